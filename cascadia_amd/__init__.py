@@ -11,8 +11,8 @@ was not built (``python cascadia_amd/build.py``).  There is no CPU fallback.
 import torch  # noqa: F401
 
 from ._lib import (ROUTE_IDS, ROUTE_SIGMOID_BIAS, ROUTE_SOFTMAX_TOPK, CascadiaInt4Error,
-                   LIB_PATH, SCALE_BF16, SCALE_F16, SIGNATURES, TILING_CRATE, TILING_MFMA,
-                   TILING_MFMA_UP_ROWS, check, lib)
+                   LIB_PATH, SCALE_BF16, SCALE_F16, SCORE_SIGMOID, SCORE_SOFTMAX, SIGNATURES,
+                   TILING_CRATE, TILING_MFMA, TILING_MFMA_UP_ROWS, check, lib)
 
 lib()  # fail loudly at import when the HIP library is missing
 
@@ -33,6 +33,8 @@ from .api import (GROUP_SIZE, HIDDEN, INTERMEDIATE, NIBBLES_PER_INT32, ExpertSou
                   dequant_axpy_int4_active_auto, fill_bytes, fill_normal,
                   fill_scales, gate_up_silu, gemm_int4_bf16, gemm_workspace_bytes, MoEExperts,
                   moe_forward,
+                  Fp8Experts, fp8_gemm, fp8_gemm_workspace_bytes, fp8_moe_forward,
+                  fp8_moe_workspace_bytes, quantize_fp8, quantize_fp8_blocks, route_experts,
                   moe_workspace_bytes, ov_gemv, ov_to_crate, quantize_int4_group, tile_weights,
                   tiled_sizes)
 
@@ -56,4 +58,7 @@ __all__ = [
     "build_active_mask_per_channel", "dequant_gemv_int4_rows_subset",
     "dequant_gemv_int4_rows_subset_auto", "expert_forward_sparse_mode",
     "ffn_forward_sparse_f32_mode", "stream_read",
+    "SCORE_SIGMOID", "SCORE_SOFTMAX", "Fp8Experts", "fp8_gemm", "fp8_gemm_workspace_bytes",
+    "fp8_moe_forward", "fp8_moe_workspace_bytes", "quantize_fp8", "quantize_fp8_blocks",
+    "route_experts",
 ]

@@ -69,9 +69,29 @@ class Routing(C.Structure):
                 ("ids", C.c_void_p), ("weights", C.c_void_p), ("threshold", C.c_float)]
 
 
+SCORE_SOFTMAX = 0
+SCORE_SIGMOID = 1
+FP8_X_BF16 = 0
+FP8_X_F32 = 1
+FP8_X_E4M3 = 2
+
+
+class Router(C.Structure):
+    _fields_ = [("n_experts", C.c_uint32), ("top_k", C.c_uint32), ("score", C.c_uint32),
+                ("n_groups", C.c_uint32), ("top_groups", C.c_uint32), ("group_best", C.c_uint32),
+                ("normalize", C.c_uint32), ("scale", C.c_float), ("bias", C.c_void_p)]
+
+
+class Fp8MoeLayer(C.Structure):
+    _fields_ = [("hidden", C.c_uint32), ("inter", C.c_uint32), ("n_experts", C.c_uint32),
+                ("gate_up", C.c_void_p), ("gate_up_scales", C.c_void_p), ("down", C.c_void_p),
+                ("down_scales", C.c_void_p)]
+
+
 _vp, _u32, _u64, _sz, _f64, _i32 = C.c_void_p, C.c_uint32, C.c_uint64, C.c_size_t, C.c_double, C.c_int
 _LP, _EP = C.POINTER(Layout), C.POINTER(Expert)
 _MP, _RP = C.POINTER(MoeLayer), C.POINTER(Routing)
+_FP = C.POINTER(Fp8MoeLayer)
 
 # Every symbol declared in include/cascadia_int4.h: (restype, argtypes).
 SIGNATURES = {
@@ -102,6 +122,15 @@ SIGNATURES = {
     "cascadia_int4_gate_up_silu": (_i32, [_u32, _u32, _u32, _u32, _EP, _vp, _u32, _u32, _vp, _vp]),
     "cascadia_int4_moe_workspace_bytes": (_sz, [_MP, _u32, _u32]),
     "cascadia_int4_moe_forward": (_i32, [_MP, _RP, _vp, _vp, _u32, _vp, _vp, _vp, _vp, _vp]),
+    "cascadia_int4_route_experts": (_i32, [C.POINTER(Router), _vp, _u32, _u32, _vp, _vp, _vp]),
+    "cascadia_int4_fp8_quantize": (_i32, [_vp, _u32, _u32, _u32, _vp, _vp, _vp]),
+    "cascadia_int4_fp8_quantize_blocks": (_i32, [_vp, _u32, _u32, _vp, _vp, _vp]),
+    "cascadia_int4_fp8_gemm_workspace_bytes": (_sz, [_u32, _u32, _u32, _u32]),
+    "cascadia_int4_fp8_gemm": (_i32, [_u32, _u32, _vp, _vp, _vp, _u32, _vp, _u32, _vp, _u32, _vp,
+                                      _vp]),
+    "cascadia_int4_fp8_moe_workspace_bytes": (_sz, [_FP, _u32, _u32]),
+    "cascadia_int4_fp8_moe_forward": (_i32, [_FP, _u32, _vp, _vp, C.c_float, _vp, _u32, _vp, _u32,
+                                             _vp, _u32, _vp, _vp]),
     "cascadia_int4_debug_dequant": (_i32, [_LP, _vp, _vp, _vp, _vp]),
     "cascadia_int4_stream_read": (_i32, [_vp, _sz, _vp, _vp]),
     "cascadia_int4_fill_synthetic": (_i32, [_u32, _u64, _u64, _sz, _f64, _f64, _u32, _vp, _vp]),

@@ -19,9 +19,10 @@ from operator import index as _index
 import numpy as np
 import torch
 
-from ._lib import (ROUTE_IDS, ROUTE_SIGMOID_BIAS, ROUTE_SOFTMAX_TOPK, Expert, Layout, MoeLayer,
-                   OvSegment, Routing, SCALE_BF16, SCALE_F16, TILING_CRATE, TILING_MFMA,
-                   TILING_MFMA_UP_ROWS, check, lib)
+from ._lib import (FP8_X_BF16, FP8_X_E4M3, FP8_X_F32, ROUTE_IDS, ROUTE_SIGMOID_BIAS,
+                   ROUTE_SOFTMAX_TOPK, Expert, Fp8MoeLayer, Layout, MoeLayer, OvSegment, Router,
+                   Routing, SCALE_BF16, SCALE_F16, SCORE_SIGMOID, SCORE_SOFTMAX, TILING_CRATE,
+                   TILING_MFMA, TILING_MFMA_UP_ROWS, check, lib)
 
 # K2.6 constants of the crate (lib.rs:71-78)
 HIDDEN = 7168
@@ -969,6 +970,239 @@ def moe_forward(experts: MoEExperts, x, out, *, top_k: int, logits=None, bias=No
             raise ValueError(f"workspace has {workspace.nbytes} bytes, the call needs {need}")
     check("cascadia_int4_moe_forward", lib().cascadia_int4_moe_forward(
         C.byref(experts._struct()), C.byref(R), x.data_ptr(), res, T, out.data_ptr(), io, wo, ws,
+        _stream()))
+    return out
+
+
+# ---------------------------------------------------------------------------
+# routing to experts, and products in 8-bit floating point
+# ---------------------------------------------------------------------------
+
+FP8_BLOCK = 128  # columns of a row's group; rows and columns of a weight block
+
+
+def _here(t: torch.Tensor, name: str) -> torch.Tensor:
+    """A contiguous tensor of the current device (the one whose stream the call
+    is enqueued on)."""
+    _dev(t, name)
+    if t.device.index != _device():
+        raise ValueError(f"{name} is on {t.device}, the current device is {_device()}")
+    return t
+
+
+def _fp8_blocks(n: int) -> int:
+    return (n + FP8_BLOCK - 1) // FP8_BLOCK
+
+
+def _is_e4m3(t: torch.Tensor) -> bool:
+    return t.dtype in (torch.float8_e4m3fn, torch.uint8)
+
+
+def _fp8_matrix(codes, scales, lead, n_rows, k_cols, name):
+    """Check e4m3 codes [*lead, n_rows, k_cols] and their blocks' scales."""
+    _here(codes, name), _here(scales, f"{name} scales")
+    if not (n_rows >= 1 and k_cols >= 16 and k_cols % 16 == 0):
+        raise ValueError(f"{name}: k_cols {k_cols} must be a multiple of 16")
+    if not (_is_e4m3(codes) and codes.numel() == lead * n_rows * k_cols):
+        raise ValueError(f"{name}: e4m3 codes of {lead * n_rows * k_cols} values")
+    need = lead * _fp8_blocks(n_rows) * _fp8_blocks(k_cols)
+    if not (scales.dtype == torch.float32 and scales.numel() == need):
+        raise ValueError(f"{name} scales: f32, one per block of 128 x 128 ({need})")
+
+
+def route_experts(logits, top_k: int, ids, weights, *, score: int = SCORE_SIGMOID, bias=None,
+                  n_groups: int = 1, top_groups: int = 1, group_best: int = 2,
+                  normalize: bool = True, scale: float = 1.0):
+    """Choose top_k experts per token from router logits [n_tokens, n_experts]
+    (f32 or bf16) into ids (int32) and weights (f32) [n_tokens, top_k], as
+    moe_forward (ROUTE_IDS) and fp8_moe_forward take them.
+    s = sigmoid(logit) or softmax over all experts; the choice goes by s + bias
+    (f32 [n_experts]; without one by the logits), within the top_groups of
+    n_groups groups of neighbouring experts whose group_best (1 or 2) best add up
+    to the most; descending, ties to the lower id.  weights: the chosen s, over
+    their sum when normalize, times scale.  A NaN logit counts as -infinity; a
+    softmax over -infinity alone gives weights of 0."""
+    _here(logits, "logits"), _here(ids, "ids"), _here(weights, "weights")
+    if logits.dim() != 2 or logits.dtype not in (torch.float32, torch.bfloat16):
+        raise ValueError("logits: f32 or bf16 [n_tokens, n_experts]")
+    T, E = logits.shape
+    if not (ids.dtype == torch.int32 and ids.numel() == T * top_k):
+        raise ValueError("ids: int32 [n_tokens, top_k]")
+    if not (weights.dtype == torch.float32 and weights.numel() == T * top_k):
+        raise ValueError("weights: f32 [n_tokens, top_k]")
+    b = 0
+    if bias is not None:
+        _here(bias, "bias")
+        _expect(bias.dtype == torch.float32 and bias.numel() == E, "bias: f32 [n_experts]")
+        b = bias.data_ptr()
+    if not (1 <= E <= 1024 and 1 <= top_k <= 16 and 1 <= n_groups <= 64 and E % n_groups == 0
+            and 1 <= top_groups <= n_groups and top_k <= top_groups * (E // n_groups)
+            and group_best in (1, 2) and score in (SCORE_SOFTMAX, SCORE_SIGMOID)):
+        raise ValueError(f"routing of {E} experts: top_k {top_k}, {top_groups} of {n_groups} groups "
+                         f"by the best {group_best}, score {score}")
+    R = Router(E, top_k, score, n_groups, top_groups, group_best, int(normalize), scale, b)
+    check("cascadia_int4_route_experts", lib().cascadia_int4_route_experts(
+        C.byref(R), logits.data_ptr(), int(logits.dtype == torch.bfloat16), T, ids.data_ptr(),
+        weights.data_ptr(), _stream()))
+    return ids, weights
+
+
+def quantize_fp8(x, rows: int, k_cols: int, codes, scales):
+    """Rows of x (f32 or bf16 [rows, k_cols]) as e4m3 codes (float8_e4m3fn or
+    uint8 [rows, k_cols]) with a scale per group of 128 columns (f32 [rows,
+    ceil(k_cols / 128)]): scale = max(max|x|, 2^-96) / 448, code = e4m3(x /
+    scale), to nearest even.  k_cols: a multiple of 16."""
+    _here(x, "x"), _here(codes, "codes"), _here(scales, "scales")
+    _expect(k_cols >= 16 and k_cols % 16 == 0, f"k_cols {k_cols} must be a multiple of 16")
+    _expect(x.dtype in (torch.float32, torch.bfloat16) and x.numel() == rows * k_cols,
+            "x: f32 or bf16 [rows, k_cols]")
+    _expect(_is_e4m3(codes) and codes.numel() == rows * k_cols, "codes: e4m3 [rows, k_cols]")
+    _expect(scales.dtype == torch.float32 and scales.numel() == rows * _fp8_blocks(k_cols),
+            "scales: f32 [rows, ceil(k_cols / 128)]")
+    check("cascadia_int4_fp8_quantize", lib().cascadia_int4_fp8_quantize(
+        x.data_ptr(), int(x.dtype == torch.float32), rows, k_cols, codes.data_ptr(),
+        scales.data_ptr(), _stream()))
+    return codes, scales
+
+
+def quantize_fp8_blocks(weight_bf16, n_rows: int, k_cols: int):
+    """Quantise bf16 weights [n_rows, k_cols] for fp8_gemm (done once, at load):
+    (codes float8_e4m3fn [n_rows, k_cols], scales f32 [ceil(n_rows / 128),
+    ceil(k_cols / 128)]), a scale per block of 128 x 128 as quantize_fp8's."""
+    _here(weight_bf16, "weight_bf16")
+    _expect(n_rows >= 1 and k_cols >= 16 and k_cols % 16 == 0,
+            f"k_cols {k_cols} must be a multiple of 16")
+    _expect(_is_bf16_bits(weight_bf16) and weight_bf16.numel() == n_rows * k_cols,
+            "weight_bf16: bf16 [n_rows, k_cols]")
+    dev = weight_bf16.device
+    codes = torch.empty((n_rows, k_cols), dtype=torch.float8_e4m3fn, device=dev)
+    scales = torch.empty((_fp8_blocks(n_rows), _fp8_blocks(k_cols)), dtype=torch.float32,
+                         device=dev)
+    check("cascadia_int4_fp8_quantize_blocks", lib().cascadia_int4_fp8_quantize_blocks(
+        weight_bf16.data_ptr(), n_rows, k_cols, codes.data_ptr(), scales.data_ptr(), _stream()))
+    return codes, scales
+
+
+def _fp8_x_type(dtype) -> int:
+    if dtype == torch.bfloat16:
+        return FP8_X_BF16
+    if dtype == torch.float32:
+        return FP8_X_F32
+    if dtype in (torch.float8_e4m3fn, torch.uint8):
+        return FP8_X_E4M3
+    raise ValueError(f"xs: bf16, f32 or e4m3, not {dtype}")
+
+
+def fp8_gemm_workspace_bytes(n_rows: int, k_cols: int, seq: int, x_dtype=torch.bfloat16) -> int:
+    """Workspace bytes of fp8_gemm for up to seq rows of x_dtype."""
+    return int(lib().cascadia_int4_fp8_gemm_workspace_bytes(n_rows, k_cols, _fp8_x_type(x_dtype),
+                                                            seq))
+
+
+def fp8_gemm(codes, scales, xs, n_rows: int, k_cols: int, seq: int, ys, x_scales=None,
+             workspace=None):
+    """ys[t, r] = sum_b x_scale[t, b] scale[r / 128, b] sum_{c in b} x[t, c] w[r, c]
+    over blocks b of 128 columns: weights as e4m3 codes [n_rows, k_cols] with
+    scales of blocks of 128 x 128 (quantize_fp8_blocks).  xs [seq, k_cols]: bf16 or
+    f32, quantised in the call as by quantize_fp8, or e4m3 codes with x_scales
+    [seq, ceil(k_cols / 128)].  ys [seq, n_rows] bf16 or f32; f32 sums, one
+    rounding.  workspace: fp8_gemm_workspace_bytes (for a graph capture)."""
+    _fp8_matrix(codes, scales, 1, n_rows, k_cols, "codes")
+    _here(xs, "xs"), _here(ys, "ys")
+    _expect(seq >= 1, "seq must be >= 1")
+    xt = _fp8_x_type(xs.dtype)
+    if xs.numel() != seq * k_cols:
+        raise ValueError(f"xs must hold seq*k_cols = {seq * k_cols} values")
+    if not (ys.dtype in (torch.float32, torch.bfloat16) and ys.numel() == seq * n_rows):
+        raise ValueError(f"ys: f32 or bf16 [seq*n_rows = {seq * n_rows}]")
+    sp = 0
+    if xt == FP8_X_E4M3:
+        _expect(x_scales is not None, "e4m3 xs need x_scales")
+        _here(x_scales, "x_scales")
+        _expect(x_scales.dtype == torch.float32 and x_scales.numel() == seq * _fp8_blocks(k_cols),
+                "x_scales: f32 [seq, ceil(k_cols / 128)]")
+        sp = x_scales.data_ptr()
+    else:
+        _expect(x_scales is None, "x_scales go with e4m3 xs")
+    ws = 0
+    if workspace is not None:
+        _here(workspace, "workspace")
+        ws = _workspace_ptr(workspace, "cascadia_int4_fp8_gemm_workspace_bytes", n_rows, k_cols,
+                            xt, seq)
+    check("cascadia_int4_fp8_gemm", lib().cascadia_int4_fp8_gemm(
+        n_rows, k_cols, codes.data_ptr(), scales.data_ptr(), xs.data_ptr(), xt, sp, seq,
+        ys.data_ptr(), int(ys.dtype == torch.float32), ws, _stream()))
+    return ys
+
+
+class Fp8Experts:
+    """One MoE layer's experts in e4m3 (float8_e4m3fn or uint8) with f32 scales of
+    blocks of 128 x 128: gate_up [n_experts, 2, inter, hidden] (gate, then up),
+    its scales [n_experts, 2, ceil(inter / 128), ceil(hidden / 128)], down
+    [n_experts, hidden, inter], its scales [n_experts, ceil(hidden / 128),
+    ceil(inter / 128)].  hidden and inter: multiples of 16."""
+
+    def __init__(self, gate_up, gate_up_scales, down, down_scales, n_experts: int, hidden: int,
+                 inter: int):
+        _expect(1 <= n_experts <= 1024, "n_experts: 1 to 1024")
+        _fp8_matrix(gate_up, gate_up_scales, 2 * n_experts, inter, hidden, "gate_up")
+        _fp8_matrix(down, down_scales, n_experts, hidden, inter, "down")
+        self.gate_up, self.gate_up_scales = gate_up, gate_up_scales
+        self.down, self.down_scales = down, down_scales
+        self.n_experts, self.hidden, self.inter = n_experts, hidden, inter
+        self._layer = Fp8MoeLayer(hidden, inter, n_experts, gate_up.data_ptr(),
+                                  gate_up_scales.data_ptr(), down.data_ptr(),
+                                  down_scales.data_ptr())
+
+
+def fp8_moe_workspace_bytes(experts: Fp8Experts, top_k: int, n_tokens: int) -> int:
+    """Workspace bytes of fp8_moe_forward for up to n_tokens rows."""
+    return int(lib().cascadia_int4_fp8_moe_workspace_bytes(C.byref(experts._layer), top_k,
+                                                           n_tokens))
+
+
+@functools.lru_cache(maxsize=1024)
+def _fp8_moe_need(tuning, device, hidden, inter, n_experts, top_k, n_tokens):
+    L = Fp8MoeLayer(hidden, inter, n_experts, 256, 256, 256, 256)
+    return int(lib().cascadia_int4_fp8_moe_workspace_bytes(C.byref(L), top_k, n_tokens))
+
+
+def fp8_moe_forward(experts: Fp8Experts, x, out, *, top_k: int, ids, weights,
+                    threshold: float = 0.0, residual=None, workspace=None):
+    """One MoE layer over e4m3 experts: out = residual + sum_k w_k bf16(down(q(silu(
+    gate(q(x))) * up(q(x))))), q as quantize_fp8, f32 sums in slot order, one
+    rounding.  x f32 or bf16, out f32 or bf16 (residual of out's type), all
+    [n_tokens, hidden]; ids (int32) / weights (f32) [n_tokens, top_k], as
+    route_experts gives them.  Slots with a weight below threshold or an id
+    outside the layer (padding: -1) are left out.  workspace:
+    fp8_moe_workspace_bytes (for a graph capture)."""
+    _here(x, "x"), _here(out, "out"), _here(ids, "ids"), _here(weights, "weights")
+    _here(experts.gate_up, "experts")
+    H = experts.hidden
+    both = (torch.float32, torch.bfloat16)
+    _expect(x.dtype in both and out.dtype in both, "x and out must be f32 or bf16")
+    T = x.numel() // H
+    _expect(x.numel() == T * H and out.numel() == T * H and T >= 1, "x/out must be [n_tokens, hidden]")
+    _expect(1 <= top_k <= 16, "top_k: 1 to 16")
+    _expect(ids.dtype == torch.int32 and ids.numel() == T * top_k, "ids: int32 [n_tokens, top_k]")
+    _expect(weights.dtype == torch.float32 and weights.numel() == T * top_k,
+            "weights: f32 [n_tokens, top_k]")
+    res = 0
+    if residual is not None:
+        _here(residual, "residual")
+        _expect(residual.dtype == out.dtype and residual.numel() == T * H,
+                "residual: [n_tokens, hidden] of out's type")
+        res = residual.data_ptr()
+    ws = 0
+    if workspace is not None:
+        ws = _here(workspace, "workspace").data_ptr()
+        need = _fp8_moe_need(lib().cascadia_int4_tuning_generation(), _device(), H, experts.inter,
+                             experts.n_experts, int(top_k), T)
+        if workspace.nbytes < need:
+            raise ValueError(f"workspace has {workspace.nbytes} bytes, the call needs {need}")
+    check("cascadia_int4_fp8_moe_forward", lib().cascadia_int4_fp8_moe_forward(
+        C.byref(experts._layer), top_k, ids.data_ptr(), weights.data_ptr(), threshold, x.data_ptr(),
+        int(x.dtype == torch.float32), res, T, out.data_ptr(), int(out.dtype == torch.float32), ws,
         _stream()))
     return out
 

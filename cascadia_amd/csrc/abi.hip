@@ -17,6 +17,7 @@
 #include "ov.hpp"
 #include "gemv.hpp"
 #include "few.hpp"
+#include "fp8.hpp"
 #include "grouped.hpp"
 #include "quant.hpp"
 #include "skinny.hpp"
@@ -2335,6 +2336,188 @@ int cascadia_int4_moe_forward(const cascadia_int4_moe_layer *layer,
                               void *stream) {
   return moe_forward(layer, routing, x, residual, n_tokens, out, ids_out, weights_out, workspace,
                      (hipStream_t)stream);
+}
+
+// ---- routing to experts, 8-bit floating point ----
+
+namespace {
+
+constexpr uint32_t kFp8MaxRows = 1u << 24, kFp8MaxCols = 1u << 20;
+
+bool fp8_dims_ok(uint32_t n_rows, uint32_t k_cols) {
+  return n_rows >= 1 && n_rows <= kFp8MaxRows && k_cols >= 16 && k_cols <= kFp8MaxCols &&
+         k_cols % 16 == 0;
+}
+
+// Codes and scales of rows quantised within a call.
+size_t fp8_rows_bytes(uint32_t rows, uint32_t k_cols) {
+  return (((size_t)rows * k_cols + 255) & ~(size_t)255) +
+         (size_t)rows * cai4::fp8_blocks((int)k_cols) * 4;
+}
+
+int fp8_moe_check(const cascadia_int4_fp8_moe_layer *L, uint32_t top_k, uint32_t n_tokens) {
+  if (!L || !L->gate_up || !L->gate_up_scales || !L->down || !L->down_scales)
+    return CASCADIA_INT4_ERR_NULL;
+  if (!fp8_dims_ok(L->hidden, L->inter) || !fp8_dims_ok(L->inter, L->hidden) ||
+      L->n_experts == 0 || L->n_experts > (uint32_t)cai4::kRouteMaxExperts || top_k == 0 ||
+      top_k > (uint32_t)cai4::kRouteMaxTopK || n_tokens == 0 || n_tokens > (1u << 20))
+    return CASCADIA_INT4_ERR_ARG;
+  if (!aligned(L->gate_up, 16) || !aligned(L->down, 16) || !aligned(L->gate_up_scales, 4) ||
+      !aligned(L->down_scales, 4))
+    return CASCADIA_INT4_ERR_ARG;
+  return CASCADIA_INT4_OK;
+}
+
+}  // namespace
+
+int cascadia_int4_route_experts(const cascadia_int4_router *R, const void *logits,
+                                uint32_t logits_bf16, uint32_t n_tokens, int32_t *ids,
+                                float *weights, void *stream) {
+  if (!R) return CASCADIA_INT4_ERR_NULL;
+  if (R->n_experts == 0 || R->n_experts > (uint32_t)cai4::kRouteMaxExperts || R->top_k == 0 ||
+      R->top_k > (uint32_t)cai4::kRouteMaxTopK || R->score > CASCADIA_INT4_SCORE_SIGMOID ||
+      R->n_groups == 0 || R->n_groups > (uint32_t)cai4::kRouteMaxGroups ||
+      R->n_experts % R->n_groups || R->top_groups == 0 || R->top_groups > R->n_groups ||
+      R->top_k > R->top_groups * (R->n_experts / R->n_groups) || R->group_best == 0 ||
+      R->group_best > 2 || logits_bf16 > 1 || n_tokens > (1u << 30))
+    return CASCADIA_INT4_ERR_ARG;
+  if (n_tokens == 0) return CASCADIA_INT4_OK;
+  if (!logits || !ids || !weights) return CASCADIA_INT4_ERR_NULL;
+  if (!aligned(logits, logits_bf16 ? 2 : 4) || !aligned(ids, 4) || !aligned(weights, 4) ||
+      !aligned(R->bias, 4))
+    return CASCADIA_INT4_ERR_ARG;
+  cai4::RouteExperts r{};
+  r.logits = logits;
+  r.bias = R->bias;
+  r.T = (int)n_tokens;
+  r.E = (int)R->n_experts;
+  r.top_k = (int)R->top_k;
+  r.x_f32 = !logits_bf16;
+  r.sigmoid = R->score == CASCADIA_INT4_SCORE_SIGMOID;
+  r.n_groups = (int)R->n_groups;
+  r.top_groups = (int)R->top_groups;
+  r.group_best = (int)R->group_best;
+  r.normalize = R->normalize != 0;
+  r.scale = R->scale;
+  r.ids = ids;
+  r.weights = weights;
+  return hip_status(cai4::route_experts(r, (hipStream_t)stream));
+}
+
+int cascadia_int4_fp8_quantize(const void *x, uint32_t x_is_f32, uint32_t rows, uint32_t k_cols,
+                               uint8_t *codes, float *scales, void *stream) {
+  if (!fp8_dims_ok(1, k_cols) || rows > kFp8MaxRows || x_is_f32 > 1) return CASCADIA_INT4_ERR_ARG;
+  if (rows == 0) return CASCADIA_INT4_OK;
+  if (!x || !codes || !scales) return CASCADIA_INT4_ERR_NULL;
+  if (!aligned(x, 16) || !aligned(codes, 16) || !aligned(scales, 4)) return CASCADIA_INT4_ERR_ARG;
+  return hip_status(cai4::fp8_quantize_rows(x, x_is_f32 != 0, rows, (int)k_cols, codes, scales,
+                                            (hipStream_t)stream));
+}
+
+int cascadia_int4_fp8_quantize_blocks(const uint16_t *w_bf16, uint32_t n_rows, uint32_t k_cols,
+                                      uint8_t *codes, float *scales, void *stream) {
+  if (!w_bf16 || !codes || !scales) return CASCADIA_INT4_ERR_NULL;
+  if (!fp8_dims_ok(n_rows, k_cols) || n_rows > (1u << 22)) return CASCADIA_INT4_ERR_ARG;
+  if (!aligned(w_bf16, 16) || !aligned(codes, 16) || !aligned(scales, 4))
+    return CASCADIA_INT4_ERR_ARG;
+  return hip_status(cai4::fp8_quantize_blocks(w_bf16, (int)n_rows, (int)k_cols, codes, scales,
+                                              (hipStream_t)stream));
+}
+
+size_t cascadia_int4_fp8_gemm_workspace_bytes(uint32_t n_rows, uint32_t k_cols, uint32_t x_type,
+                                              uint32_t seq) {
+  if (!fp8_dims_ok(n_rows, k_cols) || seq == 0 || seq > kFp8MaxRows ||
+      x_type > CASCADIA_INT4_FP8_X_E4M3)
+    return 0;
+  return x_type == CASCADIA_INT4_FP8_X_E4M3 ? 0 : fp8_rows_bytes(seq, k_cols);
+}
+
+int cascadia_int4_fp8_gemm(uint32_t n_rows, uint32_t k_cols, const uint8_t *w,
+                           const float *w_scales, const void *xs, uint32_t x_type,
+                           const float *x_scales, uint32_t seq, void *ys, uint32_t y_is_f32,
+                           void *workspace, void *stream) {
+  if (!w || !w_scales || !xs || !ys) return CASCADIA_INT4_ERR_NULL;
+  const bool codes = x_type == CASCADIA_INT4_FP8_X_E4M3;
+  if (codes && !x_scales) return CASCADIA_INT4_ERR_NULL;
+  if (!fp8_dims_ok(n_rows, k_cols) || seq == 0 || seq > kFp8MaxRows ||
+      x_type > CASCADIA_INT4_FP8_X_E4M3 || (!codes && x_scales) || y_is_f32 > 1)
+    return CASCADIA_INT4_ERR_ARG;
+  if (!aligned(w, 16) || !aligned(w_scales, 4) || !aligned(xs, 16) || !aligned(x_scales, 4) ||
+      !aligned(ys, y_is_f32 ? 4 : 2) || !aligned(workspace, 16))
+    return CASCADIA_INT4_ERR_ARG;
+  int dev;
+  if (int rc = current_device(&dev)) return rc;
+  const hipStream_t st = (hipStream_t)stream;
+  Workspace own;
+  const size_t need = cascadia_int4_fp8_gemm_workspace_bytes(n_rows, k_cols, x_type, seq);
+  if (need && !workspace)
+    if (int rc = own.get(dev, need, st, &workspace)) return rc;
+  cai4::Fp8Gemm g{};
+  g.w = w;
+  g.ws = w_scales;
+  g.x = static_cast<const uint8_t *>(xs);
+  g.xs = x_scales;
+  g.y = ys;
+  g.N = (int)n_rows;
+  g.K = (int)k_cols;
+  g.M = (int)seq;
+  g.out_f32 = (int)y_is_f32;
+  if (!codes) {
+    uint8_t *q = static_cast<uint8_t *>(workspace);
+    float *s = reinterpret_cast<float *>(q + (((size_t)seq * k_cols + 255) & ~(size_t)255));
+    if (int rc = hip_status(cai4::fp8_quantize_rows(xs, x_type == CASCADIA_INT4_FP8_X_F32, seq,
+                                                    (int)k_cols, q, s, st)))
+      return rc;
+    g.x = q;
+    g.xs = s;
+  }
+  return hip_status(cai4::fp8_gemm(g, st));
+}
+
+size_t cascadia_int4_fp8_moe_workspace_bytes(const cascadia_int4_fp8_moe_layer *L, uint32_t top_k,
+                                             uint32_t n_tokens) {
+  if (fp8_moe_check(L, top_k, n_tokens)) return 0;
+  return cai4::fp8_moe_workspace((int)L->hidden, (int)L->inter, (int)L->n_experts, (int)top_k,
+                                 (int)n_tokens);
+}
+
+int cascadia_int4_fp8_moe_forward(const cascadia_int4_fp8_moe_layer *L, uint32_t top_k,
+                                  const int32_t *ids, const float *weights, float threshold,
+                                  const void *x, uint32_t x_is_f32, const void *residual,
+                                  uint32_t n_tokens, void *out, uint32_t out_is_f32,
+                                  void *workspace, void *stream) {
+  if (int rc = fp8_moe_check(L, top_k, n_tokens)) return rc;
+  if (!ids || !weights || !x || !out) return CASCADIA_INT4_ERR_NULL;
+  if (x_is_f32 > 1 || out_is_f32 > 1 || !aligned(ids, 4) || !aligned(weights, 4) ||
+      !aligned(x, 16) || !aligned(residual, 16) || !aligned(out, 16) || !aligned(workspace, 16))
+    return CASCADIA_INT4_ERR_ARG;
+  int dev;
+  if (int rc = current_device(&dev)) return rc;
+  const hipStream_t st = (hipStream_t)stream;
+  Workspace own;
+  if (!workspace) {
+    const size_t need = cascadia_int4_fp8_moe_workspace_bytes(L, top_k, n_tokens);
+    if (int rc = own.get(dev, need, st, &workspace)) return rc;
+  }
+  cai4::Fp8Moe m{};
+  m.H = (int)L->hidden;
+  m.I = (int)L->inter;
+  m.E = (int)L->n_experts;
+  m.gate_up = L->gate_up;
+  m.down = L->down;
+  m.gate_up_s = L->gate_up_scales;
+  m.down_s = L->down_scales;
+  m.T = (int)n_tokens;
+  m.top_k = (int)top_k;
+  m.ids = ids;
+  m.weights = weights;
+  m.threshold = threshold;
+  m.x = x;
+  m.x_f32 = (int)x_is_f32;
+  m.residual = residual;
+  m.out = out;
+  m.out_f32 = (int)out_is_f32;
+  return hip_status(cai4::fp8_moe_forward(m, workspace, st));
 }
 
 }  // extern "C"

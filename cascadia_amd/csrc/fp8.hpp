@@ -1,0 +1,75 @@
+// fp8.hpp -- 8-bit floating point (OCP e4m3) with a scale per block of 128, and
+// the routing of tokens to experts: what abi.hip calls.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stddef.h>
+#include <stdint.h>
+
+#include "skinny.hpp"
+
+namespace cai4 {
+
+// Choice of top_k of E experts per token from router logits (route.hip).
+struct RouteExperts {
+  const void *logits;  // [T, E], f32 or bf16
+  const float *bias;   // [E] or null: added to the scores for the choice only
+  int T, E, top_k;
+  int x_f32, sigmoid;                      // logits' type; scores: sigmoid, else softmax
+  int n_groups, top_groups, group_best;    // groups of E / n_groups neighbours
+  int normalize;
+  float scale;
+  int32_t *ids;    // [T, top_k]
+  float *weights;  // [T, top_k]
+};
+constexpr int kRouteMaxExperts = 1024, kRouteMaxTopK = 16, kRouteMaxGroups = 64;
+hipError_t route_experts(const RouteExperts &r, hipStream_t st);
+
+constexpr int kFp8Block = 128;
+inline int fp8_blocks(int n) { return (n + kFp8Block - 1) / kFp8Block; }
+
+// x [rows, K] (bf16 or f32) -> e4m3 codes [rows, K] and scales [rows, ceil(K / 128)].
+// K a multiple of 16; x, codes 16-byte aligned.
+hipError_t fp8_quantize_rows(const void *x, bool x_f32, size_t rows, int K, uint8_t *codes,
+                             float *scales, hipStream_t st);
+// w bf16 [N, K] -> codes [N, K] and scales [ceil(N / 128), ceil(K / 128)].
+hipError_t fp8_quantize_blocks(const uint16_t *w, int N, int K, uint8_t *codes, float *scales,
+                               hipStream_t st);
+
+// y = x w^T over e4m3 codes and their blocks' scales, for one matrix or for the
+// row groups of many experts in one launch (chunks).
+struct Fp8Gemm {
+  const uint8_t *w;  // [N, K] codes (SwiGLU: gate [N, K], then up [N, K])
+  const float *ws;   // [ceil(N / 128), KB] (SwiGLU: gate's, then up's)
+  const uint8_t *x;  // [rows, K] codes
+  const float *xs;   // [rows, KB]
+  void *y;           // [M, N]
+  int N, K, M;       // M: rows of y
+  int out_f32;       // y f32, else bf16
+  // experts: chunks of grouped rows (null: one matrix over M rows)
+  const SkinnyChunk *chunks;
+  int max_chunks;
+  const int32_t *row_map;      // grouped row -> row of x (null: the same)
+  size_t w_stride, ws_stride;  // between experts
+  int swiglu;                  // y = silu(gate) * up, f32
+};
+hipError_t fp8_gemm(const Fp8Gemm &g, hipStream_t st);
+
+// One layer's experts in e4m3.
+struct Fp8Moe {
+  int H, I, E;
+  const uint8_t *gate_up, *down;      // [E, 2, I, H], [E, H, I]
+  const float *gate_up_s, *down_s;    // [E, 2, ib, hb], [E, hb, ib]
+  int T, top_k;
+  const int32_t *ids;
+  const float *weights;
+  float threshold;
+  const void *x;
+  int x_f32;
+  const void *residual;  // [T, H] of out's type, or null
+  void *out;
+  int out_f32;
+};
+size_t fp8_moe_workspace(int H, int I, int E, int top_k, int T);
+hipError_t fp8_moe_forward(const Fp8Moe &m, void *workspace, hipStream_t st);
+
+}  // namespace cai4

@@ -435,6 +435,101 @@ int cascadia_int4_moe_forward(const cascadia_int4_moe_layer *layer,
                               int32_t *ids_out, float *weights_out, void *workspace,
                               void *stream);
 
+/* ---- routing to experts, and products in 8-bit floating point ---- */
+
+/* Choice of top_k experts per token from router logits [n_tokens, n_experts],
+ * f32 (logits_bf16 0) or bf16 bits (1): what a layer's ROUTE_IDS form and
+ * cascadia_int4_fp8_moe_forward take.  No counterpart in the crate, whose two
+ * rules are ROUTE_SIGMOID_BIAS and ROUTE_SOFTMAX_TOPK above.
+ *   s = sigmoid(logit), or softmax over all experts; c = s + bias.
+ *   n_groups > 1: the experts form n_groups groups of neighbours, a group's
+ *     score is the sum of its group_best (1 or 2) largest c, and only the
+ *     experts of the top_groups best groups (ties to the lower group) stay.
+ *   ids: the top_k by c (bias NULL: by logit), descending, ties to the lower
+ *     id; scores are computed and compared in 64 bits.
+ *   weights: s of the chosen (without the bias); divided by their sum + 1e-20
+ *     when normalize; times scale.
+ * A NaN logit counts as -infinity.  Where the largest logit of a softmax is
+ * +infinity its mass is shared by those that have it; a row of -infinity has
+ * s = 0 throughout (weights 0).  top_k <= top_groups * n_experts / n_groups. */
+#define CASCADIA_INT4_SCORE_SOFTMAX 0u
+#define CASCADIA_INT4_SCORE_SIGMOID 1u
+typedef struct cascadia_int4_router {
+  uint32_t n_experts; /* <= 1024 */
+  uint32_t top_k;     /* <= 16 */
+  uint32_t score;     /* CASCADIA_INT4_SCORE_* */
+  uint32_t n_groups, top_groups; /* n_groups <= 64 divides n_experts; 1, 1: none */
+  uint32_t group_best;           /* 1 or 2 */
+  uint32_t normalize;
+  float scale;
+  const float *bias; /* f32 [n_experts] or NULL */
+} cascadia_int4_router;
+int cascadia_int4_route_experts(const cascadia_int4_router *router, const void *logits,
+                                uint32_t logits_bf16, uint32_t n_tokens, int32_t *ids,
+                                float *weights, void *stream);
+
+/* Quantisation to OCP e4m3 with f32 scales: top = max(max|x|, 2^-96) of a
+ * group, scale = top / 448, code = e4m3(x / scale) to nearest even; the codes
+ * stand for code * scale.  _quantize: rows of x (f32 when x_is_f32, else bf16
+ * bits) [rows, k_cols] in groups of 128 columns, scales
+ * [rows, ceil(k_cols / 128)].  _quantize_blocks: bf16 weights [n_rows, k_cols]
+ * in blocks of 128 x 128, scales [ceil(n_rows / 128), ceil(k_cols / 128)] (done
+ * once, at load).  The last group of a row and the last blocks may be short.
+ * k_cols: a multiple of 16; x, w and codes 16-byte aligned.  A group that holds
+ * an infinity or NaN stands for NaN wherever a product meets it (a NaN alone:
+ * for its own code). */
+int cascadia_int4_fp8_quantize(const void *x, uint32_t x_is_f32, uint32_t rows, uint32_t k_cols,
+                               uint8_t *codes, float *scales, void *stream);
+int cascadia_int4_fp8_quantize_blocks(const uint16_t *w_bf16, uint32_t n_rows, uint32_t k_cols,
+                                      uint8_t *codes, float *scales, void *stream);
+
+/* ys[t, r] = sum over blocks b of 128 columns of x_scale[t, b] *
+ * w_scale[r / 128, b] * sum_{c in b} x[t, c] w[r, c], f32 sums, one rounding:
+ * ys [seq, n_rows] f32 (y_is_f32) or bf16.  w: e4m3 codes [n_rows, k_cols] with
+ * scales as _quantize_blocks lays them out.  xs [seq, k_cols]: bf16 or f32
+ * (quantised in the call as by _quantize; x_scales NULL), or e4m3 codes with
+ * x_scales [seq, ceil(k_cols / 128)].  k_cols a multiple of 16; w and xs 16-byte
+ * aligned.  workspace: 16-byte aligned, of at least _workspace_bytes for seq
+ * rows or more, or NULL for the library's.  seq >= 1. */
+#define CASCADIA_INT4_FP8_X_BF16 0u
+#define CASCADIA_INT4_FP8_X_F32 1u
+#define CASCADIA_INT4_FP8_X_E4M3 2u
+size_t cascadia_int4_fp8_gemm_workspace_bytes(uint32_t n_rows, uint32_t k_cols, uint32_t x_type,
+                                              uint32_t seq);
+int cascadia_int4_fp8_gemm(uint32_t n_rows, uint32_t k_cols, const uint8_t *w,
+                           const float *w_scales, const void *xs, uint32_t x_type,
+                           const float *x_scales, uint32_t seq, void *ys, uint32_t y_is_f32,
+                           void *workspace, void *stream);
+
+/* One MoE layer's experts in e4m3: gate_up [n_experts, 2, inter, hidden] (each
+ * expert's gate, then its up) with scales [n_experts, 2, ceil(inter / 128),
+ * ceil(hidden / 128)]; down [n_experts, hidden, inter] with scales [n_experts,
+ * ceil(hidden / 128), ceil(inter / 128)].  hidden and inter multiples of 16. */
+typedef struct cascadia_int4_fp8_moe_layer {
+  uint32_t hidden, inter, n_experts; /* n_experts <= 1024 */
+  const uint8_t *gate_up;
+  const float *gate_up_scales;
+  const uint8_t *down;
+  const float *down_scales;
+} cascadia_int4_fp8_moe_layer;
+
+/* out_t = residual_t + sum_k weights[t, k] * y_{t,k} in slot order, one
+ * rounding, with y_{t,k} = bf16(down_e(q(silu(gate_e(q(x_t))) * up_e(q(x_t)))))
+ * for e = ids[t, k] and q the quantisation above in groups of 128; f32 sums.
+ * ids (int32) / weights (f32) [n_tokens, top_k], as route_experts or the caller
+ * gives them: a slot with weight < threshold or an id outside the layer is left
+ * out (padding: -1).  A shared expert is an expert of the stack that every
+ * token lists.  x [n_tokens, hidden] f32 (x_is_f32) or bf16; out f32
+ * (out_is_f32) or bf16, residual of out's type or NULL.  x, residual and out
+ * 16-byte aligned; top_k <= 16; n_tokens >= 1.  workspace as above. */
+size_t cascadia_int4_fp8_moe_workspace_bytes(const cascadia_int4_fp8_moe_layer *layer,
+                                             uint32_t top_k, uint32_t n_tokens);
+int cascadia_int4_fp8_moe_forward(const cascadia_int4_fp8_moe_layer *layer, uint32_t top_k,
+                                  const int32_t *ids, const float *weights, float threshold,
+                                  const void *x, uint32_t x_is_f32, const void *residual,
+                                  uint32_t n_tokens, void *out, uint32_t out_is_f32,
+                                  void *workspace, void *stream);
+
 /* Dequantise to f32 [n_rows, k_cols] (bit-exact w = q*s; the kernel's own
  * decode path).  No crate counterpart; the parity check of the weights. */
 int cascadia_int4_debug_dequant(const cascadia_int4_layout *layout, const uint8_t *packed,

@@ -1,0 +1,134 @@
+"""64-bit reference of the routing and 8-bit floating-point operators (numpy,
+on the CPU), with bounds on what 32-bit arithmetic may add."""
+import numpy as np
+import torch
+
+U32 = 2.0 ** -24   # half a step of f32, relative
+BF16 = 2.0 ** -8   # half a step of bf16, relative
+
+
+def e4m3(codes):
+    """Codes (uint8 array or float8 tensor) as the values they stand for."""
+    if isinstance(codes, torch.Tensor):
+        codes = codes.cpu().view(torch.uint8).numpy()
+    return torch.from_numpy(np.ascontiguousarray(codes)).view(torch.float8_e4m3fn).double().numpy()
+
+
+def e4m3_step(v):
+    """The distance between neighbouring e4m3 values around |v|."""
+    a = np.maximum(np.abs(v), 2.0 ** -6)
+    return 2.0 ** (np.floor(np.log2(a)) - 3)
+
+
+def round_e4m3(v):
+    s = e4m3_step(v)
+    return np.round(v / s) * s
+
+
+def blocks(n):
+    return (n + 127) // 128
+
+
+def spread(s, n, k, rows=128):
+    return np.repeat(np.repeat(s, rows, -2)[..., :n, :], 128, -1)[..., :k]
+
+
+def tops(x, rows):
+    """Group maxima (groups of `rows` x 128) of x [n, k], at least 2^-96."""
+    n, k = x.shape
+    nb, kb = -(-n // rows), blocks(k)
+    p = np.zeros((nb * rows, kb * 128))
+    p[:n, :k] = np.abs(x)
+    return np.maximum(p.reshape(nb, rows, kb, 128).max((1, 3)), 2.0 ** -96)
+
+
+def quotients(x, rows):
+    """(x / (top / 448), top / 448) in 64 bits."""
+    x = np.asarray(x, np.float64)
+    t = tops(x, rows)
+    return x * 448.0 / spread(t, *x.shape, rows=rows), t / 448.0
+
+
+def gemm(xq, xs, wq, ws):
+    """(y, bound): the product in 64 bits, and how far f32 sums may be off: the
+    products are exact; a block's 128 are added in some order, each sum within
+    2^-23 of itself (a matrix core may truncate rather than round), then scaled
+    (two products) and added over the blocks."""
+    n, k = wq.shape
+    xd = xq * np.repeat(xs, 128, 1)[:, :k]
+    wd = wq * spread(ws, n, k)
+    y = xd @ wd.T
+    return y, (128 + blocks(k) + 4) * 2 * U32 * (np.abs(xd) @ np.abs(wd).T)
+
+
+def silu(g):
+    with np.errstate(over="ignore"):
+        return g / (1.0 + np.exp(-g))
+
+
+def moe(x, gate_up, gate_up_s, down, down_s, ids, weights, threshold, residual):
+    """(out, bound) of one layer in 64 bits (codes as values), bound without the
+    output's own rounding."""
+    T, H = x.shape
+    E, _, I, _ = gate_up.shape
+    q, s = quotients(x, 1)
+    xq = round_e4m3(q)
+    out = np.zeros((T, H)) if residual is None else np.array(residual, np.float64)
+    bound = np.zeros((T, H))
+    total = np.abs(out).copy()
+    for t in range(T):
+        for j in range(ids.shape[1]):
+            e, w = int(ids[t, j]), float(weights[t, j])
+            if w < threshold or not 0 <= e < E:
+                continue
+            (g, bg), (u, bu) = (gemm(xq[t:t + 1], s[t:t + 1], gate_up[e, i], gate_up_s[e, i])
+                                for i in (0, 1))
+            h = silu(g) * u
+            # |silu'| <= 1.1; the exponential, the division and two products round
+            bh = 1.1 * bg * np.abs(u) + np.abs(silu(g)) * bu + 1.1 * bg * bu + 16 * U32 * np.abs(h)
+            hq, hs = quotients(h, 1)
+            code = round_e4m3(hq)
+            # a quotient off by more than its distance from the border between two
+            # codes may take the neighbouring one; the group's maximum is off too
+            top_off = tops(bh, 1) / tops(h, 1) + 4 * U32
+            off = bh / spread(hs, 1, I, rows=1) + np.abs(hq) * spread(top_off, 1, I, rows=1)
+            step = e4m3_step(hq)
+            border = np.abs(np.abs(hq - code) - step / 2) <= off
+            dh = np.where(border, step, 0.0) + np.abs(code) * spread(top_off, 1, I, rows=1)
+            y, by = gemm(code, hs, down[e], down_s[e])
+            wd = np.abs(down[e] * spread(down_s[e], H, I))
+            by = by + (dh * spread(hs, 1, I, rows=1)) @ wd.T
+            y, by = y[0], by[0]
+            out[t] += w * y
+            bound[t] += abs(w) * (by + BF16 * (np.abs(y) + by))
+            total[t] += np.abs(w * y)
+    return out, bound + (ids.shape[1] + 2) * 2 * U32 * total
+
+
+def route(logits, top_k, score, bias, n_groups, top_groups, group_best, normalize, scale):
+    """(ids, weights) in 64 bits, straight from the definition."""
+    ids, weights = [], []
+    for row in np.asarray(logits, np.float64):
+        l = np.where(np.isnan(row), -np.inf, row)
+        E = l.size
+        with np.errstate(over="ignore", invalid="ignore"):
+            if score == "sigmoid":
+                s = 1.0 / (1.0 + np.exp(-l))
+            elif l.max() == -np.inf:
+                s = np.zeros(E)
+            else:
+                s = np.where(l == l.max(), 1.0, np.exp(l - l.max()))
+                s = s / s.sum()
+        c = s if bias is None else s + np.asarray(bias, np.float64)
+        per = E // n_groups
+        g = [sum(sorted(c[i * per:(i + 1) * per])[::-1][:group_best]) for i in range(n_groups)]
+        kept = sorted(range(n_groups), key=lambda i: (-g[i], i))[:top_groups]
+        order = c if bias is not None else l
+        left = [e for e in range(E) if e // per in kept]
+        chosen = sorted(left, key=lambda e: (-order[e], e))[:top_k]
+        w = s[chosen]
+        if normalize:
+            w = w / (w.sum() + 1e-20)
+        ids.append(chosen)
+        weights.append(w * scale)
+    return np.array(ids, np.int32), np.array(weights)
