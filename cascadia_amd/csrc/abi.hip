@@ -2360,7 +2360,8 @@ int fp8_moe_check(const cascadia_int4_fp8_moe_layer *L, uint32_t top_k, uint32_t
     return CASCADIA_INT4_ERR_NULL;
   if (!fp8_dims_ok(L->hidden, L->inter) || !fp8_dims_ok(L->inter, L->hidden) ||
       L->n_experts == 0 || L->n_experts > (uint32_t)cai4::kRouteMaxExperts || top_k == 0 ||
-      top_k > (uint32_t)cai4::kRouteMaxTopK || n_tokens == 0 || n_tokens > (1u << 20))
+      top_k > (uint32_t)cai4::kRouteMaxTopK || n_tokens == 0 || n_tokens > (1u << 20) ||
+      (size_t)n_tokens * L->hidden > 0x7FFFFFFFu)
     return CASCADIA_INT4_ERR_ARG;
   if (!aligned(L->gate_up, 16) || !aligned(L->down, 16) || !aligned(L->gate_up_scales, 4) ||
       !aligned(L->down_scales, 4))

@@ -47,12 +47,15 @@ struct Fp8Gemm {
   int out_f32;       // y f32, else bf16
   // experts: chunks of grouped rows (null: one matrix over M rows)
   const SkinnyChunk *chunks;
-  int max_chunks;
+  int max_chunks, chunk_rows;
   const int32_t *row_map;      // grouped row -> row of x (null: the same)
+  int x_rows;                  // rows of x (row_map)
   size_t w_stride, ws_stride;  // between experts
   int swiglu;                  // y = silu(gate) * up, f32
 };
 hipError_t fp8_gemm(const Fp8Gemm &g, hipStream_t st);
+constexpr int kFp8TileRows = 128;  // rows of a chunk on the tile kernel (16 else)
+hipError_t fp8_tile_gemm(const Fp8Gemm &g, hipStream_t st);
 
 // One layer's experts in e4m3.
 struct Fp8Moe {

@@ -18,11 +18,14 @@
 namespace cai4 {
 namespace {
 
-constexpr int kFp8ChunkRows = 16;
+// Rows of a chunk: the tile kernel's from a mean of 16 rows per expert.
+int chunk_rows(int T, int E, int top_k) {
+  return (int64_t)T * top_k >= (int64_t)16 * E ? kFp8TileRows : 16;
+}
 
 struct Layout {
   size_t xq, xs, pos, row_map, chunks, counts, h, hq, hs, y, total;
-  int max_chunks;
+  int max_chunks, chunk_rows;
 };
 
 Layout layout_of(int H, int I, int E, int top_k, int T) {
@@ -34,7 +37,8 @@ Layout layout_of(int H, int I, int E, int top_k, int T) {
     o += (bytes + 255) & ~(size_t)255;
     return at;
   };
-  w.max_chunks = moe_max_chunks(T, E, top_k, kFp8ChunkRows);
+  w.chunk_rows = chunk_rows(T, E, top_k);
+  w.max_chunks = moe_max_chunks(T, E, top_k, w.chunk_rows);
   w.xq = take((size_t)T * H);
   w.xs = take((size_t)T * fp8_blocks(H) * 4);
   w.pos = take(n * 4);
@@ -98,7 +102,7 @@ hipError_t fp8_moe_forward(const Fp8Moe &m, void *workspace, hipStream_t st) {
   const int n = m.T * m.top_k, hb = fp8_blocks(m.H), ib = fp8_blocks(m.I);
   hipError_t e = fp8_quantize_rows(m.x, m.x_f32, m.T, m.H, xq, xs, st);
   if (e != hipSuccess) return e;
-  e = moe_group(m.ids, m.weights, m.threshold, m.T, m.E, m.top_k, kFp8ChunkRows, w.max_chunks, pos,
+  e = moe_group(m.ids, m.weights, m.threshold, m.T, m.E, m.top_k, w.chunk_rows, w.max_chunks, pos,
                 row_map, chunks, reinterpret_cast<int32_t *>(b + w.counts), st);
   if (e != hipSuccess) return e;
   Fp8Gemm g{};
@@ -113,6 +117,8 @@ hipError_t fp8_moe_forward(const Fp8Moe &m, void *workspace, hipStream_t st) {
   g.out_f32 = 1;
   g.chunks = chunks;
   g.max_chunks = w.max_chunks;
+  g.chunk_rows = w.chunk_rows;
+  g.x_rows = m.T;
   g.row_map = row_map;
   g.w_stride = (size_t)2 * m.I * m.H;
   g.ws_stride = (size_t)2 * ib * hb;

@@ -273,6 +273,17 @@ def gemm_ref(w, ws, x, xs):
     return y, b + d @ np.abs(wd * ref.spread(wsd, *wd.shape)).T
 
 
+def eight_bit(w, ws, x, xs):
+    n, k = w.shape
+    if xs is None:
+        q, s = ref.quotients(x.double().numpy(), 1)
+        xq = ref.round_e4m3(q)
+    else:
+        xq, s = ref.e4m3(x), xs.double().numpy()
+    return ref.eight_bit_sums(xq * np.repeat(s, 128, 1)[:, :k],
+                              ref.e4m3(w) * ref.spread(ws.double().numpy(), n, k))
+
+
 def check_gemm(cl, w, ws, x, xs, y_dtype, workspace=None):
     m, k = x.shape
     n = w.shape[0]
@@ -281,6 +292,8 @@ def check_gemm(cl, w, ws, x, xs, y_dtype, workspace=None):
                 x_scales=None if xs is None else xs.cuda(), workspace=workspace)
     want, bound = gemm_ref(w, ws, x, xs)
     if y_dtype == torch.bfloat16:
+        if m > 16:  # products of many rows may run on the 8-bit MFMAs
+            bound = bound + eight_bit(w, ws, x, xs)
         bound = bound + ref.BF16 * (np.abs(want) + bound)
     off = np.abs(y.double().cpu().numpy() - want) - bound
     assert np.all(off <= 0), (off.max(), np.unravel_index(np.argmax(off), off.shape))
