@@ -48,6 +48,7 @@ struct Fp8Gemm {
   // experts: chunks of grouped rows (null: one matrix over M rows)
   const SkinnyChunk *chunks;
   int max_chunks, chunk_rows;
+  const int32_t *n_chunks;     // how many of them there are (device)
   const int32_t *row_map;      // grouped row -> row of x (null: the same)
   int x_rows;                  // rows of x (row_map)
   size_t w_stride, ws_stride;  // between experts

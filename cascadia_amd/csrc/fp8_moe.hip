@@ -118,6 +118,7 @@ hipError_t fp8_moe_forward(const Fp8Moe &m, void *workspace, hipStream_t st) {
   g.chunks = chunks;
   g.max_chunks = w.max_chunks;
   g.chunk_rows = w.chunk_rows;
+  g.n_chunks = reinterpret_cast<const int32_t *>(b + w.counts) + 1;
   g.x_rows = m.T;
   g.row_map = row_map;
   g.w_stride = (size_t)2 * m.I * m.H;

@@ -3,7 +3,7 @@
 // groups of many experts in one launch.
 //
 // A block of 128 columns is one step: both operands' codes go global -> LDS by
-// loads with an LDS destination (two stages), each wave reads the fragments of
+// loads with an LDS destination (S stages), each wave reads the fragments of
 // its 16 NI weight rows and 16 NJ tokens, and every 16 x 16 tile's partial sum
 // over the block (starting from zero) enters its f32 sum with the product of the
 // two scales: one f32 scale per token and block, since a wave's weight rows lie
@@ -27,8 +27,10 @@
 // Order: weight tiles outside, tokens inside.  The tokens' fragments stay in
 // registers for the block, the weights' are read one tile ahead.  Before the
 // last weight tile nothing of the stage is left to read: there the one barrier
-// of the block stands, which also publishes the next stage; its loads were
-// issued one block earlier, those of the stage after it go into the freed one.
+// of the block stands, which also publishes the next stage; the freed one takes
+// the loads of the block S further (past the last block: loads out of range, so
+// that every wait counts the same number).  The tokens' scales come with the
+// stage, each wave's own.
 #include "fp8.hpp"
 #include "fp8_common.hpp"
 #include "fp8_rows.hpp"
@@ -62,27 +64,50 @@ CAI4_DEV void pin(f32x4_t &v) {
 
 // WN x WM waves of 16 NI weight rows x 16 NJ tokens.  SW: a wave's first NI / 2
 // tiles are gate rows, the others the same rows of up.
-template <int NI, int NJ, int WN, int WM, bool SW>
+template <int NI, int NJ, int WN, int WM, bool SW, int S>
 struct Tile {
   static constexpr int W = WN * WM, BN = 16 * NI * WN, BM = 16 * NJ * WM;
   static constexpr int OUT = SW ? BN / 2 : BN;  // output columns
-  static constexpr int STAGE = (BN + BM) * 128;
+  static constexpr int XS = (BN + BM) * 128, STAGE = XS + W * 256;  // codes, then scales
   static constexpr int PW = BN / 8 / W, PX = BM / 8 / W;  // 1 KB loads per wave and stage
   static_assert(PW * W * 8 == BN && PX * W * 8 == BM, "pieces");
   static_assert(128 % (16 * NI / (SW ? 2 : 1)) == 0, "a wave's rows lie in one scale block");
-  static_assert(2 * STAGE <= 160 * 1024, "LDS");
+  static constexpr int LOADS = PW + PX + 1;
+  static_assert(S >= 2 && S * STAGE <= 160 * 1024, "LDS");
+  static_assert(NJ <= 4, "a wave's scales are one load");
 };
 
-template <int NI, int NJ, int WN, int WM, bool SW, bool EXACT>
+// A workgroup's place: m tile (or chunk) and n tile.  Workgroups go round the
+// eight XCDs; each takes a run of neighbouring tiles, so that those that run
+// together share rows of both operands in its L2.  One matrix: groups of 4 m
+// tiles, n outside, m inside (32 workgroups: 4 x 8 tiles).  Experts: n outside,
+// the chunks inside, where neighbours are one expert's; `tiles` counts the chunks
+// there are, not the table's length.
+struct Place {
+  int m, n;
+};
+CAI4_DEV Place place_of(int id, int mtiles, int ntiles, bool grouped) {
+  const int total = mtiles * ntiles, per = (total + 7) >> 3, t = (id & 7) * per + (id >> 3);
+  if ((id >> 3) >= per || t >= total) return Place{-1, 0};
+  if (grouped) return Place{t % mtiles, t / mtiles};
+  const int group = t / (4 * ntiles), r = t - group * 4 * ntiles;
+  const int gm = mtiles - group * 4 < 4 ? mtiles - group * 4 : 4;
+  return Place{group * 4 + r % gm, r / gm};
+}
+
+template <int NI, int NJ, int WN, int WM, bool SW, bool EXACT, int S>
 __global__ __launch_bounds__(64 * WN * WM) void fp8_tile_kernel(Fp8Gemm g, int ntiles) {
-  using P = Tile<NI, NJ, WN, WM, SW>;
-  __shared__ __attribute__((aligned(1024))) uint8_t st[2 * P::STAGE];
+  using P = Tile<NI, NJ, WN, WM, SW, S>;
+  __shared__ __attribute__((aligned(1024))) uint8_t st[S * P::STAGE];
   const int lane = threadIdx.x & 63, l15 = lane & 15, c = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wn = wave % WN, wm = wave / WN;
-  const int mt = blockIdx.x / ntiles, n0 = (blockIdx.x - mt * ntiles) * P::OUT;
-  const Rows rows = rows_of(g, mt, P::BM);
-  if (rows.count <= 0) return;  // the whole workgroup
+  const int mtiles = g.chunks ? __builtin_amdgcn_readfirstlane(*g.n_chunks)
+                              : (g.M + P::BM - 1) / P::BM;
+  const Place at = place_of(blockIdx.x, mtiles, ntiles, g.chunks != nullptr);
+  if (at.m < 0) return;  // the whole workgroup
+  const int n0 = at.n * P::OUT;
+  const Rows rows = rows_of(g, at.m, P::BM);
   const int KB = (g.K + 127) >> 7, NB = (g.N + 127) >> 7;
   const int nr = g.N - n0 < P::OUT ? g.N - n0 : P::OUT;
   // this wave loads rows of the weights (SwiGLU: the first half gate, the others up)
@@ -114,8 +139,15 @@ __global__ __launch_bounds__(64 * WN * WM) void fp8_tile_kernel(Fp8Gemm g, int n
             : (g.row_map ? (uint32_t)g.row_map[rows.row0 + r] * (uint32_t)g.K
                          : (uint32_t)(r * g.K)) + 16 * chunk_of(r);
   }
-  auto issue = [&](int kb) {
-    const uint32_t to = lds0 + (kb & 1) * P::STAGE, soff = (uint32_t)kb * 128;
+  // this wave's tokens' scales
+  uint32_t vs = kDmaOOB;
+  {
+    const int r = wm * NJ * 16 + lane;
+    if (lane < NJ * 16 && r < rows.count)
+      vs = (g.row_map ? (uint32_t)g.row_map[rows.row0 + r] : (uint32_t)r) * (uint32_t)KB * 4;
+  }
+  auto issue = [&](int kb, uint32_t to) {
+    const uint32_t soff = (uint32_t)kb * 128;
     const int left = g.K - 128 * kb;  // a short last block reads zeros past it
 #pragma unroll
     for (int q = 0; q < P::PW; ++q) {
@@ -129,35 +161,24 @@ __global__ __launch_bounds__(64 * WN * WM) void fp8_tile_kernel(Fp8Gemm g, int n
       const uint32_t v = 16 * chunk_of(piece * 8 + (lane >> 3)) < left ? vx[q] : kDmaOOB;
       lds_dma<16>(xr, to + P::BN * 128 + piece * 1024, v, soff);
     }
+    lds_dma<4>(sr, to + P::XS + wave * 256, left > 0 ? vs : kDmaOOB, (uint32_t)kb * 4);
   };
 
-  // ---- scales: one per token and block, times the weight rows' ----
-  uint32_t so[NJ];
-#pragma unroll
-  for (int j = 0; j < NJ; ++j) {
-    const int r = (wm * NJ + j) * 16 + l15;
-    so[j] = r >= rows.count ? kDmaOOB
-            : g.row_map     ? (uint32_t)g.row_map[rows.row0 + r] * (uint32_t)KB * 4
-                            : (uint32_t)(r * KB) * 4;
-  }
+  // ---- scales: a token's times the weight rows' ----
   const int nw = SW ? n0 + wn * 8 * NI : n0 + wn * 16 * NI;  // this wave's first row
   const bool idle = nw >= g.N;
-  const size_t eo = (size_t)rows.expert * g.ws_stride;
-  const float *ws = g.ws + eo + (size_t)((idle ? n0 : nw) >> 7) * KB;
+  typedef const __attribute__((address_space(4))) float *scalar_t;  // scalar loads
+  const scalar_t ws = (scalar_t)(g.ws + (size_t)rows.expert * g.ws_stride +
+                                 (size_t)((idle ? n0 : nw) >> 7) * KB);
   constexpr int NS = SW ? 2 : 1;
-  float xv[NJ], wv[NS], s[NS][NJ];
-  auto load_scales = [&](int kb) {
+  const uint32_t fs = lds0 + P::XS + wave * 256 + l15 * 4;
+  auto take_scales = [&](uint32_t base, int kb, float (&to)[NS][NJ]) {
 #pragma unroll
-    for (int j = 0; j < NJ; ++j)
-      xv[j] = bitsf(__builtin_amdgcn_raw_buffer_load_b32(sr, so[j], kb * 4, 0));
-    wv[0] = ws[kb];
-    if (SW) wv[NS - 1] = ws[(size_t)NB * KB + kb];
-  };
-  auto take_scales = [&](float (&to)[NS][NJ]) {
+    for (int m = 0; m < NS; ++m) {
+      const float f = ws[(size_t)m * NB * KB + kb];
 #pragma unroll
-    for (int m = 0; m < NS; ++m)
-#pragma unroll
-      for (int j = 0; j < NJ; ++j) to[m][j] = xv[j] * wv[m];
+      for (int j = 0; j < NJ; ++j) to[m][j] = lds_at<float>(base + fs, j * 64) * f;
+    }
   };
 
   // ---- fragments: chunks c and c + 4 of rows 16 i + l15 ----
@@ -181,19 +202,19 @@ __global__ __launch_bounds__(64 * WN * WM) void fp8_tile_kernel(Fp8Gemm g, int n
 #pragma unroll
     for (int j = 0; j < NJ; ++j) acc[i][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 
-  load_scales(0);
-  issue(0);
-  dma_wait_barrier<0>();
-  take_scales(s);
-  if (KB > 1) issue(1);
+  float s[NS][NJ];
+#pragma unroll
+  for (int q = 0; q < S; ++q) issue(q, lds0 + q * P::STAGE);
+  dma_wait_barrier<(S - 1) * P::LOADS>();
+  take_scales(0, 0, s);
 #pragma unroll
   for (int j = 0; j < NJ; ++j) read_b(0, j);
   read_a(0, 0, 0);
   constexpr int LAG = 2;  // MFMAs between one and the use of its result
   f32x4_t p[LAG + 1];
+  uint32_t base = 0;
   for (int kb = 0; kb < KB; ++kb) {
-    const uint32_t base = (kb & 1) * P::STAGE, next = P::STAGE - base;
-    load_scales(kb + 1 < KB ? kb + 1 : kb);
+    const uint32_t next = base + P::STAGE == S * P::STAGE ? 0 : base + P::STAGE;
     float sn[NS][NJ];
     auto add = [&](int slot) {
       const int i = slot / NJ, j = slot % NJ;
@@ -208,9 +229,9 @@ __global__ __launch_bounds__(64 * WN * WM) void fp8_tile_kernel(Fp8Gemm g, int n
       if (i + 1 < NI) {
         read_a(base, i + 1, (i + 1) & 1);
       } else {
-        dma_wait_barrier<0>();
-        take_scales(sn);
-        if (kb + 2 < KB) issue(kb + 2);
+        dma_wait_barrier<(S - 2) * P::LOADS>();
+        issue(kb + S, lds0 + base);
+        take_scales(next, kb + 1 < KB ? kb + 1 : kb, sn);
       }
 #pragma unroll
       for (int j = 0; j < NJ; ++j) {
@@ -231,8 +252,10 @@ __global__ __launch_bounds__(64 * WN * WM) void fp8_tile_kernel(Fp8Gemm g, int n
     for (int m = 0; m < NS; ++m)
 #pragma unroll
       for (int j = 0; j < NJ; ++j) s[m][j] = sn[m][j];
+    base = next;
   }
 
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // nothing may land in LDS after the end
   if (idle) return;
 #pragma unroll
   for (int j = 0; j < NJ; ++j) {
@@ -254,24 +277,24 @@ __global__ __launch_bounds__(64 * WN * WM) void fp8_tile_kernel(Fp8Gemm g, int n
   }
 }
 
-template <int NI, int NJ, int WN, int WM, bool SW, bool EXACT>
+template <int NI, int NJ, int WN, int WM, bool SW, bool EXACT, int S>
 hipError_t launch(const Fp8Gemm &g, hipStream_t st) {
-  using P = Tile<NI, NJ, WN, WM, SW>;
+  using P = Tile<NI, NJ, WN, WM, SW, S>;
   const int nt = (g.N + P::OUT - 1) / P::OUT;
   const size_t tiles = (size_t)nt * (g.chunks ? g.max_chunks : (g.M + P::BM - 1) / P::BM);
-  if (tiles > 0x7FFFFFFFu) return hipErrorInvalidValue;
-  hipLaunchKernelGGL((fp8_tile_kernel<NI, NJ, WN, WM, SW, EXACT>), dim3((unsigned)tiles),
-                     dim3(64 * P::W), 0, st, g, nt);
+  if (tiles > 0x7FFFFFF0u) return hipErrorInvalidValue;
+  hipLaunchKernelGGL((fp8_tile_kernel<NI, NJ, WN, WM, SW, EXACT, S>),
+                     dim3((unsigned)((tiles + 7) / 8 * 8)), dim3(64 * P::W), 0, st, g, nt);
   return hipGetLastError();
 }
 
 }  // namespace
 
 hipError_t fp8_tile_gemm(const Fp8Gemm &g, hipStream_t st) {
-  if (g.swiglu) return launch<8, 2, 2, 4, true, true>(g, st);
-  if (g.out_f32) return launch<8, 2, 2, 4, false, true>(g, st);
-  if (g.chunks) return launch<8, 2, 2, 4, false, false>(g, st);
-  return launch<8, 4, 2, 4, false, false>(g, st);
+  if (g.swiglu) return launch<8, 2, 2, 4, true, true, 3>(g, st);
+  if (g.out_f32) return launch<8, 2, 2, 4, false, true, 3>(g, st);
+  if (g.chunks) return launch<8, 2, 2, 4, false, false, 3>(g, st);
+  return launch<8, 4, 2, 4, false, false, 2>(g, st);
 }
 
 }  // namespace cai4
