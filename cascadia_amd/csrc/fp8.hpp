@@ -5,8 +5,6 @@
 #include <stddef.h>
 #include <stdint.h>
 
-#include "skinny.hpp"
-
 namespace cai4 {
 
 // Choice of top_k of E experts per token from router logits (route.hip).
@@ -35,6 +33,12 @@ hipError_t fp8_quantize_rows(const void *x, bool x_f32, size_t rows, int K, uint
 hipError_t fp8_quantize_blocks(const uint16_t *w, int N, int K, uint8_t *codes, float *scales,
                                hipStream_t st);
 
+// Rows row0 .. row0 + count of the grouped rows, of one expert; chunk first +
+// [0, number) are that expert's.
+struct Fp8Chunk {
+  int expert, row0, count, first, number;
+};
+
 // y = x w^T over e4m3 codes and their blocks' scales, for one matrix or for the
 // row groups of many experts in one launch (chunks).
 struct Fp8Gemm {
@@ -46,13 +50,14 @@ struct Fp8Gemm {
   int N, K, M;       // M: rows of y
   int out_f32;       // y f32, else bf16
   // experts: chunks of grouped rows (null: one matrix over M rows)
-  const SkinnyChunk *chunks;
+  const Fp8Chunk *chunks;
   int max_chunks, chunk_rows;
   const int32_t *n_chunks;     // how many of them there are (device)
   const int32_t *row_map;      // grouped row -> row of x (null: the same)
   int x_rows;                  // rows of x (row_map)
   size_t w_stride, ws_stride;  // between experts
-  int swiglu;                  // y = silu(gate) * up, f32
+  int swiglu;                  // y = silu(gate) * up: f32, or codes with ys
+  float *ys;                   // SwiGLU on tiles: y's scales [rows, ceil(N / 128)]
 };
 hipError_t fp8_gemm(const Fp8Gemm &g, hipStream_t st);
 constexpr int kFp8TileRows = 128;  // rows of a chunk on the tile kernel (16 else)

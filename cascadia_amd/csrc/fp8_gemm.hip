@@ -43,8 +43,8 @@ __global__ __launch_bounds__(64 * kFewWaves) void fp8_few_kernel(Fp8Gemm g) {
   const int lane = threadIdx.x & 63, l15 = lane & 15, c = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int ntiles = (g.N + 15) >> 4, mt = blockIdx.x / ntiles;
+  if (g.chunks && mt >= *g.n_chunks) return;  // the whole workgroup
   const Rows rows = rows_of(g, mt, 16);
-  if (rows.count <= 0) return;  // the whole workgroup
   const int n0 = (blockIdx.x - mt * ntiles) * 16, KB = (g.K + 127) >> 7, NB = (g.N + 127) >> 7;
   const int nr = g.N - n0 < 16 ? g.N - n0 : 16;
   const uint8_t *w = g.w + (size_t)rows.expert * g.w_stride + (size_t)n0 * g.K;

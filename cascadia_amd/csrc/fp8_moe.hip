@@ -8,12 +8,16 @@
 // intermediate (top_k times its output), and their rounding is no coarser than
 // that of a bf16 output.
 //
-// Rows are grouped by expert (moe_group): position in a group varies between
-// calls, results do not, since a grouped row's products do not depend on its
-// place and the sum reads slots in order.
+// Rows are grouped by expert.  Position in a group varies between calls, results
+// do not: a grouped row's products do not depend on its place, and the sum reads
+// slots in order.
+//
+// Launches: x's codes and, in workgroups of the same launch, the experts' counts
+// (for up to 1,024 slots the whole grouping); the grouping; gate / up; h's codes
+// (on tiles in the gate / up launch itself); down; the weighted sum.
 #include "fp8.hpp"
 #include "fp8_common.hpp"
-#include "moe.hpp"
+#include "fp8_quant.hpp"
 
 namespace cai4 {
 namespace {
@@ -23,9 +27,17 @@ int chunk_rows(int T, int E, int top_k) {
   return (int64_t)T * top_k >= (int64_t)16 * E ? kFp8TileRows : 16;
 }
 
+// Workgroups that count: 1,024 slots each, at most 64 (a placing workgroup adds
+// up all counts before its own).
+constexpr int kCountSlots = 1024, kMaxCounters = 64;
+int counters(size_t n) {
+  const size_t b = (n + kCountSlots - 1) / kCountSlots;
+  return b < (size_t)kMaxCounters ? (int)b : kMaxCounters;
+}
+
 struct Layout {
-  size_t xq, xs, pos, row_map, chunks, counts, h, hq, hs, y, total;
-  int max_chunks, chunk_rows;
+  size_t xq, xs, pos, row_map, chunks, counts, hist, h, hq, hs, y, total;
+  int max_chunks, chunk_rows, counters;
 };
 
 Layout layout_of(int H, int I, int E, int top_k, int T) {
@@ -38,19 +50,159 @@ Layout layout_of(int H, int I, int E, int top_k, int T) {
     return at;
   };
   w.chunk_rows = chunk_rows(T, E, top_k);
-  w.max_chunks = moe_max_chunks(T, E, top_k, w.chunk_rows);
+  // sum of ceil(c_e / C) <= A + (n - A) / C for A experts with rows
+  const size_t a = n < (size_t)E ? n : E;
+  w.max_chunks = (int)(a + (n - a) / w.chunk_rows);
+  w.counters = counters(n);
   w.xq = take((size_t)T * H);
   w.xs = take((size_t)T * fp8_blocks(H) * 4);
   w.pos = take(n * 4);
   w.row_map = take(n * 4);
-  w.chunks = take((size_t)w.max_chunks * sizeof(SkinnyChunk));
+  w.chunks = take((size_t)w.max_chunks * sizeof(Fp8Chunk));
   w.counts = take(16);
-  w.h = take(n * I * 4);
+  w.hist = take((size_t)w.counters * E * 4);
+  w.h = take(w.chunk_rows == kFp8TileRows ? 0 : n * I * 4);
   w.hq = take(n * I);
   w.hs = take(n * fp8_blocks(I) * 4);
   w.y = take(n * H * 2);
   w.total = o;
   return w;
+}
+
+struct Group {
+  const int32_t *ids;
+  const float *weights;
+  float threshold;
+  int n, top_k, E, chunk_rows, counters;
+  int32_t *pos, *row_map, *hist;  // hist: [counters, E]
+  Fp8Chunk *chunks;
+  int32_t *n_chunks;
+};
+
+constexpr int kGroupThreads = 256, kPer = kRouteMaxExperts / kGroupThreads;
+struct GroupLds {
+  int cnt[kRouteMaxExperts];  // counts; then first rows
+  int waves[2][4];
+};
+
+// The slots of counter b: [first, last).
+CAI4_DEV void slots_of(const Group &g, int b, int &first, int &last) {
+  const int per = (g.n + g.counters - 1) / g.counters;
+  first = b * per;
+  last = first + per < g.n ? first + per : g.n;
+}
+
+// Counts a share of the slots; pos[i] becomes slot i's rank among its expert's in
+// the share, or -1 for a slot that is left out.
+CAI4_DEV void count_slots(const Group &g, int b, GroupLds &l) {
+  for (int e = threadIdx.x; e < g.E; e += kGroupThreads) l.cnt[e] = 0;
+  __syncthreads();
+  int first, last;
+  slots_of(g, b, first, last);
+  for (int i = first + (int)threadIdx.x; i < last; i += kGroupThreads) {
+    const int e = g.ids[i];
+    const bool in = !(g.weights[i] < g.threshold) && e >= 0 && e < g.E;
+    g.pos[i] = in ? atomicAdd(&l.cnt[e], 1) : -1;
+  }
+  __syncthreads();
+}
+
+// Inclusive sum over the workgroup's threads of v.
+CAI4_DEV int group_scan(int v, int *waves) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) {
+    const int u = __shfl_up(v, d);
+    if (lane >= d) v += u;
+  }
+  if (lane == 63) waves[wave] = v;
+  __syncthreads();
+  for (int q = 0; q < wave; ++q) v += waves[q];
+  return v;
+}
+
+// From the experts' counts over all slots (total) and over the shares before this
+// one (before), kPer neighbouring experts per thread: first rows, chunks (by
+// share 0), and the places of the share's slots.
+CAI4_DEV void place_slots(const Group &g, int b, const int *total, const int *before,
+                          GroupLds &l) {
+  const int e0 = threadIdx.x * kPer;
+  int rows = 0, chunks = 0;
+#pragma unroll
+  for (int q = 0; q < kPer; ++q) {
+    rows += total[q];
+    chunks += (total[q] + g.chunk_rows - 1) / g.chunk_rows;
+  }
+  int row = group_scan(rows, l.waves[0]) - rows;
+  int chunk = group_scan(chunks, l.waves[1]) - chunks;
+  __syncthreads();  // (counts read by every thread before they are replaced)
+#pragma unroll
+  for (int q = 0; q < kPer; ++q) {
+    const int e = e0 + q, nc = (total[q] + g.chunk_rows - 1) / g.chunk_rows;
+    if (e < g.E) {
+      l.cnt[e] = row + before[q];
+      if (b == 0)
+        for (int i = 0; i < nc; ++i) {
+          const int left = total[q] - i * g.chunk_rows;
+          g.chunks[chunk + i] = Fp8Chunk{e, row + i * g.chunk_rows,
+                                         left < g.chunk_rows ? left : g.chunk_rows, chunk, nc};
+        }
+    }
+    row += total[q];
+    chunk += nc;
+  }
+  if (b == 0 && threadIdx.x == kGroupThreads - 1) *g.n_chunks = chunk;
+  __syncthreads();
+  int first, last;
+  slots_of(g, b, first, last);
+  for (int i = first + (int)threadIdx.x; i < last; i += kGroupThreads) {
+    const int rank = g.pos[i];
+    if (rank < 0) continue;
+    const int p = l.cnt[g.ids[i]] + rank;
+    g.pos[i] = p;
+    g.row_map[p] = i / g.top_k;
+  }
+}
+
+// The first `counters` workgroups count (one alone: also places), the others
+// quantise x.
+template <bool F32>
+__global__ __launch_bounds__(256) void fp8_moe_prep_kernel(Group g, const void *x, size_t groups,
+                                                           int K, int KB, uint8_t *codes,
+                                                           float *scales) {
+  __shared__ GroupLds l;
+  const int b = blockIdx.x;
+  if (b >= g.counters) {
+    quantize_rows_step<F32>((size_t)(b - g.counters), x, groups, K, KB, codes, scales);
+    return;
+  }
+  count_slots(g, b, l);
+  const int e0 = threadIdx.x * kPer;
+  if (g.counters == 1) {
+    int total[kPer], before[kPer];
+#pragma unroll
+    for (int q = 0; q < kPer; ++q) {
+      total[q] = e0 + q < g.E ? l.cnt[e0 + q] : 0;
+      before[q] = 0;
+    }
+    place_slots(g, 0, total, before, l);
+  } else {
+    for (int e = threadIdx.x; e < g.E; e += kGroupThreads) g.hist[(size_t)b * g.E + e] = l.cnt[e];
+  }
+}
+
+__global__ __launch_bounds__(256) void fp8_moe_place_kernel(Group g) {
+  __shared__ GroupLds l;
+  const int b = blockIdx.x, e0 = threadIdx.x * kPer;
+  int total[kPer] = {}, before[kPer] = {};
+  for (int s = 0; s < g.counters; ++s)
+#pragma unroll
+    for (int q = 0; q < kPer; ++q) {
+      const int v = e0 + q < g.E ? g.hist[(size_t)s * g.E + e0 + q] : 0;
+      total[q] += v;
+      before[q] += s < b ? v : 0;
+    }
+  place_slots(g, b, total, before, l);
 }
 
 CAI4_DEV f32x4_t load4(const void *p, size_t at, bool f32) {
@@ -96,37 +248,57 @@ hipError_t fp8_moe_forward(const Fp8Moe &m, void *workspace, hipStream_t st) {
   uint8_t *b = static_cast<uint8_t *>(workspace);
   uint8_t *xq = b + w.xq, *hq = b + w.hq;
   float *xs = reinterpret_cast<float *>(b + w.xs), *hs = reinterpret_cast<float *>(b + w.hs);
-  int32_t *pos = reinterpret_cast<int32_t *>(b + w.pos);
-  int32_t *row_map = reinterpret_cast<int32_t *>(b + w.row_map);
-  SkinnyChunk *chunks = reinterpret_cast<SkinnyChunk *>(b + w.chunks);
   const int n = m.T * m.top_k, hb = fp8_blocks(m.H), ib = fp8_blocks(m.I);
-  hipError_t e = fp8_quantize_rows(m.x, m.x_f32, m.T, m.H, xq, xs, st);
+  Group gr{};
+  gr.ids = m.ids;
+  gr.weights = m.weights;
+  gr.threshold = m.threshold;
+  gr.n = n;
+  gr.top_k = m.top_k;
+  gr.E = m.E;
+  gr.chunk_rows = w.chunk_rows;
+  gr.counters = w.counters;
+  gr.pos = reinterpret_cast<int32_t *>(b + w.pos);
+  gr.row_map = reinterpret_cast<int32_t *>(b + w.row_map);
+  gr.hist = reinterpret_cast<int32_t *>(b + w.hist);
+  gr.chunks = reinterpret_cast<Fp8Chunk *>(b + w.chunks);
+  gr.n_chunks = reinterpret_cast<int32_t *>(b + w.counts);
+  const size_t groups = (size_t)m.T * hb;
+  const dim3 grid((unsigned)(w.counters + (groups + kRowGroups - 1) / kRowGroups));
+  if (m.x_f32)
+    hipLaunchKernelGGL(fp8_moe_prep_kernel<true>, grid, dim3(256), 0, st, gr, m.x, groups, m.H, hb,
+                       xq, xs);
+  else
+    hipLaunchKernelGGL(fp8_moe_prep_kernel<false>, grid, dim3(256), 0, st, gr, m.x, groups, m.H,
+                       hb, xq, xs);
+  if (w.counters > 1)
+    hipLaunchKernelGGL(fp8_moe_place_kernel, dim3(w.counters), dim3(256), 0, st, gr);
+  hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
-  e = moe_group(m.ids, m.weights, m.threshold, m.T, m.E, m.top_k, w.chunk_rows, w.max_chunks, pos,
-                row_map, chunks, reinterpret_cast<int32_t *>(b + w.counts), st);
-  if (e != hipSuccess) return e;
+  const bool tiles = w.chunk_rows == kFp8TileRows;
   Fp8Gemm g{};
   g.w = m.gate_up;
   g.ws = m.gate_up_s;
   g.x = xq;
   g.xs = xs;
-  g.y = b + w.h;
+  g.y = tiles ? hq : b + w.h;
+  g.ys = hs;
   g.N = m.I;
   g.K = m.H;
   g.M = n;
   g.out_f32 = 1;
-  g.chunks = chunks;
+  g.chunks = gr.chunks;
   g.max_chunks = w.max_chunks;
   g.chunk_rows = w.chunk_rows;
-  g.n_chunks = reinterpret_cast<const int32_t *>(b + w.counts) + 1;
+  g.n_chunks = gr.n_chunks;
   g.x_rows = m.T;
-  g.row_map = row_map;
+  g.row_map = gr.row_map;
   g.w_stride = (size_t)2 * m.I * m.H;
   g.ws_stride = (size_t)2 * ib * hb;
   g.swiglu = 1;
   e = fp8_gemm(g, st);
   if (e != hipSuccess) return e;
-  e = fp8_quantize_rows(b + w.h, true, n, m.I, hq, hs, st);
+  if (!tiles) e = fp8_quantize_rows(b + w.h, true, n, m.I, hq, hs, st);
   if (e != hipSuccess) return e;
   g.w = m.down;
   g.ws = m.down_s;
@@ -143,7 +315,7 @@ hipError_t fp8_moe_forward(const Fp8Moe &m, void *workspace, hipStream_t st) {
   e = fp8_gemm(g, st);
   if (e != hipSuccess) return e;
   hipLaunchKernelGGL(fp8_combine_kernel, dim3(m.T, (m.H + 1023) / 1024), dim3(256), 0, st,
-                     m.residual, reinterpret_cast<const uint16_t *>(b + w.y), pos, m.weights, m.H,
+                     m.residual, reinterpret_cast<const uint16_t *>(b + w.y), gr.pos, m.weights, m.H,
                      m.top_k, m.out, m.out_f32);
   return hipGetLastError();
 }

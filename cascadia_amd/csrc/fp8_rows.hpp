@@ -14,7 +14,7 @@ struct Rows {
 CAI4_DEV Rows rows_of(const Fp8Gemm &g, int chunk, int per) {
   Rows r;
   if (g.chunks) {
-    const SkinnyChunk c = g.chunks[chunk];
+    const Fp8Chunk c = g.chunks[chunk];
     r.expert = __builtin_amdgcn_readfirstlane(c.expert);
     r.row0 = __builtin_amdgcn_readfirstlane(c.row0);
     r.count = __builtin_amdgcn_readfirstlane(c.count);

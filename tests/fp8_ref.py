@@ -82,7 +82,7 @@ def silu(g):
 
 def moe(x, gate_up, gate_up_s, down, down_s, ids, weights, threshold, residual):
     """(out, bound) of one layer in 64 bits (codes as values), bound without the
-    output's own rounding.  Of many tokens the down products may run on the 8-bit
+    output's own rounding.  Of many tokens the products may run on the 8-bit
     MFMAs."""
     T, H = x.shape
     E, _, I, _ = gate_up.shape
@@ -98,6 +98,10 @@ def moe(x, gate_up, gate_up_s, down, down_s, ids, weights, threshold, residual):
                 continue
             (g, bg), (u, bu) = (gemm(xq[t:t + 1], s[t:t + 1], gate_up[e, i], gate_up_s[e, i])
                                 for i in (0, 1))
+            if T > 16:
+                xd = xq[t:t + 1] * np.repeat(s[t:t + 1], 128, 1)[:, :H]
+                bg, bu = (b + eight_bit_sums(xd, gate_up[e, i] * spread(gate_up_s[e, i], I, H))
+                          for i, b in ((0, bg), (1, bu)))
             h = silu(g) * u
             # |silu'| <= 1.1; the exponential, the division and two products round
             bh = 1.1 * bg * np.abs(u) + np.abs(silu(g)) * bu + 1.1 * bg * bu + 16 * U32 * np.abs(h)
