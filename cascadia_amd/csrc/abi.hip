@@ -2349,10 +2349,18 @@ bool fp8_dims_ok(uint32_t n_rows, uint32_t k_cols) {
          k_cols % 16 == 0;
 }
 
-// Codes and scales of rows quantised within a call.
-size_t fp8_rows_bytes(uint32_t rows, uint32_t k_cols) {
-  return (((size_t)rows * k_cols + 255) & ~(size_t)255) +
-         (size_t)rows * cai4::fp8_blocks((int)k_cols) * 4;
+// A call's workspace: scales in rows of fp8_ld, then, of rows that it quantises,
+// their codes.
+struct Fp8Workspace {
+  size_t codes, total;
+};
+Fp8Workspace fp8_workspace(uint32_t n_rows, uint32_t k_cols, uint32_t x_type, uint32_t seq) {
+  const bool given = x_type == CASCADIA_INT4_FP8_X_E4M3;
+  Fp8Workspace w{};
+  if (given && !cai4::fp8_tiles((int)seq, (int)n_rows, (int)k_cols)) return w;
+  w.codes = ((size_t)seq * cai4::fp8_ld((int)k_cols) * 4 + 255) & ~(size_t)255;
+  w.total = w.codes + (given ? 0 : (size_t)seq * k_cols);
+  return w;
 }
 
 int fp8_moe_check(const cascadia_int4_fp8_moe_layer *L, uint32_t top_k, uint32_t n_tokens) {
@@ -2412,7 +2420,7 @@ int cascadia_int4_fp8_quantize(const void *x, uint32_t x_is_f32, uint32_t rows, 
   if (!x || !codes || !scales) return CASCADIA_INT4_ERR_NULL;
   if (!aligned(x, 16) || !aligned(codes, 16) || !aligned(scales, 4)) return CASCADIA_INT4_ERR_ARG;
   return hip_status(cai4::fp8_quantize_rows(x, x_is_f32 != 0, rows, (int)k_cols, codes, scales,
-                                            (hipStream_t)stream));
+                                            cai4::fp8_blocks((int)k_cols), (hipStream_t)stream));
 }
 
 int cascadia_int4_fp8_quantize_blocks(const uint16_t *w_bf16, uint32_t n_rows, uint32_t k_cols,
@@ -2430,7 +2438,7 @@ size_t cascadia_int4_fp8_gemm_workspace_bytes(uint32_t n_rows, uint32_t k_cols, 
   if (!fp8_dims_ok(n_rows, k_cols) || seq == 0 || seq > kFp8MaxRows ||
       x_type > CASCADIA_INT4_FP8_X_E4M3)
     return 0;
-  return x_type == CASCADIA_INT4_FP8_X_E4M3 ? 0 : fp8_rows_bytes(seq, k_cols);
+  return fp8_workspace(n_rows, k_cols, x_type, seq).total;
 }
 
 int cascadia_int4_fp8_gemm(uint32_t n_rows, uint32_t k_cols, const uint8_t *w,
@@ -2450,9 +2458,12 @@ int cascadia_int4_fp8_gemm(uint32_t n_rows, uint32_t k_cols, const uint8_t *w,
   if (int rc = current_device(&dev)) return rc;
   const hipStream_t st = (hipStream_t)stream;
   Workspace own;
-  const size_t need = cascadia_int4_fp8_gemm_workspace_bytes(n_rows, k_cols, x_type, seq);
-  if (need && !workspace)
-    if (int rc = own.get(dev, need, st, &workspace)) return rc;
+  const Fp8Workspace need = fp8_workspace(n_rows, k_cols, x_type, seq);
+  const int blocks = cai4::fp8_blocks((int)k_cols), ld = cai4::fp8_ld((int)k_cols);
+  // given scales are read where they are unless tiles want their rows aligned
+  const bool pad = codes && need.total && (blocks != ld || !aligned(x_scales, 16));
+  if ((!codes || pad) && !workspace)
+    if (int rc = own.get(dev, need.total, st, &workspace)) return rc;
   cai4::Fp8Gemm g{};
   g.w = w;
   g.ws = w_scales;
@@ -2463,14 +2474,18 @@ int cascadia_int4_fp8_gemm(uint32_t n_rows, uint32_t k_cols, const uint8_t *w,
   g.K = (int)k_cols;
   g.M = (int)seq;
   g.out_f32 = (int)y_is_f32;
-  if (!codes) {
-    uint8_t *q = static_cast<uint8_t *>(workspace);
-    float *s = reinterpret_cast<float *>(q + (((size_t)seq * k_cols + 255) & ~(size_t)255));
-    if (int rc = hip_status(cai4::fp8_quantize_rows(xs, x_type == CASCADIA_INT4_FP8_X_F32, seq,
-                                                    (int)k_cols, q, s, st)))
-      return rc;
-    g.x = q;
+  g.ld_xs = blocks;
+  if (!codes || pad) {
+    float *s = static_cast<float *>(workspace);
+    uint8_t *q = static_cast<uint8_t *>(workspace) + need.codes;
+    const hipError_t e =
+        pad ? cai4::fp8_pad_scales(x_scales, seq, blocks, s, ld, st)
+            : cai4::fp8_quantize_rows(xs, x_type == CASCADIA_INT4_FP8_X_F32, seq, (int)k_cols, q, s,
+                                      ld, st);
+    if (e != hipSuccess) return CASCADIA_INT4_ERR_DEVICE;
     g.xs = s;
+    g.ld_xs = ld;
+    if (!codes) g.x = q;
   }
   return hip_status(cai4::fp8_gemm(g, st));
 }

@@ -25,10 +25,16 @@ hipError_t route_experts(const RouteExperts &r, hipStream_t st);
 constexpr int kFp8Block = 128;
 inline int fp8_blocks(int n) { return (n + kFp8Block - 1) / kFp8Block; }
 
-// x [rows, K] (bf16 or f32) -> e4m3 codes [rows, K] and scales [rows, ceil(K / 128)].
-// K a multiple of 16; x, codes 16-byte aligned.
+// Scales per row inside a workspace: rows of 16 bytes' multiple.
+inline int fp8_ld(int K) { return (fp8_blocks(K) + 3) & ~3; }
+
+// x [rows, K] (bf16 or f32) -> e4m3 codes [rows, K] and scales [rows, ld], ceil(K /
+// 128) of them.  K a multiple of 16; x, codes 16-byte aligned.
 hipError_t fp8_quantize_rows(const void *x, bool x_f32, size_t rows, int K, uint8_t *codes,
-                             float *scales, hipStream_t st);
+                             float *scales, int ld, hipStream_t st);
+// Scales [rows, KB] to rows of ld.
+hipError_t fp8_pad_scales(const float *scales, size_t rows, int KB, float *to, int ld,
+                          hipStream_t st);
 // w bf16 [N, K] -> codes [N, K] and scales [ceil(N / 128), ceil(K / 128)].
 hipError_t fp8_quantize_blocks(const uint16_t *w, int N, int K, uint8_t *codes, float *scales,
                                hipStream_t st);
@@ -45,7 +51,8 @@ struct Fp8Gemm {
   const uint8_t *w;  // [N, K] codes (SwiGLU: gate [N, K], then up [N, K])
   const float *ws;   // [ceil(N / 128), KB] (SwiGLU: gate's, then up's)
   const uint8_t *x;  // [rows, K] codes
-  const float *xs;   // [rows, KB]
+  const float *xs;   // [rows, ld_xs], KB of them used (tiles: 16-byte aligned rows)
+  int ld_xs;
   void *y;           // [M, N]
   int N, K, M;       // M: rows of y
   int out_f32;       // y f32, else bf16
@@ -57,9 +64,12 @@ struct Fp8Gemm {
   int x_rows;                  // rows of x (row_map)
   size_t w_stride, ws_stride;  // between experts
   int swiglu;                  // y = silu(gate) * up: f32, or codes with ys
-  float *ys;                   // SwiGLU on tiles: y's scales [rows, ceil(N / 128)]
+  float *ys;                   // SwiGLU on tiles: y's scales [rows, ld_ys]
+  int ld_ys;
 };
 hipError_t fp8_gemm(const Fp8Gemm &g, hipStream_t st);
+// Whether a product of M rows runs on tiles, and how many scales it wants per row.
+bool fp8_tiles(int M, int N, int K);
 constexpr int kFp8TileRows = 128;  // rows of a chunk on the tile kernel (16 else)
 hipError_t fp8_tile_gemm(const Fp8Gemm &g, hipStream_t st);
 

@@ -55,7 +55,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void fp8_few_kernel(Fp8Gemm g) {
   const int grow = rows.row0 + (tok ? l15 : 0);
   const int xrow = g.row_map ? g.row_map[grow] : grow;
   const uint8_t *x = g.x + (size_t)xrow * g.K;
-  const float *xs = g.xs + (size_t)xrow * KB;
+  const float *xs = g.xs + (size_t)xrow * g.ld_xs;
   f32x4_t acc[MT];
 #pragma unroll
   for (int m = 0; m < MT; ++m) acc[m] = f32x4_t{0.f, 0.f, 0.f, 0.f};
@@ -101,8 +101,10 @@ __global__ __launch_bounds__(64 * kFewWaves) void fp8_few_kernel(Fp8Gemm g) {
 
 }  // namespace
 
+bool fp8_tiles(int M, int N, int K) { return M > 64; }
+
 hipError_t fp8_gemm(const Fp8Gemm &g, hipStream_t st) {
-  if (g.chunks ? g.chunk_rows > 16 : g.M > 64) return fp8_tile_gemm(g, st);
+  if (g.chunks ? g.chunk_rows > 16 : fp8_tiles(g.M, g.N, g.K)) return fp8_tile_gemm(g, st);
   const size_t tiles = (size_t)((g.N + 15) / 16) * (g.chunks ? g.max_chunks : (g.M + 15) / 16);
   if (tiles > 0x7FFFFFFFu) return hipErrorInvalidValue;
   const dim3 grid((unsigned)tiles);

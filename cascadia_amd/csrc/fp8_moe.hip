@@ -55,7 +55,7 @@ Layout layout_of(int H, int I, int E, int top_k, int T) {
   w.max_chunks = (int)(a + (n - a) / w.chunk_rows);
   w.counters = counters(n);
   w.xq = take((size_t)T * H);
-  w.xs = take((size_t)T * fp8_blocks(H) * 4);
+  w.xs = take((size_t)T * fp8_ld(H) * 4);
   w.pos = take(n * 4);
   w.row_map = take(n * 4);
   w.chunks = take((size_t)w.max_chunks * sizeof(Fp8Chunk));
@@ -63,7 +63,7 @@ Layout layout_of(int H, int I, int E, int top_k, int T) {
   w.hist = take((size_t)w.counters * E * 4);
   w.h = take(w.chunk_rows == kFp8TileRows ? 0 : n * I * 4);
   w.hq = take(n * I);
-  w.hs = take(n * fp8_blocks(I) * 4);
+  w.hs = take(n * fp8_ld(I) * 4);
   w.y = take(n * H * 2);
   w.total = o;
   return w;
@@ -169,11 +169,11 @@ CAI4_DEV void place_slots(const Group &g, int b, const int *total, const int *be
 template <bool F32>
 __global__ __launch_bounds__(256) void fp8_moe_prep_kernel(Group g, const void *x, size_t groups,
                                                            int K, int KB, uint8_t *codes,
-                                                           float *scales) {
+                                                           float *scales, int ld) {
   __shared__ GroupLds l;
   const int b = blockIdx.x;
   if (b >= g.counters) {
-    quantize_rows_step<F32>((size_t)(b - g.counters), x, groups, K, KB, codes, scales);
+    quantize_rows_step<F32>((size_t)(b - g.counters), x, groups, K, KB, codes, scales, ld);
     return;
   }
   count_slots(g, b, l);
@@ -240,7 +240,11 @@ __global__ __launch_bounds__(256) void fp8_combine_kernel(const void *residual, 
 }  // namespace
 
 size_t fp8_moe_workspace(int H, int I, int E, int top_k, int T) {
-  return layout_of(H, I, E, top_k, T).total;
+  const size_t bytes = layout_of(H, I, E, top_k, T).total;
+  // (the largest batch in 16-row chunks may need more than one on tiles)
+  const int few = (int)(((int64_t)16 * E - 1) / top_k);
+  const size_t less = few >= 1 && few < T ? layout_of(H, I, E, top_k, few).total : 0;
+  return less > bytes ? less : bytes;
 }
 
 hipError_t fp8_moe_forward(const Fp8Moe &m, void *workspace, hipStream_t st) {
@@ -267,10 +271,10 @@ hipError_t fp8_moe_forward(const Fp8Moe &m, void *workspace, hipStream_t st) {
   const dim3 grid((unsigned)(w.counters + (groups + kRowGroups - 1) / kRowGroups));
   if (m.x_f32)
     hipLaunchKernelGGL(fp8_moe_prep_kernel<true>, grid, dim3(256), 0, st, gr, m.x, groups, m.H, hb,
-                       xq, xs);
+                       xq, xs, fp8_ld(m.H));
   else
     hipLaunchKernelGGL(fp8_moe_prep_kernel<false>, grid, dim3(256), 0, st, gr, m.x, groups, m.H,
-                       hb, xq, xs);
+                       hb, xq, xs, fp8_ld(m.H));
   if (w.counters > 1)
     hipLaunchKernelGGL(fp8_moe_place_kernel, dim3(w.counters), dim3(256), 0, st, gr);
   hipError_t e = hipGetLastError();
@@ -281,8 +285,10 @@ hipError_t fp8_moe_forward(const Fp8Moe &m, void *workspace, hipStream_t st) {
   g.ws = m.gate_up_s;
   g.x = xq;
   g.xs = xs;
+  g.ld_xs = fp8_ld(m.H);
   g.y = tiles ? hq : b + w.h;
   g.ys = hs;
+  g.ld_ys = fp8_ld(m.I);
   g.N = m.I;
   g.K = m.H;
   g.M = n;
@@ -298,12 +304,13 @@ hipError_t fp8_moe_forward(const Fp8Moe &m, void *workspace, hipStream_t st) {
   g.swiglu = 1;
   e = fp8_gemm(g, st);
   if (e != hipSuccess) return e;
-  if (!tiles) e = fp8_quantize_rows(b + w.h, true, n, m.I, hq, hs, st);
+  if (!tiles) e = fp8_quantize_rows(b + w.h, true, n, m.I, hq, hs, fp8_ld(m.I), st);
   if (e != hipSuccess) return e;
   g.w = m.down;
   g.ws = m.down_s;
   g.x = hq;
   g.xs = hs;
+  g.ld_xs = fp8_ld(m.I);
   g.y = b + w.y;
   g.N = m.H;
   g.K = m.I;

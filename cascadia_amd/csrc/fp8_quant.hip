@@ -16,8 +16,16 @@ namespace {
 
 template <bool F32>
 __global__ __launch_bounds__(256) void fp8_rows_kernel(const void *x, size_t groups, int K, int KB,
-                                                       uint8_t *codes, float *scales) {
-  quantize_rows_step<F32>(blockIdx.x, x, groups, K, KB, codes, scales);
+                                                       uint8_t *codes, float *scales, int ld) {
+  quantize_rows_step<F32>(blockIdx.x, x, groups, K, KB, codes, scales, ld);
+}
+
+__global__ __launch_bounds__(256) void fp8_pad_kernel(const float *scales, size_t n, int KB,
+                                                      float *to, int ld) {
+  const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= n) return;
+  const size_t row = i / KB;
+  to[row * ld + (i - row * KB)] = scales[i];
 }
 
 // A workgroup per block: 16 rows at a time, eight passes, held in registers.
@@ -53,15 +61,25 @@ __global__ __launch_bounds__(256) void fp8_blocks_kernel(const uint16_t *w, int 
 }  // namespace
 
 hipError_t fp8_quantize_rows(const void *x, bool x_f32, size_t rows, int K, uint8_t *codes,
-                             float *scales, hipStream_t st) {
+                             float *scales, int ld, hipStream_t st) {
   const int KB = fp8_blocks(K);
   const size_t groups = rows * KB;
   if (groups == 0) return hipSuccess;
   const dim3 grid((unsigned)((groups + kRowGroups - 1) / kRowGroups)), block(256);
   if (x_f32)
-    hipLaunchKernelGGL(fp8_rows_kernel<true>, grid, block, 0, st, x, groups, K, KB, codes, scales);
+    hipLaunchKernelGGL(fp8_rows_kernel<true>, grid, block, 0, st, x, groups, K, KB, codes, scales,
+                       ld);
   else
-    hipLaunchKernelGGL(fp8_rows_kernel<false>, grid, block, 0, st, x, groups, K, KB, codes, scales);
+    hipLaunchKernelGGL(fp8_rows_kernel<false>, grid, block, 0, st, x, groups, K, KB, codes, scales,
+                       ld);
+  return hipGetLastError();
+}
+
+hipError_t fp8_pad_scales(const float *scales, size_t rows, int KB, float *to, int ld,
+                          hipStream_t st) {
+  const size_t n = rows * KB;
+  hipLaunchKernelGGL(fp8_pad_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, scales, n,
+                     KB, to, ld);
   return hipGetLastError();
 }
 

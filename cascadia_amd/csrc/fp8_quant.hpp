@@ -40,7 +40,7 @@ CAI4_DEV u32x2_t codes_f32(u32x4_t v, u32x4_t w, const Fp8Div &d) {
 constexpr int kRowGroups = 16;  // groups per workgroup of 256 threads
 template <bool F32>
 CAI4_DEV void quantize_rows_step(size_t block, const void *x, size_t groups, int K, int KB,
-                                 uint8_t *codes, float *scales) {
+                                 uint8_t *codes, float *scales, int ld) {
   const size_t g = block * kRowGroups + (threadIdx.x >> 4);
   if (g >= groups) return;  // whole groups of 16 lanes
   const size_t row = g / KB;
@@ -64,7 +64,7 @@ CAI4_DEV void quantize_rows_step(size_t block, const void *x, size_t groups, int
   const Fp8Div d = fp8_div(top);
   if (in)
     *reinterpret_cast<u32x2_t *>(codes + at) = F32 ? codes_f32(v, w, d) : codes_bf16(v, d);
-  if ((threadIdx.x & 15) == 0) scales[g] = d.scale;
+  if ((threadIdx.x & 15) == 0) scales[row * ld + kb] = d.scale;
 }
 
 }  // namespace

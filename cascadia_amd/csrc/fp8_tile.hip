@@ -31,8 +31,12 @@
 // last weight tile nothing of the stage is left to read: there the one barrier
 // of the block stands, which also publishes the next stage; the freed one takes
 // the loads of the block S further (past the last block: loads out of range, so
-// that every wait counts the same number).  The tokens' scales come with the
-// stage, each wave's own.
+// that every wait counts the same number).
+//
+// What bounds it: a CU keeps some 64 cache lines in flight to its L2, about 14
+// bytes a cycle at 390 cycles each, so requests count.  The tokens' scales, rows
+// padded to 16 bytes, are read four blocks at a time; one by one they were a third
+// of all requests (4096 x 14336 x 4096: 289 us).
 #include "fp8.hpp"
 #include "fp8_common.hpp"
 #include "fp8_rows.hpp"
@@ -70,13 +74,15 @@ template <int NI, int NJ, int WN, int WM, bool SW, int S>
 struct Tile {
   static constexpr int W = WN * WM, BN = 16 * NI * WN, BM = 16 * NJ * WM;
   static constexpr int OUT = SW ? BN / 2 : BN;  // output columns
-  static constexpr int XS = (BN + BM) * 128, STAGE = XS + W * 256;  // codes, then scales
+  static constexpr int STAGE = (BN + BM) * 128, WINDOW = BM * 16;  // codes; scales of four blocks
+  static constexpr int SL = 16 * NJ / WN;  // tokens whose scales a wave loads
+  static constexpr int XS = S * STAGE, NONE = XS + 2 * WINDOW, BYTES = NONE + SL * 16;
   static constexpr int PW = BN / 8 / W, PX = BM / 8 / W;  // 1 KB loads per wave and stage
   static_assert(PW * W * 8 == BN && PX * W * 8 == BM, "pieces");
   static_assert(128 % (16 * NI / (SW ? 2 : 1)) == 0, "a wave's rows lie in one scale block");
   static constexpr int LOADS = PW + PX + 1;
-  static_assert(S >= 2 && S * STAGE <= 160 * 1024, "LDS");
-  static_assert(NJ <= 4, "a wave's scales are one load");
+  static_assert(S >= 2 && S <= 4 && BYTES + (SW ? WN * BM * 4 : 0) <= 160 * 1024, "LDS");
+  static_assert(SL * WN == 16 * NJ && SL <= 64, "a wave's scales are one load");
 };
 
 // A workgroup's place: m tile (or chunk) and n tile.  Workgroups go round the
@@ -104,7 +110,7 @@ CAI4_DEV Place place_of(const Fp8Gemm &g, int id, int mtiles, int ntiles) {
 template <int NI, int NJ, int WN, int WM, bool SW, bool EXACT, int S>
 __global__ __launch_bounds__(64 * WN * WM) void fp8_tile_kernel(Fp8Gemm g, int ntiles) {
   using P = Tile<NI, NJ, WN, WM, SW, S>;
-  __shared__ __attribute__((aligned(1024))) uint8_t st[S * P::STAGE];
+  __shared__ __attribute__((aligned(1024))) uint8_t st[P::BYTES];
   __shared__ float tops[SW ? WN : 1][SW ? P::BM : 1];
   const int lane = threadIdx.x & 63, l15 = lane & 15, c = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -124,9 +130,9 @@ __global__ __launch_bounds__(64 * WN * WM) void fp8_tile_kernel(Fp8Gemm g, int n
   const rsrc_t xr = g.row_map ? rsrc_scalar(g.x, (size_t)g.x_rows * g.K)
                               : rsrc_scalar(g.x + (size_t)rows.row0 * g.K,
                                             (size_t)rows.count * g.K);
-  const rsrc_t sr = g.row_map ? rsrc_scalar(g.xs, (size_t)g.x_rows * KB * 4)
-                              : rsrc_scalar(g.xs + (size_t)rows.row0 * KB,
-                                            (size_t)rows.count * KB * 4);
+  const rsrc_t sr = g.row_map ? rsrc_scalar(g.xs, (size_t)g.x_rows * g.ld_xs * 4)
+                              : rsrc_scalar(g.xs + (size_t)rows.row0 * g.ld_xs,
+                                            (size_t)rows.count * g.ld_xs * 4);
   const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(const lds_void *)st);
 
   // ---- this wave's loads of a stage: 1 KB pieces of eight rows, PW of the
@@ -146,29 +152,38 @@ __global__ __launch_bounds__(64 * WN * WM) void fp8_tile_kernel(Fp8Gemm g, int n
             : (g.row_map ? (uint32_t)g.row_map[rows.row0 + r] * (uint32_t)g.K
                          : (uint32_t)(r * g.K)) + 16 * chunk_of(r);
   }
-  // this wave's tokens' scales
+  // scales: 16 bytes, four blocks' of a token, with every fourth stage (two windows)
   uint32_t vs = kDmaOOB;
-  {
-    const int r = wm * NJ * 16 + lane;
-    if (lane < NJ * 16 && r < rows.count)
-      vs = (g.row_map ? (uint32_t)g.row_map[rows.row0 + r] : (uint32_t)r) * (uint32_t)KB * 4;
-  }
-  auto issue = [&](int kb, uint32_t to) {
+  const int s0 = wm * NJ * 16 + wn * P::SL;
+  if (s0 + lane < rows.count)
+    vs = (g.row_map && lane < P::SL ? (uint32_t)g.row_map[rows.row0 + s0 + lane]
+                                    : (uint32_t)(s0 + lane)) * (uint32_t)g.ld_xs * 4;
+  auto load = [&](int kb, uint32_t to, int left) {
     const uint32_t soff = (uint32_t)kb * 128;
-    const int left = g.K - 128 * kb;  // a short last block reads zeros past it
 #pragma unroll
     for (int q = 0; q < P::PW; ++q) {
       const int piece = wave * P::PW + q;
-      const uint32_t v = 16 * chunk_of(piece * 8 + (lane >> 3)) < left ? vw[q] : kDmaOOB;
-      lds_dma<16>(wr, to + piece * 1024, v, soff);
+      const bool in = left >= 128 || 16 * chunk_of(piece * 8 + (lane >> 3)) < left;
+      lds_dma<16>(wr, to + piece * 1024, in ? vw[q] : kDmaOOB, soff);
     }
 #pragma unroll
     for (int q = 0; q < P::PX; ++q) {
       const int piece = wave * P::PX + q;
-      const uint32_t v = 16 * chunk_of(piece * 8 + (lane >> 3)) < left ? vx[q] : kDmaOOB;
-      lds_dma<16>(xr, to + P::BN * 128 + piece * 1024, v, soff);
+      const bool in = left >= 128 || 16 * chunk_of(piece * 8 + (lane >> 3)) < left;
+      lds_dma<16>(xr, to + P::BN * 128 + piece * 1024, in ? vx[q] : kDmaOOB, soff);
     }
-    lds_dma<4>(sr, to + P::XS + wave * 256, left > 0 ? vs : kDmaOOB, (uint32_t)kb * 4);
+    // (in the other stages, and past the end, zeros to a place that nothing reads)
+    const bool window = left > 0 && (kb & 3) == 0;
+    if (lane < P::SL)
+      lds_dma<16>(sr, lds0 + (window ? P::XS + ((kb >> 2) & 1) * P::WINDOW + s0 * 16 : P::NONE),
+                  window ? vs : kDmaOOB, (uint32_t)kb * 4);
+  };
+  auto issue = [&](int kb, uint32_t to) {
+    const int left = g.K - 128 * kb;
+    if (left >= 128)
+      load(kb, to, 128);
+    else  // a short last block reads zeros past its end
+      load(kb, to, left);
   };
 
   // ---- scales: a token's times the weight rows' ----
@@ -178,13 +193,14 @@ __global__ __launch_bounds__(64 * WN * WM) void fp8_tile_kernel(Fp8Gemm g, int n
   const scalar_t ws = (scalar_t)(g.ws + (size_t)rows.expert * g.ws_stride +
                                  (size_t)((idle ? n0 : nw) >> 7) * KB);
   constexpr int NS = SW ? 2 : 1;
-  const uint32_t fs = lds0 + P::XS + wave * 256 + l15 * 4;
-  auto take_scales = [&](uint32_t base, int kb, float (&to)[NS][NJ]) {
+  const uint32_t fs = lds0 + P::XS + (wm * NJ * 16 + l15) * 16;
+  auto take_scales = [&](int kb, float (&to)[NS][NJ]) {
+    const uint32_t at = fs + ((kb >> 2) & 1) * P::WINDOW + (kb & 3) * 4;
 #pragma unroll
     for (int m = 0; m < NS; ++m) {
       const float f = ws[(size_t)m * NB * KB + kb];
 #pragma unroll
-      for (int j = 0; j < NJ; ++j) to[m][j] = lds_at<float>(base + fs, j * 64) * f;
+      for (int j = 0; j < NJ; ++j) to[m][j] = lds_at<float>(at, j * 256) * f;
     }
   };
 
@@ -213,11 +229,11 @@ __global__ __launch_bounds__(64 * WN * WM) void fp8_tile_kernel(Fp8Gemm g, int n
 #pragma unroll
   for (int q = 0; q < S; ++q) issue(q, lds0 + q * P::STAGE);
   dma_wait_barrier<(S - 1) * P::LOADS>();
-  take_scales(0, 0, s);
+  take_scales(0, s);
 #pragma unroll
   for (int j = 0; j < NJ; ++j) read_b(0, j);
   read_a(0, 0, 0);
-  constexpr int LAG = 2;  // MFMAs between one and the use of its result
+  constexpr int LAG = 3;  // MFMAs between one and the use of its result
   f32x4_t p[LAG + 1];
   uint32_t base = 0;
   for (int kb = 0; kb < KB; ++kb) {
@@ -238,7 +254,7 @@ __global__ __launch_bounds__(64 * WN * WM) void fp8_tile_kernel(Fp8Gemm g, int n
       } else {
         dma_wait_barrier<(S - 2) * P::LOADS>();
         issue(kb + S, lds0 + base);
-        take_scales(next, kb + 1 < KB ? kb + 1 : kb, sn);
+        take_scales(kb + 1 < KB ? kb + 1 : kb, sn);
       }
 #pragma unroll
       for (int j = 0; j < NJ; ++j) {
@@ -247,6 +263,7 @@ __global__ __launch_bounds__(64 * WN * WM) void fp8_tile_kernel(Fp8Gemm g, int n
           p[slot % (LAG + 1)] = mfma_codes(a[i & 1], b[j], f32x4_t{0.f, 0.f, 0.f, 0.f});
         else
           p[slot % (LAG + 1)] = mfma_fp8(a[i & 1], b[j]);
+        __builtin_amdgcn_sched_barrier(0);
         if (slot >= LAG) add(slot - LAG);
         if (i + 1 == NI) read_b(next, j);  // (past the last block: not used)
         __builtin_amdgcn_sched_barrier(0);
@@ -290,7 +307,7 @@ __global__ __launch_bounds__(64 * WN * WM) void fp8_tile_kernel(Fp8Gemm g, int n
 #pragma unroll
       for (int q = 1; q < WN; ++q) top = fmaxf(top, tops[q][r]);
       const Fp8Div d = fp8_div(top);
-      if (wn == 0 && c == 0) g.ys[row * NB + (n0 >> 7)] = d.scale;
+      if (wn == 0 && c == 0) g.ys[row * g.ld_ys + (n0 >> 7)] = d.scale;
       uint8_t *y = static_cast<uint8_t *>(g.y) + row * g.N + nw + 4 * c;
 #pragma unroll
       for (int i = 0; i < NH; ++i)
