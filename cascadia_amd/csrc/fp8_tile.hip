@@ -29,9 +29,11 @@
 // Order: weight tiles outside, tokens inside.  The tokens' fragments stay in
 // registers for the block, the weights' are read one tile ahead.  Before the
 // last weight tile nothing of the stage is left to read: there the one barrier
-// of the block stands, which also publishes the next stage; the freed one takes
-// the loads of the block S further (past the last block: loads out of range, so
-// that every wait counts the same number).
+// of the block stands, which also publishes the next stage.  The freed one takes
+// the loads of the block S further during the next block, one or two a pass
+// (past the last block: loads out of range, so that every wait counts the same
+// number).  Issued all at once behind the barrier they held up every wave while
+// the address unit worked through them (4096 x 14336 x 4096: 260 us).
 //
 // What bounds it: a CU keeps some 64 cache lines in flight to its L2, about 14
 // bytes a cycle at 390 cycles each, so requests count.  The tokens' scales, rows
@@ -158,32 +160,27 @@ __global__ __launch_bounds__(64 * WN * WM) void fp8_tile_kernel(Fp8Gemm g, int n
   if (s0 + lane < rows.count)
     vs = (g.row_map && lane < P::SL ? (uint32_t)g.row_map[rows.row0 + s0 + lane]
                                     : (uint32_t)(s0 + lane)) * (uint32_t)g.ld_xs * 4;
-  auto load = [&](int kb, uint32_t to, int left) {
-    const uint32_t soff = (uint32_t)kb * 128;
-#pragma unroll
-    for (int q = 0; q < P::PW; ++q) {
-      const int piece = wave * P::PW + q;
-      const bool in = left >= 128 || 16 * chunk_of(piece * 8 + (lane >> 3)) < left;
-      lds_dma<16>(wr, to + piece * 1024, in ? vw[q] : kDmaOOB, soff);
-    }
-#pragma unroll
-    for (int q = 0; q < P::PX; ++q) {
-      const int piece = wave * P::PX + q;
-      const bool in = left >= 128 || 16 * chunk_of(piece * 8 + (lane >> 3)) < left;
-      lds_dma<16>(xr, to + P::BN * 128 + piece * 1024, in ? vx[q] : kDmaOOB, soff);
-    }
-    // (in the other stages, and past the end, zeros to a place that nothing reads)
-    const bool window = left > 0 && (kb & 3) == 0;
-    if (lane < P::SL)
-      lds_dma<16>(sr, lds0 + (window ? P::XS + ((kb >> 2) & 1) * P::WINDOW + s0 * 16 : P::NONE),
-                  window ? vs : kDmaOOB, (uint32_t)kb * 4);
+  // load q of this wave for block kb into the stage at `to`.  A short last block
+  // reads zeros past its end: chunks of pieces of one parity are cut alike.
+  auto cut = [&](int kb, int parity) {
+    return 16 * (((lane & 7) ^ ((4 * parity + (lane >> 4)) & 7))) < g.K - 128 * kb;
   };
-  auto issue = [&](int kb, uint32_t to) {
-    const int left = g.K - 128 * kb;
-    if (left >= 128)
-      load(kb, to, 128);
-    else  // a short last block reads zeros past its end
-      load(kb, to, left);
+  auto load1 = [&](int q, int kb, uint32_t to, bool even, bool odd) {
+    if (q < P::PW) {
+      const int piece = wave * P::PW + q;
+      lds_dma<16>(wr, to + piece * 1024, (piece & 1 ? odd : even) ? vw[q] : kDmaOOB,
+                  (uint32_t)kb * 128);
+    } else if (q < P::PW + P::PX) {
+      const int piece = wave * P::PX + q - P::PW;
+      lds_dma<16>(xr, to + P::BN * 128 + piece * 1024,
+                  (piece & 1 ? odd : even) ? vx[q - P::PW] : kDmaOOB, (uint32_t)kb * 128);
+    } else {
+      // (in the other stages, and past the end, zeros to a place that nothing reads)
+      const bool window = kb < KB && (kb & 3) == 0;
+      if (lane < P::SL)
+        lds_dma<16>(sr, lds0 + (window ? P::XS + ((kb >> 2) & 1) * P::WINDOW + s0 * 16 : P::NONE),
+                    window ? vs : kDmaOOB, (uint32_t)kb * 4);
+    }
   };
 
   // ---- scales: a token's times the weight rows' ----
@@ -227,17 +224,21 @@ __global__ __launch_bounds__(64 * WN * WM) void fp8_tile_kernel(Fp8Gemm g, int n
 
   float s[NS][NJ];
 #pragma unroll
-  for (int q = 0; q < S; ++q) issue(q, lds0 + q * P::STAGE);
-  dma_wait_barrier<(S - 1) * P::LOADS>();
+  for (int t = 0; t + 1 < S; ++t)
+#pragma unroll
+    for (int q = 0; q < P::LOADS; ++q)
+      load1(q, t, lds0 + t * P::STAGE, cut(t, 0), cut(t, 1));
+  dma_wait_barrier<(S - 2) * P::LOADS>();
   take_scales(0, s);
 #pragma unroll
   for (int j = 0; j < NJ; ++j) read_b(0, j);
   read_a(0, 0, 0);
   constexpr int LAG = 3;  // MFMAs between one and the use of its result
   f32x4_t p[LAG + 1];
-  uint32_t base = 0;
+  uint32_t base = 0, last = (S - 1) * P::STAGE;  // stages of this block, of the one before
   for (int kb = 0; kb < KB; ++kb) {
     const uint32_t next = base + P::STAGE == S * P::STAGE ? 0 : base + P::STAGE;
+    const bool even = cut(kb + S - 1, 0), odd = cut(kb + S - 1, 1);
     float sn[NS][NJ];
     auto add = [&](int slot) {
       const int i = slot / NJ, j = slot % NJ;
@@ -253,7 +254,6 @@ __global__ __launch_bounds__(64 * WN * WM) void fp8_tile_kernel(Fp8Gemm g, int n
         read_a(base, i + 1, (i + 1) & 1);
       } else {
         dma_wait_barrier<(S - 2) * P::LOADS>();
-        issue(kb + S, lds0 + base);
         take_scales(kb + 1 < KB ? kb + 1 : kb, sn);
       }
 #pragma unroll
@@ -265,6 +265,11 @@ __global__ __launch_bounds__(64 * WN * WM) void fp8_tile_kernel(Fp8Gemm g, int n
           p[slot % (LAG + 1)] = mfma_fp8(a[i & 1], b[j]);
         __builtin_amdgcn_sched_barrier(0);
         if (slot >= LAG) add(slot - LAG);
+        // the stage of the block before takes the loads of S - 1 blocks ahead, PER a pass
+        constexpr int PER = S == 2 ? 2 : (P::LOADS + NI - 2) / (NI - 1);
+        static_assert(PER * (NI - 1) >= P::LOADS, "loads");
+        if (j % (NJ / PER) == 0 && i + 1 < NI && i * PER + j / (NJ / PER) < P::LOADS)
+          load1(i * PER + j / (NJ / PER), kb + S - 1, lds0 + last, even, odd);
         if (i + 1 == NI) read_b(next, j);  // (past the last block: not used)
         __builtin_amdgcn_sched_barrier(0);
       }
@@ -276,6 +281,7 @@ __global__ __launch_bounds__(64 * WN * WM) void fp8_tile_kernel(Fp8Gemm g, int n
     for (int m = 0; m < NS; ++m)
 #pragma unroll
       for (int j = 0; j < NJ; ++j) s[m][j] = sn[m][j];
+    last = base;
     base = next;
   }
 
