@@ -2461,8 +2461,9 @@ int cascadia_int4_fp8_gemm(uint32_t n_rows, uint32_t k_cols, const uint8_t *w,
   const Fp8Workspace need = fp8_workspace(n_rows, k_cols, x_type, seq);
   const int blocks = cai4::fp8_blocks((int)k_cols), ld = cai4::fp8_ld((int)k_cols);
   // given scales are read where they are unless tiles want their rows aligned
+  const bool one = seq == 1 && !codes && cai4::fp8_one_row((int)k_cols);  // quantised in its kernel
   const bool pad = codes && need.total && (blocks != ld || !aligned(x_scales, 16));
-  if ((!codes || pad) && !workspace)
+  if (((!codes && !one) || pad) && !workspace)
     if (int rc = own.get(dev, need.total, st, &workspace)) return rc;
   cai4::Fp8Gemm g{};
   g.w = w;
@@ -2475,6 +2476,8 @@ int cascadia_int4_fp8_gemm(uint32_t n_rows, uint32_t k_cols, const uint8_t *w,
   g.M = (int)seq;
   g.out_f32 = (int)y_is_f32;
   g.ld_xs = blocks;
+  if (one)
+    return hip_status(cai4::fp8_gemv(g, xs, x_type == CASCADIA_INT4_FP8_X_F32, st));
   if (!codes || pad) {
     float *s = static_cast<float *>(workspace);
     uint8_t *q = static_cast<uint8_t *>(workspace) + need.codes;

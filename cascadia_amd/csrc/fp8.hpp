@@ -88,6 +88,13 @@ struct Fp8Moe {
   void *out;
   int out_f32;
 };
+// One row of x (bf16 or f32), quantised in the kernel (fp8_one_row).
+bool fp8_one_row(int K);
+bool fp8_one_token(int H, int I, int top_k);
+hipError_t fp8_gemv(const Fp8Gemm &g, const void *x, bool x_f32, hipStream_t st);
+// One token (fp8_one_token): gate / up into h [top_k, I], down and the weighted sum.
+hipError_t fp8_moe_one(const Fp8Moe &m, const Fp8Gemm &gate_up, const Fp8Gemm &down, float *h,
+                       hipStream_t st);
 size_t fp8_moe_workspace(int H, int I, int E, int top_k, int T);
 hipError_t fp8_moe_forward(const Fp8Moe &m, void *workspace, hipStream_t st);
 

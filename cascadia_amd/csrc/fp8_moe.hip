@@ -12,7 +12,8 @@
 // do not: a grouped row's products do not depend on its place, and the sum reads
 // slots in order.
 //
-// Launches: x's codes and, in workgroups of the same launch, the experts' counts
+// One token: two launches, each quantising the rows it reads (fp8_gemm.hip).
+// More: x's codes and, in workgroups of the same launch, the experts' counts
 // (for up to 1,024 slots the whole grouping); the grouping; gate / up; h's codes
 // (on tiles in the gate / up launch itself); down; the weighted sum.
 #include "fp8.hpp"
@@ -61,7 +62,7 @@ Layout layout_of(int H, int I, int E, int top_k, int T) {
   w.chunks = take((size_t)w.max_chunks * sizeof(Fp8Chunk));
   w.counts = take(16);
   w.hist = take((size_t)w.counters * E * 4);
-  w.h = take(w.chunk_rows == kFp8TileRows ? 0 : n * I * 4);
+  w.h = take(T > 1 && w.chunk_rows == kFp8TileRows ? 0 : n * I * 4);
   w.hq = take(n * I);
   w.hs = take(n * fp8_ld(I) * 4);
   w.y = take(n * H * 2);
@@ -253,6 +254,32 @@ hipError_t fp8_moe_forward(const Fp8Moe &m, void *workspace, hipStream_t st) {
   uint8_t *xq = b + w.xq, *hq = b + w.hq;
   float *xs = reinterpret_cast<float *>(b + w.xs), *hs = reinterpret_cast<float *>(b + w.hs);
   const int n = m.T * m.top_k, hb = fp8_blocks(m.H), ib = fp8_blocks(m.I);
+  Fp8Gemm up{}, down{};
+  up.w = m.gate_up;
+  up.ws = m.gate_up_s;
+  up.N = m.I;
+  up.K = m.H;
+  up.M = n;
+  up.w_stride = (size_t)2 * m.I * m.H;
+  up.ws_stride = (size_t)2 * ib * hb;
+  up.swiglu = 1;
+  up.out_f32 = 1;
+  down.w = m.down;
+  down.ws = m.down_s;
+  down.N = m.H;
+  down.K = m.I;
+  down.M = n;
+  down.w_stride = (size_t)m.H * m.I;
+  down.ws_stride = (size_t)hb * ib;
+
+  if (m.T == 1 && fp8_one_token(m.H, m.I, m.top_k)) {
+    float *h = reinterpret_cast<float *>(b + w.h);
+    up.y = h;
+    down.y = m.out;
+    down.out_f32 = m.out_f32;
+    return fp8_moe_one(m, up, down, h, st);
+  }
+
   Group gr{};
   gr.ids = m.ids;
   gr.weights = m.weights;
@@ -279,47 +306,33 @@ hipError_t fp8_moe_forward(const Fp8Moe &m, void *workspace, hipStream_t st) {
     hipLaunchKernelGGL(fp8_moe_place_kernel, dim3(w.counters), dim3(256), 0, st, gr);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
+
   const bool tiles = w.chunk_rows == kFp8TileRows;
-  Fp8Gemm g{};
-  g.w = m.gate_up;
-  g.ws = m.gate_up_s;
-  g.x = xq;
-  g.xs = xs;
-  g.ld_xs = fp8_ld(m.H);
-  g.y = tiles ? hq : b + w.h;
-  g.ys = hs;
-  g.ld_ys = fp8_ld(m.I);
-  g.N = m.I;
-  g.K = m.H;
-  g.M = n;
-  g.out_f32 = 1;
-  g.chunks = gr.chunks;
-  g.max_chunks = w.max_chunks;
-  g.chunk_rows = w.chunk_rows;
-  g.n_chunks = gr.n_chunks;
-  g.x_rows = m.T;
-  g.row_map = gr.row_map;
-  g.w_stride = (size_t)2 * m.I * m.H;
-  g.ws_stride = (size_t)2 * ib * hb;
-  g.swiglu = 1;
-  e = fp8_gemm(g, st);
+  up.x = xq;
+  up.xs = xs;
+  up.ld_xs = fp8_ld(m.H);
+  up.y = tiles ? hq : b + w.h;
+  up.ys = hs;
+  up.ld_ys = fp8_ld(m.I);
+  up.chunks = gr.chunks;
+  up.max_chunks = w.max_chunks;
+  up.chunk_rows = w.chunk_rows;
+  up.n_chunks = gr.n_chunks;
+  up.row_map = gr.row_map;
+  up.x_rows = m.T;
+  e = fp8_gemm(up, st);
+  if (e == hipSuccess && !tiles)
+    e = fp8_quantize_rows(b + w.h, true, n, m.I, hq, hs, fp8_ld(m.I), st);
   if (e != hipSuccess) return e;
-  if (!tiles) e = fp8_quantize_rows(b + w.h, true, n, m.I, hq, hs, fp8_ld(m.I), st);
-  if (e != hipSuccess) return e;
-  g.w = m.down;
-  g.ws = m.down_s;
-  g.x = hq;
-  g.xs = hs;
-  g.ld_xs = fp8_ld(m.I);
-  g.y = b + w.y;
-  g.N = m.H;
-  g.K = m.I;
-  g.out_f32 = 0;
-  g.row_map = nullptr;
-  g.w_stride = (size_t)m.H * m.I;
-  g.ws_stride = (size_t)hb * ib;
-  g.swiglu = 0;
-  e = fp8_gemm(g, st);
+  down.x = hq;
+  down.xs = hs;
+  down.ld_xs = fp8_ld(m.I);
+  down.y = b + w.y;
+  down.chunks = gr.chunks;
+  down.max_chunks = w.max_chunks;
+  down.chunk_rows = w.chunk_rows;
+  down.n_chunks = gr.n_chunks;
+  e = fp8_gemm(down, st);
   if (e != hipSuccess) return e;
   hipLaunchKernelGGL(fp8_combine_kernel, dim3(m.T, (m.H + 1023) / 1024), dim3(256), 0, st,
                      m.residual, reinterpret_cast<const uint16_t *>(b + w.y), gr.pos, m.weights, m.H,
