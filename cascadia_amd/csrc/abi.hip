@@ -2350,16 +2350,18 @@ bool fp8_dims_ok(uint32_t n_rows, uint32_t k_cols) {
 }
 
 // A call's workspace: scales in rows of fp8_ld, then, of rows that it quantises,
-// their codes.
+// their codes, then the partial sums of a split K.
 struct Fp8Workspace {
-  size_t codes, total;
+  size_t codes, part, total;
 };
 Fp8Workspace fp8_workspace(uint32_t n_rows, uint32_t k_cols, uint32_t x_type, uint32_t seq) {
   const bool given = x_type == CASCADIA_INT4_FP8_X_E4M3;
   Fp8Workspace w{};
-  if (given && !cai4::fp8_tiles((int)seq, (int)n_rows, (int)k_cols)) return w;
+  const bool tiles = cai4::fp8_tiles((int)seq, (int)n_rows, (int)k_cols);
+  if (given && !tiles) return w;
   w.codes = ((size_t)seq * cai4::fp8_ld((int)k_cols) * 4 + 255) & ~(size_t)255;
-  w.total = w.codes + (given ? 0 : (size_t)seq * k_cols);
+  w.part = (w.codes + (given ? 0 : (size_t)seq * k_cols) + 255) & ~(size_t)255;
+  w.total = w.part + (tiles ? cai4::fp8_partial_bytes((int)seq, (int)n_rows, (int)k_cols) : 0);
   return w;
 }
 
@@ -2463,7 +2465,8 @@ int cascadia_int4_fp8_gemm(uint32_t n_rows, uint32_t k_cols, const uint8_t *w,
   // given scales are read where they are unless tiles want their rows aligned
   const bool one = seq == 1 && !codes && cai4::fp8_one_row((int)k_cols);  // quantised in its kernel
   const bool pad = codes && need.total && (blocks != ld || !aligned(x_scales, 16));
-  if (((!codes && !one) || pad) && !workspace)
+  const bool use = (!codes && !one) || pad || need.total > need.part;
+  if (use && !workspace)
     if (int rc = own.get(dev, need.total, st, &workspace)) return rc;
   cai4::Fp8Gemm g{};
   g.w = w;
@@ -2476,6 +2479,7 @@ int cascadia_int4_fp8_gemm(uint32_t n_rows, uint32_t k_cols, const uint8_t *w,
   g.M = (int)seq;
   g.out_f32 = (int)y_is_f32;
   g.ld_xs = blocks;
+  g.part = reinterpret_cast<float *>(static_cast<uint8_t *>(workspace) + need.part);
   if (one)
     return hip_status(cai4::fp8_gemv(g, xs, x_type == CASCADIA_INT4_FP8_X_F32, st));
   if (!codes || pad) {

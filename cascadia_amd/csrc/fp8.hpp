@@ -66,10 +66,14 @@ struct Fp8Gemm {
   int swiglu;                  // y = silu(gate) * up: f32, or codes with ys
   float *ys;                   // SwiGLU on tiles: y's scales [rows, ld_ys]
   int ld_ys;
+  float *part;                 // tiles: workspace of fp8_partial_bytes
+  int kper;                    // (set by fp8_tile_gemm)
 };
 hipError_t fp8_gemm(const Fp8Gemm &g, hipStream_t st);
 // Whether a product of M rows runs on tiles, and how many scales it wants per row.
 bool fp8_tiles(int M, int N, int K);
+// Bytes of partial sums of a product on tiles, for any number of rows up to M.
+size_t fp8_partial_bytes(int M, int N, int K);
 constexpr int kFp8TileRows = 128;  // rows of a chunk on the tile kernel (16 else)
 hipError_t fp8_tile_gemm(const Fp8Gemm &g, hipStream_t st);
 

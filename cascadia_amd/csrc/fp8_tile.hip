@@ -124,6 +124,10 @@ __global__ __launch_bounds__(64 * WN * WM) void fp8_tile_kernel(Fp8Gemm g, int n
   const int n0 = at.n * P::OUT;
   const Rows rows = rows_of(g, at.m, P::BM);
   const int KB = (g.K + 127) >> 7, NB = (g.N + 127) >> 7;
+  // this workgroup's blocks: all, or slice blockIdx.y of g.kper (a multiple of 4)
+  const int first = g.kper ? (int)blockIdx.y * g.kper : 0;
+  const int end = g.kper && first + g.kper < KB ? first + g.kper : KB;
+  const int cols = end * 128 < g.K ? end * 128 : g.K;
   const int nr = g.N - n0 < P::OUT ? g.N - n0 : P::OUT;
   // this wave loads rows of the weights (SwiGLU: the first half gate, the others up)
   const uint8_t *w = g.w + (size_t)rows.expert * g.w_stride + (size_t)n0 * g.K +
@@ -163,7 +167,7 @@ __global__ __launch_bounds__(64 * WN * WM) void fp8_tile_kernel(Fp8Gemm g, int n
   // load q of this wave for block kb into the stage at `to`.  A short last block
   // reads zeros past its end: chunks of pieces of one parity are cut alike.
   auto cut = [&](int kb, int parity) {
-    return 16 * (((lane & 7) ^ ((4 * parity + (lane >> 4)) & 7))) < g.K - 128 * kb;
+    return 16 * (((lane & 7) ^ ((4 * parity + (lane >> 4)) & 7))) < cols - 128 * kb;
   };
   auto load1 = [&](int q, int kb, uint32_t to, bool even, bool odd) {
     if (q < P::PW) {
@@ -176,7 +180,7 @@ __global__ __launch_bounds__(64 * WN * WM) void fp8_tile_kernel(Fp8Gemm g, int n
                   (piece & 1 ? odd : even) ? vx[q - P::PW] : kDmaOOB, (uint32_t)kb * 128);
     } else {
       // (in the other stages, and past the end, zeros to a place that nothing reads)
-      const bool window = kb < KB && (kb & 3) == 0;
+      const bool window = kb < end && (kb & 3) == 0;
       if (lane < P::SL)
         lds_dma<16>(sr, lds0 + (window ? P::XS + ((kb >> 2) & 1) * P::WINDOW + s0 * 16 : P::NONE),
                     window ? vs : kDmaOOB, (uint32_t)kb * 4);
@@ -227,16 +231,16 @@ __global__ __launch_bounds__(64 * WN * WM) void fp8_tile_kernel(Fp8Gemm g, int n
   for (int t = 0; t + 1 < S; ++t)
 #pragma unroll
     for (int q = 0; q < P::LOADS; ++q)
-      load1(q, t, lds0 + t * P::STAGE, cut(t, 0), cut(t, 1));
+      load1(q, first + t, lds0 + t * P::STAGE, cut(first + t, 0), cut(first + t, 1));
   dma_wait_barrier<(S - 2) * P::LOADS>();
-  take_scales(0, s);
+  take_scales(first, s);
 #pragma unroll
   for (int j = 0; j < NJ; ++j) read_b(0, j);
   read_a(0, 0, 0);
   constexpr int LAG = 3;  // MFMAs between one and the use of its result
   f32x4_t p[LAG + 1];
   uint32_t base = 0, last = (S - 1) * P::STAGE;  // stages of this block, of the one before
-  for (int kb = 0; kb < KB; ++kb) {
+  for (int kb = first; kb < end; ++kb) {
     const uint32_t next = base + P::STAGE == S * P::STAGE ? 0 : base + P::STAGE;
     const bool even = cut(kb + S - 1, 0), odd = cut(kb + S - 1, 1);
     float sn[NS][NJ];
@@ -254,7 +258,7 @@ __global__ __launch_bounds__(64 * WN * WM) void fp8_tile_kernel(Fp8Gemm g, int n
         read_a(base, i + 1, (i + 1) & 1);
       } else {
         dma_wait_barrier<(S - 2) * P::LOADS>();
-        take_scales(kb + 1 < KB ? kb + 1 : kb, sn);
+        take_scales(kb + 1 < end ? kb + 1 : kb, sn);
       }
 #pragma unroll
       for (int j = 0; j < NJ; ++j) {
@@ -266,8 +270,8 @@ __global__ __launch_bounds__(64 * WN * WM) void fp8_tile_kernel(Fp8Gemm g, int n
         __builtin_amdgcn_sched_barrier(0);
         if (slot >= LAG) add(slot - LAG);
         // the stage of the block before takes the loads of S - 1 blocks ahead, PER a pass
-        constexpr int PER = S == 2 ? 2 : (P::LOADS + NI - 2) / (NI - 1);
-        static_assert(PER * (NI - 1) >= P::LOADS, "loads");
+        constexpr int PER = (NI - 1) >= P::LOADS ? 1 : 2;
+        static_assert(PER * (NI - 1) >= P::LOADS && NJ % PER == 0, "loads");
         if (j % (NJ / PER) == 0 && i + 1 < NI && i * PER + j / (NJ / PER) < P::LOADS)
           load1(i * PER + j / (NJ / PER), kb + S - 1, lds0 + last, even, odd);
         if (i + 1 == NI) read_b(next, j);  // (past the last block: not used)
@@ -326,6 +330,10 @@ __global__ __launch_bounds__(64 * WN * WM) void fp8_tile_kernel(Fp8Gemm g, int n
     }
   } else {
     if (idle) return;
+    if (g.kper) {  // partial sums [slices, M, N], f32
+      g.y = g.part + (size_t)blockIdx.y * g.M * g.N;
+      g.out_f32 = 1;
+    }
 #pragma unroll
     for (int j = 0; j < NJ; ++j) {
       const int r = (wm * NJ + j) * 16 + l15;
@@ -337,24 +345,104 @@ __global__ __launch_bounds__(64 * WN * WM) void fp8_tile_kernel(Fp8Gemm g, int n
   }
 }
 
+// Sums the slices' partials in order: four neighbouring outputs per thread.
+template <bool F32>
+__global__ __launch_bounds__(256) void fp8_slices_kernel(const float *part, size_t n, int slices,
+                                                         void *y) {
+  const size_t i = ((size_t)blockIdx.x * 256 + threadIdx.x) * 4;
+  if (i >= n) return;
+  const int left = n - i < 4 ? (int)(n - i) : 4;
+  float v[4] = {};
+  if (left == 4 && n % 4 == 0) {
+    f32x4_t t = *reinterpret_cast<const f32x4_t *>(part + i);
+    for (int s = 1; s < slices; ++s) t += *reinterpret_cast<const f32x4_t *>(part + s * n + i);
+    for (int q = 0; q < 4; ++q) v[q] = t[q];
+  } else {
+    for (int s = 0; s < slices; ++s)
+      for (int q = 0; q < left; ++q) v[q] += part[s * n + i + q];
+  }
+  if (F32) {
+    float *to = static_cast<float *>(y) + i;
+    if (left == 4 && ((uintptr_t)to & 15) == 0)
+      *reinterpret_cast<f32x4_t *>(to) = f32x4_t{v[0], v[1], v[2], v[3]};
+    else
+      for (int q = 0; q < left; ++q) to[q] = v[q];
+  } else {
+    uint16_t *to = static_cast<uint16_t *>(y) + i;
+    const u32x2_t b = {f32_to_bf16_rne(v[0]) | (f32_to_bf16_rne(v[1]) << 16),
+                       f32_to_bf16_rne(v[2]) | (f32_to_bf16_rne(v[3]) << 16)};
+    if (left == 4 && ((uintptr_t)to & 7) == 0)
+      *reinterpret_cast<u32x2_t *>(to) = b;
+    else
+      for (int q = 0; q < left; ++q) to[q] = (uint16_t)(b[q >> 1] >> (16 * (q & 1)));
+  }
+}
+
 template <int NI, int NJ, int WN, int WM, bool SW, bool EXACT, int S>
 hipError_t launch(const Fp8Gemm &g, hipStream_t st) {
   using P = Tile<NI, NJ, WN, WM, SW, S>;
   const int nt = (g.N + P::OUT - 1) / P::OUT;
+  const int slices = g.kper ? (fp8_blocks(g.K) + g.kper - 1) / g.kper : 1;
   const size_t tiles = (size_t)nt * (g.chunks ? g.max_chunks : (g.M + P::BM - 1) / P::BM);
   if (tiles > 0x7FFFFFF0u) return hipErrorInvalidValue;
   hipLaunchKernelGGL((fp8_tile_kernel<NI, NJ, WN, WM, SW, EXACT, S>),
-                     dim3((unsigned)((tiles + 7) / 8 * 8)), dim3(64 * P::W), 0, st, g, nt);
+                     dim3((unsigned)((tiles + 7) / 8 * 8), slices), dim3(64 * P::W), 0, st, g, nt);
+  if (slices > 1) {
+    const size_t n = (size_t)g.M * g.N;
+    const dim3 grid((unsigned)((n + 1023) / 1024));
+    if (g.out_f32)
+      hipLaunchKernelGGL(fp8_slices_kernel<true>, grid, dim3(256), 0, st, g.part, n, slices, g.y);
+    else
+      hipLaunchKernelGGL(fp8_slices_kernel<false>, grid, dim3(256), 0, st, g.part, n, slices, g.y);
+  }
   return hipGetLastError();
+}
+
+// Slices of K for a product whose 128 x 128 tiles are fewer than the CUs take (two
+// each): 4 blocks or a multiple per slice, 0 where one slice is left.
+int slice_blocks(int M, int N, int K) {
+  const int KB = fp8_blocks(K), tiles = fp8_blocks(M) * fp8_blocks(N);
+  const int want = tiles >= 512 ? 1 : 512 / tiles;
+  const int per = ((KB + want - 1) / want + 3) & ~3;
+  return per < KB ? per : 0;
+}
+
+enum Form { SMALL, MIDDLE, LARGE };  // 128 x 128, 256 x 128, 256 x 256
+// The largest tiles that still occupy three quarters of the CUs.
+Form form_of(int M, int N, bool out_f32) {
+  const int n = (N + 255) / 256;
+  if (!out_f32 && (int64_t)n * ((M + 255) / 256) >= 192) return LARGE;
+  return (int64_t)n * fp8_blocks(M) >= 192 ? MIDDLE : SMALL;
 }
 
 }  // namespace
 
-hipError_t fp8_tile_gemm(const Fp8Gemm &g, hipStream_t st) {
+size_t fp8_partial_bytes(int M, int N, int K) {
+  size_t most = 0;  // over all calls of up to M rows
+  for (int m = 1; m <= fp8_blocks(M) && m * fp8_blocks(N) < 512; ++m) {
+    const int rows = m * 128 < M ? m * 128 : M, per = slice_blocks(rows, N, K);
+    if (!per || form_of(rows, N, true) != SMALL) continue;
+    const size_t b = (size_t)((fp8_blocks(K) + per - 1) / per) * rows * N * 4;
+    most = b > most ? b : most;
+  }
+  return most;
+}
+
+hipError_t fp8_tile_gemm(const Fp8Gemm &g0, hipStream_t st) {
+  Fp8Gemm g = g0;
+  g.kper = 0;
   if (g.swiglu) return launch<8, 2, 2, 4, true, false, 3>(g, st);
-  if (g.out_f32) return launch<8, 2, 2, 4, false, true, 3>(g, st);
   if (g.chunks) return launch<8, 2, 2, 4, false, false, 3>(g, st);
-  return launch<8, 4, 2, 4, false, false, 2>(g, st);
+  switch (form_of(g.M, g.N, g.out_f32)) {
+    case LARGE: return launch<8, 4, 2, 4, false, false, 2>(g, st);
+    case MIDDLE:
+      if (g.out_f32) return launch<8, 2, 2, 4, false, true, 3>(g, st);
+      return launch<8, 2, 2, 4, false, false, 3>(g, st);
+    default: break;
+  }
+  g.kper = slice_blocks(g.M, g.N, g.K);
+  if (g.out_f32) return launch<4, 2, 2, 4, false, true, 2>(g, st);
+  return launch<4, 2, 2, 4, false, false, 2>(g, st);
 }
 
 }  // namespace cai4
