@@ -981,13 +981,21 @@ def moe_forward(experts: MoEExperts, x, out, *, top_k: int, logits=None, bias=No
 FP8_BLOCK = 128  # columns of a row's group; rows and columns of a weight block
 
 
-def _here(t: torch.Tensor, name: str) -> torch.Tensor:
-    """A contiguous tensor of the current device (the one whose stream the call
-    is enqueued on)."""
+def _here(dev: int, t: torch.Tensor, name: str) -> None:
+    """Check a contiguous tensor of the current device dev (the one whose stream
+    the call is enqueued on)."""
+    if not (isinstance(t, torch.Tensor) and t.is_cuda and t.is_contiguous()):
+        _dev(t, name)
+    if t.get_device() != dev:
+        raise ValueError(f"{name} is on {t.device}, the current device is {dev}")
+
+
+def _home(t: torch.Tensor, name: str) -> int:
+    """The current device, which a call's first tensor is checked to be on."""
     _dev(t, name)
-    if t.device.index != _device():
-        raise ValueError(f"{name} is on {t.device}, the current device is {_device()}")
-    return t
+    dev = _device()
+    _here(dev, t, name)
+    return dev
 
 
 def _fp8_blocks(n: int) -> int:
@@ -998,14 +1006,15 @@ def _is_e4m3(t: torch.Tensor) -> bool:
     return t.dtype in (torch.float8_e4m3fn, torch.uint8)
 
 
-def _fp8_matrix(codes, scales, lead, n_rows, k_cols, name):
+def _fp8_matrix(dev, codes, scales, lead, n_rows, k_cols, name):
     """Check e4m3 codes [*lead, n_rows, k_cols] and their blocks' scales."""
-    _here(codes, name), _here(scales, f"{name} scales")
+    _here(dev, codes, name)
+    _here(dev, scales, "scales")
     if not (n_rows >= 1 and k_cols >= 16 and k_cols % 16 == 0):
         raise ValueError(f"{name}: k_cols {k_cols} must be a multiple of 16")
     if not (_is_e4m3(codes) and codes.numel() == lead * n_rows * k_cols):
         raise ValueError(f"{name}: e4m3 codes of {lead * n_rows * k_cols} values")
-    need = lead * _fp8_blocks(n_rows) * _fp8_blocks(k_cols)
+    need = lead * ((n_rows + 127) // 128) * ((k_cols + 127) // 128)
     if not (scales.dtype == torch.float32 and scales.numel() == need):
         raise ValueError(f"{name} scales: f32, one per block of 128 x 128 ({need})")
 
@@ -1022,8 +1031,11 @@ def route_experts(logits, top_k: int, ids, weights, *, score: int = SCORE_SIGMOI
     to the most; descending, ties to the lower id.  weights: the chosen s, over
     their sum when normalize, times scale.  A NaN logit counts as -infinity; a
     softmax over -infinity alone gives weights of 0."""
-    _here(logits, "logits"), _here(ids, "ids"), _here(weights, "weights")
-    if logits.dim() != 2 or logits.dtype not in (torch.float32, torch.bfloat16):
+    dev = _home(logits, "logits")
+    _here(dev, ids, "ids")
+    _here(dev, weights, "weights")
+    bf16 = logits.dtype is torch.bfloat16
+    if logits.dim() != 2 or not (bf16 or logits.dtype is torch.float32):
         raise ValueError("logits: f32 or bf16 [n_tokens, n_experts]")
     T, E = logits.shape
     if not (ids.dtype == torch.int32 and ids.numel() == T * top_k):
@@ -1032,8 +1044,8 @@ def route_experts(logits, top_k: int, ids, weights, *, score: int = SCORE_SIGMOI
         raise ValueError("weights: f32 [n_tokens, top_k]")
     b = 0
     if bias is not None:
-        _here(bias, "bias")
-        _expect(bias.dtype == torch.float32 and bias.numel() == E, "bias: f32 [n_experts]")
+        _here(dev, bias, "bias")
+        _expect(bias.dtype is torch.float32 and bias.numel() == E, "bias: f32 [n_experts]")
         b = bias.data_ptr()
     if not (1 <= E <= 1024 and 1 <= top_k <= 16 and 1 <= n_groups <= 64 and E % n_groups == 0
             and 1 <= top_groups <= n_groups and top_k <= top_groups * (E // n_groups)
@@ -1042,7 +1054,7 @@ def route_experts(logits, top_k: int, ids, weights, *, score: int = SCORE_SIGMOI
                          f"by the best {group_best}, score {score}")
     R = Router(E, top_k, score, n_groups, top_groups, group_best, int(normalize), scale, b)
     check("cascadia_int4_route_experts", lib().cascadia_int4_route_experts(
-        C.byref(R), logits.data_ptr(), int(logits.dtype == torch.bfloat16), T, ids.data_ptr(),
+        C.byref(R), logits.data_ptr(), int(bf16), T, ids.data_ptr(),
         weights.data_ptr(), _stream()))
     return ids, weights
 
@@ -1052,7 +1064,9 @@ def quantize_fp8(x, rows: int, k_cols: int, codes, scales):
     uint8 [rows, k_cols]) with a scale per group of 128 columns (f32 [rows,
     ceil(k_cols / 128)]): scale = max(max|x|, 2^-96) / 448, code = e4m3(x /
     scale), to nearest even.  k_cols: a multiple of 16."""
-    _here(x, "x"), _here(codes, "codes"), _here(scales, "scales")
+    dev = _home(x, "x")
+    _here(dev, codes, "codes")
+    _here(dev, scales, "scales")
     _expect(k_cols >= 16 and k_cols % 16 == 0, f"k_cols {k_cols} must be a multiple of 16")
     _expect(x.dtype in (torch.float32, torch.bfloat16) and x.numel() == rows * k_cols,
             "x: f32 or bf16 [rows, k_cols]")
@@ -1069,7 +1083,7 @@ def quantize_fp8_blocks(weight_bf16, n_rows: int, k_cols: int):
     """Quantise bf16 weights [n_rows, k_cols] for fp8_gemm (done once, at load):
     (codes float8_e4m3fn [n_rows, k_cols], scales f32 [ceil(n_rows / 128),
     ceil(k_cols / 128)]), a scale per block of 128 x 128 as quantize_fp8's."""
-    _here(weight_bf16, "weight_bf16")
+    _home(weight_bf16, "weight_bf16")
     _expect(n_rows >= 1 and k_cols >= 16 and k_cols % 16 == 0,
             f"k_cols {k_cols} must be a multiple of 16")
     _expect(_is_bf16_bits(weight_bf16) and weight_bf16.numel() == n_rows * k_cols,
@@ -1107,18 +1121,21 @@ def fp8_gemm(codes, scales, xs, n_rows: int, k_cols: int, seq: int, ys, x_scales
     f32, quantised in the call as by quantize_fp8, or e4m3 codes with x_scales
     [seq, ceil(k_cols / 128)].  ys [seq, n_rows] bf16 or f32; f32 sums, one
     rounding.  workspace: fp8_gemm_workspace_bytes (for a graph capture)."""
-    _fp8_matrix(codes, scales, 1, n_rows, k_cols, "codes")
-    _here(xs, "xs"), _here(ys, "ys")
+    dev = _home(codes, "codes")
+    _fp8_matrix(dev, codes, scales, 1, n_rows, k_cols, "codes")
+    _here(dev, xs, "xs")
+    _here(dev, ys, "ys")
     _expect(seq >= 1, "seq must be >= 1")
     xt = _fp8_x_type(xs.dtype)
     if xs.numel() != seq * k_cols:
         raise ValueError(f"xs must hold seq*k_cols = {seq * k_cols} values")
-    if not (ys.dtype in (torch.float32, torch.bfloat16) and ys.numel() == seq * n_rows):
+    f32 = ys.dtype is torch.float32
+    if not ((f32 or ys.dtype is torch.bfloat16) and ys.numel() == seq * n_rows):
         raise ValueError(f"ys: f32 or bf16 [seq*n_rows = {seq * n_rows}]")
     sp = 0
     if xt == FP8_X_E4M3:
         _expect(x_scales is not None, "e4m3 xs need x_scales")
-        _here(x_scales, "x_scales")
+        _here(dev, x_scales, "x_scales")
         _expect(x_scales.dtype == torch.float32 and x_scales.numel() == seq * _fp8_blocks(k_cols),
                 "x_scales: f32 [seq, ceil(k_cols / 128)]")
         sp = x_scales.data_ptr()
@@ -1126,12 +1143,15 @@ def fp8_gemm(codes, scales, xs, n_rows: int, k_cols: int, seq: int, ys, x_scales
         _expect(x_scales is None, "x_scales go with e4m3 xs")
     ws = 0
     if workspace is not None:
-        _here(workspace, "workspace")
-        ws = _workspace_ptr(workspace, "cascadia_int4_fp8_gemm_workspace_bytes", n_rows, k_cols,
-                            xt, seq)
+        _here(dev, workspace, "workspace")
+        need = _need("cascadia_int4_fp8_gemm_workspace_bytes",
+                     lib().cascadia_int4_tuning_generation(), dev, n_rows, k_cols, xt, seq)
+        if workspace.nbytes < need:
+            raise ValueError(f"workspace has {workspace.nbytes} bytes, the call needs {need}")
+        ws = workspace.data_ptr()
     check("cascadia_int4_fp8_gemm", lib().cascadia_int4_fp8_gemm(
         n_rows, k_cols, codes.data_ptr(), scales.data_ptr(), xs.data_ptr(), xt, sp, seq,
-        ys.data_ptr(), int(ys.dtype == torch.float32), ws, _stream()))
+        ys.data_ptr(), int(f32), ws, _stream()))
     return ys
 
 
@@ -1145,20 +1165,21 @@ class Fp8Experts:
     def __init__(self, gate_up, gate_up_scales, down, down_scales, n_experts: int, hidden: int,
                  inter: int):
         _expect(1 <= n_experts <= 1024, "n_experts: 1 to 1024")
-        _fp8_matrix(gate_up, gate_up_scales, 2 * n_experts, inter, hidden, "gate_up")
-        _fp8_matrix(down, down_scales, n_experts, hidden, inter, "down")
+        dev = _home(gate_up, "gate_up")
+        _fp8_matrix(dev, gate_up, gate_up_scales, 2 * n_experts, inter, hidden, "gate_up")
+        _fp8_matrix(dev, down, down_scales, n_experts, hidden, inter, "down")
         self.gate_up, self.gate_up_scales = gate_up, gate_up_scales
         self.down, self.down_scales = down, down_scales
         self.n_experts, self.hidden, self.inter = n_experts, hidden, inter
         self._layer = Fp8MoeLayer(hidden, inter, n_experts, gate_up.data_ptr(),
                                   gate_up_scales.data_ptr(), down.data_ptr(),
                                   down_scales.data_ptr())
+        self._ref = C.byref(self._layer)  # (the library only reads it)
 
 
 def fp8_moe_workspace_bytes(experts: Fp8Experts, top_k: int, n_tokens: int) -> int:
     """Workspace bytes of fp8_moe_forward for up to n_tokens rows."""
-    return int(lib().cascadia_int4_fp8_moe_workspace_bytes(C.byref(experts._layer), top_k,
-                                                           n_tokens))
+    return int(lib().cascadia_int4_fp8_moe_workspace_bytes(experts._ref, top_k, n_tokens))
 
 
 @functools.lru_cache(maxsize=1024)
@@ -1176,11 +1197,15 @@ def fp8_moe_forward(experts: Fp8Experts, x, out, *, top_k: int, ids, weights,
     route_experts gives them.  Slots with a weight below threshold or an id
     outside the layer (padding: -1) are left out.  workspace:
     fp8_moe_workspace_bytes (for a graph capture)."""
-    _here(x, "x"), _here(out, "out"), _here(ids, "ids"), _here(weights, "weights")
-    _here(experts.gate_up, "experts")
+    dev = _home(x, "x")
+    _here(dev, out, "out")
+    _here(dev, ids, "ids")
+    _here(dev, weights, "weights")
+    _here(dev, experts.gate_up, "experts")
     H = experts.hidden
-    both = (torch.float32, torch.bfloat16)
-    _expect(x.dtype in both and out.dtype in both, "x and out must be f32 or bf16")
+    x_f32, out_f32 = x.dtype is torch.float32, out.dtype is torch.float32
+    _expect((x_f32 or x.dtype is torch.bfloat16) and (out_f32 or out.dtype is torch.bfloat16),
+            "x and out must be f32 or bf16")
     T = x.numel() // H
     _expect(x.numel() == T * H and out.numel() == T * H and T >= 1, "x/out must be [n_tokens, hidden]")
     _expect(1 <= top_k <= 16, "top_k: 1 to 16")
@@ -1189,21 +1214,21 @@ def fp8_moe_forward(experts: Fp8Experts, x, out, *, top_k: int, ids, weights,
             "weights: f32 [n_tokens, top_k]")
     res = 0
     if residual is not None:
-        _here(residual, "residual")
-        _expect(residual.dtype == out.dtype and residual.numel() == T * H,
+        _here(dev, residual, "residual")
+        _expect(residual.dtype is out.dtype and residual.numel() == T * H,
                 "residual: [n_tokens, hidden] of out's type")
         res = residual.data_ptr()
     ws = 0
     if workspace is not None:
-        ws = _here(workspace, "workspace").data_ptr()
-        need = _fp8_moe_need(lib().cascadia_int4_tuning_generation(), _device(), H, experts.inter,
-                             experts.n_experts, int(top_k), T)
+        _here(dev, workspace, "workspace")
+        ws = workspace.data_ptr()
+        need = _fp8_moe_need(lib().cascadia_int4_tuning_generation(), dev, H, experts.inter,
+                             experts.n_experts, top_k, T)
         if workspace.nbytes < need:
             raise ValueError(f"workspace has {workspace.nbytes} bytes, the call needs {need}")
     check("cascadia_int4_fp8_moe_forward", lib().cascadia_int4_fp8_moe_forward(
-        C.byref(experts._layer), top_k, ids.data_ptr(), weights.data_ptr(), threshold, x.data_ptr(),
-        int(x.dtype == torch.float32), res, T, out.data_ptr(), int(out.dtype == torch.float32), ws,
-        _stream()))
+        experts._ref, top_k, ids.data_ptr(), weights.data_ptr(), threshold, x.data_ptr(),
+        int(x_f32), res, T, out.data_ptr(), int(out_f32), ws, _stream()))
     return out
 
 
