@@ -85,7 +85,7 @@ class Router(C.Structure):
 class Fp8MoeLayer(C.Structure):
     _fields_ = [("hidden", C.c_uint32), ("inter", C.c_uint32), ("n_experts", C.c_uint32),
                 ("gate_up", C.c_void_p), ("gate_up_scales", C.c_void_p), ("down", C.c_void_p),
-                ("down_scales", C.c_void_p)]
+                ("down_scales", C.c_void_p), ("tiled", C.c_uint32)]
 
 
 _vp, _u32, _u64, _sz, _f64, _i32 = C.c_void_p, C.c_uint32, C.c_uint64, C.c_size_t, C.c_double, C.c_int
@@ -128,6 +128,8 @@ SIGNATURES = {
     "cascadia_int4_fp8_gemm_workspace_bytes": (_sz, [_u32, _u32, _u32, _u32]),
     "cascadia_int4_fp8_gemm": (_i32, [_u32, _u32, _vp, _vp, _vp, _u32, _vp, _u32, _vp, _u32, _vp,
                                       _vp]),
+    "cascadia_int4_fp8_tiled_bytes": (_sz, [_u32, _u32]),
+    "cascadia_int4_fp8_tile_weights": (_i32, [_u32, _u32, _u32, _vp, _vp, _vp]),
     "cascadia_int4_fp8_moe_workspace_bytes": (_sz, [_FP, _u32, _u32]),
     "cascadia_int4_fp8_moe_forward": (_i32, [_FP, _u32, _vp, _vp, C.c_float, _vp, _u32, _vp, _u32,
                                              _vp, _u32, _vp, _vp]),

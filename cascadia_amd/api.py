@@ -1155,25 +1155,40 @@ def fp8_gemm(codes, scales, xs, n_rows: int, k_cols: int, seq: int, ys, x_scales
     return ys
 
 
+def _fp8_tiled(codes, count, n_rows, k_cols):
+    """A copy of `count` matrices of e4m3 codes in blocks of 128 x 128."""
+    per = int(lib().cascadia_int4_fp8_tiled_bytes(n_rows, k_cols))
+    out = torch.empty(count * per, dtype=torch.uint8, device=codes.device)
+    check("cascadia_int4_fp8_tile_weights", lib().cascadia_int4_fp8_tile_weights(
+        count, n_rows, k_cols, codes.data_ptr(), out.data_ptr(), _stream()))
+    return out
+
+
 class Fp8Experts:
     """One MoE layer's experts in e4m3 (float8_e4m3fn or uint8) with f32 scales of
     blocks of 128 x 128: gate_up [n_experts, 2, inter, hidden] (gate, then up),
     its scales [n_experts, 2, ceil(inter / 128), ceil(hidden / 128)], down
     [n_experts, hidden, inter], its scales [n_experts, ceil(hidden / 128),
-    ceil(inter / 128)].  hidden and inter: multiples of 16."""
+    ceil(inter / 128)].  hidden and inter: multiples of 16.
+    tiled (the default): the codes are copied once into blocks that stream faster,
+    on the current stream; the tensors of codes are not kept and may be freed or
+    changed (the scales are read where they are).  tiled=False: they are read where they are."""
 
     def __init__(self, gate_up, gate_up_scales, down, down_scales, n_experts: int, hidden: int,
-                 inter: int):
+                 inter: int, tiled: bool = True):
         _expect(1 <= n_experts <= 1024, "n_experts: 1 to 1024")
         dev = _home(gate_up, "gate_up")
         _fp8_matrix(dev, gate_up, gate_up_scales, 2 * n_experts, inter, hidden, "gate_up")
         _fp8_matrix(dev, down, down_scales, n_experts, hidden, inter, "down")
+        if tiled:
+            gate_up = _fp8_tiled(gate_up, 2 * n_experts, inter, hidden)
+            down = _fp8_tiled(down, n_experts, hidden, inter)
         self.gate_up, self.gate_up_scales = gate_up, gate_up_scales
         self.down, self.down_scales = down, down_scales
-        self.n_experts, self.hidden, self.inter = n_experts, hidden, inter
+        self.n_experts, self.hidden, self.inter, self.tiled = n_experts, hidden, inter, bool(tiled)
         self._layer = Fp8MoeLayer(hidden, inter, n_experts, gate_up.data_ptr(),
                                   gate_up_scales.data_ptr(), down.data_ptr(),
-                                  down_scales.data_ptr())
+                                  down_scales.data_ptr(), int(self.tiled))
         self._ref = C.byref(self._layer)  # (the library only reads it)
 
 
@@ -1184,7 +1199,7 @@ def fp8_moe_workspace_bytes(experts: Fp8Experts, top_k: int, n_tokens: int) -> i
 
 @functools.lru_cache(maxsize=1024)
 def _fp8_moe_need(tuning, device, hidden, inter, n_experts, top_k, n_tokens):
-    L = Fp8MoeLayer(hidden, inter, n_experts, 256, 256, 256, 256)
+    L = Fp8MoeLayer(hidden, inter, n_experts, 256, 256, 256, 256, 0)
     return int(lib().cascadia_int4_fp8_moe_workspace_bytes(C.byref(L), top_k, n_tokens))
 
 

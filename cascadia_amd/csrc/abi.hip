@@ -2369,7 +2369,8 @@ int fp8_moe_check(const cascadia_int4_fp8_moe_layer *L, uint32_t top_k, uint32_t
   if (!L || !L->gate_up || !L->gate_up_scales || !L->down || !L->down_scales)
     return CASCADIA_INT4_ERR_NULL;
   if (!fp8_dims_ok(L->hidden, L->inter) || !fp8_dims_ok(L->inter, L->hidden) ||
-      L->n_experts == 0 || L->n_experts > (uint32_t)cai4::kRouteMaxExperts || top_k == 0 ||
+      L->n_experts == 0 || L->n_experts > (uint32_t)cai4::kRouteMaxExperts || L->tiled > 1 ||
+      top_k == 0 ||
       top_k > (uint32_t)cai4::kRouteMaxTopK || n_tokens == 0 || n_tokens > (1u << 20) ||
       (size_t)n_tokens * L->hidden > 0x7FFFFFFFu)
     return CASCADIA_INT4_ERR_ARG;
@@ -2497,6 +2498,22 @@ int cascadia_int4_fp8_gemm(uint32_t n_rows, uint32_t k_cols, const uint8_t *w,
   return hip_status(cai4::fp8_gemm(g, st));
 }
 
+size_t cascadia_int4_fp8_tiled_bytes(uint32_t n_rows, uint32_t k_cols) {
+  return fp8_dims_ok(n_rows, k_cols) ? cai4::fp8_tiled_bytes((int)n_rows, (int)k_cols) : 0;
+}
+
+int cascadia_int4_fp8_tile_weights(uint32_t n_matrices, uint32_t n_rows, uint32_t k_cols,
+                                   const uint8_t *codes, uint8_t *tiled, void *stream) {
+  if (!codes || !tiled) return CASCADIA_INT4_ERR_NULL;
+  if (!fp8_dims_ok(n_rows, k_cols) || n_matrices == 0 || n_matrices > (1u << 20) ||
+      (size_t)n_matrices * (cai4::fp8_tiled_bytes((int)n_rows, (int)k_cols) / cai4::kFp8BlockBytes) >
+          0x7FFFFFFFu)
+    return CASCADIA_INT4_ERR_ARG;
+  if (!aligned(codes, 16) || !aligned(tiled, 16)) return CASCADIA_INT4_ERR_ARG;
+  return hip_status(cai4::fp8_tile_weights(codes, (int)n_matrices, (int)n_rows, (int)k_cols, tiled,
+                                           (hipStream_t)stream));
+}
+
 size_t cascadia_int4_fp8_moe_workspace_bytes(const cascadia_int4_fp8_moe_layer *L, uint32_t top_k,
                                              uint32_t n_tokens) {
   if (fp8_moe_check(L, top_k, n_tokens)) return 0;
@@ -2526,6 +2543,7 @@ int cascadia_int4_fp8_moe_forward(const cascadia_int4_fp8_moe_layer *L, uint32_t
   m.H = (int)L->hidden;
   m.I = (int)L->inter;
   m.E = (int)L->n_experts;
+  m.tiled = (int)L->tiled;
   m.gate_up = L->gate_up;
   m.down = L->down;
   m.gate_up_s = L->gate_up_scales;

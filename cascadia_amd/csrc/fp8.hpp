@@ -45,10 +45,20 @@ struct Fp8Chunk {
   int expert, row0, count, first, number;
 };
 
+// Codes [count, N, K] -> blocks of 128 rows x 128 columns, each contiguous (16 KB, row
+// by row), padded with zeros: [count, ceil(N / 128), ceil(K / 128), 128, 128].
+constexpr size_t kFp8BlockBytes = 128 * 128;
+inline size_t fp8_tiled_bytes(int N, int K) {
+  return (size_t)fp8_blocks(N) * fp8_blocks(K) * kFp8BlockBytes;
+}
+hipError_t fp8_tile_weights(const uint8_t *codes, int count, int N, int K, uint8_t *tiled,
+                            hipStream_t st);
+
 // y = x w^T over e4m3 codes and their blocks' scales, for one matrix or for the
 // row groups of many experts in one launch (chunks).
 struct Fp8Gemm {
   const uint8_t *w;  // [N, K] codes (SwiGLU: gate [N, K], then up [N, K])
+  int w_tiled;       // w in blocks (fp8_tile_weights)
   const float *ws;   // [ceil(N / 128), KB] (SwiGLU: gate's, then up's)
   const uint8_t *x;  // [rows, K] codes
   const float *xs;   // [rows, ld_xs], KB of them used (tiles: 16-byte aligned rows)
@@ -79,7 +89,7 @@ hipError_t fp8_tile_gemm(const Fp8Gemm &g, hipStream_t st);
 
 // One layer's experts in e4m3.
 struct Fp8Moe {
-  int H, I, E;
+  int H, I, E, tiled;
   const uint8_t *gate_up, *down;      // [E, 2, I, H], [E, H, I]
   const float *gate_up_s, *down_s;    // [E, 2, ib, hb], [E, hb, ib]
   int T, top_k;

@@ -40,16 +40,33 @@ struct Weights {
   rsrc_t r;
   scalar_t ws;
   int rows;
+  uint32_t row, block;  // bytes between rows, between blocks of K
 };
 CAI4_DEV Weights weights_of(const Fp8Gemm &g, int expert, int n0, int m) {
   const int KB = (g.K + 127) >> 7, NB = (g.N + 127) >> 7;
   Weights w;
   w.rows = n0 >= g.N ? 0 : g.N - n0 < 16 ? g.N - n0 : 16;
   const int n = w.rows ? n0 : 0;
-  w.r = rsrc_scalar(g.w + (size_t)expert * g.w_stride + ((size_t)m * g.N + n) * g.K,
-                    (size_t)w.rows * g.K);
+  const uint8_t *p = g.w + (size_t)expert * g.w_stride;
+  if (g.w_tiled) {
+    const size_t band = KB * kFp8BlockBytes, in = (size_t)(n & 127) * 128;
+    w.r = rsrc_scalar(p + ((size_t)m * NB + (n >> 7)) * band + in, w.rows ? band - in : 0);
+    w.row = 128;
+    w.block = kFp8BlockBytes;
+  } else {
+    w.r = rsrc_scalar(p + ((size_t)m * g.N + n) * g.K, (size_t)w.rows * g.K);
+    w.row = g.K;
+    w.block = 128;
+  }
   w.ws = (scalar_t)(g.ws + (size_t)expert * g.ws_stride + ((size_t)m * NB + (n >> 7)) * KB);
   return w;
+}
+// This lane's two chunks of block kb (past the rows or columns: zeros).
+CAI4_DEV void load_weights(const Weights &w, int kb, int K, int l15, int c, u32x4_t (&a)[2]) {
+  const uint32_t at = (uint32_t)l15 * w.row + (uint32_t)kb * w.block + 16 * c;
+  const int c0 = kb * 128 + 16 * c;
+  a[0] = load16(w.r, l15 < w.rows && c0 < K ? at : kDmaOOB);
+  a[1] = load16(w.r, l15 < w.rows && c0 + 64 < K ? at + 64 : kDmaOOB);
 }
 
 // 16 MT weight rows (SW: the same 16 of gate and of up) x 16 NT rows of x per
@@ -83,7 +100,6 @@ __global__ __launch_bounds__(512) void fp8_few_kernel(Fp8Gemm g) {
     xo[t] = r >= rows.count ? kDmaOOB
             : (g.row_map ? (uint32_t)g.row_map[rows.row0 + r] : (uint32_t)r) * (uint32_t)g.K;
   }
-  const uint32_t wo = (uint32_t)l15 * g.K;
   f32x4_t acc[MT][NT];
 #pragma unroll
   for (int m = 0; m < MT; ++m)
@@ -108,10 +124,7 @@ __global__ __launch_bounds__(512) void fp8_few_kernel(Fp8Gemm g) {
       const int c0 = kb * 128 + 16 * c, c1 = c0 + 64;
       u32x4_t a[MT][2], b[NT][2];
 #pragma unroll
-      for (int m = 0; m < MT; ++m) {
-        a[m][0] = load16(w[m].r, l15 < w[m].rows && c0 < g.K ? wo + c0 : kDmaOOB);
-        a[m][1] = load16(w[m].r, l15 < w[m].rows && c1 < g.K ? wo + c1 : kDmaOOB);
-      }
+      for (int m = 0; m < MT; ++m) load_weights(w[m], kb, g.K, l15, c, a[m]);
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
         b[t][0] = load16(xr, xo[t] != kDmaOOB && c0 < g.K ? xo[t] + c0 : kDmaOOB);
@@ -206,15 +219,10 @@ CAI4_DEV void stream_row(const Weights (&w)[MT], int K, int first, int step, int
                          const uint8_t (*codes)[128], const float *scales, f32x4_t (&acc)[MT],
                          Row row) {
   const int l15 = lane & 15, c = lane >> 4, KB = (K + 127) >> 7;
-  const uint32_t wo = (uint32_t)l15 * K;
   u32x4_t a[2][MT][2];
   auto load = [&](u32x4_t (&to)[MT][2], int kb) {  // (past the end: out of range)
-    const int c0 = kb * 128 + 16 * c, c1 = c0 + 64;
 #pragma unroll
-    for (int m = 0; m < MT; ++m) {
-      to[m][0] = load16(w[m].r, l15 < w[m].rows && c0 < K ? wo + c0 : kDmaOOB);
-      to[m][1] = load16(w[m].r, l15 < w[m].rows && c1 < K ? wo + c1 : kDmaOOB);
-    }
+    for (int m = 0; m < MT; ++m) load_weights(w[m], kb, K, l15, c, to[m]);
   };
   auto add = [&](const u32x4_t (&from)[MT][2], int kb) {
     const u32x4_t b[2] = {*reinterpret_cast<const u32x4_t *>(&codes[kb][16 * c]),

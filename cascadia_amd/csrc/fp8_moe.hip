@@ -260,7 +260,8 @@ hipError_t fp8_moe_forward(const Fp8Moe &m, void *workspace, hipStream_t st) {
   up.N = m.I;
   up.K = m.H;
   up.M = n;
-  up.w_stride = (size_t)2 * m.I * m.H;
+  up.w_tiled = down.w_tiled = m.tiled;
+  up.w_stride = 2 * (m.tiled ? fp8_tiled_bytes(m.I, m.H) : (size_t)m.I * m.H);
   up.ws_stride = (size_t)2 * ib * hb;
   up.swiglu = 1;
   up.out_f32 = 1;
@@ -269,7 +270,7 @@ hipError_t fp8_moe_forward(const Fp8Moe &m, void *workspace, hipStream_t st) {
   down.N = m.H;
   down.K = m.I;
   down.M = n;
-  down.w_stride = (size_t)m.H * m.I;
+  down.w_stride = m.tiled ? fp8_tiled_bytes(m.H, m.I) : (size_t)m.H * m.I;
   down.ws_stride = (size_t)hb * ib;
 
   if (m.T == 1 && fp8_one_token(m.H, m.I, m.top_k)) {

@@ -58,7 +58,34 @@ __global__ __launch_bounds__(256) void fp8_blocks_kernel(const uint16_t *w, int 
   if (threadIdx.x == 0) scales[(size_t)nb * KB + kb] = d.scale;
 }
 
+// A workgroup per block: half a row per thread.
+__global__ __launch_bounds__(256) void fp8_tile_kernel(const uint8_t *codes, int N, int K, int NB,
+                                                       int KB, uint8_t *tiled) {
+  const size_t b = blockIdx.x, m = b / ((size_t)NB * KB);
+  const int r = (int)(b - m * NB * KB), nb = r / KB, kb = r - nb * KB;
+  const int row = threadIdx.x >> 1, n = nb * kFp8Block + row;
+  const int half = (threadIdx.x & 1) * 64, col = kb * kFp8Block + half;
+  const uint8_t *from = codes + (m * N + n) * K + col;
+  uint8_t *to = tiled + b * kFp8BlockBytes + row * 128 + half;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    u32x4_t v = {0u, 0u, 0u, 0u};
+    if (n < N && col + 16 * i < K) v = *reinterpret_cast<const u32x4_t *>(from + 16 * i);
+    *reinterpret_cast<u32x4_t *>(to + 16 * i) = v;
+  }
+}
+
 }  // namespace
+
+hipError_t fp8_tile_weights(const uint8_t *codes, int count, int N, int K, uint8_t *tiled,
+                            hipStream_t st) {
+  const int NB = fp8_blocks(N), KB = fp8_blocks(K);
+  const size_t blocks = (size_t)count * NB * KB;
+  if (blocks > 0x7FFFFFFFu) return hipErrorInvalidValue;
+  hipLaunchKernelGGL(fp8_tile_kernel, dim3((unsigned)blocks), dim3(256), 0, st, codes, N, K, NB, KB,
+                     tiled);
+  return hipGetLastError();
+}
 
 hipError_t fp8_quantize_rows(const void *x, bool x_f32, size_t rows, int K, uint8_t *codes,
                              float *scales, int ld, hipStream_t st) {

@@ -130,9 +130,14 @@ __global__ __launch_bounds__(64 * WN * WM) void fp8_tile_kernel(Fp8Gemm g, int n
   const int cols = end * 128 < g.K ? end * 128 : g.K;
   const int nr = g.N - n0 < P::OUT ? g.N - n0 : P::OUT;
   // this wave loads rows of the weights (SwiGLU: the first half gate, the others up)
-  const uint8_t *w = g.w + (size_t)rows.expert * g.w_stride + (size_t)n0 * g.K +
-                     (SW && wave >= P::W / 2 ? (size_t)g.N * g.K : 0);
-  const rsrc_t wr = rsrc_scalar(w, (size_t)nr * g.K);
+  const uint32_t band = (uint32_t)(KB * kFp8BlockBytes);  // 128 rows, in blocks
+  const size_t matrix = g.w_tiled ? (size_t)NB * band : (size_t)g.N * g.K;
+  const uint8_t *w = g.w + (size_t)rows.expert * g.w_stride +
+                     (g.w_tiled ? (size_t)(n0 >> 7) * band : (size_t)n0 * g.K) +
+                     (SW && wave >= P::W / 2 ? matrix : 0);
+  const rsrc_t wr = rsrc_scalar(w, g.w_tiled ? (size_t)((nr + 127) >> 7) * band
+                                             : (size_t)nr * g.K);
+  const uint32_t wstep = g.w_tiled ? (uint32_t)kFp8BlockBytes : 128u;  // per block of K
   const rsrc_t xr = g.row_map ? rsrc_scalar(g.x, (size_t)g.x_rows * g.K)
                               : rsrc_scalar(g.x + (size_t)rows.row0 * g.K,
                                             (size_t)rows.count * g.K);
@@ -149,7 +154,9 @@ __global__ __launch_bounds__(64 * WN * WM) void fp8_tile_kernel(Fp8Gemm g, int n
 #pragma unroll
   for (int q = 0; q < P::PW; ++q) {
     const int row = (wave * P::PW + q) * 8 + (lane >> 3), r = SW ? row & (P::BN / 2 - 1) : row;
-    vw[q] = r < nr ? (uint32_t)(r * g.K) + 16 * chunk_of(row) : kDmaOOB;
+    const uint32_t at = g.w_tiled ? (uint32_t)(r >> 7) * band + (uint32_t)(r & 127) * 128
+                                  : (uint32_t)(r * g.K);
+    vw[q] = r < nr ? at + 16 * chunk_of(row) : kDmaOOB;
   }
 #pragma unroll
   for (int q = 0; q < P::PX; ++q) {
@@ -173,7 +180,7 @@ __global__ __launch_bounds__(64 * WN * WM) void fp8_tile_kernel(Fp8Gemm g, int n
     if (q < P::PW) {
       const int piece = wave * P::PW + q;
       lds_dma<16>(wr, to + piece * 1024, (piece & 1 ? odd : even) ? vw[q] : kDmaOOB,
-                  (uint32_t)kb * 128);
+                  (uint32_t)kb * wstep);
     } else if (q < P::PW + P::PX) {
       const int piece = wave * P::PX + q - P::PW;
       lds_dma<16>(xr, to + P::BN * 128 + piece * 1024,

@@ -501,16 +501,28 @@ int cascadia_int4_fp8_gemm(uint32_t n_rows, uint32_t k_cols, const uint8_t *w,
                            const float *x_scales, uint32_t seq, void *ys, uint32_t y_is_f32,
                            void *workspace, void *stream);
 
+/* Weight codes in blocks: each 128 rows x 128 columns contiguous (16 KB, row by
+ * row), [n_matrices, ceil(n_rows / 128), ceil(k_cols / 128), 128, 128], rows and
+ * columns past the matrix zero; _tiled_bytes is one matrix's size (0 on bad
+ * dimensions).  Same codes, moved (once, at load): products over few rows per
+ * expert stream them faster.  codes and tiled 16-byte aligned. */
+size_t cascadia_int4_fp8_tiled_bytes(uint32_t n_rows, uint32_t k_cols);
+int cascadia_int4_fp8_tile_weights(uint32_t n_matrices, uint32_t n_rows, uint32_t k_cols,
+                                   const uint8_t *codes, uint8_t *tiled, void *stream);
+
 /* One MoE layer's experts in e4m3: gate_up [n_experts, 2, inter, hidden] (each
  * expert's gate, then its up) with scales [n_experts, 2, ceil(inter / 128),
  * ceil(hidden / 128)]; down [n_experts, hidden, inter] with scales [n_experts,
- * ceil(hidden / 128), ceil(inter / 128)].  hidden and inter multiples of 16. */
+ * ceil(hidden / 128), ceil(inter / 128)].  hidden and inter multiples of 16.
+ * tiled 1: both in blocks, as cascadia_int4_fp8_tile_weights makes them of 2 *
+ * n_experts and of n_experts matrices (the scales stay as they are). */
 typedef struct cascadia_int4_fp8_moe_layer {
   uint32_t hidden, inter, n_experts; /* n_experts <= 1024 */
   const uint8_t *gate_up;
   const float *gate_up_scales;
   const uint8_t *down;
   const float *down_scales;
+  uint32_t tiled;
 } cascadia_int4_fp8_moe_layer;
 
 /* out_t = residual_t + sum_k weights[t, k] * y_{t,k} in slot order, one

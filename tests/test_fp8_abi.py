@@ -88,7 +88,7 @@ def test_moe_refusals(cl):
 
     def call(k=2, ids=P, w=P, x=P, xf=0, res=None, T=4, out=P, of=0, buf=None, **kw):
         a = dict(hidden=64, inter=32, n_experts=4, gate_up=P, gate_up_scales=P, down=P,
-                 down_scales=P)
+                 down_scales=P, tiled=0)
         a.update(kw)
         return L.cascadia_int4_fp8_moe_forward(C.byref(Layer(**a)), k, ids, w, 0.0, x, xf, res, T,
                                                out, of, buf, None)
@@ -101,14 +101,25 @@ def test_moe_refusals(cl):
     for kw in (dict(hidden=0), dict(hidden=72), dict(inter=24), dict(n_experts=0),
                dict(n_experts=1025), dict(k=0), dict(k=17), dict(T=0), dict(T=(1 << 20) + 1),
                dict(gate_up=P + 8), dict(down=P + 4), dict(gate_up_scales=P + 2), dict(xf=2),
-               dict(of=2), dict(x=P + 8), dict(out=P + 8), dict(res=P + 8), dict(buf=P + 8),
+               dict(of=2), dict(tiled=2), dict(x=P + 8), dict(out=P + 8), dict(res=P + 8), dict(buf=P + 8),
                dict(ids=P + 2), dict(w=P + 2)):
         assert call(**kw) == arg, kw
     need = L.cascadia_int4_fp8_moe_workspace_bytes
-    lay = Layer(256, 128, 16, P, P, P, P)
+    lay = Layer(256, 128, 16, P, P, P, P, 1)
     sizes = [need(C.byref(lay), 4, t) for t in range(1, 600)]
     assert sizes == sorted(sizes) and sizes[0] > 0
     assert need(C.byref(lay), 0, 4) == 0
+
+
+def test_tile_refusals(cl):
+    L, arg, nul = cl.lib(), cl._lib.ERR_ARG, cl._lib.ERR_NULL
+    f = L.cascadia_int4_fp8_tile_weights
+    assert f(1, 4, 32, None, P, None) == nul and f(1, 4, 32, P, None, None) == nul
+    for a in ((0, 4, 32, P, P), (1, 0, 32, P, P), (1, 4, 40, P, P), (1, 4, 32, P + 8, P),
+              (1, 4, 32, P, P + 8), ((1 << 20) + 1, 4, 32, P, P), (1 << 20, 1 << 20, 1 << 14, P, P)):
+        assert f(*a, None) == arg
+    b = L.cascadia_int4_fp8_tiled_bytes
+    assert b(1, 16) == 128 * 128 and b(129, 272) == 2 * 3 * 128 * 128 and b(4, 40) == 0
 
 
 def test_host_tensors_are_refused(cl):

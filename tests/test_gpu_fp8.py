@@ -429,10 +429,10 @@ def moe_ref(case, threshold, residual):
     return out, bound
 
 
-def run_moe(cl, case, out_dtype, threshold, residual, workspace=None):
+def run_moe(cl, case, out_dtype, threshold, residual, workspace=None, tiled=True):
     gu, gus, dn, dns, x, ids, w, _ = case
     E, _, I, H = gu.shape
-    ex = cl.Fp8Experts(gu.cuda(), gus.cuda(), dn.cuda(), dns.cuda(), E, H, I)
+    ex = cl.Fp8Experts(gu.cuda(), gus.cuda(), dn.cuda(), dns.cuda(), E, H, I, tiled=tiled)
     out = torch.full(x.shape, float("nan"), dtype=out_dtype, device="cuda")
     cl.fp8_moe_forward(ex, x.cuda(), out, top_k=ids.shape[1], ids=ids.cuda(), weights=w.cuda(),
                        threshold=threshold, workspace=workspace,
@@ -461,6 +461,30 @@ def check_moe(cl, case, out_dtype=torch.bfloat16, threshold=0.0, residual=True):
 def test_moe(cl, T, H, I, E, k, x_dtype):
     case = moe_case(T + H + I, T, H, I, E, k, x_dtype)
     check_moe(cl, case, torch.float32 if (T + k) % 2 else torch.bfloat16, residual=T % 3 != 0)
+
+
+@pytest.mark.parametrize("T,H,I,E,k", [(1, 400, 272, 5, 3), (9, 144, 1040, 4, 2),
+                                       (90, 272, 400, 3, 2), (300, 128, 16, 2, 1)])
+def test_moe_tiled_codes_are_the_same_codes(cl, T, H, I, E, k):
+    case = moe_case(T, T, H, I, E, k, torch.bfloat16)
+    a, b = (run_moe(cl, case, torch.float32, 0.0, None, tiled=t) for t in (True, False))
+    assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("count,n,k", [(1, 1, 16), (3, 128, 128), (2, 130, 272), (5, 300, 144)])
+def test_tile_weights(cl, count, n, k):
+    w = codes(gen(n), count, n, k).view(torch.uint8).cuda()
+    L = cl.lib()
+    per = L.cascadia_int4_fp8_tiled_bytes(n, k)
+    nb, kb = ref.blocks(n), ref.blocks(k)
+    assert per == nb * kb * 128 * 128
+    out = torch.full((count * per + 64,), 7, dtype=torch.uint8, device="cuda")
+    cl.check("tile", L.cascadia_int4_fp8_tile_weights(count, n, k, w.data_ptr(), out.data_ptr(),
+                                                      torch.cuda.current_stream().cuda_stream))
+    want = torch.zeros((count, nb * 128, kb * 128), dtype=torch.uint8)
+    want[:, :n, :k] = w.cpu()
+    want = want.view(count, nb, 128, kb, 128).permute(0, 1, 3, 2, 4).reshape(-1)
+    assert torch.equal(out[:-64].cpu(), want) and torch.all(out[-64:] == 7)
 
 
 def test_moe_one_expert_takes_every_token(cl):
@@ -552,7 +576,7 @@ def load_layer(cl, H, I, E, w1, w2):
         for j in (0, 1):
             gu[e, j], gus[e, j] = cl.quantize_fp8_blocks(w1[e, j].cuda(), I, H)
         dn[e], dns[e] = cl.quantize_fp8_blocks(w2[e].cuda(), H, I)
-    return cl.Fp8Experts(gu, gus, dn, dns, E, H, I)
+    return (gu, gus, dn, dns), cl.Fp8Experts(gu, gus, dn, dns, E, H, I)
 
 
 class Layer:
@@ -563,7 +587,7 @@ class Layer:
         (self.H, self.I, self.E, self.k, gate, self.bias, w1, w2, x) = layer_case(T, seed)
         self.x = x.cuda()
         self.gate, self.gate_s = cl.quantize_fp8_blocks(gate.cuda(), self.E, self.H)
-        self.ex = load_layer(cl, self.H, self.I, self.E, w1, w2)
+        self.given, self.ex = load_layer(cl, self.H, self.I, self.E, w1, w2)
         self.bias = self.bias.cuda()
         self.logits = torch.empty((T, self.E), device="cuda")
         self.ids = torch.empty((T, self.k), dtype=torch.int32, device="cuda")
@@ -596,10 +620,9 @@ def test_layer_from_router_to_experts(cl, T):
     ids, w = ref.route(L.logits.double().cpu().numpy(), L.k, "sigmoid",
                        L.bias.double().cpu().numpy(), 4, 2, 2, True, 2.5)
     assert np.array_equal(L.ids.cpu().numpy(), ids)
-    ex = L.ex
-    want, bound = ref.moe(L.x.double().cpu().numpy(), ref.e4m3(ex.gate_up),
-                          ex.gate_up_scales.double().cpu().numpy(), ref.e4m3(ex.down),
-                          ex.down_scales.double().cpu().numpy(), ids,
+    gu, gus, dn, dns = L.given
+    want, bound = ref.moe(L.x.double().cpu().numpy(), ref.e4m3(gu), gus.double().cpu().numpy(),
+                          ref.e4m3(dn), dns.double().cpu().numpy(), ids,
                           L.w.double().cpu().numpy(), 0.0, L.x.double().cpu().numpy())
     bound = bound + ref.BF16 * (np.abs(want) + bound)
     assert np.all(np.abs(out - want) <= bound)
