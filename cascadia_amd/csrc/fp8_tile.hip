@@ -247,6 +247,17 @@ __global__ __launch_bounds__(64 * WN * WM) void fp8_tile_kernel(Fp8Gemm g, int n
   constexpr int LAG = 3;  // MFMAs between one and the use of its result
   f32x4_t p[LAG + 1];
   uint32_t base = 0, last = (S - 1) * P::STAGE;  // stages of this block, of the one before
+  // a wave without tokens only loads and waits with the others
+  if (wm * NJ * 16 >= rows.count) {
+    for (int kb = first; kb < end; ++kb) {
+      const bool even = cut(kb + S - 1, 0), odd = cut(kb + S - 1, 1);
+#pragma unroll
+      for (int q = 0; q < P::LOADS; ++q) load1(q, kb + S - 1, lds0 + last, even, odd);
+      dma_wait_barrier<(S - 2) * P::LOADS>();
+      last = base;
+      base = base + P::STAGE == S * P::STAGE ? 0 : base + P::STAGE;
+    }
+  } else
   for (int kb = first; kb < end; ++kb) {
     const uint32_t next = base + P::STAGE == S * P::STAGE ? 0 : base + P::STAGE;
     const bool even = cut(kb + S - 1, 0), odd = cut(kb + S - 1, 1);
@@ -277,7 +288,7 @@ __global__ __launch_bounds__(64 * WN * WM) void fp8_tile_kernel(Fp8Gemm g, int n
         __builtin_amdgcn_sched_barrier(0);
         if (slot >= LAG) add(slot - LAG);
         // the stage of the block before takes the loads of S - 1 blocks ahead, PER a pass
-        constexpr int PER = (NI - 1) >= P::LOADS ? 1 : 2;
+        constexpr int PER = NI - 1 >= P::LOADS ? 1 : 2;
         static_assert(PER * (NI - 1) >= P::LOADS && NJ % PER == 0, "loads");
         if (j % (NJ / PER) == 0 && i + 1 < NI && i * PER + j / (NJ / PER) < P::LOADS)
           load1(i * PER + j / (NJ / PER), kb + S - 1, lds0 + last, even, odd);
