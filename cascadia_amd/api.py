@@ -1032,6 +1032,7 @@ def route_experts(logits, top_k: int, ids, weights, *, score: int = SCORE_SIGMOI
     their sum when normalize, times scale.  A NaN logit counts as -infinity; a
     softmax over -infinity alone gives weights of 0."""
     dev = _home(logits, "logits")
+    top_k = _index(top_k)
     _here(dev, ids, "ids")
     _here(dev, weights, "weights")
     bf16 = logits.dtype is torch.bfloat16
@@ -1065,6 +1066,7 @@ def quantize_fp8(x, rows: int, k_cols: int, codes, scales):
     ceil(k_cols / 128)]): scale = max(max|x|, 2^-96) / 448, code = e4m3(x /
     scale), to nearest even.  k_cols: a multiple of 16."""
     dev = _home(x, "x")
+    rows, k_cols = _index(rows), _index(k_cols)
     _here(dev, codes, "codes")
     _here(dev, scales, "scales")
     _expect(k_cols >= 16 and k_cols % 16 == 0, f"k_cols {k_cols} must be a multiple of 16")
@@ -1084,6 +1086,7 @@ def quantize_fp8_blocks(weight_bf16, n_rows: int, k_cols: int):
     (codes float8_e4m3fn [n_rows, k_cols], scales f32 [ceil(n_rows / 128),
     ceil(k_cols / 128)]), a scale per block of 128 x 128 as quantize_fp8's."""
     _home(weight_bf16, "weight_bf16")
+    n_rows, k_cols = _index(n_rows), _index(k_cols)
     _expect(n_rows >= 1 and k_cols >= 16 and k_cols % 16 == 0,
             f"k_cols {k_cols} must be a multiple of 16")
     _expect(_is_bf16_bits(weight_bf16) and weight_bf16.numel() == n_rows * k_cols,
@@ -1122,6 +1125,7 @@ def fp8_gemm(codes, scales, xs, n_rows: int, k_cols: int, seq: int, ys, x_scales
     [seq, ceil(k_cols / 128)].  ys [seq, n_rows] bf16 or f32; f32 sums, one
     rounding.  workspace: fp8_gemm_workspace_bytes (for a graph capture)."""
     dev = _home(codes, "codes")
+    n_rows, k_cols, seq = _index(n_rows), _index(k_cols), _index(seq)
     _fp8_matrix(dev, codes, scales, 1, n_rows, k_cols, "codes")
     _here(dev, xs, "xs")
     _here(dev, ys, "ys")
@@ -1178,6 +1182,7 @@ class Fp8Experts:
                  inter: int, tiled: bool = True):
         _expect(1 <= n_experts <= 1024, "n_experts: 1 to 1024")
         dev = _home(gate_up, "gate_up")
+        n_experts, hidden, inter = _index(n_experts), _index(hidden), _index(inter)
         _fp8_matrix(dev, gate_up, gate_up_scales, 2 * n_experts, inter, hidden, "gate_up")
         _fp8_matrix(dev, down, down_scales, n_experts, hidden, inter, "down")
         if tiled:
@@ -1210,14 +1215,14 @@ def fp8_moe_forward(experts: Fp8Experts, x, out, *, top_k: int, ids, weights,
     rounding.  x f32 or bf16, out f32 or bf16 (residual of out's type), all
     [n_tokens, hidden]; ids (int32) / weights (f32) [n_tokens, top_k], as
     route_experts gives them.  Slots with a weight below threshold or an id
-    outside the layer (padding: -1) are left out.  workspace:
-    fp8_moe_workspace_bytes (for a graph capture)."""
+    outside the layer (padding: -1) are left out.  out may be residual or x.
+    workspace: fp8_moe_workspace_bytes (for a graph capture)."""
     dev = _home(x, "x")
     _here(dev, out, "out")
     _here(dev, ids, "ids")
     _here(dev, weights, "weights")
     _here(dev, experts.gate_up, "experts")
-    H = experts.hidden
+    H, top_k = experts.hidden, _index(top_k)
     x_f32, out_f32 = x.dtype is torch.float32, out.dtype is torch.float32
     _expect((x_f32 or x.dtype is torch.bfloat16) and (out_f32 or out.dtype is torch.bfloat16),
             "x and out must be f32 or bf16")

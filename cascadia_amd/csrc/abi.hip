@@ -2349,6 +2349,11 @@ bool fp8_dims_ok(uint32_t n_rows, uint32_t k_cols) {
          k_cols % 16 == 0;
 }
 
+// Rows whose groups one launch takes.
+bool fp8_rows_ok(uint32_t rows, uint32_t k_cols) {
+  return (size_t)rows * cai4::fp8_blocks((int)k_cols) <= (size_t)1 << 34;
+}
+
 // A call's workspace: scales in rows of fp8_ld, then, of rows that it quantises,
 // their codes, then the partial sums of a split K.
 struct Fp8Workspace {
@@ -2418,7 +2423,9 @@ int cascadia_int4_route_experts(const cascadia_int4_router *R, const void *logit
 
 int cascadia_int4_fp8_quantize(const void *x, uint32_t x_is_f32, uint32_t rows, uint32_t k_cols,
                                uint8_t *codes, float *scales, void *stream) {
-  if (!fp8_dims_ok(1, k_cols) || rows > kFp8MaxRows || x_is_f32 > 1) return CASCADIA_INT4_ERR_ARG;
+  if (!fp8_dims_ok(1, k_cols) || rows > kFp8MaxRows || x_is_f32 > 1 ||
+      !fp8_rows_ok(rows, k_cols))
+    return CASCADIA_INT4_ERR_ARG;
   if (rows == 0) return CASCADIA_INT4_OK;
   if (!x || !codes || !scales) return CASCADIA_INT4_ERR_NULL;
   if (!aligned(x, 16) || !aligned(codes, 16) || !aligned(scales, 4)) return CASCADIA_INT4_ERR_ARG;
@@ -2439,7 +2446,7 @@ int cascadia_int4_fp8_quantize_blocks(const uint16_t *w_bf16, uint32_t n_rows, u
 size_t cascadia_int4_fp8_gemm_workspace_bytes(uint32_t n_rows, uint32_t k_cols, uint32_t x_type,
                                               uint32_t seq) {
   if (!fp8_dims_ok(n_rows, k_cols) || seq == 0 || seq > kFp8MaxRows ||
-      x_type > CASCADIA_INT4_FP8_X_E4M3)
+      x_type > CASCADIA_INT4_FP8_X_E4M3 || !fp8_rows_ok(seq, k_cols))
     return 0;
   return fp8_workspace(n_rows, k_cols, x_type, seq).total;
 }
@@ -2452,7 +2459,8 @@ int cascadia_int4_fp8_gemm(uint32_t n_rows, uint32_t k_cols, const uint8_t *w,
   const bool codes = x_type == CASCADIA_INT4_FP8_X_E4M3;
   if (codes && !x_scales) return CASCADIA_INT4_ERR_NULL;
   if (!fp8_dims_ok(n_rows, k_cols) || seq == 0 || seq > kFp8MaxRows ||
-      x_type > CASCADIA_INT4_FP8_X_E4M3 || (!codes && x_scales) || y_is_f32 > 1)
+      x_type > CASCADIA_INT4_FP8_X_E4M3 || (!codes && x_scales) || y_is_f32 > 1 ||
+      !fp8_rows_ok(seq, k_cols))
     return CASCADIA_INT4_ERR_ARG;
   if (!aligned(w, 16) || !aligned(w_scales, 4) || !aligned(xs, 16) || !aligned(x_scales, 4) ||
       !aligned(ys, y_is_f32 ? 4 : 2) || !aligned(workspace, 16))
@@ -2480,7 +2488,7 @@ int cascadia_int4_fp8_gemm(uint32_t n_rows, uint32_t k_cols, const uint8_t *w,
   g.M = (int)seq;
   g.out_f32 = (int)y_is_f32;
   g.ld_xs = blocks;
-  g.part = reinterpret_cast<float *>(static_cast<uint8_t *>(workspace) + need.part);
+  if (use) g.part = reinterpret_cast<float *>(static_cast<uint8_t *>(workspace) + need.part);
   if (one)
     return hip_status(cai4::fp8_gemv(g, xs, x_type == CASCADIA_INT4_FP8_X_F32, st));
   if (!codes || pad) {

@@ -532,9 +532,9 @@ typedef struct cascadia_int4_fp8_moe_layer {
  * gives them: a slot with weight < threshold or an id outside the layer is left
  * out (padding: -1).  A shared expert is an expert of the stack that every
  * token lists.  x [n_tokens, hidden] f32 (x_is_f32) or bf16; out f32
- * (out_is_f32) or bf16, residual of out's type or NULL.  x, residual and out
- * 16-byte aligned; top_k <= 16; 1 <= n_tokens <= 2^20, n_tokens * hidden < 2^31.
- * workspace as above. */
+ * (out_is_f32) or bf16, residual of out's type or NULL (out may be either).  x,
+ * residual and out 16-byte aligned; top_k <= 16; 1 <= n_tokens <= 2^20,
+ * n_tokens * hidden < 2^31.  workspace as above. */
 size_t cascadia_int4_fp8_moe_workspace_bytes(const cascadia_int4_fp8_moe_layer *layer,
                                              uint32_t top_k, uint32_t n_tokens);
 int cascadia_int4_fp8_moe_forward(const cascadia_int4_fp8_moe_layer *layer, uint32_t top_k,

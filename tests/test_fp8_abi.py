@@ -70,7 +70,8 @@ def test_gemm_refusals(cl):
     for kw in (dict(n=0), dict(k=0), dict(k=72), dict(seq=0), dict(xt=3), dict(xt=0), dict(f32=2),
                dict(w=P + 8), dict(x=P + 4), dict(ws=P + 2), dict(xs=P + 2), dict(y=P + 2),
                dict(y=P + 1, f32=0), dict(buf=P + 8), dict(n=(1 << 24) + 1),
-               dict(k=(1 << 20) + 16), dict(seq=(1 << 24) + 1)):
+               dict(k=(1 << 20) + 16), dict(seq=(1 << 24) + 1),
+               dict(seq=1 << 24, k=1 << 20)):
         assert call(**kw) == arg, kw
     need = L.cascadia_int4_fp8_gemm_workspace_bytes
     for a in ((0, 64, 0, 4), (32, 72, 0, 4), (32, 64, 3, 4), (32, 64, 0, 0)):
@@ -78,8 +79,9 @@ def test_gemm_refusals(cl):
     assert need(32, 64, 0, 4) >= 4 * 64 + 4 * 4
     # one workspace of the largest call serves every smaller one
     for x_type in (0, 1, 2):
-        sizes = [need(4096, 4096, x_type, m) for m in range(1, 600)]
-        assert sizes == sorted(sizes)
+        for n, k in ((4096, 4096), (576, 7168), (100, 20496), (14336, 4096)):
+            sizes = [need(n, k, x_type, m) for m in range(1, 600)]
+            assert sizes == sorted(sizes)
 
 
 def test_moe_refusals(cl):

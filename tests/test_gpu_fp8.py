@@ -315,6 +315,31 @@ def test_gemm(cl, m, n, k, kind):
     check_gemm(cl, w, ws, x, xs, torch.float32 if (m + n) % 2 else torch.bfloat16)
 
 
+@pytest.mark.parametrize("m,n,k", [(1, 32, 17408), (2, 40, 33040), (20, 16, 20496), (70, 24, 33040)])
+@pytest.mark.parametrize("kind", ["fp8", "bf16"])
+def test_gemm_long_rows(cl, m, n, k, kind):
+    """More blocks than the few-row kernels hold scales for at once."""
+    w, ws, x, xs = gemm_case(m + k, m, n, k, kind)
+    check_gemm(cl, w, ws, x, xs, torch.float32)
+
+
+@pytest.mark.parametrize("m,n,k", [(3500, 3600, 272), (1700, 3600, 400), (1000, 1100, 144)])
+@pytest.mark.parametrize("y_dtype", [torch.float32, torch.bfloat16])
+def test_gemm_many_tiles(cl, m, n, k, y_dtype):
+    """Ragged products on the larger tiles: every output written, the rows at the
+    tiles' edges and some between against the reference."""
+    w, ws, x, xs = gemm_case(m, m, n, k, "fp8")
+    y = torch.full((m, n), float("nan"), dtype=y_dtype, device="cuda")
+    cl.fp8_gemm(w.cuda(), ws.cuda(), x.cuda(), n, k, m, y, x_scales=xs.cuda())
+    assert torch.isfinite(y).all()
+    rows = sorted({0, 1, 127, 128, 255, 256, m // 2, m - 2, m - 1, *range(77, m, 997)})
+    want, bound = gemm_ref(w, ws, x[rows], xs[rows])
+    if y_dtype == torch.bfloat16:
+        bound = bound + eight_bit(w, ws, x[rows], xs[rows])
+        bound = bound + ref.BF16 * (np.abs(want) + bound)
+    assert np.all(np.abs(y[rows].double().cpu().numpy() - want) <= bound)
+
+
 @pytest.mark.parametrize("y_dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("m", [1, 4, 20, 70, 300])
 def test_gemm_scales_belong_to_their_blocks(cl, m, y_dtype):
@@ -456,6 +481,7 @@ def check_moe(cl, case, out_dtype=torch.bfloat16, threshold=0.0, residual=True):
 @pytest.mark.parametrize("T,H,I,E,k", [
     (1, 256, 128, 8, 2), (1, 16, 16, 1, 1), (1, 1040, 400, 16, 8), (2, 144, 272, 4, 4),
     (3, 512, 96, 5, 3), (17, 256, 256, 3, 2), (40, 128, 144, 2, 1), (33, 272, 128, 64, 16),
+    (1, 64, 144, 20, 16), (1, 32, 4096, 16, 16), (120, 16, 16, 700, 8), (200, 32, 16, 700, 8),
     (70, 256, 160, 2, 2), (150, 144, 128, 3, 2), (400, 128, 272, 5, 4), (600, 64, 48, 3, 2)])
 @pytest.mark.parametrize("x_dtype", [torch.float32, torch.bfloat16])
 def test_moe(cl, T, H, I, E, k, x_dtype):
@@ -524,6 +550,46 @@ def test_moe_nan_stays_in_its_token(cl, T):
     out = run_moe(cl, case, torch.float32, 0.0, None).cpu()
     bad = torch.isnan(out).any(1)
     assert bad[T // 2] and int(bad.sum()) == 1
+
+
+@pytest.mark.parametrize("T", [1, 20, 200])
+def test_moe_in_place(cl, T):
+    """out is the residual, or x itself."""
+    case = moe_case(7, T, 144, 128, 4, 2, torch.bfloat16)
+    gu, gus, dn, dns, x, ids, w, res = (t.cuda() for t in case)
+    ex = cl.Fp8Experts(gu, gus, dn, dns, 4, 144, 128)
+    kw = dict(top_k=2, ids=ids, weights=w)
+    res = res.to(torch.bfloat16)
+    want = cl.fp8_moe_forward(ex, x, torch.empty_like(x), residual=res, **kw)
+    a = res.clone()
+    assert torch.equal(cl.fp8_moe_forward(ex, x, a, residual=a, **kw), want)
+    want = cl.fp8_moe_forward(ex, x, torch.empty_like(x), residual=x, **kw)
+    b = x.clone()
+    assert torch.equal(cl.fp8_moe_forward(ex, b, b, residual=b, **kw), want)
+
+
+def test_one_workspace_serves_smaller_calls(cl):
+    """A workspace of the largest batch, for every smaller one."""
+    n, k = 320, 1040
+    w, ws, x, xs = (t.cuda() for t in gemm_case(8, 400, n, k, "fp8"))
+    for kind, scales_of in ((x, xs), (x.float(), None)):
+        buf = torch.empty(cl.fp8_gemm_workspace_bytes(n, k, 400, kind.dtype), dtype=torch.uint8,
+                          device="cuda")
+        for m in (400, 300, 129, 65, 64, 33, 17, 2, 1):
+            sc = None if scales_of is None else scales_of[:m]
+            a, b = (torch.empty((m, n), device="cuda") for _ in range(2))
+            cl.fp8_gemm(w, ws, kind[:m], n, k, m, a, x_scales=sc, workspace=buf)
+            cl.fp8_gemm(w, ws, kind[:m], n, k, m, b, x_scales=sc)
+            assert torch.equal(a, b)
+    gu, gus, dn, dns, x, ids, wt, _ = (t.cuda() for t in moe_case(8, 200, 144, 400, 6, 2, torch.float32))
+    ex = cl.Fp8Experts(gu, gus, dn, dns, 6, 144, 400)
+    buf = torch.empty(cl.fp8_moe_workspace_bytes(ex, 2, 200), dtype=torch.uint8, device="cuda")
+    for t in (200, 100, 48, 47, 20, 2, 1):
+        a, b = (torch.empty((t, 144), device="cuda") for _ in range(2))
+        kw = dict(top_k=2, ids=ids[:t], weights=wt[:t])
+        cl.fp8_moe_forward(ex, x[:t], a, workspace=buf, **kw)
+        cl.fp8_moe_forward(ex, x[:t], b, **kw)
+        assert torch.equal(a, b)
 
 
 @pytest.mark.parametrize("T", [1, 30, 200])
