@@ -88,7 +88,7 @@ struct Tile {
 };
 
 // A workgroup's place: m tile (or chunk) and n tile.  Workgroups go round the
-// // eight XCDs; each takes a run of neighbouring tiles, so that those that run
+// eight XCDs; each takes a run of neighbouring tiles, so that those that run
 // together share rows of both operands in its L2.  One matrix: groups of 4 m
 // tiles, n outside, m inside (32 workgroups: 4 x 8 tiles).  Experts, one after
 // the other: n outside, the expert's chunks inside.

@@ -953,6 +953,197 @@ inline void moe_forward(const MoeLayer &layer, const Routing &routing,
   detail::finish(call);
 }
 
+// ---- routing to experts, and products in 8-bit floating point ----
+//
+// No counterpart in the crate: cascadia_int4.h states what each computes.
+// Options supply the stream, the synchronisation and the workspace.
+
+using Router = cascadia_int4_router;  // (bias: device memory or NULL)
+
+// ids / weights [n_tokens, router.top_k] from logits [n_tokens, n_experts], f32 or
+// bf16 bits.
+namespace detail {
+inline void route(const Router &router, const void *logits, bool bf16, size_t len,
+                  DeviceSlice<int32_t> ids, DeviceSlice<float> weights, const Options &call) {
+  require(router.n_experts > 0 && len % router.n_experts == 0, "logits: n_tokens x n_experts");
+  const size_t t = len / router.n_experts;
+  require(t <= UINT32_MAX && ids.len == t * router.top_k && weights.len == ids.len,
+          "ids and weights: n_tokens x top_k");
+  check(cascadia_int4_route_experts(&router, logits, bf16, (uint32_t)t, ids.data, weights.data,
+                                    call.stream),
+        "cascadia_int4_route_experts");
+  finish(call);
+}
+inline size_t fp8_blocks(size_t n) { return (n + 127) / 128; }
+}  // namespace detail
+inline void route_experts(const Router &router, DeviceSlice<const float> logits,
+                          DeviceSlice<int32_t> ids, DeviceSlice<float> weights,
+                          const Options &call = {}) {
+  detail::route(router, logits.data, false, logits.len, ids, weights, call);
+}
+inline void route_experts(const Router &router, DeviceSlice<const uint16_t> logits_bf16,
+                          DeviceSlice<int32_t> ids, DeviceSlice<float> weights,
+                          const Options &call = {}) {
+  detail::route(router, logits_bf16.data, true, logits_bf16.len, ids, weights, call);
+}
+
+// Rows of x as a product takes them: f32, bf16 bits, or e4m3 codes with a scale per
+// 128 columns.
+struct Fp8Rows {
+  const void *data;
+  size_t len;
+  uint32_t type;
+  DeviceSlice<const float> scales;
+  Fp8Rows(DeviceSlice<const float> x) : data(x.data), len(x.len), type(CASCADIA_INT4_FP8_X_F32) {}
+  Fp8Rows(DeviceSlice<const uint16_t> x_bf16)
+      : data(x_bf16.data), len(x_bf16.len), type(CASCADIA_INT4_FP8_X_BF16) {}
+  Fp8Rows(DeviceSlice<const uint8_t> codes, DeviceSlice<const float> scales)
+      : data(codes.data), len(codes.len), type(CASCADIA_INT4_FP8_X_E4M3), scales(scales) {}
+};
+
+// Rows of x (f32 or bf16) as e4m3 codes [rows, k_cols], scales [rows, ceil(k_cols / 128)].
+inline void quantize_fp8(const Fp8Rows &x, size_t rows, size_t k_cols, DeviceSlice<uint8_t> codes,
+                         DeviceSlice<float> scales, const Options &call = {}) {
+  detail::require(x.type != CASCADIA_INT4_FP8_X_E4M3, "x is f32 or bf16");
+  detail::require(rows <= UINT32_MAX && k_cols <= UINT32_MAX && x.len == rows * k_cols &&
+                      codes.len == x.len && scales.len == rows * detail::fp8_blocks(k_cols),
+                  "x and codes: rows x k_cols, scales: rows x ceil(k_cols / 128)");
+  detail::check(cascadia_int4_fp8_quantize(x.data, x.type == CASCADIA_INT4_FP8_X_F32,
+                                           (uint32_t)rows, (uint32_t)k_cols, codes.data,
+                                           scales.data, call.stream),
+                "cascadia_int4_fp8_quantize");
+  detail::finish(call);
+}
+
+// bf16 weights [n_rows, k_cols] as (codes, scales of blocks of 128 x 128).
+inline std::pair<DeviceBuffer<uint8_t>, DeviceBuffer<float>> quantize_fp8_blocks(
+    DeviceSlice<const uint16_t> weight_bf16, size_t n_rows, size_t k_cols,
+    const Options &call = {}) {
+  detail::require(n_rows <= UINT32_MAX && k_cols <= UINT32_MAX &&
+                      weight_bf16.len == n_rows * k_cols,
+                  "weight_bf16: n_rows x k_cols");
+  std::pair<DeviceBuffer<uint8_t>, DeviceBuffer<float>> out{
+      DeviceBuffer<uint8_t>(n_rows * k_cols),
+      DeviceBuffer<float>(detail::fp8_blocks(n_rows) * detail::fp8_blocks(k_cols))};
+  detail::check(cascadia_int4_fp8_quantize_blocks(weight_bf16.data, (uint32_t)n_rows,
+                                                  (uint32_t)k_cols, out.first.data(),
+                                                  out.second.data(), call.stream),
+                "cascadia_int4_fp8_quantize_blocks");
+  detail::finish(call);
+  return out;
+}
+
+// ys[t, r] = sum over blocks of x_scale w_scale sum x w: ys f32 or bf16 [seq, n_rows].
+namespace detail {
+inline void fp8_gemm(DeviceSlice<const uint8_t> codes, DeviceSlice<const float> scales,
+                     const Fp8Rows &xs, size_t n_rows, size_t k_cols, size_t seq, void *ys,
+                     size_t ys_len, bool ys_f32, const Options &call) {
+  require(n_rows <= UINT32_MAX && k_cols <= UINT32_MAX && seq <= UINT32_MAX &&
+              codes.len == n_rows * k_cols &&
+              scales.len == fp8_blocks(n_rows) * fp8_blocks(k_cols),
+          "codes: n_rows x k_cols, scales: one per block of 128 x 128");
+  require(xs.len == seq * k_cols && ys_len == seq * n_rows &&
+              (xs.type != CASCADIA_INT4_FP8_X_E4M3 ||
+               xs.scales.len == seq * fp8_blocks(k_cols)),
+          "xs: seq x k_cols (codes: with seq x ceil(k_cols / 128) scales), ys: seq x n_rows");
+  check(cascadia_int4_fp8_gemm((uint32_t)n_rows, (uint32_t)k_cols, codes.data, scales.data,
+                               xs.data, xs.type, xs.scales.data, (uint32_t)seq, ys, ys_f32,
+                               call.workspace, call.stream),
+        "cascadia_int4_fp8_gemm");
+  finish(call);
+}
+}  // namespace detail
+inline void fp8_gemm(DeviceSlice<const uint8_t> codes, DeviceSlice<const float> scales,
+                     const Fp8Rows &xs, size_t n_rows, size_t k_cols, size_t seq,
+                     DeviceSlice<float> ys, const Options &call = {}) {
+  detail::fp8_gemm(codes, scales, xs, n_rows, k_cols, seq, ys.data, ys.len, true, call);
+}
+inline void fp8_gemm(DeviceSlice<const uint8_t> codes, DeviceSlice<const float> scales,
+                     const Fp8Rows &xs, size_t n_rows, size_t k_cols, size_t seq,
+                     DeviceSlice<uint16_t> ys_bf16, const Options &call = {}) {
+  detail::fp8_gemm(codes, scales, xs, n_rows, k_cols, seq, ys_bf16.data, ys_bf16.len, false, call);
+}
+
+// One MoE layer's experts in e4m3: owns a copy of the codes in blocks, refers to
+// the scales.
+class Fp8Experts {
+ public:
+  Fp8Experts(DeviceSlice<const uint8_t> gate_up, DeviceSlice<const float> gate_up_scales,
+             DeviceSlice<const uint8_t> down, DeviceSlice<const float> down_scales,
+             size_t n_experts, size_t hidden, size_t intermediate, const Options &call = {}) {
+    const size_t e = n_experts, h = hidden, i = intermediate;
+    const size_t blocks = detail::fp8_blocks(h) * detail::fp8_blocks(i);
+    detail::require(e >= 1 && e <= 1024 && h <= UINT32_MAX && i <= UINT32_MAX, "1 to 1024 experts");
+    detail::require(gate_up.len == 2 * e * i * h && down.len == e * h * i &&
+                        gate_up_scales.len == 2 * e * blocks && down_scales.len == e * blocks,
+                    "gate_up: n_experts x 2 x intermediate x hidden, down: n_experts x hidden x "
+                    "intermediate, a scale per block of 128 x 128");
+    const size_t u = cascadia_int4_fp8_tiled_bytes((uint32_t)i, (uint32_t)h);
+    const size_t d = cascadia_int4_fp8_tiled_bytes((uint32_t)h, (uint32_t)i);
+    detail::require(u > 0 && d > 0, "unsupported expert dims");
+    gate_up_ = DeviceBuffer<uint8_t>(2 * e * u);
+    down_ = DeviceBuffer<uint8_t>(e * d);
+    detail::check(cascadia_int4_fp8_tile_weights((uint32_t)(2 * e), (uint32_t)i, (uint32_t)h,
+                                                 gate_up.data, gate_up_.data(), call.stream),
+                  "cascadia_int4_fp8_tile_weights");
+    detail::check(cascadia_int4_fp8_tile_weights((uint32_t)e, (uint32_t)h, (uint32_t)i, down.data,
+                                                 down_.data(), call.stream),
+                  "cascadia_int4_fp8_tile_weights");
+    detail::finish(call);
+    l_ = {(uint32_t)h, (uint32_t)i, (uint32_t)e, gate_up_.data(), gate_up_scales.data,
+          down_.data(), down_scales.data, 1u};
+  }
+  size_t hidden() const { return l_.hidden; }
+  const cascadia_int4_fp8_moe_layer &c_layer() const { return l_; }
+  size_t workspace_bytes(size_t top_k, size_t n_tokens) const {
+    return cascadia_int4_fp8_moe_workspace_bytes(&l_, (uint32_t)top_k, (uint32_t)n_tokens);
+  }
+
+ private:
+  DeviceBuffer<uint8_t> gate_up_, down_;
+  cascadia_int4_fp8_moe_layer l_{};
+};
+
+// out = residual + the weighted sum of the chosen experts: x f32 or bf16, out and
+// residual (empty: zero) both f32 or both bf16, [n_tokens, hidden]; ids / weights
+// [n_tokens, top_k].
+namespace detail {
+inline void fp8_moe(const Fp8Experts &experts, const Fp8Rows &x, DeviceSlice<const int32_t> ids,
+                    DeviceSlice<const float> weights, size_t top_k, float threshold, void *out,
+                    size_t out_len, bool out_f32, const void *residual, size_t residual_len,
+                    const Options &call) {
+  const size_t h = experts.hidden(), t = x.len / h;
+  require(x.type != CASCADIA_INT4_FP8_X_E4M3, "x is f32 or bf16");
+  require(t > 0 && t <= UINT32_MAX && x.len == t * h && out_len == x.len &&
+              (!residual || residual_len == x.len),
+          "x, out and residual: n_tokens x hidden");
+  require(top_k <= UINT32_MAX && ids.len == t * top_k && weights.len == ids.len,
+          "ids and weights: n_tokens x top_k");
+  check(cascadia_int4_fp8_moe_forward(&experts.c_layer(), (uint32_t)top_k, ids.data, weights.data,
+                                      threshold, x.data, x.type == CASCADIA_INT4_FP8_X_F32,
+                                      residual, (uint32_t)t, out, out_f32, call.workspace,
+                                      call.stream),
+        "cascadia_int4_fp8_moe_forward");
+  finish(call);
+}
+}  // namespace detail
+inline void fp8_moe_forward(const Fp8Experts &experts, const Fp8Rows &x,
+                            DeviceSlice<const int32_t> ids, DeviceSlice<const float> weights,
+                            size_t top_k, DeviceSlice<float> out,
+                            DeviceSlice<const float> residual = {}, float threshold = 0.0f,
+                            const Options &call = {}) {
+  detail::fp8_moe(experts, x, ids, weights, top_k, threshold, out.data, out.len, true,
+                  residual.data, residual.len, call);
+}
+inline void fp8_moe_forward(const Fp8Experts &experts, const Fp8Rows &x,
+                            DeviceSlice<const int32_t> ids, DeviceSlice<const float> weights,
+                            size_t top_k, DeviceSlice<uint16_t> out_bf16,
+                            DeviceSlice<const uint16_t> residual_bf16 = {},
+                            float threshold = 0.0f, const Options &call = {}) {
+  detail::fp8_moe(experts, x, ids, weights, top_k, threshold, out_bf16.data, out_bf16.len, false,
+                  residual_bf16.data, residual_bf16.len, call);
+}
+
 // ---- the crate's C handle API (c_ffi.rs:35-341) as an owning object ----
 
 // A model directory (safetensors, or an int4_bin manifest with flat expert
