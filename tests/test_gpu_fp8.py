@@ -123,6 +123,17 @@ def test_route_infinities_and_nan(cl, score, groups, top_groups):
     check_route(cl, x, 6, score, normal(g, 48) * 0.1, groups, top_groups, 1, True, 2.0)
 
 
+def test_route_groups_whose_biases_cancel(cl):
+    """A group's best two, of opposite signs and far larger than their sum: added in
+    32 bits that sum would be off by 2^-24 of them, more than groups are apart."""
+    g = torch.Generator().manual_seed(18)
+    logits = torch.randn((512, 16), generator=g)
+    for big in (30.0, 1000.0, 65536.0):
+        bias = torch.tensor([big, -big] * 8)
+        check_route(cl, logits, 4, "sigmoid", bias, 8, 3, 2, True, 1.0)
+        check_route(cl, logits, 4, "softmax", bias, 8, 3, 2, True, 1.0)
+
+
 def test_route_nothing_and_refusals(cl):
     ids = torch.empty((0, 2), dtype=torch.int32, device="cuda")
     w = torch.empty((0, 2), device="cuda")
@@ -323,7 +334,8 @@ def test_gemm_long_rows(cl, m, n, k, kind):
     check_gemm(cl, w, ws, x, xs, torch.float32)
 
 
-@pytest.mark.parametrize("m,n,k", [(3500, 3600, 272), (1700, 3600, 400), (1000, 1100, 144)])
+@pytest.mark.parametrize("m,n,k", [(3500, 3600, 272), (1700, 3600, 400), (1000, 1100, 144),
+                                   (4100, 4200, 144), (2300, 8100, 272)])
 @pytest.mark.parametrize("y_dtype", [torch.float32, torch.bfloat16])
 def test_gemm_many_tiles(cl, m, n, k, y_dtype):
     """Ragged products on the larger tiles: every output written, the rows at the
