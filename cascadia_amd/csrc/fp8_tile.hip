@@ -110,7 +110,7 @@ CAI4_DEV Place place_of(const Fp8Gemm &g, int id, int mtiles, int ntiles) {
 }
 
 template <int NI, int NJ, int WN, int WM, bool SW, bool EXACT, int S>
-__global__ __launch_bounds__(64 * WN * WM) void fp8_tile_kernel(Fp8Gemm g, int ntiles) {
+__global__ __launch_bounds__(64 * WN * WM) void fp8_tile_kernel(Fp8Gemm g, int n_first, int ntiles) {
   using P = Tile<NI, NJ, WN, WM, SW, S>;
   __shared__ __attribute__((aligned(1024))) uint8_t st[P::BYTES];
   __shared__ float tops[SW ? WN : 1][SW ? P::BM : 1];
@@ -121,7 +121,7 @@ __global__ __launch_bounds__(64 * WN * WM) void fp8_tile_kernel(Fp8Gemm g, int n
                               : (g.M + P::BM - 1) / P::BM;
   const Place at = place_of(g, blockIdx.x, mtiles, ntiles);
   if (at.m < 0) return;  // the whole workgroup
-  const int n0 = at.n * P::OUT;
+  const int n0 = n_first + at.n * P::OUT;
   const Rows rows = rows_of(g, at.m, P::BM);
   const int KB = (g.K + 127) >> 7, NB = (g.N + 127) >> 7;
   // this workgroup's blocks: all, or slice blockIdx.y of g.kper (a multiple of 4)
@@ -396,15 +396,17 @@ __global__ __launch_bounds__(256) void fp8_slices_kernel(const float *part, size
   }
 }
 
+// Weight rows [n_first, n_first + count); count -1: all.
 template <int NI, int NJ, int WN, int WM, bool SW, bool EXACT, int S>
-hipError_t launch(const Fp8Gemm &g, hipStream_t st) {
+hipError_t launch(const Fp8Gemm &g, hipStream_t st, int n_first = 0, int count = -1) {
   using P = Tile<NI, NJ, WN, WM, SW, S>;
-  const int nt = (g.N + P::OUT - 1) / P::OUT;
+  const int nt = ((count < 0 ? g.N : count) + P::OUT - 1) / P::OUT;
   const int slices = g.kper ? (fp8_blocks(g.K) + g.kper - 1) / g.kper : 1;
   const size_t tiles = (size_t)nt * (g.chunks ? g.max_chunks : (g.M + P::BM - 1) / P::BM);
   if (tiles > 0x7FFFFFF0u) return hipErrorInvalidValue;
   hipLaunchKernelGGL((fp8_tile_kernel<NI, NJ, WN, WM, SW, EXACT, S>),
-                     dim3((unsigned)((tiles + 7) / 8 * 8), slices), dim3(64 * P::W), 0, st, g, nt);
+                     dim3((unsigned)((tiles + 7) / 8 * 8), slices), dim3(64 * P::W), 0, st, g,
+                     n_first, nt);
   if (slices > 1) {
     const size_t n = (size_t)g.M * g.N;
     const dim3 grid((unsigned)((n + 1023) / 1024));
@@ -425,12 +427,26 @@ int slice_blocks(int M, int N, int K) {
   return per < KB ? per : 0;
 }
 
+constexpr int kCUs = 256;
 enum Form { SMALL, MIDDLE, LARGE };  // 128 x 128, 256 x 128, 256 x 256
 // The largest tiles that still occupy three quarters of the CUs.
 Form form_of(int M, int N, bool out_f32) {
   const int n = (N + 255) / 256;
   if (!out_f32 && (int64_t)n * ((M + 255) / 256) >= 192) return LARGE;
   return (int64_t)n * fp8_blocks(M) >= 192 ? MIDDLE : SMALL;
+}
+
+// Weight rows whose tiles of 256 x bm would fill at most half of a last round over
+// the CUs: in tiles of half the size they fill twice as many, in a launch of their
+// own.  Measured, us, one launch / two: bf16 out, 256 x 256, K = 4096: N = M = 4096
+// and 256 rows more (272 tiles) 116 / 100, 12000 x 1500 (282) 115 / 101, 14336 x 4096
+// (896) 276 / 266; f32 out, 256 x 128: 4352 x 4096 (544) 187 / 179, 4096 x 2100 (272)
+// 120 / 108.  bf16 out on 256 x 128 tiles loses 4 % by it (72 / 75) and stays whole.
+int last_round(int M, int N, int bm) {
+  const int nt = (N + 255) / 256, mt = (M + bm - 1) / bm;
+  const int full = (int)((int64_t)nt * mt / kCUs * kCUs / mt);  // n tiles of whole rounds
+  if (full == 0 || full == nt || (int64_t)(nt - full) * mt > kCUs / 2) return 0;
+  return N - full * 256;
 }
 
 }  // namespace
@@ -451,13 +467,18 @@ hipError_t fp8_tile_gemm(const Fp8Gemm &g0, hipStream_t st) {
   g.kper = 0;
   if (g.swiglu) return launch<8, 2, 2, 4, true, false, 3>(g, st);
   if (g.chunks) return launch<8, 2, 2, 4, false, false, 3>(g, st);
-  switch (form_of(g.M, g.N, g.out_f32)) {
-    case LARGE: return launch<8, 4, 2, 4, false, false, 2>(g, st);
-    case MIDDLE:
-      // (exact: waves of 64 x 64 convert a fifth fewer codes than of 128 x 32)
-      if (g.out_f32) return launch<4, 4, 4, 2, false, true, 3>(g, st);
-      return launch<8, 2, 2, 4, false, false, 3>(g, st);
-    default: break;
+  const Form f = form_of(g.M, g.N, g.out_f32);
+  if (f == LARGE) {
+    const int left = last_round(g.M, g.N, 256), most = g.N - left;
+    const hipError_t e = launch<8, 4, 2, 4, false, false, 2>(g, st, 0, most);
+    return e != hipSuccess || !left ? e : launch<8, 2, 2, 4, false, false, 3>(g, st, most, left);
+  }
+  if (f == MIDDLE) {
+    if (!g.out_f32) return launch<8, 2, 2, 4, false, false, 3>(g, st);
+    // (exact: waves of 64 x 64 convert a fifth fewer codes than of 128 x 32)
+    const int left = last_round(g.M, g.N, 128), most = g.N - left;
+    const hipError_t e = launch<4, 4, 4, 2, false, true, 3>(g, st, 0, most);
+    return e != hipSuccess || !left ? e : launch<4, 2, 2, 4, false, true, 2>(g, st, most, left);
   }
   g.kper = slice_blocks(g.M, g.N, g.K);
   if (g.out_f32) return launch<4, 2, 2, 4, false, true, 2>(g, st);
