@@ -58,21 +58,23 @@ __global__ __launch_bounds__(256) void fp8_blocks_kernel(const uint16_t *w, int 
   if (threadIdx.x == 0) scales[(size_t)nb * KB + kb] = d.scale;
 }
 
-// A workgroup per block: half a row per thread.
+// A workgroup per block: 16 bytes per thread, eight threads to a row, 32 rows at a time.
 __global__ __launch_bounds__(256) void fp8_arrange_kernel(const uint8_t *codes, int N, int K, int NB,
-                                                       int KB, uint8_t *tiled) {
+                                                          int KB, uint8_t *tiled) {
   const size_t b = blockIdx.x, m = b / ((size_t)NB * KB);
   const int r = (int)(b - m * NB * KB), nb = r / KB, kb = r - nb * KB;
-  const int row = threadIdx.x >> 1, n = nb * kFp8Block + row;
-  const int half = (threadIdx.x & 1) * 64, col = kb * kFp8Block + half;
-  const uint8_t *from = codes + (m * N + n) * K + col;
-  uint8_t *to = tiled + b * kFp8BlockBytes + row * 128 + half;
+  const int row = threadIdx.x >> 3, at = (threadIdx.x & 7) * 16, col = kb * kFp8Block + at;
+  uint8_t *to = tiled + b * kFp8BlockBytes + at;
+  u32x4_t v[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    u32x4_t v = {0u, 0u, 0u, 0u};
-    if (n < N && col + 16 * i < K) v = *reinterpret_cast<const u32x4_t *>(from + 16 * i);
-    *reinterpret_cast<u32x4_t *>(to + 16 * i) = v;
+    const int n = nb * kFp8Block + row + 32 * i;
+    v[i] = u32x4_t{0u, 0u, 0u, 0u};
+    if (n < N && col < K)
+      v[i] = *reinterpret_cast<const u32x4_t *>(codes + (m * N + n) * K + col);
   }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) *reinterpret_cast<u32x4_t *>(to + (row + 32 * i) * 128) = v[i];
 }
 
 }  // namespace
