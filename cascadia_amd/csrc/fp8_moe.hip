@@ -36,6 +36,9 @@ int counters(size_t n) {
   return b < (size_t)kMaxCounters ? (int)b : kMaxCounters;
 }
 
+// Counts in rows of whole 16 bytes.
+__host__ __device__ inline int fp8_ld_experts(int E) { return (E + 3) & ~3; }
+
 struct Layout {
   size_t xq, xs, pos, row_map, chunks, counts, hist, h, hq, hs, y, total;
   int max_chunks, chunk_rows, counters;
@@ -61,7 +64,7 @@ Layout layout_of(int H, int I, int E, int top_k, int T) {
   w.row_map = take(n * 4);
   w.chunks = take((size_t)w.max_chunks * sizeof(Fp8Chunk));
   w.counts = take(16);
-  w.hist = take((size_t)w.counters * E * 4);
+  w.hist = take((size_t)w.counters * fp8_ld_experts(E) * 4);
   w.h = take(T > 1 && w.chunk_rows == kFp8TileRows ? 0 : n * I * 4);
   w.hq = take(n * I);
   w.hs = take(n * fp8_ld(I) * 4);
@@ -75,7 +78,7 @@ struct Group {
   const float *weights;
   float threshold;
   int n, top_k, E, chunk_rows, counters;
-  int32_t *pos, *row_map, *hist;  // hist: [counters, E]
+  int32_t *pos, *row_map, *hist;  // hist: [counters, fp8_ld_experts(E)]
   Fp8Chunk *chunks;
   int32_t *n_chunks;
 };
@@ -188,7 +191,10 @@ __global__ __launch_bounds__(256) void fp8_moe_prep_kernel(Group g, const void *
     }
     place_slots(g, 0, total, before, l);
   } else {
-    for (int e = threadIdx.x; e < g.E; e += kGroupThreads) g.hist[(size_t)b * g.E + e] = l.cnt[e];
+    // (kPer is 4: a thread's experts are one load)
+    const int ld = fp8_ld_experts(g.E);
+    for (int e = threadIdx.x; e < ld; e += kGroupThreads)
+      g.hist[(size_t)b * ld + e] = e < g.E ? l.cnt[e] : 0;
   }
 }
 
@@ -196,12 +202,24 @@ __global__ __launch_bounds__(256) void fp8_moe_place_kernel(Group g) {
   __shared__ GroupLds l;
   const int b = blockIdx.x, e0 = threadIdx.x * kPer;
   int total[kPer] = {}, before[kPer] = {};
-  for (int s = 0; s < g.counters; ++s)
+  static_assert(kPer == 4, "one load per share");
+  const int ld = fp8_ld_experts(g.E);
+  if (e0 < g.E)
+    for (int s0 = 0; s0 < g.counters; s0 += 8) {  // eight loads in flight
+      u32x4_t v[8];
 #pragma unroll
-    for (int q = 0; q < kPer; ++q) {
-      const int v = e0 + q < g.E ? g.hist[(size_t)s * g.E + e0 + q] : 0;
-      total[q] += v;
-      before[q] += s < b ? v : 0;
+      for (int i = 0; i < 8; ++i) {
+        const int s = s0 + i < g.counters ? s0 + i : s0;
+        v[i] = *reinterpret_cast<const u32x4_t *>(g.hist + (size_t)s * ld + e0);
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int q = 0; q < kPer; ++q) {
+          const int c = s0 + i < g.counters ? (int)v[i][q] : 0;
+          total[q] += c;
+          before[q] += s0 + i < b ? c : 0;
+        }
     }
   place_slots(g, b, total, before, l);
 }
