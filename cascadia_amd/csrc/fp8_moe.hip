@@ -23,9 +23,13 @@
 namespace cai4 {
 namespace {
 
-// Rows of a chunk: the tile kernel's from a mean of 16 rows per expert.
+// Rows of a chunk: the tile kernel's from a mean of 8 rows per expert.  Measured, us,
+// 16-row chunks / tiles at a mean of 4, 8, 12 and 16 rows: 60 experts of 3584 x 1408,
+// even 176 / 194, 191 / 196, 214 / 201, 259 / 205; Zipf 154 / 163, 201 / 196, 235 /
+// 200, 269 / 207; 128 of 2048 x 1024, Zipf 132 / 131, 189 / 171, 234 / 183, 272 / 186.
+constexpr int kTileMean = 8;
 int chunk_rows(int T, int E, int top_k) {
-  return (int64_t)T * top_k >= (int64_t)16 * E ? kFp8TileRows : 16;
+  return (int64_t)T * top_k >= (int64_t)kTileMean * E ? kFp8TileRows : 16;
 }
 
 // Workgroups that count: 1,024 slots each, at most 64 (a placing workgroup adds
@@ -261,7 +265,7 @@ __global__ __launch_bounds__(256) void fp8_combine_kernel(const void *residual, 
 size_t fp8_moe_workspace(int H, int I, int E, int top_k, int T) {
   const size_t bytes = layout_of(H, I, E, top_k, T).total;
   // (the largest batch in 16-row chunks may need more than one on tiles)
-  const int few = (int)(((int64_t)16 * E - 1) / top_k);
+  const int few = (int)(((int64_t)kTileMean * E - 1) / top_k);
   const size_t less = few >= 1 && few < T ? layout_of(H, I, E, top_k, few).total : 0;
   return less > bytes ? less : bytes;
 }

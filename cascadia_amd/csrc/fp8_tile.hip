@@ -429,11 +429,14 @@ int slice_blocks(int M, int N, int K) {
 
 constexpr int kCUs = 256;
 enum Form { SMALL, MIDDLE, LARGE };  // 128 x 128, 256 x 128, 256 x 256
-// The largest tiles that still occupy three quarters of the CUs.
+// The next larger tiles once the smaller ones take more than a round over the CUs.
+// Measured, us, K = 4096, bf16 out, 128 x 128 / 256 x 128: 4096 x 1024 (256 / 128
+// tiles) 38.3 / 36.7 (f32 out 52.8 / 63.0), 2048 x 2304 (288 / 144) 41.9 / 38.0 (f32
+// out 71.7 / 65.7); 256 x 128 / 256 x 256: 4096 x 2048 (256 / 128) 41.5 / 58.0, 3328 x
+// 3328 (338 / 169) 71.0 / 58.7.  (256 x 256 with f32 outputs: too few registers.)
 Form form_of(int M, int N, bool out_f32) {
-  const int n = (N + 255) / 256;
-  if (!out_f32 && (int64_t)n * ((M + 255) / 256) >= 192) return LARGE;
-  return (int64_t)n * fp8_blocks(M) >= 192 ? MIDDLE : SMALL;
+  const int64_t middle = (int64_t)((N + 255) / 256) * fp8_blocks(M);
+  return !out_f32 && middle > kCUs ? LARGE : middle > kCUs / 2 ? MIDDLE : SMALL;
 }
 
 // Weight rows whose tiles of 256 x bm would fill at most half of a last round over
@@ -441,7 +444,7 @@ Form form_of(int M, int N, bool out_f32) {
 // own.  Measured, us, one launch / two: bf16 out, 256 x 256, K = 4096: N = M = 4096
 // and 256 rows more (272 tiles) 116 / 100, 12000 x 1500 (282) 115 / 101, 14336 x 4096
 // (896) 276 / 266; f32 out, 256 x 128: 4352 x 4096 (544) 187 / 179, 4096 x 2100 (272)
-// 120 / 108.  bf16 out on 256 x 128 tiles loses 4 % by it (72 / 75) and stays whole.
+// 120 / 108.
 int last_round(int M, int N, int bm) {
   const int nt = (N + 255) / 256, mt = (M + bm - 1) / bm;
   const int full = (int)((int64_t)nt * mt / kCUs * kCUs / mt);  // n tiles of whole rounds
