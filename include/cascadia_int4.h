@@ -446,7 +446,7 @@ int cascadia_int4_moe_forward(const cascadia_int4_moe_layer *layer,
  *     score is the sum of its group_best (1 or 2) largest c, and only the
  *     experts of the top_groups best groups (ties to the lower group) stay.
  *   ids: the top_k by c (bias NULL: by logit), descending, ties to the lower
- *     id; scores are computed and compared in 64 bits.
+ *     id; the choice is that of scores in 64 bits.
  *   weights: s of the chosen (without the bias); divided by their sum + 1e-20
  *     when normalize; times scale.
  * A NaN logit counts as -infinity.  Where the largest logit of a softmax is
@@ -485,12 +485,14 @@ int cascadia_int4_fp8_quantize_blocks(const uint16_t *w_bf16, uint32_t n_rows, u
 
 /* ys[t, r] = sum over blocks b of 128 columns of x_scale[t, b] *
  * w_scale[r / 128, b] * sum_{c in b} x[t, c] w[r, c], f32 sums, one rounding:
- * ys [seq, n_rows] f32 (y_is_f32) or bf16.  w: e4m3 codes [n_rows, k_cols] with
+ * ys [seq, n_rows] f32 (y_is_f32) or bf16.  (bf16 ys of more than 32 rows may add
+ * a block's products on the 8-bit matrix instructions, which keep of every eight
+ * the bits down to 2^-13 of the largest: about 1.5e-5 of a result.)  w: e4m3 codes [n_rows, k_cols] with
  * scales as _quantize_blocks lays them out.  xs [seq, k_cols]: bf16 or f32
  * (quantised in the call as by _quantize; x_scales NULL), or e4m3 codes with
  * x_scales [seq, ceil(k_cols / 128)].  k_cols a multiple of 16; w and xs 16-byte
- * aligned.  workspace: 16-byte aligned, of at least _workspace_bytes for seq
- * rows or more, or NULL for the library's.  seq >= 1. */
+ * aligned; ys overlaps no input.  workspace: 16-byte aligned, of at least
+ * _workspace_bytes for seq rows or more, or NULL for the library's.  seq >= 1. */
 #define CASCADIA_INT4_FP8_X_BF16 0u
 #define CASCADIA_INT4_FP8_X_F32 1u
 #define CASCADIA_INT4_FP8_X_E4M3 2u
@@ -527,13 +529,14 @@ typedef struct cascadia_int4_fp8_moe_layer {
 
 /* out_t = residual_t + sum_k weights[t, k] * y_{t,k} in slot order, one
  * rounding, with y_{t,k} = bf16(down_e(q(silu(gate_e(q(x_t))) * up_e(q(x_t)))))
- * for e = ids[t, k] and q the quantisation above in groups of 128; f32 sums.
+ * for e = ids[t, k] and q the quantisation above in groups of 128; f32 sums
+ * (with many rows per expert a block's as cascadia_int4_fp8_gemm's for bf16 ys).
  * ids (int32) / weights (f32) [n_tokens, top_k], as route_experts or the caller
  * gives them: a slot with weight < threshold or an id outside the layer is left
  * out (padding: -1).  A shared expert is an expert of the stack that every
  * token lists.  x [n_tokens, hidden] f32 (x_is_f32) or bf16; out f32
- * (out_is_f32) or bf16, residual of out's type or NULL (out may be either).  x,
- * residual and out 16-byte aligned; top_k <= 16; 1 <= n_tokens <= 2^20,
+ * (out_is_f32) or bf16, residual of out's type or NULL; out may be x or
+ * residual.  x, residual and out 16-byte aligned; top_k <= 16; 1 <= n_tokens <= 2^20,
  * n_tokens * hidden < 2^31.  workspace as above. */
 size_t cascadia_int4_fp8_moe_workspace_bytes(const cascadia_int4_fp8_moe_layer *layer,
                                              uint32_t top_k, uint32_t n_tokens);
