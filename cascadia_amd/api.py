@@ -1123,7 +1123,7 @@ def fp8_gemm(codes, scales, xs, n_rows: int, k_cols: int, seq: int, ys, x_scales
     scales of blocks of 128 x 128 (quantize_fp8_blocks).  xs [seq, k_cols]: bf16 or
     f32, quantised in the call as by quantize_fp8, or e4m3 codes with x_scales
     [seq, ceil(k_cols / 128)].  ys [seq, n_rows] bf16 or f32, apart from the
-    inputs; f32 sums, one rounding (bf16 of more than 32 rows: a block's products
+    inputs; f32 sums, one rounding (bf16 of more than 16 rows: a block's products
     may be added on the 8-bit matrix instructions, about 1.5e-5 of a result off).
     workspace: fp8_gemm_workspace_bytes (for a graph capture)."""
     dev = _home(codes, "codes")

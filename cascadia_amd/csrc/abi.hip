@@ -2354,15 +2354,16 @@ bool fp8_rows_ok(uint32_t rows, uint32_t k_cols) {
   return (size_t)rows * cai4::fp8_blocks((int)k_cols) <= (size_t)1 << 34;
 }
 
-// A call's workspace: scales in rows of fp8_ld, then, of rows that it quantises,
-// their codes, then the partial sums of a split K.
+// The workspace of a call of up to seq rows: scales in rows of fp8_ld, then, of rows
+// that it quantises, their codes, then the partial sums of a split K (more rows
+// may leave the tiles, so any above kFp8FewRows count as on tiles).
 struct Fp8Workspace {
   size_t codes, part, total;
 };
 Fp8Workspace fp8_workspace(uint32_t n_rows, uint32_t k_cols, uint32_t x_type, uint32_t seq) {
   const bool given = x_type == CASCADIA_INT4_FP8_X_E4M3;
   Fp8Workspace w{};
-  const bool tiles = cai4::fp8_tiles((int)seq, (int)n_rows, (int)k_cols);
+  const bool tiles = seq > (uint32_t)cai4::kFp8FewRows;
   if (given && !tiles) return w;
   w.codes = ((size_t)seq * cai4::fp8_ld((int)k_cols) * 4 + 255) & ~(size_t)255;
   w.part = (w.codes + (given ? 0 : (size_t)seq * k_cols) + 255) & ~(size_t)255;
@@ -2473,8 +2474,9 @@ int cascadia_int4_fp8_gemm(uint32_t n_rows, uint32_t k_cols, const uint8_t *w,
   const int blocks = cai4::fp8_blocks((int)k_cols), ld = cai4::fp8_ld((int)k_cols);
   // given scales are read where they are unless tiles want their rows aligned
   const bool one = seq == 1 && !codes && cai4::fp8_one_row((int)k_cols);  // quantised in its kernel
-  const bool pad = codes && need.total && (blocks != ld || !aligned(x_scales, 16));
-  const bool use = (!codes && !one) || pad || need.total > need.part;
+  const bool tiles = cai4::fp8_tiles((int)seq, (int)n_rows, (int)k_cols);
+  const bool pad = codes && tiles && (blocks != ld || !aligned(x_scales, 16));
+  const bool use = (!codes && !one) || pad || (tiles && need.total > need.part);
   if (use && !workspace)
     if (int rc = own.get(dev, need.total, st, &workspace)) return rc;
   cai4::Fp8Gemm g{};

@@ -80,7 +80,8 @@ struct Fp8Gemm {
   int kper;                    // (set by fp8_tile_gemm)
 };
 hipError_t fp8_gemm(const Fp8Gemm &g, hipStream_t st);
-// Whether a product of M rows runs on tiles, and how many scales it wants per row.
+// Whether a product of M rows runs on tiles: none of up to kFp8FewRows does.
+constexpr int kFp8FewRows = 16;
 bool fp8_tiles(int M, int N, int K);
 // Bytes of partial sums of a product on tiles, for any number of rows up to M.
 size_t fp8_partial_bytes(int M, int N, int K);

@@ -16,7 +16,8 @@
 // (exact) give 1e-8.  The kernels here stream weights and have time to spare: the
 // products run on the bf16 MFMAs, codes converted in registers.
 //
-// Bound: HBM, every weight read once per 16 or 32 rows of x.  A workgroup's
+// Bound: HBM, every weight read once per 16 or 32 rows of x (of more rows: the
+// conversion of codes, and latency).  A workgroup's
 // waves take the k-blocks of its rows in turn, so that together they read
 // contiguous kilobytes of each row; their sums are added through LDS in wave order.
 #include "fp8.hpp"
@@ -354,11 +355,21 @@ hipError_t few(const Fp8Gemm &g, hipStream_t st) {
 
 }  // namespace
 
-// Measured, us, few rows / tiles (bf16 out): 14336 x 4096 17 rows 17.5 / 22.8 (65
-// rows), 48: 31.8 / 22.8; 4096 x 4096 64: 12.0 / 16.7; 1536 x 7168 64: 16.7 / 17.7;
-// 7168 x 2048 64: 12.4 / 15.2.
+// Tiles, or 32 x 32 outputs per workgroup: some 7.5 us and 0.2 us per round over the
+// CUs and block of K, where tiles take 11.5 us (with the joining of K's slices) and
+// grow slower.  Few workgroups over a long K leave CUs idle that slices of K use.
+// Measured, us, 32 x 32 / tiles, bf16 out: 1024 x 4096 (N x K), 96 rows 11.3 / 12.5,
+// 200 11.9 / 15.6, 333 19.0 / 18.1; 2048 x 2048, 333 15.8 / 17.2, 512 20.7 / 20.0; 4096
+// x 1024, 200 12.8 / 14.1, 512 24.4 / 20.6; 4096 x 4096, 64 12.0 / 16.7, 96 18.4 /
+// 18.8, 200 31.3 / 22.3; 576 x 7168, 65 16.9 / 14.2, 333 17.8 / 19.3, 512 30.1 / 21.0;
+// 4096 x 14336, 32 30.9 / 21.9; 14336 x 4096, 32 19.8 / 19.7, 48 31.8 / 19.7.  (f32
+// out: up to 3 more for tiles.)
 bool fp8_tiles(int M, int N, int K) {
-  return M > 64 || (M > 32 && (int64_t)N * K >= (int64_t)32 << 20);
+  if (M <= kFp8FewRows) return false;
+  const int64_t groups = (int64_t)((N + 31) / 32) * ((M + 31) / 32);
+  const int64_t rounds = (groups + 255) / 256;
+  const int KB = fp8_blocks(K);
+  return rounds * (KB + 2) > 72 || (groups < 128 && KB > 32);
 }
 
 hipError_t fp8_gemm(const Fp8Gemm &g, hipStream_t st) {

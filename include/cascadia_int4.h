@@ -485,7 +485,7 @@ int cascadia_int4_fp8_quantize_blocks(const uint16_t *w_bf16, uint32_t n_rows, u
 
 /* ys[t, r] = sum over blocks b of 128 columns of x_scale[t, b] *
  * w_scale[r / 128, b] * sum_{c in b} x[t, c] w[r, c], f32 sums, one rounding:
- * ys [seq, n_rows] f32 (y_is_f32) or bf16.  (bf16 ys of more than 32 rows may add
+ * ys [seq, n_rows] f32 (y_is_f32) or bf16.  (bf16 ys of more than 16 rows may add
  * a block's products on the 8-bit matrix instructions, which keep of every eight
  * the bits down to 2^-13 of the largest: about 1.5e-5 of a result.)  w: e4m3 codes [n_rows, k_cols] with
  * scales as _quantize_blocks lays them out.  xs [seq, k_cols]: bf16 or f32
