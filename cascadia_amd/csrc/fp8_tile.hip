@@ -418,16 +418,23 @@ hipError_t launch(const Fp8Gemm &g, hipStream_t st, int n_first = 0, int count =
   return hipGetLastError();
 }
 
+constexpr int kCUs = 256;
+
 // Slices of K for a product whose 128 x 128 tiles are fewer than the CUs take (two
-// each): 4 blocks or a multiple per slice, 0 where one slice is left.
+// each): a multiple of 4 blocks per slice, 0 where one slice is left.  A workgroup's
+// start and end weigh as much as some 8 blocks, so that is the least, unless 4 leave
+// half the CUs idle; none where all of a short K fills half of them.  Measured, us, least 4 / 8, bf16 out: N x K 576 x 7168, 65 rows 15.0
+// / 14.7 (f32 out 15.1 / 16.9), 512 21.8 / 19.2; 1536 x 7168, 333 27.0 / 22.9; 576 x
+// 14336, 128 23.2 / 19.8; two slices / one: 7168 x 2048, 333 25.3 / 19.5, 512 26.3 / 20.6.
 int slice_blocks(int M, int N, int K) {
   const int KB = fp8_blocks(K), tiles = fp8_blocks(M) * fp8_blocks(N);
   const int want = tiles >= 512 ? 1 : 512 / tiles;
-  const int per = ((KB + want - 1) / want + 3) & ~3;
+  if (tiles > kCUs / 2 && KB <= 16) return 0;
+  const int least = (int64_t)tiles * ((KB + 3) / 4) <= kCUs / 2 ? 4 : 8;
+  const int even = ((KB + want - 1) / want + 3) & ~3, per = even > least ? even : least;
   return per < KB ? per : 0;
 }
 
-constexpr int kCUs = 256;
 enum Form { SMALL, MIDDLE, LARGE };  // 128 x 128, 256 x 128, 256 x 256
 // The next larger tiles once the smaller ones take more than a round over the CUs.
 // Measured, us, K = 4096, bf16 out, 128 x 128 / 256 x 128: 4096 x 1024 (256 / 128
