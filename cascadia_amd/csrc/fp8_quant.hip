@@ -6,7 +6,9 @@
 // divisor growing past f32.)  A group that holds an infinity gives NaN codes or
 // an infinite scale, and so a NaN in every product with it.
 //
-// Bound: HBM, each value read and its code written once.
+// Bound: HBM, each value read and its code written once.  4096 x 7168 bf16 rows: 17
+// us (5.2 TB/s, some of it from the Infinity Cache); 7104 x 8112 in blocks: 39 us (4.4
+// TB/s; a copy reaches 4.87).
 #include "fp8.hpp"
 #include "fp8_common.hpp"
 #include "fp8_quant.hpp"

@@ -19,7 +19,7 @@
 // SwiGLU takes the fast form: its result is quantised to 4 bits of precision
 // right here, where 1.5e-5 moves one value in some 3,000 to the neighbouring code;
 // a layer's bf16 output is 1.9e-3 off the 64-bit one, with exact sums 1.7e-3
-// (2,048 tokens over 128 experts; gate and up take 855 us that way, 555 so).
+// (2,048 tokens over 128 experts; gate and up took 855 us that way, 555 so).
 //
 // LDS: a row of 128 bytes is eight 16-byte chunks, chunk c of row r in slot
 // c ^ (r / 2 & 7), so that the 16 rows that a fragment read touches at once lie
@@ -32,13 +32,16 @@
 // of the block stands, which also publishes the next stage.  The freed one takes
 // the loads of the block S further during the next block, one or two a pass
 // (past the last block: loads out of range, so that every wait counts the same
-// number).  Issued all at once behind the barrier they held up every wave while
-// the address unit worked through them (4096 x 14336 x 4096: 260 us).
+// number).  Issued all at once behind the barrier they hold up every wave while the
+// address unit works through them.
 //
 // What bounds it: a CU keeps some 64 cache lines in flight to its L2, about 14
 // bytes a cycle at 390 cycles each, so requests count.  The tokens' scales, rows
 // padded to 16 bytes, are read four blocks at a time; one by one they were a third
-// of all requests (4096 x 14336 x 4096: 289 us).
+// of all requests.  Measured, M x N x K 4096 x 14336 x 4096, bf16 out: 257 us, 1.87
+// PFLOP/s (one large library product of codes under one scale: 2.65 PFLOP/s; scales
+// one by one and stores at the end: 282 us); f32 out 460 us, 1.05 PFLOP/s.  Of 2,048 tokens
+// over 128 experts of 4096 x 1536: gate and up 450 to 477 us, down 266 to 292.
 #include "fp8.hpp"
 #include "fp8_common.hpp"
 #include "fp8_rows.hpp"
