@@ -265,11 +265,17 @@ __global__ __launch_bounds__(256) void fp8_combine_kernel(const void *residual, 
 }  // namespace
 
 size_t fp8_moe_workspace(int H, int I, int E, int top_k, int T) {
-  const size_t bytes = layout_of(H, I, E, top_k, T).total;
-  // (the largest batch in 16-row chunks may need more than one on tiles)
+  size_t most = 0;  // over all calls of up to T tokens
+  auto take = [&](int t) {
+    const size_t bytes = layout_of(H, I, E, top_k, t).total;
+    most = bytes > most ? bytes : most;
+  };
+  take(T);
+  // (one token, and the largest batch in 16-row chunks, may need more than one on tiles)
+  take(1);
   const int few = (int)(((int64_t)kTileMean * E - 1) / top_k);
-  const size_t less = few >= 1 && few < T ? layout_of(H, I, E, top_k, few).total : 0;
-  return less > bytes ? less : bytes;
+  if (few >= 1 && few < T) take(few);
+  return most;
 }
 
 hipError_t fp8_moe_forward(const Fp8Moe &m, void *workspace, hipStream_t st) {

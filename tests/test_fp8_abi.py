@@ -183,3 +183,14 @@ def test_reference_route_on_a_case_by_hand():
     bias = np.array([9.0, 0, 0, 0, 0, 0, 0, 9.0])
     ids, w = ref.route(logits, 2, "sigmoid", bias, 1, 1, 1, False, 1.0)
     assert ids.tolist() == [[0, 7]] and abs(w[0, 0] - 1 / (1 + np.exp(-1.0))) < 1e-12
+
+
+def test_layer_workspace_of_more_tokens_serves_fewer(cl):
+    """One token keeps its slots' h in f32, more of them (here on tiles at once: one
+    expert takes all 16 slots) only its codes."""
+    Layer, need = cl._lib.Fp8MoeLayer, cl.lib().cascadia_int4_fp8_moe_workspace_bytes
+    for hidden, inter, experts, k in ((16, 4096, 1, 16), (16, 4096, 2, 16), (32, 4096, 4, 16),
+                                      (16, 2048, 3, 8), (256, 128, 1, 1)):
+        lay = Layer(hidden, inter, experts, P, P, P, P, 0)
+        sizes = [need(C.byref(lay), k, t) for t in range(1, 300)]
+        assert sizes == sorted(sizes), (hidden, inter, experts, k)
