@@ -82,10 +82,11 @@ def silu(g):
 
 def moe(x, gate_up, gate_up_s, down, down_s, ids, weights, threshold, residual):
     """(out, bound) of one layer in 64 bits (codes as values), bound without the
-    output's own rounding.  Of many tokens the products may run on the 8-bit
-    MFMAs."""
+    output's own rounding.  Of many tokens, or of eight rows per expert, the
+    products may run on the 8-bit MFMAs (eight_bit_sums: how far off)."""
     T, H = x.shape
     E, _, I, _ = gate_up.shape
+    many = T > 16 or T * ids.shape[1] >= 8 * E
     q, s = quotients(x, 1)
     xq = round_e4m3(q)
     out = np.zeros((T, H)) if residual is None else np.array(residual, np.float64)
@@ -98,7 +99,7 @@ def moe(x, gate_up, gate_up_s, down, down_s, ids, weights, threshold, residual):
                 continue
             (g, bg), (u, bu) = (gemm(xq[t:t + 1], s[t:t + 1], gate_up[e, i], gate_up_s[e, i])
                                 for i in (0, 1))
-            if T > 16:
+            if many:
                 xd = xq[t:t + 1] * np.repeat(s[t:t + 1], 128, 1)[:, :H]
                 bg, bu = (b + eight_bit_sums(xd, gate_up[e, i] * spread(gate_up_s[e, i], I, H))
                           for i, b in ((0, bg), (1, bu)))
@@ -116,7 +117,7 @@ def moe(x, gate_up, gate_up_s, down, down_s, ids, weights, threshold, residual):
             dh = np.where(border, step, 0.0) + np.abs(code) * spread(top_off, 1, I, rows=1)
             y, by = gemm(code, hs, down[e], down_s[e])
             wd = np.abs(down[e] * spread(down_s[e], H, I))
-            if T > 16:
+            if many:
                 by = by + eight_bit_sums(code * spread(hs, 1, I, rows=1), wd)
             by = by + (dh * spread(hs, 1, I, rows=1)) @ wd.T
             y, by = y[0], by[0]

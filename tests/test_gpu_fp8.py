@@ -501,6 +501,14 @@ def test_moe(cl, T, H, I, E, k, x_dtype):
     check_moe(cl, case, torch.float32 if (T + k) % 2 else torch.bfloat16, residual=T % 3 != 0)
 
 
+@pytest.mark.parametrize("T,H,I,E,k", [(8, 256, 144, 1, 1), (16, 400, 272, 4, 2),
+                                       (15, 144, 128, 4, 2), (2, 64, 1040, 1, 16)])
+def test_moe_about_eight_rows_per_expert(cl, T, H, I, E, k):
+    """Either side of the step from 16-row chunks to tiles, and a few tokens on tiles."""
+    ids = torch.randint(0, E, (T, k), generator=gen(T), dtype=torch.int32)
+    check_moe(cl, moe_case(T + H, T, H, I, E, k, torch.bfloat16, ids))
+
+
 @pytest.mark.parametrize("T,H,I,E,k", [(1, 400, 272, 5, 3), (9, 144, 1040, 4, 2),
                                        (90, 272, 400, 3, 2), (300, 128, 16, 2, 1)])
 def test_moe_tiled_codes_are_the_same_codes(cl, T, H, I, E, k):
