@@ -1212,8 +1212,8 @@ def _fp8_moe_need(tuning, device, hidden, inter, n_experts, top_k, n_tokens):
 
 def fp8_moe_forward(experts: Fp8Experts, x, out, *, top_k: int, ids, weights,
                     threshold: float = 0.0, residual=None, workspace=None):
-    """One MoE layer over e4m3 experts: out = residual + sum_k w_k bf16(down(q(silu(
-    gate(q(x))) * up(q(x))))), q as quantize_fp8, f32 sums in slot order, one
+    """One MoE layer over e4m3 experts: out = residual + sum_k w_k down(q(silu(
+    gate(q(x))) * up(q(x)))), q as quantize_fp8, f32 sums in slot order, one
     rounding.  x f32 or bf16, out f32 or bf16 (residual of out's type), all
     [n_tokens, hidden]; ids (int32) / weights (f32) [n_tokens, top_k], as
     route_experts gives them.  Slots with a weight below threshold or an id

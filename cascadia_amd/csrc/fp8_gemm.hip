@@ -335,7 +335,7 @@ __global__ __launch_bounds__(1024) void fp8_one_down_kernel(Fp8Gemm g, const flo
     float y = 0.f;
     for (int q = 0; q < per; ++q)
       y += reinterpret_cast<const float *>(part[s * per + q])[threadIdx.x];
-    v += weights[s] * bf16_to_f32(f32_to_bf16_rne(y));
+    v += weights[s] * y;
   }
   if (g.out_f32) {
     if (residual) v = static_cast<const float *>(residual)[n] + v;

@@ -2,11 +2,8 @@
 //
 // Per token t and slot j with weight w >= threshold and an expert id inside the
 // layer: h = silu(W_gate x) (W_up x) in f32 over x's codes, requantised, and
-// y = bf16(W_down h); out_t = residual_t + sum_j w_j y_j in slot order (multiply,
-// then add), rounded once.  y is kept in 16 bits between its product and the
-// sum, as the INT4 layer keeps it: the slots' rows are the layer's largest
-// intermediate (top_k times its output), and their rounding is no coarser than
-// that of a bf16 output.
+// y = W_down h in f32; out_t = residual_t + sum_j w_j y_j in slot order (multiply,
+// then add), rounded once.
 //
 // Rows are grouped by expert.  Position in a group varies between calls, results
 // do not: a grouped row's products do not depend on its place, and the sum reads
@@ -74,7 +71,7 @@ Layout layout_of(int H, int I, int E, int top_k, int T) {
   w.h = take(T > 1 && w.chunk_rows == kFp8TileRows ? 0 : n * I * 4);
   w.hq = take(n * I);
   w.hs = take(n * fp8_ld(I) * 4);
-  w.y = take(n * H * 2);
+  w.y = take(n * H * 4);
   w.total = o;
   return w;
 }
@@ -238,7 +235,7 @@ CAI4_DEV f32x4_t load4(const void *p, size_t at, bool f32) {
 }
 
 // Four outputs of a token per thread (H is a multiple of 16).
-__global__ __launch_bounds__(256) void fp8_combine_kernel(const void *residual, const uint16_t *y,
+__global__ __launch_bounds__(256) void fp8_combine_kernel(const void *residual, const float *y,
                                                           const int32_t *pos, const float *w,
                                                           int H, int k, void *out, int out_f32) {
 #pragma clang fp contract(off)
@@ -249,7 +246,7 @@ __global__ __launch_bounds__(256) void fp8_combine_kernel(const void *residual, 
   for (int s = 0; s < k; ++s) {
     const int p = pos[(size_t)t * k + s];
     if (p < 0) continue;
-    v += w[(size_t)t * k + s] * load4(y, (size_t)p * H + j, false);
+    v += w[(size_t)t * k + s] * load4(y, (size_t)p * H + j, true);
   }
   if (residual) v = load4(residual, o, out_f32) + v;
   if (out_f32) {
@@ -359,6 +356,7 @@ hipError_t fp8_moe_forward(const Fp8Moe &m, void *workspace, hipStream_t st) {
   down.xs = hs;
   down.ld_xs = fp8_ld(m.I);
   down.y = b + w.y;
+  down.out_f32 = 1;
   down.chunks = gr.chunks;
   down.max_chunks = w.max_chunks;
   down.chunk_rows = w.chunk_rows;
@@ -366,7 +364,7 @@ hipError_t fp8_moe_forward(const Fp8Moe &m, void *workspace, hipStream_t st) {
   e = fp8_gemm(down, st);
   if (e != hipSuccess) return e;
   hipLaunchKernelGGL(fp8_combine_kernel, dim3(m.T, (m.H + 1023) / 1024), dim3(256), 0, st,
-                     m.residual, reinterpret_cast<const uint16_t *>(b + w.y), gr.pos, m.weights, m.H,
+                     m.residual, reinterpret_cast<const float *>(b + w.y), gr.pos, m.weights, m.H,
                      m.top_k, m.out, m.out_f32);
   return hipGetLastError();
 }
