@@ -1214,7 +1214,8 @@ def fp8_moe_forward(experts: Fp8Experts, x, out, *, top_k: int, ids, weights,
                     threshold: float = 0.0, residual=None, workspace=None):
     """One MoE layer over e4m3 experts: out = residual + sum_k w_k down(q(silu(
     gate(q(x))) * up(q(x)))), q as quantize_fp8, f32 sums in slot order, one
-    rounding.  x f32 or bf16, out f32 or bf16 (residual of out's type), all
+    rounding (bf16 out of eight or more rows per expert: a block's products may be
+    added on the 8-bit matrix instructions, as fp8_gemm's).  x f32 or bf16, out f32 or bf16 (residual of out's type), all
     [n_tokens, hidden]; ids (int32) / weights (f32) [n_tokens, top_k], as
     route_experts gives them.  Slots with a weight below threshold or an id
     outside the layer (padding: -1) are left out.  out may be residual or x.

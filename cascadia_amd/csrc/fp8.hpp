@@ -74,6 +74,7 @@ struct Fp8Gemm {
   int x_rows;                  // rows of x (row_map)
   size_t w_stride, ws_stride;  // between experts
   int swiglu;                  // y = silu(gate) * up: f32, or codes with ys
+  int exact;                   // experts on tiles: no 8-bit sums
   float *ys;                   // SwiGLU on tiles: y's scales [rows, ld_ys]
   int ld_ys;
   float *part;                 // tiles: workspace of fp8_partial_bytes

@@ -292,6 +292,7 @@ hipError_t fp8_moe_forward(const Fp8Moe &m, void *workspace, hipStream_t st) {
   up.ws_stride = (size_t)2 * ib * hb;
   up.swiglu = 1;
   up.out_f32 = 1;
+  up.exact = down.exact = m.out_f32;
   down.w = m.down;
   down.ws = m.down_s;
   down.N = m.H;

@@ -16,10 +16,11 @@
 //          takes 2e-3.  Used where the output is bf16.
 //   exact  the codes converted to bf16 in registers (exact) and four 16x16x32
 //          MFMAs: f32 sums, at half the rate.  Used for f32 outputs.
-// SwiGLU takes the fast form: its result is quantised to 4 bits of precision
-// right here, where 1.5e-5 moves one value in some 3,000 to the neighbouring code;
-// a layer's bf16 output is 1.9e-3 off the 64-bit one, with exact sums 1.7e-3
-// (2,048 tokens over 128 experts; gate and up took 855 us that way, 555 so).
+// A layer takes the form of its output for all its products.  SwiGLU's result is
+// quantised to 4 bits of precision right here, where 1.5e-5 moves one value in some
+// 3,000 to the neighbouring code.  2,048 tokens over 128 experts of 4096 x 1536, off
+// the 64-bit output (relative, as a whole) and time: bf16 out 1.75e-3 (rounding it
+// alone 1.66e-3), 770 us; f32 out 2.1e-4, 1100 us (8-bit sums: 0.85e-3).
 //
 // LDS: a row of 128 bytes is eight 16-byte chunks, chunk c of row r in slot
 // c ^ (r / 2 & 7), so that the 16 rows that a fragment read touches at once lie
@@ -478,8 +479,12 @@ size_t fp8_partial_bytes(int M, int N, int K) {
 hipError_t fp8_tile_gemm(const Fp8Gemm &g0, hipStream_t st) {
   Fp8Gemm g = g0;
   g.kper = 0;
-  if (g.swiglu) return launch<8, 2, 2, 4, true, false, 3>(g, st);
-  if (g.chunks) return launch<8, 2, 2, 4, false, false, 3>(g, st);
+  if (g.swiglu)
+    return g.exact ? launch<4, 4, 4, 2, true, true, 3>(g, st)
+                   : launch<8, 2, 2, 4, true, false, 3>(g, st);
+  if (g.chunks)
+    return g.exact ? launch<4, 4, 4, 2, false, true, 3>(g, st)
+                   : launch<8, 2, 2, 4, false, false, 3>(g, st);
   const Form f = form_of(g.M, g.N, g.out_f32);
   if (f == LARGE) {
     const int left = last_round(g.M, g.N, 256), most = g.N - left;

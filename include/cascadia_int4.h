@@ -530,7 +530,7 @@ typedef struct cascadia_int4_fp8_moe_layer {
 /* out_t = residual_t + sum_k weights[t, k] * y_{t,k} in slot order, one
  * rounding, with y_{t,k} = down_e(q(silu(gate_e(q(x_t))) * up_e(q(x_t)))) in f32
  * for e = ids[t, k] and q the quantisation above in groups of 128; f32 sums
- * (with many rows per expert a block's as cascadia_int4_fp8_gemm's for bf16 ys).
+ * (bf16 out and many rows per expert: a block's as cascadia_int4_fp8_gemm's for bf16 ys).
  * ids (int32) / weights (f32) [n_tokens, top_k], as route_experts or the caller
  * gives them: a slot with weight < threshold or an id outside the layer is left
  * out (padding: -1).  A shared expert is an expert of the stack that every
