@@ -133,6 +133,8 @@ SIGNATURES = {
     "cascadia_int4_fp8_moe_workspace_bytes": (_sz, [_FP, _u32, _u32]),
     "cascadia_int4_fp8_moe_forward": (_i32, [_FP, _u32, _vp, _vp, C.c_float, _vp, _u32, _vp, _u32,
                                              _vp, _u32, _vp, _vp]),
+    "cascadia_int4_debug_fp8_gemm_form": (_i32, [_u32, _u32, _u32, _u32, _u32]),
+    "cascadia_int4_debug_fp8_moe_form": (_i32, [_FP, _u32, _u32]),
     "cascadia_int4_debug_dequant": (_i32, [_LP, _vp, _vp, _vp, _vp]),
     "cascadia_int4_stream_read": (_i32, [_vp, _sz, _vp, _vp]),
     "cascadia_int4_fill_synthetic": (_i32, [_u32, _u64, _u64, _sz, _f64, _f64, _u32, _vp, _vp]),

@@ -2474,7 +2474,8 @@ int cascadia_int4_fp8_gemm(uint32_t n_rows, uint32_t k_cols, const uint8_t *w,
   const int blocks = cai4::fp8_blocks((int)k_cols), ld = cai4::fp8_ld((int)k_cols);
   // given scales are read where they are unless tiles want their rows aligned
   const bool one = seq == 1 && !codes && cai4::fp8_one_row((int)k_cols);  // quantised in its kernel
-  const bool tiles = cai4::fp8_tiles((int)seq, (int)n_rows, (int)k_cols);
+  const bool tiles =
+      cai4::fp8_form((int)seq, (int)n_rows, (int)k_cols, y_is_f32 != 0) >= cai4::kFp8Tiles128;
   const bool pad = codes && tiles && (blocks != ld || !aligned(x_scales, 16));
   const bool use = (!codes && !one) || pad || (tiles && need.total > need.part);
   if (use && !workspace)
@@ -2506,6 +2507,22 @@ int cascadia_int4_fp8_gemm(uint32_t n_rows, uint32_t k_cols, const uint8_t *w,
     if (!codes) g.x = q;
   }
   return hip_status(cai4::fp8_gemm(g, st));
+}
+
+int cascadia_int4_debug_fp8_gemm_form(uint32_t n_rows, uint32_t k_cols, uint32_t x_type,
+                                      uint32_t seq, uint32_t y_is_f32) {
+  if (!fp8_dims_ok(n_rows, k_cols) || seq == 0 || seq > kFp8MaxRows ||
+      x_type > CASCADIA_INT4_FP8_X_E4M3 || y_is_f32 > 1)
+    return CASCADIA_INT4_ERR_ARG;
+  if (seq == 1 && x_type != CASCADIA_INT4_FP8_X_E4M3 && cai4::fp8_one_row((int)k_cols)) return 0;
+  return cai4::fp8_form((int)seq, (int)n_rows, (int)k_cols, y_is_f32 != 0);
+}
+
+int cascadia_int4_debug_fp8_moe_form(const cascadia_int4_fp8_moe_layer *L, uint32_t top_k,
+                                     uint32_t n_tokens) {
+  if (int rc = fp8_moe_check(L, top_k, n_tokens)) return rc;
+  if (n_tokens == 1 && cai4::fp8_one_token((int)L->hidden, (int)L->inter, (int)top_k)) return 0;
+  return cai4::fp8_moe_chunk_rows((int)n_tokens, (int)L->n_experts, (int)top_k);
 }
 
 size_t cascadia_int4_fp8_tiled_bytes(uint32_t n_rows, uint32_t k_cols) {

@@ -81,9 +81,20 @@ struct Fp8Gemm {
   int kper;                    // (set by fp8_tile_gemm)
 };
 hipError_t fp8_gemm(const Fp8Gemm &g, hipStream_t st);
-// Whether a product of M rows runs on tiles: none of up to kFp8FewRows does.
-constexpr int kFp8FewRows = 16;
-bool fp8_tiles(int M, int N, int K);
+// Forms of a product of one matrix: 16 x 32 or 32 x 32 outputs per workgroup, or tiles
+// of 128 x 128 (with K in slices or not), 256 x 128, 256 x 256.
+enum Fp8Form {
+  kFp8Rows16 = 1,
+  kFp8Rows32,
+  kFp8Tiles128,
+  kFp8Slices128,
+  kFp8Tiles256x128,
+  kFp8Tiles256
+};
+constexpr int kFp8FewRows = 16;  // no more rows than these run on tiles
+Fp8Form fp8_form(int M, int N, int K, bool out_f32);
+Fp8Form fp8_tile_form(int M, int N, int K, bool out_f32);  // of one on tiles
+float fp8_tile_us(int M, int N, int K, bool out_f32);      // its estimated time
 // Bytes of partial sums of a product on tiles, for any number of rows up to M.
 size_t fp8_partial_bytes(int M, int N, int K);
 constexpr int kFp8TileRows = 128;  // rows of a chunk on the tile kernel (16 else)
@@ -112,6 +123,7 @@ hipError_t fp8_gemv(const Fp8Gemm &g, const void *x, bool x_f32, hipStream_t st)
 hipError_t fp8_moe_one(const Fp8Moe &m, const Fp8Gemm &gate_up, const Fp8Gemm &down, float *h,
                        hipStream_t st);
 size_t fp8_moe_workspace(int H, int I, int E, int top_k, int T);
+int fp8_moe_chunk_rows(int T, int E, int top_k);  // 16, or kFp8TileRows: on tiles
 hipError_t fp8_moe_forward(const Fp8Moe &m, void *workspace, hipStream_t st);
 
 }  // namespace cai4

@@ -358,28 +358,34 @@ hipError_t few(const Fp8Gemm &g, hipStream_t st) {
 
 }  // namespace
 
-// Tiles, or 32 x 32 outputs per workgroup: some 7.5 us and 0.2 us per round over the
-// CUs and block of K, where tiles take 11.5 us (with the joining of K's slices) and
-// grow slower.  Few workgroups over a long K leave CUs idle that slices of K use.
-// Measured, us, 32 x 32 / tiles, bf16 out: 1024 x 4096 (N x K), 96 rows 11.3 / 12.5,
-// 200 11.9 / 15.6, 333 19.0 / 18.1; 2048 x 2048, 333 15.8 / 17.2, 512 20.7 / 20.0; 4096
-// x 1024, 200 12.8 / 14.1, 512 24.4 / 20.6; 4096 x 4096, 64 12.0 / 16.7, 96 18.4 /
-// 18.8, 200 31.3 / 22.3; 576 x 7168, 65 16.9 / 14.2, 333 17.8 / 19.3, 512 30.1 / 21.0;
-// 4096 x 14336, 32 30.9 / 21.9; 14336 x 4096, 32 19.8 / 19.7, 48 31.8 / 19.7.  (f32
-// out: up to 3 more for tiles.)
-bool fp8_tiles(int M, int N, int K) {
-  if (M <= kFp8FewRows) return false;
+// Estimated time of a product in 32 x 32 outputs per workgroup, us: a round over the
+// CUs costs 0.2 us per block of K (off 10 % as a whole over 1,260 products of 17 to
+// 1,024 rows, 246 to 24,576 x 272 to 14,336).
+static float few_us(int M, int N, int K) {
   const int64_t groups = (int64_t)((N + 31) / 32) * ((M + 31) / 32);
-  const int64_t rounds = (groups + 255) / 256;
-  const int KB = fp8_blocks(K);
-  return rounds * (KB + 2) > 72 || (groups < 128 && KB > 32);
+  return 3.0f + (float)((groups + 255) / 256) * (0.2f * fp8_blocks(K) + 0.6f);
+}
+
+// Tiles where fp8_tile_us says less.  Measured, us, 32 x 32 / tiles, bf16 out (f32
+// out), N x K: 4096 x 1024, 256 rows 13.0 / 14.8, 448 20.8 / 11.0 (20.4 / 14.0); 2395 x
+// 272, 640 12.6 / 12.5, 1024 19.2 / 12.9; 576 x 7168, 96 16.3 / 14.0 (16.2 / 15.2), 333
+// 16.8 / 16.8 (16.7 / 19.2), 512 29.1 / 18.6; 246 x 4336, 333 9.3 / 20.7; 1137 x 9152,
+// 200 17.2 / 23.2, 512 41.6 / 33.1; 4096 x 4096, 96 19.2 / 17.2; 14336 x 4096, 32 21.9 /
+// 19.2.  Over those products the choice costs 0.8 % more than the faster form of each.
+Fp8Form fp8_form(int M, int N, int K, bool out_f32) {
+  if (M <= kFp8FewRows) return kFp8Rows16;
+  return fp8_tile_us(M, N, K, out_f32) < few_us(M, N, K) ? fp8_tile_form(M, N, K, out_f32)
+                                                         : kFp8Rows32;
 }
 
 hipError_t fp8_gemm(const Fp8Gemm &g, hipStream_t st) {
-  if (g.chunks ? g.chunk_rows > 16 : fp8_tiles(g.M, g.N, g.K)) return fp8_tile_gemm(g, st);
-  if (g.swiglu) return few<1, true>(g, st);
-  if (!g.chunks && g.M > 16) return few<2, false>(g, st);
-  return few<1, false>(g, st);
+  if (g.chunks) {
+    if (g.chunk_rows > 16) return fp8_tile_gemm(g, st);
+    return g.swiglu ? few<1, true>(g, st) : few<1, false>(g, st);
+  }
+  const Fp8Form f = fp8_form(g.M, g.N, g.K, g.out_f32);
+  if (f == kFp8Rows16) return few<1, false>(g, st);
+  return f == kFp8Rows32 ? few<2, false>(g, st) : fp8_tile_gemm(g, st);
 }
 
 bool fp8_one_row(int K) { return K <= kOneBlocks * 128; }

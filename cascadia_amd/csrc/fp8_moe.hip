@@ -27,9 +27,6 @@ namespace {
 // even 176 / 194, 191 / 196, 214 / 201, 259 / 205; Zipf 154 / 163, 201 / 196, 235 /
 // 200, 269 / 207; 128 of 2048 x 1024, Zipf 132 / 131, 189 / 171, 234 / 183, 272 / 186.
 constexpr int kTileMean = 8;
-int chunk_rows(int T, int E, int top_k) {
-  return (int64_t)T * top_k >= (int64_t)kTileMean * E ? kFp8TileRows : 16;
-}
 
 // Workgroups that count: 1,024 slots each, at most 64 (a placing workgroup adds
 // up all counts before its own).
@@ -56,7 +53,7 @@ Layout layout_of(int H, int I, int E, int top_k, int T) {
     o += (bytes + 255) & ~(size_t)255;
     return at;
   };
-  w.chunk_rows = chunk_rows(T, E, top_k);
+  w.chunk_rows = fp8_moe_chunk_rows(T, E, top_k);
   // sum of ceil(c_e / C) <= A + (n - A) / C for A experts with rows
   const size_t a = n < (size_t)E ? n : E;
   w.max_chunks = (int)(a + (n - a) / w.chunk_rows);
@@ -260,6 +257,10 @@ __global__ __launch_bounds__(256) void fp8_combine_kernel(const void *residual, 
 }
 
 }  // namespace
+
+int fp8_moe_chunk_rows(int T, int E, int top_k) {
+  return (int64_t)T * top_k >= (int64_t)kTileMean * E ? kFp8TileRows : 16;
+}
 
 size_t fp8_moe_workspace(int H, int I, int E, int top_k, int T) {
   size_t most = 0;  // over all calls of up to T tokens

@@ -439,15 +439,16 @@ int slice_blocks(int M, int N, int K) {
   return per < KB ? per : 0;
 }
 
-enum Form { SMALL, MIDDLE, LARGE };  // 128 x 128, 256 x 128, 256 x 256
 // The next larger tiles once the smaller ones take more than a round over the CUs.
 // Measured, us, K = 4096, bf16 out, 128 x 128 / 256 x 128: 4096 x 1024 (256 / 128
 // tiles) 38.3 / 36.7 (f32 out 52.8 / 63.0), 2048 x 2304 (288 / 144) 41.9 / 38.0 (f32
 // out 71.7 / 65.7); 256 x 128 / 256 x 256: 4096 x 2048 (256 / 128) 41.5 / 58.0, 3328 x
 // 3328 (338 / 169) 71.0 / 58.7.  (256 x 256 with f32 outputs: too few registers.)
-Form form_of(int M, int N, bool out_f32) {
+Fp8Form tile_size(int M, int N, bool out_f32) {
   const int64_t middle = (int64_t)((N + 255) / 256) * fp8_blocks(M);
-  return !out_f32 && middle > kCUs ? LARGE : middle > kCUs / 2 ? MIDDLE : SMALL;
+  return !out_f32 && middle > kCUs ? kFp8Tiles256
+         : middle > kCUs / 2       ? kFp8Tiles256x128
+                                   : kFp8Tiles128;
 }
 
 // Weight rows whose tiles of 256 x bm would fill at most half of a last round over
@@ -469,11 +470,35 @@ size_t fp8_partial_bytes(int M, int N, int K) {
   size_t most = 0;  // over all calls of up to M rows
   for (int m = 1; m <= fp8_blocks(M) && m * fp8_blocks(N) < 512; ++m) {
     const int rows = m * 128 < M ? m * 128 : M, per = slice_blocks(rows, N, K);
-    if (!per || form_of(rows, N, true) != SMALL) continue;
+    if (!per || tile_size(rows, N, true) != kFp8Tiles128) continue;
     const size_t b = (size_t)((fp8_blocks(K) + per - 1) / per) * rows * N * 4;
     most = b > most ? b : most;
   }
   return most;
+}
+
+Fp8Form fp8_tile_form(int M, int N, int K, bool out_f32) {
+  const Fp8Form f = tile_size(M, N, out_f32);
+  return f == kFp8Tiles128 && slice_blocks(M, N, K) ? kFp8Slices128 : f;
+}
+
+// Fitted to the products named at fp8_form (off 7 to 18 % by form).  In slices: 0.75
+// us per block of K of one, and the writing and joining of the partial sums, 2.5 us a
+// million.
+float fp8_tile_us(int M, int N, int K, bool out_f32) {
+  const float KB = (float)fp8_blocks(K);
+  switch (fp8_tile_form(M, N, K, out_f32)) {
+    case kFp8Slices128: {
+      const int per = slice_blocks(M, N, K), slices = (fp8_blocks(K) + per - 1) / per;
+      return 10.0f + 0.75f * per + 2.5e-6f * M * N * slices;
+    }
+    case kFp8Tiles128:
+      return 8.0f + KB * (0.6f + 0.5f * fp8_blocks(M) * fp8_blocks(N) / kCUs);
+    case kFp8Tiles256x128:
+      return 12.0f + KB * (out_f32 ? 1.7f : 0.95f);  // (one round; of more, 32 x 32 takes far longer)
+    default:
+      return 18.0f + 0.7f * KB * (float)(((int64_t)((M + 255) / 256) * ((N + 255) / 256) + kCUs - 1) / kCUs);
+  }
 }
 
 hipError_t fp8_tile_gemm(const Fp8Gemm &g0, hipStream_t st) {
@@ -485,20 +510,20 @@ hipError_t fp8_tile_gemm(const Fp8Gemm &g0, hipStream_t st) {
   if (g.chunks)
     return g.exact ? launch<4, 4, 4, 2, false, true, 3>(g, st)
                    : launch<8, 2, 2, 4, false, false, 3>(g, st);
-  const Form f = form_of(g.M, g.N, g.out_f32);
-  if (f == LARGE) {
+  const Fp8Form f = fp8_tile_form(g.M, g.N, g.K, g.out_f32);
+  if (f == kFp8Tiles256) {
     const int left = last_round(g.M, g.N, 256), most = g.N - left;
     const hipError_t e = launch<8, 4, 2, 4, false, false, 2>(g, st, 0, most);
     return e != hipSuccess || !left ? e : launch<8, 2, 2, 4, false, false, 3>(g, st, most, left);
   }
-  if (f == MIDDLE) {
+  if (f == kFp8Tiles256x128) {
     if (!g.out_f32) return launch<8, 2, 2, 4, false, false, 3>(g, st);
     // (exact: waves of 64 x 64 convert a fifth fewer codes than of 128 x 32)
     const int left = last_round(g.M, g.N, 128), most = g.N - left;
     const hipError_t e = launch<4, 4, 4, 2, false, true, 3>(g, st, 0, most);
     return e != hipSuccess || !left ? e : launch<4, 2, 2, 4, false, true, 2>(g, st, most, left);
   }
-  g.kper = slice_blocks(g.M, g.N, g.K);
+  if (f == kFp8Slices128) g.kper = slice_blocks(g.M, g.N, g.K);
   if (g.out_f32) return launch<4, 2, 2, 4, false, true, 2>(g, st);
   return launch<4, 2, 2, 4, false, false, 2>(g, st);
 }

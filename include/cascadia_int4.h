@@ -546,6 +546,17 @@ int cascadia_int4_fp8_moe_forward(const cascadia_int4_fp8_moe_layer *layer, uint
                                   uint32_t n_tokens, void *out, uint32_t out_is_f32,
                                   void *workspace, void *stream);
 
+/* The kernel that a cascadia_int4_fp8_gemm of these sizes takes: 0 one row quantised
+ * where it is multiplied; 1, 2 outputs in 16 x 32 or 32 x 32 (rows x weight rows);
+ * 3, 4 tiles of 128 x 128, with K whole or in slices; 5, 6 tiles of 128 x 256, 256 x
+ * 256.  And the rows of a chunk in a cascadia_int4_fp8_moe_forward: 0 one token, 16,
+ * or 128 (on tiles).  Negative: CASCADIA_INT4_ERR_*.  Host only; for tests and
+ * profiles, the values may change with the rules. */
+int cascadia_int4_debug_fp8_gemm_form(uint32_t n_rows, uint32_t k_cols, uint32_t x_type,
+                                      uint32_t seq, uint32_t y_is_f32);
+int cascadia_int4_debug_fp8_moe_form(const cascadia_int4_fp8_moe_layer *layer, uint32_t top_k,
+                                     uint32_t n_tokens);
+
 /* Dequantise to f32 [n_rows, k_cols] (bit-exact w = q*s; the kernel's own
  * decode path).  No crate counterpart; the parity check of the weights. */
 int cascadia_int4_debug_dequant(const cascadia_int4_layout *layout, const uint8_t *packed,
