@@ -1,7 +1,11 @@
-"""Which kernel an 8-bit product takes (host only), and what the queries refuse."""
+"""Which kernel an 8-bit product takes (host only): every form is reached by sizes of
+the GPU tests, and what the queries refuse."""
 import ctypes as C
 
 import pytest
+
+from test_gpu_fp8 import GEMM_SIZES
+from test_gpu_fp8_tiles import SIZES, F32
 
 
 @pytest.fixture(scope="module")
@@ -9,6 +13,16 @@ def cl():
     import cascadia_amd
 
     return cascadia_amd
+
+
+def test_sizes_of_the_gpu_tests_take_every_form(cl):
+    f = cl.lib().cascadia_int4_debug_fp8_gemm_form
+    for want, m, n, k, dtype in SIZES:
+        assert f(n, k, 2, m, int(dtype == F32)) == want, (m, n, k)
+    # both output types of every tile form but the largest, which f32 does not take
+    assert {(w, d == F32) for w, _, _, _, d in SIZES} == {
+        (w, f32) for w in (3, 4, 5, 6) for f32 in (False, True) if w < 6 or not f32}
+    assert {f(n, k, t, m, 0) for m, n, k in GEMM_SIZES for t in (0, 2)} >= {0, 1, 2}
 
 
 @pytest.mark.parametrize("m,n,k,f32,tiles", [
