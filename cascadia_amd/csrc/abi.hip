@@ -2474,12 +2474,17 @@ int cascadia_int4_fp8_gemm(uint32_t n_rows, uint32_t k_cols, const uint8_t *w,
   const int blocks = cai4::fp8_blocks((int)k_cols), ld = cai4::fp8_ld((int)k_cols);
   // given scales are read where they are unless tiles want their rows aligned
   const bool one = seq == 1 && !codes && cai4::fp8_one_row((int)k_cols);  // quantised in its kernel
-  const bool tiles =
-      cai4::fp8_form((int)seq, (int)n_rows, (int)k_cols, y_is_f32 != 0) >= cai4::kFp8Tiles128;
-  const bool pad = codes && tiles && (blocks != ld || !aligned(x_scales, 16));
-  const bool use = (!codes && !one) || pad || (tiles && need.total > need.part);
+  const cai4::Fp8Form form =
+      cai4::fp8_form((int)seq, (int)n_rows, (int)k_cols, y_is_f32 != 0);
+  const bool split = form == cai4::kFp8Slices128;
+  const bool pad =
+      codes && form >= cai4::kFp8Tiles128 && (blocks != ld || !aligned(x_scales, 16));
+  // (what this call uses; _workspace_bytes, and what graphs record after it, are also
+  // for calls of fewer rows)
+  const bool use = (!codes && !one) || pad || split;
   if (use && !workspace)
-    if (int rc = own.get(dev, need.total, st, &workspace)) return rc;
+    if (int rc = own.get(dev, split ? need.total : need.part, st, &workspace, need.total))
+      return rc;
   cai4::Fp8Gemm g{};
   g.w = w;
   g.ws = w_scales;
