@@ -2349,9 +2349,14 @@ bool fp8_dims_ok(uint32_t n_rows, uint32_t k_cols) {
          k_cols % 16 == 0;
 }
 
-// Rows whose groups one launch takes.
+// Rows whose groups one launch takes (16 of them per 256 threads).
 bool fp8_rows_ok(uint32_t rows, uint32_t k_cols) {
-  return (size_t)rows * cai4::fp8_blocks((int)k_cols) <= (size_t)1 << 34;
+  return (size_t)rows * cai4::fp8_blocks((int)k_cols) < (size_t)1 << 28;
+}
+
+// Products whose tiles (of 256 x 128 outputs at least, 512 threads each) one launch takes.
+bool fp8_outputs_ok(uint32_t seq, uint32_t n_rows) {
+  return (size_t)seq * n_rows <= (size_t)1 << 37;
 }
 
 // The workspace of a call of up to seq rows: scales in rows of fp8_ld, then, of rows
@@ -2378,7 +2383,9 @@ int fp8_moe_check(const cascadia_int4_fp8_moe_layer *L, uint32_t top_k, uint32_t
       L->n_experts == 0 || L->n_experts > (uint32_t)cai4::kRouteMaxExperts || L->tiled > 1 ||
       top_k == 0 ||
       top_k > (uint32_t)cai4::kRouteMaxTopK || n_tokens == 0 || n_tokens > (1u << 20) ||
-      (size_t)n_tokens * L->hidden > 0x7FFFFFFFu)
+      (size_t)n_tokens * L->hidden > 0x7FFFFFFFu ||
+      !cai4::fp8_moe_fits((int)L->hidden, (int)L->inter, (int)L->n_experts, (int)top_k,
+                          (int)n_tokens))
     return CASCADIA_INT4_ERR_ARG;
   if (!aligned(L->gate_up, 16) || !aligned(L->down, 16) || !aligned(L->gate_up_scales, 4) ||
       !aligned(L->down_scales, 4))
@@ -2397,7 +2404,7 @@ int cascadia_int4_route_experts(const cascadia_int4_router *R, const void *logit
       R->n_groups == 0 || R->n_groups > (uint32_t)cai4::kRouteMaxGroups ||
       R->n_experts % R->n_groups || R->top_groups == 0 || R->top_groups > R->n_groups ||
       R->top_k > R->top_groups * (R->n_experts / R->n_groups) || R->group_best == 0 ||
-      R->group_best > 2 || logits_bf16 > 1 || n_tokens > (1u << 30))
+      R->group_best > 2 || logits_bf16 > 1 || n_tokens > (uint32_t)cai4::kRouteMaxTokens)
     return CASCADIA_INT4_ERR_ARG;
   if (n_tokens == 0) return CASCADIA_INT4_OK;
   if (!logits || !ids || !weights) return CASCADIA_INT4_ERR_NULL;
@@ -2447,7 +2454,8 @@ int cascadia_int4_fp8_quantize_blocks(const uint16_t *w_bf16, uint32_t n_rows, u
 size_t cascadia_int4_fp8_gemm_workspace_bytes(uint32_t n_rows, uint32_t k_cols, uint32_t x_type,
                                               uint32_t seq) {
   if (!fp8_dims_ok(n_rows, k_cols) || seq == 0 || seq > kFp8MaxRows ||
-      x_type > CASCADIA_INT4_FP8_X_E4M3 || !fp8_rows_ok(seq, k_cols))
+      x_type > CASCADIA_INT4_FP8_X_E4M3 || !fp8_rows_ok(seq, k_cols) ||
+      !fp8_outputs_ok(seq, n_rows))
     return 0;
   return fp8_workspace(n_rows, k_cols, x_type, seq).total;
 }
@@ -2461,7 +2469,7 @@ int cascadia_int4_fp8_gemm(uint32_t n_rows, uint32_t k_cols, const uint8_t *w,
   if (codes && !x_scales) return CASCADIA_INT4_ERR_NULL;
   if (!fp8_dims_ok(n_rows, k_cols) || seq == 0 || seq > kFp8MaxRows ||
       x_type > CASCADIA_INT4_FP8_X_E4M3 || (!codes && x_scales) || y_is_f32 > 1 ||
-      !fp8_rows_ok(seq, k_cols))
+      !fp8_rows_ok(seq, k_cols) || !fp8_outputs_ok(seq, n_rows))
     return CASCADIA_INT4_ERR_ARG;
   if (!aligned(w, 16) || !aligned(w_scales, 4) || !aligned(xs, 16) || !aligned(x_scales, 4) ||
       !aligned(ys, y_is_f32 ? 4 : 2) || !aligned(workspace, 16))
@@ -2517,7 +2525,8 @@ int cascadia_int4_fp8_gemm(uint32_t n_rows, uint32_t k_cols, const uint8_t *w,
 int cascadia_int4_debug_fp8_gemm_form(uint32_t n_rows, uint32_t k_cols, uint32_t x_type,
                                       uint32_t seq, uint32_t y_is_f32) {
   if (!fp8_dims_ok(n_rows, k_cols) || seq == 0 || seq > kFp8MaxRows ||
-      x_type > CASCADIA_INT4_FP8_X_E4M3 || y_is_f32 > 1)
+      x_type > CASCADIA_INT4_FP8_X_E4M3 || y_is_f32 > 1 || !fp8_rows_ok(seq, k_cols) ||
+      !fp8_outputs_ok(seq, n_rows))
     return CASCADIA_INT4_ERR_ARG;
   if (seq == 1 && x_type != CASCADIA_INT4_FP8_X_E4M3 && cai4::fp8_one_row((int)k_cols)) return 0;
   return cai4::fp8_form((int)seq, (int)n_rows, (int)k_cols, y_is_f32 != 0);
@@ -2538,8 +2547,9 @@ int cascadia_int4_fp8_tile_weights(uint32_t n_matrices, uint32_t n_rows, uint32_
                                    const uint8_t *codes, uint8_t *tiled, void *stream) {
   if (!codes || !tiled) return CASCADIA_INT4_ERR_NULL;
   if (!fp8_dims_ok(n_rows, k_cols) || n_matrices == 0 || n_matrices > (1u << 20) ||
-      (size_t)n_matrices * (cai4::fp8_tiled_bytes((int)n_rows, (int)k_cols) / cai4::kFp8BlockBytes) >
-          0x7FFFFFFFu)
+      !cai4::launch_fits((size_t)n_matrices * (cai4::fp8_tiled_bytes((int)n_rows, (int)k_cols) /
+                                               cai4::kFp8BlockBytes),
+                         256))
     return CASCADIA_INT4_ERR_ARG;
   if (!aligned(codes, 16) || !aligned(tiled, 16)) return CASCADIA_INT4_ERR_ARG;
   return hip_status(cai4::fp8_tile_weights(codes, (int)n_matrices, (int)n_rows, (int)k_cols, tiled,

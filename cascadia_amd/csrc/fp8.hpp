@@ -7,6 +7,12 @@
 
 namespace cai4 {
 
+// Whether a launch takes so many workgroups along one dimension of its grid: fewer
+// than 2^32 threads.
+inline bool launch_fits(size_t workgroups, size_t threads) {
+  return workgroups < ((size_t)1 << 32) / threads;
+}
+
 // Choice of top_k of E experts per token from router logits (route.hip).
 struct RouteExperts {
   const void *logits;  // [T, E], f32 or bf16
@@ -20,6 +26,7 @@ struct RouteExperts {
   float *weights;  // [T, top_k]
 };
 constexpr int kRouteMaxExperts = 1024, kRouteMaxTopK = 16, kRouteMaxGroups = 64;
+constexpr int kRouteMaxTokens = 1 << 25;  // (64 threads each)
 hipError_t route_experts(const RouteExperts &r, hipStream_t st);
 
 constexpr int kFp8Block = 128;
@@ -123,6 +130,7 @@ hipError_t fp8_gemv(const Fp8Gemm &g, const void *x, bool x_f32, hipStream_t st)
 hipError_t fp8_moe_one(const Fp8Moe &m, const Fp8Gemm &gate_up, const Fp8Gemm &down, float *h,
                        hipStream_t st);
 size_t fp8_moe_workspace(int H, int I, int E, int top_k, int T);
+bool fp8_moe_fits(int H, int I, int E, int top_k, int T);  // every launch_fits
 int fp8_moe_chunk_rows(int T, int E, int top_k);  // 16, or kFp8TileRows: on tiles
 hipError_t fp8_moe_forward(const Fp8Moe &m, void *workspace, hipStream_t st);
 

@@ -351,7 +351,7 @@ hipError_t few(const Fp8Gemm &g, hipStream_t st) {
   const int out = SW ? 16 : 32;
   const size_t tiles = (size_t)((g.N + out - 1) / out) *
                        (g.chunks ? g.max_chunks : (g.M + 16 * NT - 1) / (16 * NT));
-  if (tiles > 0x7FFFFFFFu) return hipErrorInvalidValue;
+  if (!launch_fits(tiles, 512)) return hipErrorInvalidValue;
   hipLaunchKernelGGL((fp8_few_kernel<NT, SW>), dim3((unsigned)tiles), dim3(512), 0, st, g);
   return hipGetLastError();
 }

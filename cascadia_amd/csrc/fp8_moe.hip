@@ -262,6 +262,14 @@ int fp8_moe_chunk_rows(int T, int E, int top_k) {
   return (int64_t)T * top_k >= (int64_t)kTileMean * E ? kFp8TileRows : 16;
 }
 
+bool fp8_moe_fits(int H, int I, int E, int top_k, int T) {
+  const Layout w = layout_of(H, I, E, top_k, T);
+  const bool tiles = w.chunk_rows == kFp8TileRows;
+  const size_t up = tiles ? (I + 127) / 128 : (I + 15) / 16;
+  const size_t down = tiles ? (H + 255) / 256 : (H + 31) / 32;
+  return launch_fits((up > down ? up : down) * w.max_chunks + 7, 512);
+}
+
 size_t fp8_moe_workspace(int H, int I, int E, int top_k, int T) {
   size_t most = 0;  // over all calls of up to T tokens
   auto take = [&](int t) {

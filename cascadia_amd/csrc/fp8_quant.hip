@@ -85,7 +85,7 @@ hipError_t fp8_tile_weights(const uint8_t *codes, int count, int N, int K, uint8
                             hipStream_t st) {
   const int NB = fp8_blocks(N), KB = fp8_blocks(K);
   const size_t blocks = (size_t)count * NB * KB;
-  if (blocks > 0x7FFFFFFFu) return hipErrorInvalidValue;
+  if (!launch_fits(blocks, 256)) return hipErrorInvalidValue;
   hipLaunchKernelGGL(fp8_arrange_kernel, dim3((unsigned)blocks), dim3(256), 0, st, codes, N, K, NB, KB,
                      tiled);
   return hipGetLastError();
@@ -96,7 +96,7 @@ hipError_t fp8_quantize_rows(const void *x, bool x_f32, size_t rows, int K, uint
   const int KB = fp8_blocks(K);
   const size_t groups = rows * KB;
   if (groups == 0) return hipSuccess;
-  if ((groups + kRowGroups - 1) / kRowGroups > 0x7FFFFFFFu) return hipErrorInvalidValue;
+  if (!launch_fits((groups + kRowGroups - 1) / kRowGroups, 256)) return hipErrorInvalidValue;
   const dim3 grid((unsigned)((groups + kRowGroups - 1) / kRowGroups)), block(256);
   if (x_f32)
     hipLaunchKernelGGL(fp8_rows_kernel<true>, grid, block, 0, st, x, groups, K, KB, codes, scales,
@@ -110,7 +110,7 @@ hipError_t fp8_quantize_rows(const void *x, bool x_f32, size_t rows, int K, uint
 hipError_t fp8_pad_scales(const float *scales, size_t rows, int KB, float *to, int ld,
                           hipStream_t st) {
   const size_t n = rows * KB;
-  if ((n + 255) / 256 > 0x7FFFFFFFu) return hipErrorInvalidValue;
+  if (!launch_fits((n + 255) / 256, 256)) return hipErrorInvalidValue;
   hipLaunchKernelGGL(fp8_pad_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, scales, n,
                      KB, to, ld);
   return hipGetLastError();

@@ -407,7 +407,7 @@ hipError_t launch(const Fp8Gemm &g, hipStream_t st, int n_first = 0, int count =
   const int nt = ((count < 0 ? g.N : count) + P::OUT - 1) / P::OUT;
   const int slices = g.kper ? (fp8_blocks(g.K) + g.kper - 1) / g.kper : 1;
   const size_t tiles = (size_t)nt * (g.chunks ? g.max_chunks : (g.M + P::BM - 1) / P::BM);
-  if (tiles > 0x7FFFFFF0u) return hipErrorInvalidValue;
+  if (!launch_fits(tiles + 7, 64 * P::W)) return hipErrorInvalidValue;
   hipLaunchKernelGGL((fp8_tile_kernel<NI, NJ, WN, WM, SW, EXACT, S>),
                      dim3((unsigned)((tiles + 7) / 8 * 8), slices), dim3(64 * P::W), 0, st, g,
                      n_first, nt);

@@ -451,7 +451,8 @@ int cascadia_int4_moe_forward(const cascadia_int4_moe_layer *layer,
  *     when normalize; times scale.
  * A NaN logit counts as -infinity.  Where the largest logit of a softmax is
  * +infinity its mass is shared by those that have it; a row of -infinity has
- * s = 0 throughout (weights 0).  top_k <= top_groups * n_experts / n_groups. */
+ * s = 0 throughout (weights 0).  top_k <= top_groups * n_experts / n_groups,
+ * n_tokens <= 2^25. */
 #define CASCADIA_INT4_SCORE_SOFTMAX 0u
 #define CASCADIA_INT4_SCORE_SIGMOID 1u
 typedef struct cascadia_int4_router {
@@ -475,7 +476,8 @@ int cascadia_int4_route_experts(const cascadia_int4_router *router, const void *
  * [rows, ceil(k_cols / 128)].  _quantize_blocks: bf16 weights [n_rows, k_cols]
  * in blocks of 128 x 128, scales [ceil(n_rows / 128), ceil(k_cols / 128)] (done
  * once, at load).  The last group of a row and the last blocks may be short.
- * k_cols: a multiple of 16; x, w and codes 16-byte aligned.  A group that holds
+ * k_cols: a multiple of 16, at most 2^20; rows <= 2^24, rows * ceil(k_cols / 128) <
+ * 2^28; n_rows of _quantize_blocks <= 2^22; x, w and codes 16-byte aligned.  A group that holds
  * an infinity or NaN stands for NaN wherever a product meets it (a NaN alone:
  * for its own code). */
 int cascadia_int4_fp8_quantize(const void *x, uint32_t x_is_f32, uint32_t rows, uint32_t k_cols,
@@ -492,7 +494,8 @@ int cascadia_int4_fp8_quantize_blocks(const uint16_t *w_bf16, uint32_t n_rows, u
  * (quantised in the call as by _quantize; x_scales NULL), or e4m3 codes with
  * x_scales [seq, ceil(k_cols / 128)].  k_cols a multiple of 16; w and xs 16-byte
  * aligned; ys overlaps no input.  workspace: 16-byte aligned, of at least
- * _workspace_bytes for seq rows or more, or NULL for the library's.  seq >= 1. */
+ * _workspace_bytes for seq rows or more, or NULL for the library's.  1 <= seq <= 2^24,
+ * seq * ceil(k_cols / 128) < 2^28, seq * n_rows <= 2^37. */
 #define CASCADIA_INT4_FP8_X_BF16 0u
 #define CASCADIA_INT4_FP8_X_F32 1u
 #define CASCADIA_INT4_FP8_X_E4M3 2u
@@ -507,7 +510,8 @@ int cascadia_int4_fp8_gemm(uint32_t n_rows, uint32_t k_cols, const uint8_t *w,
  * row), [n_matrices, ceil(n_rows / 128), ceil(k_cols / 128), 128, 128], rows and
  * columns past the matrix zero; _tiled_bytes is one matrix's size (0 on bad
  * dimensions).  Same codes, moved (once, at load): products over few rows per
- * expert stream them faster.  codes and tiled 16-byte aligned. */
+ * expert stream them faster.  codes and tiled 16-byte aligned; n_matrices <= 2^20, fewer
+ * than 2^24 blocks in all. */
 size_t cascadia_int4_fp8_tiled_bytes(uint32_t n_rows, uint32_t k_cols);
 int cascadia_int4_fp8_tile_weights(uint32_t n_matrices, uint32_t n_rows, uint32_t k_cols,
                                    const uint8_t *codes, uint8_t *tiled, void *stream);
@@ -537,7 +541,9 @@ typedef struct cascadia_int4_fp8_moe_layer {
  * token lists.  x [n_tokens, hidden] f32 (x_is_f32) or bf16; out f32
  * (out_is_f32) or bf16, residual of out's type or NULL; out may be x or
  * residual.  x, residual and out 16-byte aligned; top_k <= 16; 1 <= n_tokens <= 2^20,
- * n_tokens * hidden < 2^31.  workspace as above. */
+ * n_tokens * hidden < 2^31; chunks of an expert's rows (128, or 16 of fewer than eight
+ * rows per expert) times ceil(inter / 16) and ceil(hidden / 32) below 2^23.  workspace as
+ * above. */
 size_t cascadia_int4_fp8_moe_workspace_bytes(const cascadia_int4_fp8_moe_layer *layer,
                                              uint32_t top_k, uint32_t n_tokens);
 int cascadia_int4_fp8_moe_forward(const cascadia_int4_fp8_moe_layer *layer, uint32_t top_k,
