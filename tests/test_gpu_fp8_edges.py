@@ -7,7 +7,7 @@ import torch
 
 import fp8_ref as ref
 from test_gpu_fp8 import (check_gemm, check_moe, check_route, cl, gemm_case, gen, moe_case,  # noqa: F401
-                          normal, run_moe)
+                          normal, run_moe, run_route)
 
 pytestmark = pytest.mark.gpu
 F32, BF16 = torch.float32, torch.bfloat16
@@ -86,3 +86,19 @@ def test_one_token_slots_left_out(cl, out_dtype):
 def test_very_wide_layers(cl, T, H, I, E, k):
     for dt in (F32, BF16):
         check_moe(cl, moe_case(T + H, T, H, I, E, k, BF16), dt)
+
+
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("norm", [True, False])
+def test_route_weights_round_once(cl, score, norm):
+    """Scores, their sum, the division and the scale in 64 bits and one rounding at the
+    end.  (A softmax's sum adds exponentials e of 32 bits: each off by 2^-23 of itself,
+    and by half a step of its argument d, which renormalising takes out of the weights.)"""
+    logits = normal(gen(24), 300, 256) * 2
+    _, w = run_route(cl, logits, 8, score, None, 1, 1, 1, norm, 2.5)
+    _, want = ref.route(logits.double().numpy(), 8, score, None, 1, 1, 1, norm, 2.5)
+    steps = np.ones((300, 1))
+    if score == "softmax" and not norm:
+        d = (logits.max(1, keepdim=True).values - logits).double().numpy()
+        steps += (np.exp(-d) * (2 + d)).sum(1, keepdims=True) / np.exp(-d).sum(1, keepdims=True)
+    assert np.all(np.abs(w - want) <= steps * (1 + 1e-6) * ref.U32 * np.abs(want))
