@@ -1178,7 +1178,9 @@ class Fp8Experts:
     ceil(inter / 128)].  hidden and inter: multiples of 16.
     tiled (the default): the codes are copied once into blocks that stream faster,
     on the current stream; the tensors of codes are not kept and may be freed or
-    changed (the scales are read where they are).  tiled=False: they are read where they are."""
+    changed (the scales are read where they are).  The copy pads every matrix to whole
+    blocks (inter or hidden of 16: eight times the codes), and both are in memory while
+    it is made.  tiled=False: the codes are read where they are."""
 
     def __init__(self, gate_up, gate_up_scales, down, down_scales, n_experts: int, hidden: int,
                  inter: int, tiled: bool = True):

@@ -13,8 +13,8 @@
 // The 8-bit MFMAs do not add in f32: measured against 64 bits, the sum of a
 // block's 128 products is 1.5e-5 off (normal values; 5e-5 for codes spread over
 // all exponents), in every form of the instruction, where the same codes as bf16
-// (exact) give 1e-8.  The kernels here stream weights and have time to spare: the
-// products run on the bf16 MFMAs, codes converted in registers.
+// (exact) give 1e-8.  The kernels here stream weights (of some hundred rows they wait
+// for them), so that the products run on the bf16 MFMAs, codes converted in registers.
 //
 // Bound: HBM, every weight read once per 16 or 32 rows of x (of more rows: the
 // conversion of codes, and latency).  A workgroup's
@@ -22,7 +22,9 @@
 // contiguous kilobytes of each row; their sums are added through LDS in wave order.
 // Measured: 14336 x 4096, 16 rows 16 us (3.7 TB/s); 60 experts of 3584 x 1408 with 256
 // rows in all: gate and up 94 us (5.3 TB/s of the codes that rows meet); one row of 4096
-// x 4096 6.8 us, one token's 8 experts of 7168 x 2048 46.8 us (5.0 TB/s) and 30.5 us.
+// x 4096 6.6 us (on another card 9.3), one token's 8 experts of 7168 x 2048 46.6 us (5.0
+// TB/s) and 30.0 us.  A row whose codes are in hand takes fp8_few_kernel: 8.4 us a call
+// with weights from HBM, a bf16 row 9.1.
 #include "fp8.hpp"
 #include "fp8_common.hpp"
 #include "fp8_rows.hpp"
