@@ -1124,7 +1124,8 @@ def fp8_gemm(codes, scales, xs, n_rows: int, k_cols: int, seq: int, ys, x_scales
     f32, quantised in the call as by quantize_fp8, or e4m3 codes with x_scales
     [seq, ceil(k_cols / 128)].  ys [seq, n_rows] bf16 or f32, apart from the
     inputs; f32 sums, one rounding (bf16 of more than 16 rows: a block's products
-    may be added on the 8-bit matrix instructions, about 1.5e-5 of a result off).
+    may be added on the 8-bit matrix instructions, off by about 1.5e-5 of the
+    products' root sum of squares).
     workspace: fp8_gemm_workspace_bytes (for a graph capture)."""
     dev = _home(codes, "codes")
     n_rows, k_cols, seq = _index(n_rows), _index(k_cols), _index(seq)
@@ -1217,8 +1218,8 @@ def fp8_moe_forward(experts: Fp8Experts, x, out, *, top_k: int, ids, weights,
     """One MoE layer over e4m3 experts: out = residual + sum_k w_k down(q(silu(
     gate(q(x))) * up(q(x)))), q as quantize_fp8, f32 sums in slot order, one
     rounding (bf16 out of eight or more rows per expert: a block's products may be
-    added on the 8-bit matrix instructions, as fp8_gemm's).  x f32 or bf16, out f32 or bf16 (residual of out's type), all
-    [n_tokens, hidden]; ids (int32) / weights (f32) [n_tokens, top_k], as
+    added on the 8-bit matrix instructions, as fp8_gemm's).  x f32 or bf16, out f32 or
+    bf16 (residual of out's type), all [n_tokens, hidden]; ids (int32) / weights (f32) [n_tokens, top_k], as
     route_experts gives them.  Slots with a weight below threshold or an id
     outside the layer (padding: -1) are left out.  out may be residual or x.
     workspace: fp8_moe_workspace_bytes (for a graph capture)."""

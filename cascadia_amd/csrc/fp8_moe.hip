@@ -24,9 +24,10 @@ namespace cai4 {
 namespace {
 
 // Rows of a chunk: the tile kernel's from a mean of 8 rows per expert.  Measured, us,
-// 16-row chunks / tiles at a mean of 4, 8, 12 and 16 rows: 60 experts of 3584 x 1408,
-// even 176 / 194, 191 / 196, 214 / 201, 259 / 205; Zipf 154 / 163, 201 / 196, 235 /
-// 200, 269 / 207; 128 of 2048 x 1024, Zipf 132 / 131, 189 / 171, 234 / 183, 272 / 186.
+// 16-row chunks / tiles at a mean of 4, 8, 12 and 16 rows, bf16 out: 60 experts of 3584 x
+// 1408, even 177 / 191, 196 / 198, 217 / 202, 262 / 206; Zipf 158 / 176, 209 / 198, 238 /
+// 203, 271 / 209; 128 of 2048 x 1024, Zipf 138 / 132, 189 / 171, 232 / 181, 270 / 186.
+// f32 out, at 8 and 12: 196 / 219, 218 / 222; 209 / 219, 239 / 230; 189 / 196, 232 / 203.
 constexpr int kTileMean = 8;
 
 // Workgroups that count: 1,024 slots each, at most 64 (a placing workgroup adds

@@ -489,7 +489,9 @@ int cascadia_int4_fp8_quantize_blocks(const uint16_t *w_bf16, uint32_t n_rows, u
  * w_scale[r / 128, b] * sum_{c in b} x[t, c] w[r, c], f32 sums, one rounding:
  * ys [seq, n_rows] f32 (y_is_f32) or bf16.  (bf16 ys of more than 16 rows may add
  * a block's products on the 8-bit matrix instructions, which keep of every eight
- * the bits down to 2^-13 of the largest: about 1.5e-5 of a result.)  w: e4m3 codes [n_rows, k_cols] with
+ * the bits down to 2^-13 of the largest: 1.5e-5 of the products' root sum of squares,
+ * and so of a result that does not cancel; at most 2^-10 of the largest of every
+ * eight.  f32 ys: never.)  w: e4m3 codes [n_rows, k_cols] with
  * scales as _quantize_blocks lays them out.  xs [seq, k_cols]: bf16 or f32
  * (quantised in the call as by _quantize; x_scales NULL), or e4m3 codes with
  * x_scales [seq, ceil(k_cols / 128)].  k_cols a multiple of 16; w and xs 16-byte
