@@ -35,6 +35,9 @@ from .api import (GROUP_SIZE, HIDDEN, INTERMEDIATE, NIBBLES_PER_INT32, ExpertSou
                   moe_forward,
                   Fp8Experts, fp8_gemm, fp8_gemm_workspace_bytes, fp8_moe_forward,
                   fp8_moe_workspace_bytes, quantize_fp8, quantize_fp8_blocks, route_experts,
+                  Adapters, adapters_forward, adapters_workspace_bytes, combine_tokens,
+                  combine_tokens_grad, gather_tokens, gather_tokens_grad, sort_tokens,
+                  sort_tokens_workspace_bytes,
                   moe_workspace_bytes, ov_gemv, ov_to_crate, quantize_int4_group, tile_weights,
                   tiled_sizes)
 
@@ -60,5 +63,7 @@ __all__ = [
     "ffn_forward_sparse_f32_mode", "stream_read",
     "SCORE_SIGMOID", "SCORE_SOFTMAX", "Fp8Experts", "fp8_gemm", "fp8_gemm_workspace_bytes",
     "fp8_moe_forward", "fp8_moe_workspace_bytes", "quantize_fp8", "quantize_fp8_blocks",
-    "route_experts",
+    "route_experts", "Adapters", "adapters_forward", "adapters_workspace_bytes", "combine_tokens",
+    "combine_tokens_grad", "gather_tokens", "gather_tokens_grad", "sort_tokens",
+    "sort_tokens_workspace_bytes",
 ]

@@ -88,10 +88,17 @@ class Fp8MoeLayer(C.Structure):
                 ("down_scales", C.c_void_p), ("tiled", C.c_uint32)]
 
 
+class AdapterSet(C.Structure):
+    _fields_ = [("k_cols", C.c_uint32), ("n_rows", C.c_uint32), ("max_rank", C.c_uint32),
+                ("n_adapters", C.c_uint32), ("a", C.c_void_p), ("b", C.c_void_p),
+                ("ranks", C.c_void_p), ("scales", C.c_void_p)]
+
+
 _vp, _u32, _u64, _sz, _f64, _i32 = C.c_void_p, C.c_uint32, C.c_uint64, C.c_size_t, C.c_double, C.c_int
 _LP, _EP = C.POINTER(Layout), C.POINTER(Expert)
 _MP, _RP = C.POINTER(MoeLayer), C.POINTER(Routing)
 _FP = C.POINTER(Fp8MoeLayer)
+_AP = C.POINTER(AdapterSet)
 
 # Every symbol declared in include/cascadia_int4.h: (restype, argtypes).
 SIGNATURES = {
@@ -133,6 +140,17 @@ SIGNATURES = {
     "cascadia_int4_fp8_moe_workspace_bytes": (_sz, [_FP, _u32, _u32]),
     "cascadia_int4_fp8_moe_forward": (_i32, [_FP, _u32, _vp, _vp, C.c_float, _vp, _u32, _vp, _u32,
                                              _vp, _u32, _vp, _vp]),
+    "cascadia_int4_sort_tokens_workspace_bytes": (_sz, [_u32, _u32, _u32]),
+    "cascadia_int4_sort_tokens": (_i32, [_vp, _vp, C.c_float, _u32, _u32, _u32, _vp, _vp, _vp, _vp,
+                                         _vp]),
+    "cascadia_int4_gather_tokens": (_i32, [_vp, _u32, _vp, _u32, _u32, _u32, _vp, _u32, _vp]),
+    "cascadia_int4_combine_tokens": (_i32, [_vp, _u32, _vp, _vp, _vp, _u32, _u32, _u32, _vp, _u32,
+                                            _vp]),
+    "cascadia_int4_combine_tokens_grad": (_i32, [_vp, _u32, _vp, _u32, _vp, _vp, _u32, _u32, _u32,
+                                                 _vp, _vp, _vp]),
+    "cascadia_int4_adapters_workspace_bytes": (_sz, [_AP, _u32]),
+    "cascadia_int4_adapters_forward": (_i32, [_AP, _vp, _vp, _vp, _u32, _sz, _vp, _u32, _sz, _u32,
+                                              _vp, _u32, _sz, _vp, _vp]),
     "cascadia_int4_debug_fp8_gemm_form": (_i32, [_u32, _u32, _u32, _u32, _u32]),
     "cascadia_int4_debug_fp8_moe_form": (_i32, [_FP, _u32, _u32]),
     "cascadia_int4_debug_dequant": (_i32, [_LP, _vp, _vp, _vp, _vp]),

@@ -19,7 +19,7 @@ from operator import index as _index
 import numpy as np
 import torch
 
-from ._lib import (FP8_X_BF16, FP8_X_E4M3, FP8_X_F32, ROUTE_IDS, ROUTE_SIGMOID_BIAS,
+from ._lib import (AdapterSet, FP8_X_BF16, FP8_X_E4M3, FP8_X_F32, ROUTE_IDS, ROUTE_SIGMOID_BIAS,
                    ROUTE_SOFTMAX_TOPK, Expert, Fp8MoeLayer, Layout, MoeLayer, OvSegment, Router,
                    Routing, SCALE_BF16, SCALE_F16, SCORE_SIGMOID, SCORE_SOFTMAX, TILING_CRATE,
                    TILING_MFMA, TILING_MFMA_UP_ROWS, check, lib)
@@ -1256,6 +1256,257 @@ def fp8_moe_forward(experts: Fp8Experts, x, out, *, top_k: int, ids, weights,
         experts._ref, top_k, ids.data_ptr(), weights.data_ptr(), threshold, x.data_ptr(),
         int(x_f32), res, T, out.data_ptr(), int(out_f32), ws, _stream()))
     return out
+
+
+# ---------------------------------------------------------------------------
+# tokens sorted by expert and back, and low-rank adapters
+# ---------------------------------------------------------------------------
+
+def sort_tokens_workspace_bytes(n_tokens: int, top_k: int, n_experts: int) -> int:
+    """Workspace bytes of sort_tokens for up to n_tokens tokens."""
+    return int(lib().cascadia_int4_sort_tokens_workspace_bytes(n_tokens, top_k, n_experts))
+
+
+def _int32(dev, t, n, name):
+    _here(dev, t, name)
+    if not (t.dtype is torch.int32 and t.numel() == n):
+        raise ValueError(f"{name}: int32 of {n} values")
+
+
+def _row_weights(dev, weights, n):
+    _here(dev, weights, "weights")
+    if not (weights.dtype is torch.float32 and weights.numel() == n):
+        raise ValueError("weights: f32 [n_tokens, top_k]")
+
+
+def sort_tokens(ids, top_k: int, n_experts: int, offsets, slots, rows, *, weights=None,
+                threshold: float = 0.0, workspace=None):
+    """Sort the slots of ids (int32 [n_tokens, top_k], as route_experts gives them;
+    slot t * top_k + j) by expert, keeping their order within one:
+      offsets [n_experts + 1]: expert e has the sorted rows offsets[e] up to
+        offsets[e + 1]; the last is the number of rows.
+      slots [n_tokens * top_k]: the slot of each sorted row; behind the last row the
+        slots left out, ascending.
+      rows [n_tokens, top_k]: the sorted row of each slot, -1 where left out.
+    All int32.  Left out: ids outside [0, n_experts) (padding: -1) and, where weights
+    (f32 [n_tokens, top_k]) are given, slots of weight < threshold.  n_experts <= 1024,
+    top_k <= 16, n_tokens <= 2^20.  With top_k 1 it groups rows by adapter
+    (adapters_forward).  workspace: sort_tokens_workspace_bytes (for a graph capture)."""
+    dev = _home(offsets, "offsets")
+    top_k, n_experts = _index(top_k), _index(n_experts)
+    n = ids.numel()
+    _expect(1 <= top_k <= 16 and n % top_k == 0, "top_k: 1 to 16, ids [n_tokens, top_k]")
+    _expect(1 <= n_experts <= 1024, "n_experts: 1 to 1024")
+    _int32(dev, ids, n, "ids")
+    _int32(dev, offsets, n_experts + 1, "offsets")
+    _int32(dev, slots, n, "slots")
+    _int32(dev, rows, n, "rows")
+    wp = 0
+    if weights is not None:
+        _row_weights(dev, weights, n)
+        wp = weights.data_ptr()
+    ws = 0
+    if workspace is not None:
+        _here(dev, workspace, "workspace")
+        need = _need("cascadia_int4_sort_tokens_workspace_bytes", 0, dev, n // top_k, top_k,
+                     n_experts)
+        if workspace.nbytes < need:
+            raise ValueError(f"workspace has {workspace.nbytes} bytes, the call needs {need}")
+        ws = workspace.data_ptr()
+    check("cascadia_int4_sort_tokens", lib().cascadia_int4_sort_tokens(
+        ids.data_ptr(), wp, threshold, n // top_k, top_k, n_experts, offsets.data_ptr(),
+        slots.data_ptr(), rows.data_ptr(), ws, _stream()))
+    return offsets, slots, rows
+
+
+def _token_rows(dev, t, rows, top_k, per, name):
+    """(n_tokens, cols) of a call over rows [n_tokens, top_k] and t [n_tokens * per, cols]."""
+    n = rows.numel()
+    if not (1 <= top_k <= 16 and n % top_k == 0):
+        raise ValueError("top_k: 1 to 16, rows [n_tokens, top_k]")
+    _int32(dev, rows, n, "rows")
+    T = n // top_k
+    if t.dim() != 2 or t.shape[0] != T * per:
+        raise ValueError(f"{name} must be [{T * per}, cols]")
+    return T, t.shape[1]
+
+
+def _values(dev, t, count, name):
+    """Whether t (count values, f32 or bf16) is f32."""
+    _here(dev, t, name)
+    f32 = t.dtype is torch.float32
+    if not ((f32 or t.dtype is torch.bfloat16) and t.numel() == count):
+        raise ValueError(f"{name}: f32 or bf16 of {count} values")
+    return f32
+
+
+def gather_tokens(x, rows, xs, *, top_k: int):
+    """xs[rows[t, j]] = x[t] for the slots that sort_tokens has not left out: x
+    [n_tokens, cols], xs [n_tokens * top_k, cols], each bf16 or f32 (rounded to
+    nearest even), or both e4m3 (or uint8).  The other rows of xs stay as they are."""
+    dev = _home(x, "x")
+    top_k = _index(top_k)
+    T, cols = _token_rows(dev, x, rows, top_k, 1, "x")
+    _here(dev, xs, "xs")
+    xt, yt = _fp8_x_type(x.dtype), _fp8_x_type(xs.dtype)
+    if (xt == FP8_X_E4M3) != (yt == FP8_X_E4M3):
+        raise ValueError("x and xs: bf16 or f32, or both e4m3")
+    if xs.numel() != T * top_k * cols:
+        raise ValueError(f"xs must hold {T * top_k} rows of {cols}")
+    check("cascadia_int4_gather_tokens", lib().cascadia_int4_gather_tokens(
+        x.data_ptr(), xt, rows.data_ptr(), T, top_k, cols, xs.data_ptr(), yt, _stream()))
+    return xs
+
+
+def combine_tokens(ys, rows, out, *, top_k: int, weights=None, residual=None):
+    """out[t] = residual[t] + sum_j weights[t, j] * ys[rows[t, j]] over the slots that
+    sort_tokens has not left out: f32 sums in slot order, one rounding.  ys
+    [n_tokens * top_k, cols] and out [n_tokens, cols] bf16 or f32, weights f32
+    [n_tokens, top_k] (None: 1), residual of out's type (None: 0); out may be
+    residual."""
+    dev = _home(ys, "ys")
+    top_k = _index(top_k)
+    T, cols = _token_rows(dev, ys, rows, top_k, top_k, "ys")
+    y_f32 = _values(dev, ys, T * top_k * cols, "ys")
+    out_f32 = _values(dev, out, T * cols, "out")
+    wp = rp = 0
+    if weights is not None:
+        _row_weights(dev, weights, T * top_k)
+        wp = weights.data_ptr()
+    if residual is not None:
+        _here(dev, residual, "residual")
+        _expect(residual.dtype is out.dtype and residual.numel() == T * cols,
+                "residual: [n_tokens, cols] of out's type")
+        rp = residual.data_ptr()
+    check("cascadia_int4_combine_tokens", lib().cascadia_int4_combine_tokens(
+        ys.data_ptr(), int(y_f32), rows.data_ptr(), wp, rp, T, top_k, cols, out.data_ptr(),
+        int(out_f32), _stream()))
+    return out
+
+
+def gather_tokens_grad(dxs, rows, dx, *, top_k: int):
+    """The gradient of gather_tokens: dx[t] = sum_j dxs[rows[t, j]] (combine_tokens
+    without weights).  dxs [n_tokens * top_k, cols], dx [n_tokens, cols], bf16 or f32."""
+    return combine_tokens(dxs, rows, dx, top_k=top_k)
+
+
+def combine_tokens_grad(dout, ys, rows, weights, dys, dweights, *, top_k: int):
+    """The gradient of combine_tokens from that of its output, dout [n_tokens, cols]
+    (which is the residual's): dys[rows[t, j]] = weights[t, j] * dout[t], of ys's type
+    (rows that no slot has stay as they are; dys may be ys), and dweights[t, j] =
+    sum_c ys[rows[t, j], c] * dout[t, c] in f32 (0 for a slot left out).  dout and ys
+    bf16 or f32."""
+    dev = _home(ys, "ys")
+    top_k = _index(top_k)
+    T, cols = _token_rows(dev, ys, rows, top_k, top_k, "ys")
+    d_f32 = _values(dev, dout, T * cols, "dout")
+    y_f32 = _values(dev, ys, T * top_k * cols, "ys")
+    _here(dev, dys, "dys")
+    _expect(dys.dtype is ys.dtype and dys.numel() == ys.numel(), "dys: as ys")
+    _row_weights(dev, weights, T * top_k)
+    _here(dev, dweights, "dweights")
+    _expect(dweights.dtype is torch.float32 and dweights.numel() == T * top_k,
+            "dweights: f32 [n_tokens, top_k]")
+    check("cascadia_int4_combine_tokens_grad", lib().cascadia_int4_combine_tokens_grad(
+        dout.data_ptr(), int(d_f32), ys.data_ptr(), int(y_f32), rows.data_ptr(),
+        weights.data_ptr(), T, top_k, cols, dys.data_ptr(), dweights.data_ptr(), _stream()))
+    return dys, dweights
+
+
+class Adapters:
+    """Low-rank adapters of one projection: a [n_adapters, max_rank, k_cols], b
+    [n_adapters, n_rows, max_rank], bf16; adapter i is scales[i] * b_i[:, :r] a_i[:r]
+    with r = ranks[i] (int32, None: max_rank; what lies past it is not used) and scales
+    f32 (None: 1), both on the device and read by each call.  The tensors are read
+    where they are: an adapter is replaced by writing its slices.  k_cols and
+    max_rank multiples of 8, max_rank <= 256, n_adapters <= 1024."""
+
+    def __init__(self, a, b, *, ranks=None, scales=None):
+        dev = _home(a, "a")
+        _here(dev, b, "b")
+        _expect(a.dtype is torch.bfloat16 and b.dtype is torch.bfloat16 and a.dim() == 3
+                and b.dim() == 3, "a, b: bf16 [n_adapters, max_rank, k_cols], "
+                "[n_adapters, n_rows, max_rank]")
+        E, R, K = a.shape
+        N = b.shape[1]
+        _expect(b.shape[0] == E and b.shape[2] == R, "a and b differ in adapters or max_rank")
+        _expect(1 <= E <= 1024 and 8 <= R <= 256 and R % 8 == 0 and K >= 8 and K % 8 == 0 and N >= 1,
+                f"{E} adapters of rank {R}, {N} x {K}: ranks and columns are multiples of 8")
+        rp = sp = 0
+        if ranks is not None:
+            _int32(dev, ranks, E, "ranks")
+            rp = ranks.data_ptr()
+        if scales is not None:
+            _here(dev, scales, "scales")
+            _expect(scales.dtype is torch.float32 and scales.numel() == E, "scales: f32 [n_adapters]")
+            sp = scales.data_ptr()
+        self.a, self.b, self.ranks, self.scales = a, b, ranks, scales
+        self.n_adapters, self.max_rank, self.k_cols, self.n_rows = E, R, K, N
+        self._set = AdapterSet(K, N, R, E, a.data_ptr(), b.data_ptr(), rp, sp)
+        self._ref = C.byref(self._set)  # (the library only reads it)
+
+
+def adapters_workspace_bytes(adapters: Adapters, n_tokens: int) -> int:
+    """Workspace bytes of adapters_forward for up to n_tokens rows."""
+    return int(lib().cascadia_int4_adapters_workspace_bytes(adapters._ref, n_tokens))
+
+
+@functools.lru_cache(maxsize=1024)
+def _adapters_need(device, k_cols, n_rows, max_rank, n_adapters, n_tokens):
+    S = AdapterSet(k_cols, n_rows, max_rank, n_adapters, 256, 256, 0, 0)
+    return int(lib().cascadia_int4_adapters_workspace_bytes(C.byref(S), n_tokens))
+
+
+def _strided(dev, t, T, cols, name):
+    """(is f32, row stride) of t [T, cols], whose rows may lie apart."""
+    if not (isinstance(t, torch.Tensor) and t.is_cuda):
+        raise ValueError(f"{name} must be a device (HBM) tensor")
+    if t.get_device() != dev:
+        raise ValueError(f"{name} is on {t.device}, the current device is {dev}")
+    f32 = t.dtype is torch.float32
+    if not ((f32 or t.dtype is torch.bfloat16) and t.dim() == 2 and t.shape[0] == T
+            and t.shape[1] == cols):
+        raise ValueError(f"{name}: f32 or bf16 [{T}, {cols}]")
+    ld = t.stride(0) if T > 1 else cols
+    if (cols > 1 and t.stride(1) != 1) or ld < cols:
+        raise ValueError(f"{name}: rows of neighbouring values that do not overlap")
+    return f32, ld
+
+
+def adapters_forward(adapters: Adapters, xs, offsets, slots, ys, *, base=None, workspace=None):
+    """ys[t] = base[t] + scale_i b_i (a_i xs[t]) for the adapter i of row t, base[t] for
+    a row without one: the rows of many requests beside a projection that they share.
+    offsets, slots: sort_tokens(ids, 1, n_adapters, ...) of the rows' adapters (int32
+    [n_tokens], -1: none), made once for all projections of a batch.  xs [n_tokens,
+    k_cols], base (None: 0) and ys [n_tokens, n_rows], each bf16 or f32; their rows may
+    lie apart (slices of wider tensors).  ys may be base (rows without an adapter are
+    then not touched), otherwise overlaps no input.  f32 sums, one rounding.
+    workspace: adapters_workspace_bytes (for a graph capture)."""
+    dev = _home(offsets, "offsets")
+    A = adapters
+    _here(dev, A.a, "adapters")
+    T = slots.numel()
+    _int32(dev, offsets, A.n_adapters + 1, "offsets")
+    _int32(dev, slots, T, "slots")
+    x_f32, ldx = _strided(dev, xs, T, A.k_cols, "xs")
+    y_f32, ldy = _strided(dev, ys, T, A.n_rows, "ys")
+    b_f32, ldb, bp = False, 0, 0
+    if base is not None:
+        b_f32, ldb = _strided(dev, base, T, A.n_rows, "base")
+        bp = base.data_ptr()
+        if bp == ys.data_ptr() and (b_f32 != y_f32 or ldb != ldy):
+            raise ValueError("ys over base: of its type and stride")
+    ws = 0
+    if workspace is not None:
+        _here(dev, workspace, "workspace")
+        need = _adapters_need(dev, A.k_cols, A.n_rows, A.max_rank, A.n_adapters, T)
+        if workspace.nbytes < need:
+            raise ValueError(f"workspace has {workspace.nbytes} bytes, the call needs {need}")
+        ws = workspace.data_ptr()
+    check("cascadia_int4_adapters_forward", lib().cascadia_int4_adapters_forward(
+        A._ref, offsets.data_ptr(), slots.data_ptr(), xs.data_ptr(), int(x_f32), ldx, bp,
+        int(b_f32), ldb, T, ys.data_ptr(), int(y_f32), ldy, ws, _stream()))
+    return ys
 
 
 # ---------------------------------------------------------------------------

@@ -23,6 +23,7 @@
 #include "skinny.hpp"
 #include "sparse.hpp"
 #include "synth.hpp"
+#include "tokens.hpp"
 #include "tuning.hpp"
 
 namespace {
@@ -2601,6 +2602,205 @@ int cascadia_int4_fp8_moe_forward(const cascadia_int4_fp8_moe_layer *L, uint32_t
   m.out = out;
   m.out_f32 = (int)out_is_f32;
   return hip_status(cai4::fp8_moe_forward(m, workspace, st));
+}
+
+// ---- tokens sorted by expert and back, low-rank adapters ----
+
+namespace {
+
+bool slots_ok(uint32_t n_tokens, uint32_t top_k) {
+  return n_tokens <= (uint32_t)cai4::kSortMaxTokens && top_k >= 1 &&
+         top_k <= (uint32_t)cai4::kSortMaxTopK;
+}
+bool row_cols_ok(uint32_t cols) { return cols >= 1 && cols <= (uint32_t)cai4::kRowMaxCols; }
+
+int adapters_check(const cascadia_int4_adapters *A, uint32_t n_tokens) {
+  if (!A || !A->a || !A->b) return CASCADIA_INT4_ERR_NULL;
+  if (A->k_cols == 0 || A->k_cols % 8 || A->k_cols > (1u << 20) || A->n_rows == 0 ||
+      A->n_rows > (1u << 22) || A->max_rank == 0 || A->max_rank % 8 ||
+      A->max_rank > (uint32_t)cai4::kAdaptersMaxRank || A->n_adapters == 0 ||
+      A->n_adapters > (uint32_t)cai4::kSortMaxGroups ||
+      n_tokens > (uint32_t)cai4::kSortMaxTokens)
+    return CASCADIA_INT4_ERR_ARG;
+  if (!aligned(A->a, 16) || !aligned(A->b, 16) || !aligned(A->ranks, 4) ||
+      !aligned(A->scales, 4))
+    return CASCADIA_INT4_ERR_ARG;
+  return CASCADIA_INT4_OK;
+}
+
+}  // namespace
+
+size_t cascadia_int4_sort_tokens_workspace_bytes(uint32_t n_tokens, uint32_t top_k,
+                                                 uint32_t n_experts) {
+  if (!slots_ok(n_tokens, top_k) || n_experts == 0 ||
+      n_experts > (uint32_t)cai4::kSortMaxGroups)
+    return 0;
+  return cai4::sort_tokens_workspace((int)(n_tokens * top_k), (int)n_experts);
+}
+
+int cascadia_int4_sort_tokens(const int32_t *ids, const float *weights, float threshold,
+                              uint32_t n_tokens, uint32_t top_k, uint32_t n_experts,
+                              int32_t *offsets, int32_t *slots, int32_t *rows, void *workspace,
+                              void *stream) {
+  if (!slots_ok(n_tokens, top_k) || n_experts == 0 ||
+      n_experts > (uint32_t)cai4::kSortMaxGroups)
+    return CASCADIA_INT4_ERR_ARG;
+  if (!offsets || (n_tokens && (!ids || !slots || !rows))) return CASCADIA_INT4_ERR_NULL;
+  if (!aligned(ids, 4) || !aligned(weights, 4) || !aligned(offsets, 4) || !aligned(slots, 4) ||
+      !aligned(rows, 4) || !aligned(workspace, 16))
+    return CASCADIA_INT4_ERR_ARG;
+  cai4::SortTokens s{};
+  s.ids = ids;
+  s.weights = weights;
+  s.threshold = threshold;
+  s.n = (int)(n_tokens * top_k);
+  s.E = (int)n_experts;
+  s.offsets = offsets;
+  s.slots = slots;
+  s.rows = rows;
+  const hipStream_t st = (hipStream_t)stream;
+  Workspace own;
+  const size_t need = cai4::sort_tokens_workspace(s.n, s.E);
+  if (need && !workspace) {
+    int dev;
+    if (int rc = current_device(&dev)) return rc;
+    if (int rc = own.get(dev, need, st, &workspace)) return rc;
+  }
+  return hip_status(cai4::sort_tokens(s, workspace, st));
+}
+
+int cascadia_int4_gather_tokens(const void *x, uint32_t x_type, const int32_t *rows,
+                                uint32_t n_tokens, uint32_t top_k, uint32_t cols, void *xs,
+                                uint32_t xs_type, void *stream) {
+  if (!slots_ok(n_tokens, top_k) || !row_cols_ok(cols) || x_type > CASCADIA_INT4_FP8_X_E4M3 ||
+      xs_type > CASCADIA_INT4_FP8_X_E4M3 ||
+      (x_type == CASCADIA_INT4_FP8_X_E4M3) != (xs_type == CASCADIA_INT4_FP8_X_E4M3))
+    return CASCADIA_INT4_ERR_ARG;
+  if (n_tokens == 0) return CASCADIA_INT4_OK;
+  if (!x || !rows || !xs) return CASCADIA_INT4_ERR_NULL;
+  constexpr size_t size[3] = {2, 4, 1};
+  if (!aligned(x, size[x_type]) || !aligned(xs, size[xs_type]) || !aligned(rows, 4))
+    return CASCADIA_INT4_ERR_ARG;
+  static_assert(CASCADIA_INT4_FP8_X_BF16 == cai4::kRowBf16 &&
+                    CASCADIA_INT4_FP8_X_F32 == cai4::kRowF32 &&
+                    CASCADIA_INT4_FP8_X_E4M3 == cai4::kRowByte,
+                "types of rows");
+  return hip_status(cai4::gather_tokens(x, (cai4::RowType)x_type, rows, (int)n_tokens, (int)top_k,
+                                        (int)cols, xs, (cai4::RowType)xs_type,
+                                        (hipStream_t)stream));
+}
+
+int cascadia_int4_combine_tokens(const void *ys, uint32_t y_is_f32, const int32_t *rows,
+                                 const float *weights, const void *residual, uint32_t n_tokens,
+                                 uint32_t top_k, uint32_t cols, void *out, uint32_t out_is_f32,
+                                 void *stream) {
+  if (!slots_ok(n_tokens, top_k) || !row_cols_ok(cols) || y_is_f32 > 1 || out_is_f32 > 1)
+    return CASCADIA_INT4_ERR_ARG;
+  if (n_tokens == 0) return CASCADIA_INT4_OK;
+  if (!ys || !rows || !out) return CASCADIA_INT4_ERR_NULL;
+  const size_t o = out_is_f32 ? 4 : 2;
+  if (!aligned(ys, y_is_f32 ? 4 : 2) || !aligned(rows, 4) || !aligned(weights, 4) ||
+      !aligned(residual, o) || !aligned(out, o))
+    return CASCADIA_INT4_ERR_ARG;
+  cai4::CombineTokens c{};
+  c.ys = ys;
+  c.rows = rows;
+  c.weights = weights;
+  c.residual = residual;
+  c.out = out;
+  c.T = (int)n_tokens;
+  c.top_k = (int)top_k;
+  c.cols = (int)cols;
+  c.y_f32 = (int)y_is_f32;
+  c.out_f32 = (int)out_is_f32;
+  return hip_status(cai4::combine_tokens(c, (hipStream_t)stream));
+}
+
+int cascadia_int4_combine_tokens_grad(const void *dout, uint32_t dout_is_f32, const void *ys,
+                                      uint32_t y_is_f32, const int32_t *rows,
+                                      const float *weights, uint32_t n_tokens, uint32_t top_k,
+                                      uint32_t cols, void *dys, float *dweights, void *stream) {
+  if (!slots_ok(n_tokens, top_k) || !row_cols_ok(cols) || y_is_f32 > 1 || dout_is_f32 > 1)
+    return CASCADIA_INT4_ERR_ARG;
+  if (n_tokens == 0) return CASCADIA_INT4_OK;
+  if (!dout || !ys || !rows || !weights || !dys || !dweights) return CASCADIA_INT4_ERR_NULL;
+  const size_t y = y_is_f32 ? 4 : 2;
+  if (!aligned(dout, dout_is_f32 ? 4 : 2) || !aligned(ys, y) || !aligned(dys, y) ||
+      !aligned(rows, 4) || !aligned(weights, 4) || !aligned(dweights, 4))
+    return CASCADIA_INT4_ERR_ARG;
+  cai4::CombineGrad c{};
+  c.dout = dout;
+  c.ys = ys;
+  c.rows = rows;
+  c.weights = weights;
+  c.dys = dys;
+  c.dweights = dweights;
+  c.T = (int)n_tokens;
+  c.top_k = (int)top_k;
+  c.cols = (int)cols;
+  c.dout_f32 = (int)dout_is_f32;
+  c.y_f32 = (int)y_is_f32;
+  return hip_status(cai4::combine_tokens_grad(c, (hipStream_t)stream));
+}
+
+size_t cascadia_int4_adapters_workspace_bytes(const cascadia_int4_adapters *A,
+                                              uint32_t n_tokens) {
+  if (adapters_check(A, n_tokens)) return 0;
+  return cai4::adapters_workspace((int)A->k_cols, (int)A->max_rank, (int)A->n_adapters,
+                                  (int)n_tokens);
+}
+
+int cascadia_int4_adapters_forward(const cascadia_int4_adapters *A, const int32_t *offsets,
+                                   const int32_t *slots, const void *xs, uint32_t x_is_f32,
+                                   size_t x_stride, const void *base, uint32_t base_is_f32,
+                                   size_t base_stride, uint32_t n_tokens, void *ys,
+                                   uint32_t y_is_f32, size_t y_stride, void *workspace,
+                                   void *stream) {
+  if (int rc = adapters_check(A, n_tokens)) return rc;
+  if (x_is_f32 > 1 || base_is_f32 > 1 || y_is_f32 > 1) return CASCADIA_INT4_ERR_ARG;
+  if (n_tokens == 0) return CASCADIA_INT4_OK;
+  if (!offsets || !slots || !xs || !ys) return CASCADIA_INT4_ERR_NULL;
+  constexpr size_t kMostStride = (size_t)1 << 40;
+  if (x_stride < A->k_cols || y_stride < A->n_rows || (base && base_stride < A->n_rows) ||
+      x_stride > kMostStride || y_stride > kMostStride || base_stride > kMostStride)
+    return CASCADIA_INT4_ERR_ARG;
+  if (!aligned(offsets, 4) || !aligned(slots, 4) || !aligned(xs, x_is_f32 ? 4 : 2) ||
+      !aligned(base, base_is_f32 ? 4 : 2) || !aligned(ys, y_is_f32 ? 4 : 2) ||
+      !aligned(workspace, 16))
+    return CASCADIA_INT4_ERR_ARG;
+  // (in place: the same values, where they are)
+  if (base == ys && (base_is_f32 != y_is_f32 || base_stride != y_stride))
+    return CASCADIA_INT4_ERR_ARG;
+  cai4::Adapters a{};
+  a.K = (int)A->k_cols;
+  a.N = (int)A->n_rows;
+  a.R = (int)A->max_rank;
+  a.E = (int)A->n_adapters;
+  a.a = A->a;
+  a.b = A->b;
+  a.ranks = A->ranks;
+  a.scales = A->scales;
+  a.offsets = offsets;
+  a.slots = slots;
+  a.T = (int)n_tokens;
+  a.x = xs;
+  a.base = base;
+  a.y = ys;
+  a.ldx = x_stride;
+  a.ldb = base_stride;
+  a.ldy = y_stride;
+  a.x_f32 = (int)x_is_f32;
+  a.base_f32 = (int)base_is_f32;
+  a.y_f32 = (int)y_is_f32;
+  const hipStream_t st = (hipStream_t)stream;
+  Workspace own;
+  if (!workspace) {
+    int dev;
+    if (int rc = current_device(&dev)) return rc;
+    const size_t need = cascadia_int4_adapters_workspace_bytes(A, n_tokens);
+    if (int rc = own.get(dev, need, st, &workspace)) return rc;
+  }
+  return hip_status(cai4::adapters_forward(a, workspace, st));
 }
 
 }  // extern "C"

@@ -565,6 +565,103 @@ int cascadia_int4_debug_fp8_gemm_form(uint32_t n_rows, uint32_t k_cols, uint32_t
 int cascadia_int4_debug_fp8_moe_form(const cascadia_int4_fp8_moe_layer *layer, uint32_t top_k,
                                      uint32_t n_tokens);
 
+/* ---- tokens sorted by expert and back, and low-rank adapters ---- */
+
+/* Slots (token t, choice j; number t * top_k + j) sorted by expert: what a caller
+ * needs that runs a layer's experts itself, one by one or on another rank.  No
+ * counterpart in the crate, whose runner loops over tokens.
+ *   ids [n_tokens, top_k] int32, weights f32 or NULL: as route_experts gives them.
+ *     A slot with an id outside [0, n_experts) (padding: -1), or with weight <
+ *     threshold where weights are given, is left out.
+ *   offsets [n_experts + 1]: expert e has the sorted rows offsets[e] ..
+ *     offsets[e + 1] - 1, offsets[n_experts] rows in all.
+ *   slots [n_tokens * top_k]: the slot of each sorted row, ascending within an
+ *     expert; behind the last row the slots left out, ascending.
+ *   rows [n_tokens, top_k]: the sorted row of each slot, -1 where left out.
+ * n_experts <= 1024, top_k <= 16, n_tokens <= 2^20; zero tokens set offsets to 0.
+ * workspace: 16-byte aligned, of at least _workspace_bytes for these sizes or larger
+ * ones, or NULL for the library's.  With top_k 1 the same call groups a batch's
+ * rows by adapter (below). */
+size_t cascadia_int4_sort_tokens_workspace_bytes(uint32_t n_tokens, uint32_t top_k,
+                                                 uint32_t n_experts);
+int cascadia_int4_sort_tokens(const int32_t *ids, const float *weights, float threshold,
+                              uint32_t n_tokens, uint32_t top_k, uint32_t n_experts,
+                              int32_t *offsets, int32_t *slots, int32_t *rows, void *workspace,
+                              void *stream);
+
+/* xs[rows[t, j]] = x[t] for every slot that is not left out: x [n_tokens, cols], xs
+ * [n_tokens * top_k, cols], of types CASCADIA_INT4_FP8_X_* (bf16 and f32 in any
+ * pair, rounded to nearest even; e4m3 codes, or any bytes, to the same).  Rows of xs
+ * that no slot has are left as they are.  Values may start at any multiple of their
+ * own size; cols <= 2^20.  xs overlaps no input.  A row number outside
+ * [0, n_tokens * top_k) counts as left out; two slots with the same one (as
+ * sort_tokens never gives them) leave either's values there. */
+int cascadia_int4_gather_tokens(const void *x, uint32_t x_type, const int32_t *rows,
+                                uint32_t n_tokens, uint32_t top_k, uint32_t cols, void *xs,
+                                uint32_t xs_type, void *stream);
+
+/* out[t] = residual[t] + sum_j weights[t, j] * ys[rows[t, j]]: f32 sums in slot
+ * order (a fused multiply-add each), then the residual, one rounding.  ys
+ * [n_tokens * top_k, cols] f32 (y_is_f32) or bf16; weights NULL: 1; residual of out's
+ * type or NULL (0); out [n_tokens, cols] f32 (out_is_f32) or bf16, may be the
+ * residual, otherwise overlaps no input.  Rows and slots that are left out are not read.
+ * Without weights and residual it is the gradient of cascadia_int4_gather_tokens: ys the
+ * gradient of xs, out that of x. */
+int cascadia_int4_combine_tokens(const void *ys, uint32_t y_is_f32, const int32_t *rows,
+                                 const float *weights, const void *residual, uint32_t n_tokens,
+                                 uint32_t top_k, uint32_t cols, void *out, uint32_t out_is_f32,
+                                 void *stream);
+
+/* The gradient of cascadia_int4_combine_tokens from that of out, dout [n_tokens, cols]
+ * f32 (dout_is_f32) or bf16 (the residual's is dout itself):
+ *   dys[rows[t, j]] = weights[t, j] * dout[t], of ys's type, one rounding; rows that
+ *     no slot has are left as they are.  dys may be ys, otherwise overlaps no input.
+ *   dweights[t, j] = sum_c ys[rows[t, j], c] * dout[t, c] in f32; 0 for a slot left
+ *     out.  Sums in an order that depends on cols alone. */
+int cascadia_int4_combine_tokens_grad(const void *dout, uint32_t dout_is_f32, const void *ys,
+                                      uint32_t y_is_f32, const int32_t *rows,
+                                      const float *weights, uint32_t n_tokens, uint32_t top_k,
+                                      uint32_t cols, void *dys, float *dweights, void *stream);
+
+/* Low-rank adapters of one projection: a [n_adapters, max_rank, k_cols], b
+ * [n_adapters, n_rows, max_rank], bf16 bits, 16-byte aligned; adapter i is
+ * scales[i] * b_i[:, :r] a_i[:r, :] with r = ranks[i] (NULL: max_rank; clamped to
+ * [0, max_rank]; what lies past it is not used) and scales NULL: 1.  ranks and scales
+ * in device memory, read by each call. */
+typedef struct cascadia_int4_adapters {
+  uint32_t k_cols;     /* a multiple of 8, <= 2^20 */
+  uint32_t n_rows;     /* <= 2^22 */
+  uint32_t max_rank;   /* a multiple of 8, <= 256 */
+  uint32_t n_adapters; /* <= 1024 */
+  const uint16_t *a, *b;
+  const int32_t *ranks;
+  const float *scales;
+} cascadia_int4_adapters;
+
+/* ys[t] = base[t] + scale_i b_i (a_i xs[t]) for the adapter i of row t, and base[t]
+ * for a row without one: the rows of many requests beside a projection that they
+ * share (base: its output, by any of the products above; NULL: 0).
+ *   offsets, slots: cascadia_int4_sort_tokens of the rows' adapters [n_tokens]
+ *     (-1: none) with top_k 1 and n_experts = n_adapters; one call of it serves all
+ *     projections of a batch.
+ *   xs [n_tokens, k_cols], base and ys [n_tokens, n_rows], f32 (*_is_f32) or bf16,
+ *     rows *_stride values apart (parts of a wider buffer: the row of several
+ *     projections); xs of a row without an adapter is not read.  ys may be base (then of
+ *     its type and stride, and rows without an adapter are not touched), otherwise
+ *     overlaps no input.
+ * f32 sums; one rounding at the end.  f32 xs enter to 24 bits, the inner a_i xs[t]
+ * to 24 bits (f32 ys) or 16 (bf16).  An infinity of b may give NaN in place of an
+ * infinity.  n_tokens <= 2^20.  workspace: 16-byte aligned, of at least
+ * _workspace_bytes for n_tokens rows or more, or NULL for the library's. */
+size_t cascadia_int4_adapters_workspace_bytes(const cascadia_int4_adapters *adapters,
+                                              uint32_t n_tokens);
+int cascadia_int4_adapters_forward(const cascadia_int4_adapters *adapters,
+                                   const int32_t *offsets, const int32_t *slots, const void *xs,
+                                   uint32_t x_is_f32, size_t x_stride, const void *base,
+                                   uint32_t base_is_f32, size_t base_stride, uint32_t n_tokens,
+                                   void *ys, uint32_t y_is_f32, size_t y_stride, void *workspace,
+                                   void *stream);
+
 /* Dequantise to f32 [n_rows, k_cols] (bit-exact w = q*s; the kernel's own
  * decode path).  No crate counterpart; the parity check of the weights. */
 int cascadia_int4_debug_dequant(const cascadia_int4_layout *layout, const uint8_t *packed,
