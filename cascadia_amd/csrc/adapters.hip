@@ -8,6 +8,7 @@
 // Both products run on bf16 MFMAs with f32 sums.  A and B are bf16; f32 x, and u,
 // enter as a sum of bf16 planes, each the rounding of what the ones before left
 // over: three hold 24 bits, two (for bf16 y) 16.
+#include <array>
 #include <type_traits>
 
 #include "adapters_common.hpp"
@@ -49,144 +50,238 @@ CAI4_DEV void operands_of(const float (&v)[8], u32x4_t (&op)[N]) {
   }
 }
 
+// Bits to keep of columns r .. r + 7 of a row of B: those below the rank (the others
+// may hold anything).
+CAI4_DEV u32x4_t keep_of(int rank, int r) {
+  u32x4_t m;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    m[i] = (r + 2 * i < rank ? 0xFFFFu : 0u) | (r + 2 * i + 1 < rank ? 0xFFFF0000u : 0u);
+  return m;
+}
+
 // ---- u = A x ----
 
-constexpr int kRankTile = 64;  // ranks of a workgroup
+constexpr int kInWaves = 8;  // of a workgroup: each has its own columns
 
-template <bool F32>
-__global__ __launch_bounds__(256) void adapters_in_kernel(Adapters a, float *u, int slices) {
-  constexpr int P = F32 ? 3 : 1, RT = kRankTile / 16;
-  __shared__ f32x4_t part[4][RT * kTiles][64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int c = lane & 15, q = lane >> 4;
-  const Chunk ch = find_chunk(a, blockIdx.x, false);
-  if (ch.rows == 0) return;
-  const int rank = rank_of(a, ch.group), r0 = blockIdx.z * kRankTile;
-  if (r0 >= rank) return;
-  const int slice = blockIdx.y;
-  // blocks of 128 columns; a wave's are neighbours
-  const int blocks = (a.K + 127) / 128, parts = slices * 4, me = slice * 4 + wave;
-  const int b0 = (int)((int64_t)blocks * me / parts), b1 = (int)((int64_t)blocks * (me + 1) / parts);
+// A workgroup's slice of K for RT * 16 ranks and NT * 16 rows of a chunk.  A wave has
+// blocks [b0, b1) of 128 columns; the waves' sums are added in LDS, eight to four to
+// one.  Rows and ranks past the last ones repeat a valid one: nobody reads their sums.
+template <bool F32, int RT, int NT>
+CAI4_DEV void adapters_in_chunk(const Adapters &a, const Chunk &ch, int rank, int r0, int b0, int b1,
+                                f32x4_t (*part)[RT * kTiles][64], float *u) {
+  constexpr int P = F32 ? 3 : 1;
+  constexpr int S = F32 && NT > 1 ? 2 : 4;  // steps of 32 columns loaded at a time
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, q = lane >> 4;
   const uint16_t *A[RT];
-  bool a_in[RT];
 #pragma unroll
   for (int i = 0; i < RT; ++i) {
     const int r = r0 + i * 16 + c;
-    a_in[i] = r < rank;
-    A[i] = a.a + ((size_t)ch.group * a.R + (a_in[i] ? r : 0)) * a.K;
+    A[i] = a.a + ((size_t)ch.group * a.R + (r < rank ? r : r0)) * a.K;
   }
-  size_t xo[kTiles];
-  bool x_in[kTiles];
+  size_t xo[NT];
 #pragma unroll
-  for (int i = 0; i < kTiles; ++i) {
-    const int t = row_of(a, ch, i * 16 + c);
-    x_in[i] = t >= 0;
+  for (int i = 0; i < NT; ++i) {
+    const int k = i * 16 + c;
+    const int t = row_of(a, ch, k < ch.rows ? k : 0);
     xo[i] = (size_t)(t < 0 ? 0 : t) * a.ldx;
   }
-  f32x4_t acc[RT][kTiles] = {};
-  for (int b = b0; b < b1; ++b) {
+  f32x4_t acc[RT][NT] = {};
+  for (int at = b0 * 128; at < b1 * 128; at += S * 32) {
+    const bool whole = at + S * 32 <= a.K;
+    u32x4_t av[S][RT], xv[S][NT];
+    f32x4_t xf[S][NT][2];
 #pragma unroll
-    for (int s = 0; s < 4; ++s) {
-      const int col = b * 128 + q * 32 + s * 8;
-      const bool in = col < a.K;
-      u32x4_t av[RT] = {}, xv[kTiles][P] = {};
+    for (int s = 0; s < S; ++s) {
+      int col = at + s * 32 + q * 8;
+      col = whole || col < a.K ? col : 0;
 #pragma unroll
-      for (int i = 0; i < RT; ++i)
-        if (in && a_in[i]) av[i] = *reinterpret_cast<const u32x4_t *>(A[i] + col);
+      for (int i = 0; i < RT; ++i) av[s][i] = *reinterpret_cast<const u32x4_t *>(A[i] + col);
 #pragma unroll
-      for (int i = 0; i < kTiles; ++i) {
-        if (!(in && x_in[i])) continue;
+      for (int i = 0; i < NT; ++i) {
         if constexpr (F32) {
           const float *p = static_cast<const float *>(a.x) + xo[i] + col;
-          const Run<float, 4> lo = load_run<float, 4>(p), hi = load_run<float, 4>(p + 4);
-          const float v[8] = {lo.v[0], lo.v[1], lo.v[2], lo.v[3],
-                              hi.v[0], hi.v[1], hi.v[2], hi.v[3]};
-          operands_of<P>(v, xv[i]);
+          xf[s][i][0] = __builtin_bit_cast(f32x4_t, load_run<float, 4>(p));
+          xf[s][i][1] = __builtin_bit_cast(f32x4_t, load_run<float, 4>(p + 4));
         } else {
-          const Run<uint16_t, 8> v =
-              load_run<uint16_t, 8>(static_cast<const uint16_t *>(a.x) + xo[i] + col);
-          xv[i][0] = __builtin_bit_cast(u32x4_t, v);
+          xv[s][i] = __builtin_bit_cast(
+              u32x4_t, load_run<uint16_t, 8>(static_cast<const uint16_t *>(a.x) + xo[i] + col));
+        }
+      }
+    }
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+      if (!whole) {  // columns past the last: zero on both sides
+        const bool in = at + s * 32 + q * 8 < a.K;
+#pragma unroll
+        for (int i = 0; i < RT; ++i) av[s][i] = in ? av[s][i] : u32x4_t{0, 0, 0, 0};
+#pragma unroll
+        for (int i = 0; i < NT; ++i) {
+          if constexpr (F32) {
+            xf[s][i][0] = in ? xf[s][i][0] : f32x4_t{0.f, 0.f, 0.f, 0.f};
+            xf[s][i][1] = in ? xf[s][i][1] : f32x4_t{0.f, 0.f, 0.f, 0.f};
+          } else {
+            xv[s][i] = in ? xv[s][i] : u32x4_t{0, 0, 0, 0};
+          }
         }
       }
 #pragma unroll
-      for (int i = 0; i < RT; ++i)
+      for (int j = 0; j < NT; ++j) {
+        u32x4_t op[P];
+        if constexpr (F32) {
+          float v[8];
 #pragma unroll
-        for (int j = 0; j < kTiles; ++j)
+          for (int i = 0; i < 8; ++i) v[i] = xf[s][j][i / 4][i % 4];
+          operands_of<P>(v, op);
+        } else {
+          op[0] = xv[s][j];
+        }
 #pragma unroll
-          for (int p = 0; p < P; ++p) acc[i][j] = mfma_bf16(av[i], xv[j][p], acc[i][j]);
+        for (int i = 0; i < RT; ++i)
+#pragma unroll
+          for (int p = 0; p < P; ++p) acc[i][j] = mfma_bf16(av[s][i], op[p], acc[i][j]);
+      }
     }
   }
+  constexpr int kHalf = kInWaves / 2;
+  if (wave >= kHalf)
 #pragma unroll
-  for (int i = 0; i < RT; ++i)
+    for (int i = 0; i < RT; ++i)
 #pragma unroll
-    for (int j = 0; j < kTiles; ++j) part[wave][i * kTiles + j][lane] = acc[i][j];
+      for (int j = 0; j < NT; ++j) part[wave - kHalf][i * NT + j][lane] = acc[i][j];
+  __syncthreads();
+  if (wave < kHalf)
+#pragma unroll
+    for (int i = 0; i < RT; ++i)
+#pragma unroll
+      for (int j = 0; j < NT; ++j) part[wave][i * NT + j][lane] += acc[i][j];
   __syncthreads();
   // tile i, j: lane holds ranks r0 + 16 i + 4 q + [0, 4) of row 16 j + c
-  for (int k = wave; k < RT * kTiles; k += 4) {
-    const int i = k / kTiles, j = k % kTiles;
+  for (int k = wave; k < RT * NT; k += kInWaves) {
     f32x4_t v = part[0][k][lane];
 #pragma unroll
-    for (int w = 1; w < 4; ++w) v += part[w][k][lane];
-    const int r = r0 + i * 16 + q * 4, row = j * 16 + c;
+    for (int w = 1; w < kHalf; ++w) v += part[w][k][lane];
+    const int r = r0 + k / NT * 16 + q * 4, row = k % NT * 16 + c;
     if (r < a.R && row < ch.rows)
-      *reinterpret_cast<f32x4_t *>(u + ((size_t)slice * a.T + ch.row0 + row) * a.R + r) = v;
+      *reinterpret_cast<f32x4_t *>(u + (size_t)(ch.row0 + row) * a.R + r) = v;
   }
+}
+
+template <bool F32, int RT>
+__global__ __launch_bounds__(64 * kInWaves) void adapters_in_kernel(Adapters a, float *u,
+                                                                    int slices) {
+  __shared__ f32x4_t part[kInWaves / 2][RT * kTiles][64];
+  const int wave = threadIdx.x >> 6;
+  const Chunk ch = find_chunk(a, blockIdx.x, false);
+  if (ch.rows == 0) return;
+  const int rank = rank_of(a, ch.group), r0 = blockIdx.z * RT * 16;
+  if (r0 >= rank) return;
+  const int slice = blockIdx.y;
+  const int blocks = (a.K + 127) / 128, parts = slices * kInWaves, me = slice * kInWaves + wave;
+  const int b0 = (int)((int64_t)blocks * me / parts), b1 = (int)((int64_t)blocks * (me + 1) / parts);
+  u += (size_t)slice * a.T * a.R;
+  if (ch.rows <= 16)
+    adapters_in_chunk<F32, RT, 1>(a, ch, rank, r0, b0, b1, part, u);
+  else
+    adapters_in_chunk<F32, RT, kTiles>(a, ch, rank, r0, b0, b1, part, u);
 }
 
 // ---- y = base + B (s u) ----
 
-constexpr int kColBlock = 64;  // columns of a wave at a time
+constexpr int kOutWaves = 4, kColBlock = 64;  // columns of a wave at a time
 
-// What a lane adds to or writes of a row: 16 neighbouring columns.
-CAI4_DEV void load16(const void *p, bool f32, size_t at, int left, float (&v)[16]) {
-  if (f32) {
-    const float *s = static_cast<const float *>(p) + at;
-    if (left >= 16) {
+enum BaseType { kBaseNone, kBaseBf16, kBaseF32 };
+
+// Columns of a block that a lane (c, q) takes part with.  Its outputs are runs of 16
+// bytes, and four lanes' runs of a row are neighbours: f32 tile m is columns 16 m +
+// [0, 16); bf16 tiles 2 h and 2 h + 1 interleave four columns each.
+template <bool F32>
+CAI4_DEV int weight_col(int m, int c) {
+  return F32 ? m * 16 + c : (m >> 1) * 32 + (c >> 2) * 8 + (m & 1) * 4 + (c & 3);
+}
+
+// One block of 64 columns for NT * 16 rows.  STEPS of 32 ranks (0: as many as there
+// are, in a loop).
+template <bool F32, int BASE, int STEPS, int NT, bool FULL>
+CAI4_DEV void adapters_out_block(const Adapters &a, const uint16_t *B, int steps, const u32x4_t *mask,
+                                 int rank, const u32x4_t *us, const int (&row)[kTiles], int n0) {
+  constexpr int P = F32 ? 3 : 2, V = F32 ? 4 : 8, RUNS = 16 / V;
+  typedef typename std::conditional<F32, float, uint16_t>::type Y;
+  typedef typename std::conditional<BASE == kBaseF32, float, uint16_t>::type X;
+  const int lane = threadIdx.x & 63, c = lane & 15, q = lane >> 4;
+  const int left = a.N - n0;
+  Run<X, V> base[NT][RUNS];
+  if constexpr (BASE != kBaseNone) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const Run<float, 4> r = load_run<float, 4>(s + 4 * i);
+    for (int j = 0; j < NT; ++j) {
+      const X *p = static_cast<const X *>(a.base) + (size_t)(row[j] < 0 ? 0 : row[j]) * a.ldb + n0;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) v[4 * i + j] = r.v[j];
+      for (int i = 0; i < RUNS; ++i) {
+        const int at = i * (kColBlock / RUNS) + q * V;
+        if (FULL || at + V <= left)
+          base[j][i] = load_run<X, V>(p + at);
+        else
+          base[j][i] = load_part<X, V>(p + at, left - at);
       }
-    } else {
-#pragma unroll
-      for (int i = 0; i < 16; ++i) v[i] = i < left ? s[i] : 0.f;
     }
+  }
+  f32x4_t acc[NT][4] = {};
+  auto step_of = [&](int step) {
+    u32x4_t bv[4];
+    const int r = step * 32 + q * 8;
+#pragma unroll
+    for (int m = 0; m < 4; ++m) {
+      const int at = weight_col<F32>(m, c), n = FULL || at < left ? n0 + at : a.N - 1;
+      bv[m] = *reinterpret_cast<const u32x4_t *>(B + (size_t)n * a.R + (r < a.R ? r : 0));
+    }
+    return std::array<u32x4_t, 4>{bv[0], bv[1], bv[2], bv[3]};
+  };
+  auto add = [&](int step, std::array<u32x4_t, 4> bv, u32x4_t keep) {
+#pragma unroll
+    for (int m = 0; m < 4; ++m) bv[m] &= keep;
+#pragma unroll
+    for (int p = 0; p < P; ++p)
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        const u32x4_t uv = us[((step * P + p) * kTiles + j) * 64 + lane];
+#pragma unroll
+        for (int m = 0; m < 4; ++m) acc[j][m] = mfma_bf16(bv[m], uv, acc[j][m]);
+      }
+  };
+  if constexpr (STEPS > 0) {
+    std::array<u32x4_t, 4> bv[STEPS];
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s) bv[s] = step_of(s);
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s) add(s, bv[s], mask[s]);
   } else {
-    const uint16_t *s = static_cast<const uint16_t *>(p) + at;
-    if (left >= 16) {
+    for (int s = 0; s < steps; ++s) add(s, step_of(s), keep_of(rank, s * 32 + q * 8));
+  }
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const Run<uint16_t, 8> r = load_run<uint16_t, 8>(s + 8 * i);
+  for (int j = 0; j < NT; ++j) {
+    if (row[j] < 0) continue;
+    Y *p = static_cast<Y *>(a.y) + (size_t)row[j] * a.ldy + n0;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[8 * i + j] = bf16_to_f32(r.v[j]);
+    for (int i = 0; i < RUNS; ++i) {
+      const int at = i * (kColBlock / RUNS) + q * V;
+      Run<Y, V> y;
+#pragma unroll
+      for (int k = 0; k < V; ++k) {
+        const float d = acc[j][i * (V / 4) + k / 4][k % 4];
+        y.v[k] = row_value<Y>(BASE == kBaseNone ? d : value_of_row(base[j][i].v[k]) + d);
       }
-    } else {
-#pragma unroll
-      for (int i = 0; i < 16; ++i) v[i] = i < left ? bf16_to_f32(s[i]) : 0.f;
+      if (FULL || at + V <= left)
+        store_run<Y, V>(p + at, y);
+      else
+        store_part<Y, V>(p + at, y, left - at);
     }
   }
 }
-template <bool F32>
-CAI4_DEV void store16(void *p, size_t at, int left, const float (&v)[16]) {
-  typedef typename std::conditional<F32, float, uint16_t>::type T;
-  constexpr int V = 16 / sizeof(T);
-  T *d = static_cast<T *>(p) + at;
-#pragma unroll
-  for (int i = 0; i < 16 / V; ++i) {
-    Run<T, V> r;
-#pragma unroll
-    for (int j = 0; j < V; ++j) r.v[j] = row_value<T>(v[V * i + j]);
-    if (left >= 16)
-      store_run<T, V>(d + V * i, r);
-    else
-      store_part<T, V>(d + V * i, r, left - V * i);
-  }
-}
 
-template <bool F32>
-__global__ __launch_bounds__(256) void adapters_out_kernel(Adapters a, const float *u, int slices,
-                                                           int cols, int bare) {
+template <bool F32, int BASE, int STEPS>
+__global__ __launch_bounds__(64 * kOutWaves) void adapters_out_kernel(Adapters a, const float *u,
+                                                                      int slices, int cols,
+                                                                      int bare) {
   constexpr int P = F32 ? 3 : 2;
   extern __shared__ u32x4_t us[];  // [steps of 32 ranks][planes][tiles][lane]
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -194,79 +289,57 @@ __global__ __launch_bounds__(256) void adapters_out_kernel(Adapters a, const flo
   const Chunk ch = find_chunk(a, blockIdx.x, bare);
   if (ch.rows == 0) return;
   const bool own = ch.group < a.E;
-  const int rank = own ? rank_of(a, ch.group) : 0, steps = (rank + 31) / 32;
-  if (steps) {
-    const float s = a.scales ? a.scales[ch.group] : 1.0f;
-    for (int k = wave; k < steps * kTiles; k += 4) {
-      const int step = k / kTiles, j = k % kTiles;
-      const int r = step * 32 + q * 8, row = j * 16 + c;
-      float v[8] = {};
-      if (row < ch.rows && r < rank) {
-        for (int h = 0; h < slices; ++h) {
-          const f32x4_t *p = reinterpret_cast<const f32x4_t *>(
-              u + ((size_t)h * a.T + ch.row0 + row) * a.R + r);
-          const f32x4_t lo = p[0], hi = p[1];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            v[i] += lo[i];
-            v[4 + i] += hi[i];
-          }
-        }
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = r + i < rank ? v[i] * s : 0.f;
-      }
-      u32x4_t op[P];
-      operands_of<P>(v, op);
-#pragma unroll
-      for (int p = 0; p < P; ++p) us[((step * P + p) * kTiles + j) * 64 + lane] = op[p];
-    }
-    __syncthreads();
-  }
+  const int rank = own ? rank_of(a, ch.group) : 0;
+  const int steps = STEPS ? STEPS : (rank + 31) / 32, tiles = ch.rows <= 16 ? 1 : kTiles;
+  const float scale = own && a.scales ? a.scales[ch.group] : 1.0f;
   int row[kTiles];
 #pragma unroll
   for (int j = 0; j < kTiles; ++j) row[j] = row_of(a, ch, j * 16 + c);
-  const uint16_t *B = a.b + (size_t)(own ? ch.group : 0) * a.N * a.R;
-  const int n_end = (blockIdx.y + 1) * cols < a.N ? (blockIdx.y + 1) * cols : a.N;
-  for (int n0 = blockIdx.y * cols + wave * kColBlock; n0 < n_end; n0 += 4 * kColBlock) {
-    f32x4_t acc[4][kTiles] = {};
-    for (int step = 0; step < steps; ++step) {
-      u32x4_t bv[4];
-      const int r = step * 32 + q * 8;
+  for (int k = wave; k < steps * tiles; k += kOutWaves) {
+    const int step = k / tiles, j = k % tiles;
+    const int r = step * 32 + q * 8, i0 = j * 16 + c;
+    float v[8] = {};
+    if (i0 < ch.rows && r < rank) {
+      const float *p = u + (size_t)(ch.row0 + i0) * a.R + r;
+      const size_t stride = (size_t)a.T * a.R;
+      for (int h0 = 0; h0 < slices; h0 += 4) {  // (in order; four slices' loads at a time)
+        f32x4_t t[4][2];
 #pragma unroll
-      for (int m = 0; m < 4; ++m) {
-        // (tile m's row i is column 16 (i / 4) + 4 m + i % 4: a lane's outputs are
-        // neighbours)
-        const int n = n0 + (c >> 2) * 16 + m * 4 + (c & 3);
-        bv[m] = u32x4_t{0, 0, 0, 0};
-        if (n < a.N && r < rank) {
-          bv[m] = *reinterpret_cast<const u32x4_t *>(B + (size_t)n * a.R + r);
-          if (r + 8 > rank)  // columns past the rank may hold anything
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              bv[m][i] &= (r + 2 * i < rank ? 0xFFFFu : 0u) | (r + 2 * i + 1 < rank ? 0xFFFF0000u : 0u);
+        for (int h = 0; h < 4; ++h) {
+          const float *s = p + (h0 + h < slices ? h0 + h : h0) * stride;
+          t[h][0] = reinterpret_cast<const f32x4_t *>(s)[0];
+          t[h][1] = reinterpret_cast<const f32x4_t *>(s)[1];
         }
+#pragma unroll
+        for (int h = 0; h < 4; ++h)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) v[i] += h0 + h < slices ? t[h][i / 4][i % 4] : 0.f;
       }
 #pragma unroll
-      for (int p = 0; p < P; ++p)
-#pragma unroll
-        for (int j = 0; j < kTiles; ++j) {
-          const u32x4_t uv = us[((step * P + p) * kTiles + j) * 64 + lane];
-#pragma unroll
-          for (int m = 0; m < 4; ++m) acc[m][j] = mfma_bf16(bv[m], uv, acc[m][j]);
-        }
+      for (int i = 0; i < 8; ++i) v[i] = r + i < rank ? v[i] * scale : 0.f;
     }
-    const int n = n0 + q * 16, left = a.N - n;
-    if (left <= 0) continue;
+    u32x4_t op[P];
+    operands_of<P>(v, op);
 #pragma unroll
-    for (int j = 0; j < kTiles; ++j) {
-      if (row[j] < 0) continue;
-      float v[16] = {};
-      if (a.base) load16(a.base, a.base_f32, (size_t)row[j] * a.ldb + n, left, v);
+    for (int p = 0; p < P; ++p) us[((step * P + p) * kTiles + j) * 64 + lane] = op[p];
+  }
+  u32x4_t mask[STEPS ? STEPS : 1];
 #pragma unroll
-      for (int m = 0; m < 4; ++m)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v[4 * m + i] += acc[m][j][i];
-      store16<F32>(a.y, (size_t)row[j] * a.ldy + n, left, v);
+  for (int s = 0; s < STEPS; ++s) mask[s] = keep_of(rank, s * 32 + q * 8);
+  __syncthreads();
+  const uint16_t *B = a.b + (size_t)(own ? ch.group : 0) * a.N * a.R;
+  const int n_end = (blockIdx.y + 1) * cols < a.N ? (blockIdx.y + 1) * cols : a.N;
+  for (int n0 = blockIdx.y * cols + wave * kColBlock; n0 < n_end; n0 += kOutWaves * kColBlock) {
+    if (n0 + kColBlock <= a.N) {
+      if (tiles == 1)
+        adapters_out_block<F32, BASE, STEPS, 1, true>(a, B, steps, mask, rank, us, row, n0);
+      else
+        adapters_out_block<F32, BASE, STEPS, kTiles, true>(a, B, steps, mask, rank, us, row, n0);
+    } else {
+      if (tiles == 1)
+        adapters_out_block<F32, BASE, STEPS, 1, false>(a, B, steps, mask, rank, us, row, n0);
+      else
+        adapters_out_block<F32, BASE, STEPS, kTiles, false>(a, B, steps, mask, rank, us, row, n0);
     }
   }
 }
@@ -277,10 +350,58 @@ int max_chunks(int T, int E) { return (T < E ? T : E) + T / kChunkRows; }
 // Slices of K: enough that the first launch has some 512 workgroups, each wave at
 // least one block of 128 columns.
 constexpr int kInWorkgroups = 512;
+int rank_tiles(int R) { return R <= 16 ? 1 : R <= 32 ? 2 : 4; }  // of a workgroup
+int rank_groups(int R) { return (R + 16 * rank_tiles(R) - 1) / (16 * rank_tiles(R)); }
 int slices_of(int K, int R, int E, int T) {
-  const int most = ((K + 127) / 128 + 3) / 4;
-  const int s = kInWorkgroups / (max_chunks(T, E) * ((R + kRankTile - 1) / kRankTile));
+  const int most = ((K + 127) / 128 + kInWaves - 1) / kInWaves;
+  const int s = kInWorkgroups / (max_chunks(T, E) * rank_groups(R));
   return s < 1 ? 1 : s < most ? s : most;
+}
+
+// Columns of a workgroup of the second launch: whole rounds of its waves.
+constexpr int kOutWorkgroups = 1536;
+int cols_of(int N, int chunks) {
+  const int each = kOutWaves * kColBlock, blocks = (N + each - 1) / each;
+  const int per = (int)(((int64_t)blocks * chunks + kOutWorkgroups - 1) / kOutWorkgroups);
+  return each * (per < 1 ? 1 : per < blocks ? per : blocks);
+}
+
+template <bool F32, int BASE>
+void launch_out(const Adapters &a, const float *u, int slices, int bare, hipStream_t st) {
+  const int chunks = max_chunks(a.T, a.E + bare), cols = cols_of(a.N, chunks);
+  const int steps = (a.R + 31) / 32;
+  const dim3 grid(chunks, (a.N + cols - 1) / cols), block(64 * kOutWaves);
+  const size_t lds = (size_t)steps * (F32 ? 3 : 2) * kTiles * 64 * 16;
+  if (steps == 1)
+    hipLaunchKernelGGL((adapters_out_kernel<F32, BASE, 1>), grid, block, lds, st, a, u, slices,
+                       cols, bare);
+  else if (steps == 2)
+    hipLaunchKernelGGL((adapters_out_kernel<F32, BASE, 2>), grid, block, lds, st, a, u, slices,
+                       cols, bare);
+  else
+    hipLaunchKernelGGL((adapters_out_kernel<F32, BASE, 0>), grid, block, lds, st, a, u, slices,
+                       cols, bare);
+}
+template <bool F32>
+void launch_out(const Adapters &a, const float *u, int slices, int bare, hipStream_t st) {
+  if (!a.base)
+    launch_out<F32, kBaseNone>(a, u, slices, bare, st);
+  else if (a.base_f32)
+    launch_out<F32, kBaseF32>(a, u, slices, bare, st);
+  else
+    launch_out<F32, kBaseBf16>(a, u, slices, bare, st);
+}
+
+template <bool F32>
+void launch_in(const Adapters &a, float *u, int slices, hipStream_t st) {
+  const dim3 grid(max_chunks(a.T, a.E), slices, rank_groups(a.R)), block(64 * kInWaves);
+  const int rt = rank_tiles(a.R);
+  if (rt == 1)
+    hipLaunchKernelGGL((adapters_in_kernel<F32, 1>), grid, block, 0, st, a, u, slices);
+  else if (rt == 2)
+    hipLaunchKernelGGL((adapters_in_kernel<F32, 2>), grid, block, 0, st, a, u, slices);
+  else
+    hipLaunchKernelGGL((adapters_in_kernel<F32, 4>), grid, block, 0, st, a, u, slices);
 }
 
 }  // namespace
@@ -288,7 +409,7 @@ int slices_of(int K, int R, int E, int T) {
 size_t adapters_workspace(int K, int R, int E, int T) {
   // (a call of fewer rows may take more slices: T * slices stays below
   // kInWorkgroups * kChunkRows where there are any)
-  const size_t most = ((size_t)((K + 127) / 128) + 3) / 4;
+  const size_t most = ((size_t)((K + 127) / 128) + kInWaves - 1) / kInWaves;
   size_t rows = (size_t)T * most;
   if (rows > (size_t)kInWorkgroups * kChunkRows) rows = (size_t)kInWorkgroups * kChunkRows;
   if (rows < (size_t)T) rows = T;
@@ -298,21 +419,15 @@ size_t adapters_workspace(int K, int R, int E, int T) {
 hipError_t adapters_forward(const Adapters &a, void *workspace, hipStream_t st) {
   float *u = static_cast<float *>(workspace);
   const int slices = slices_of(a.K, a.R, a.E, a.T);
-  const int bare = !(a.base == a.y);
-  const dim3 in(max_chunks(a.T, a.E), slices, (a.R + kRankTile - 1) / kRankTile);
   if (a.x_f32)
-    hipLaunchKernelGGL(adapters_in_kernel<true>, in, dim3(256), 0, st, a, u, slices);
+    launch_in<true>(a, u, slices, st);
   else
-    hipLaunchKernelGGL(adapters_in_kernel<false>, in, dim3(256), 0, st, a, u, slices);
-  const int cols = 4 * kColBlock;
-  const dim3 out(max_chunks(a.T, a.E + bare), (a.N + cols - 1) / cols);
-  const size_t lds = (size_t)((a.R + 31) / 32) * (a.y_f32 ? 3 : 2) * kTiles * 64 * 16;
+    launch_in<false>(a, u, slices, st);
+  const int bare = a.base != a.y;  // (in place: rows without an adapter stay)
   if (a.y_f32)
-    hipLaunchKernelGGL(adapters_out_kernel<true>, out, dim3(256), lds, st, a, u, slices, cols,
-                       bare);
+    launch_out<true>(a, u, slices, bare, st);
   else
-    hipLaunchKernelGGL(adapters_out_kernel<false>, out, dim3(256), lds, st, a, u, slices, cols,
-                       bare);
+    launch_out<false>(a, u, slices, bare, st);
   return hipGetLastError();
 }
 

@@ -13,53 +13,60 @@ struct Chunk {
   int group, row0, rows;
 };
 
-// First sorted row of group e (group E: the rows without an adapter), within [0, T]
-// whatever the offsets hold.
+// First sorted row of group e (group E: the rows without an adapter; past it T), within
+// [0, T] whatever the offsets hold.
 CAI4_DEV int first_row(const Adapters &a, int e) {
-  const int v = e > a.E ? a.T : a.offsets[e];
-  return v < 0 ? 0 : v > a.T ? a.T : v;
+  const int v = a.offsets[e < a.E ? e : a.E];  // (loaded in any case: no branch)
+  return e > a.E || v > a.T ? a.T : v < 0 ? 0 : v;
 }
 CAI4_DEV int chunks_of(int first, int last) {
   return last > first ? (last - first + kChunkRows - 1) / kChunkRows : 0;
 }
 
-// Chunk b of all groups' in order (bare: group E among them).  By each wave for
-// itself: lane i adds up the chunks of `per` neighbouring groups.
-CAI4_DEV Chunk find_chunk(const Adapters &a, int b, bool bare) {
+// Sum of v over the lanes up to this one.
+CAI4_DEV int lanes_upto(int v) {
   const int lane = threadIdx.x & 63;
-  const int groups = a.E + (bare ? 1 : 0), per = (groups + 63) / 64, e0 = lane * per;
-  int n = 0;
-  if (e0 < groups) {
-    int first = first_row(a, e0);
-    for (int e = e0; e < e0 + per && e < groups; ++e) {
-      const int last = first_row(a, e + 1);
-      n += chunks_of(first, last);
-      first = last;
-    }
-  }
-  int upto = n;
 #pragma unroll
   for (int d = 1; d < 64; d *= 2) {
-    const int v = __shfl_up(upto, d);
-    if (lane >= d) upto += v;
+    const int u = __shfl_up(v, d);
+    if (lane >= d) v += u;
   }
+  return v;
+}
+
+// Chunk b of all groups' in order (bare: group E among them), by each wave for itself:
+// lane i holds the offsets of `per` neighbouring groups and adds up their chunks.
+CAI4_DEV Chunk find_chunk(const Adapters &a, int b, bool bare) {
+  constexpr int kMostPer = (kSortMaxGroups + 1 + 63) / 64;
+  const int lane = threadIdx.x & 63;
+  const int groups = a.E + (bare ? 1 : 0), per = (groups + 63) / 64;
+  int row[kMostPer + 1], n = 0;
+#pragma unroll
+  for (int i = 0; i <= kMostPer; ++i) {  // (every load before the first use)
+    const int e = lane * per + i;
+    if (i <= per) row[i] = first_row(a, e < groups ? e : groups);
+  }
+#pragma unroll
+  for (int i = 0; i < kMostPer; ++i)
+    if (i < per) n += chunks_of(row[i], row[i + 1]);
+  const int upto = lanes_upto(n);
   const uint64_t hit = __ballot(upto > b);
   if (!hit) return Chunk{0, 0, 0};
   const int l = __builtin_ctzll(hit);
-  int left = b - (__shfl(upto, l) - __shfl(n, l));
-  for (int e = l * per; e < (l + 1) * per && e < groups; ++e) {
-    const int first = first_row(a, e), last = first_row(a, e + 1), m = chunks_of(first, last);
-    if (left < m) {
-      const int row0 = first + left * kChunkRows;
-      Chunk ch{e, row0, last - row0 < kChunkRows ? last - row0 : kChunkRows};
-      ch.group = __builtin_amdgcn_readfirstlane(ch.group);
-      ch.row0 = __builtin_amdgcn_readfirstlane(ch.row0);
-      ch.rows = __builtin_amdgcn_readfirstlane(ch.rows);
-      return ch;
+  int left = b - __builtin_amdgcn_readlane(upto - n, l);
+  Chunk ch{0, 0, 0};
+#pragma unroll
+  for (int i = 0; i < kMostPer; ++i) {
+    if (i < per) {
+      const int first = __builtin_amdgcn_readlane(row[i], l);
+      const int last = __builtin_amdgcn_readlane(row[i + 1], l), m = chunks_of(first, last);
+      const int rows = last - first - left * kChunkRows;
+      if (left >= 0 && left < m)
+        ch = Chunk{l * per + i, first + left * kChunkRows, rows < kChunkRows ? rows : kChunkRows};
+      left -= m;  // (negative once found)
     }
-    left -= m;
   }
-  return Chunk{0, 0, 0};
+  return ch;
 }
 
 // The row of x and y that is row i of the chunk; -1: none.

@@ -5,8 +5,8 @@
 namespace cai4 {
 namespace {
 
-// V neighbouring values as they are stored: one load or store of V * sizeof(T)
-// bytes (8 or 16) aligned as T only.  Rows of odd widths start between words, which
+// V neighbouring values as they are stored: loads or stores of 8 or 16 bytes (32:
+// two) aligned as T only.  Rows of odd widths start between words, which
 // vector loads and stores allow.
 template <class T, int V>
 struct Run {
@@ -36,8 +36,13 @@ struct Whole<8, 2> {
 };
 template <class T, int V>
 CAI4_DEV Run<T, V> load_run(const T *p) {
-  typedef typename Whole<sizeof(T) * V, sizeof(T)>::type W;
-  return __builtin_bit_cast(Run<T, V>, *reinterpret_cast<const W *>(p));
+  if constexpr (sizeof(T) * V == 32) {
+    const Run<T, V / 2> h[2] = {load_run<T, V / 2>(p), load_run<T, V / 2>(p + V / 2)};
+    return __builtin_bit_cast(Run<T, V>, h);
+  } else {
+    typedef typename Whole<sizeof(T) * V, sizeof(T)>::type W;
+    return __builtin_bit_cast(Run<T, V>, *reinterpret_cast<const W *>(p));
+  }
 }
 template <class T, int V>
 CAI4_DEV void store_run(T *p, const Run<T, V> &r) {
@@ -79,8 +84,8 @@ CAI4_DEV float value_of_row(float v) { return v; }
 CAI4_DEV float value_of_row(uint16_t v) { return bf16_to_f32(v); }
 template <class T>
 CAI4_DEV T row_value(float v) {
-  if constexpr (sizeof(T) == 2)
-    return (T)f32_to_bf16_rne(v);
+  if constexpr (sizeof(T) == 2)  // (to nearest even, NaN kept quiet)
+    return __builtin_bit_cast(uint16_t, (__bf16)v);
   else
     return v;
 }
