@@ -200,103 +200,117 @@ CAI4_DEV int weight_col(int m, int c) {
   return F32 ? m * 16 + c : (m >> 1) * 32 + (c >> 2) * 8 + (m & 1) * 4 + (c & 3);
 }
 
-// One block of 64 columns for NT * 16 rows.  STEPS of 32 ranks (0: as many as there
-// are, in a loop).
-template <bool F32, int BASE, int STEPS, int NT, bool FULL>
-CAI4_DEV void adapters_out_block(const Adapters &a, const uint16_t *B, int steps, const u32x4_t *mask,
-                                 int rank, const u32x4_t *us, const int (&row)[kTiles], int n0) {
-  constexpr int P = F32 ? 3 : 2, V = F32 ? 4 : 8, RUNS = 16 / V;
+// What a block of 64 columns of NT * 16 rows reads: base, and B's rows (STEPS of 32
+// ranks; 0: as many as there are, read where they are multiplied).
+template <bool F32, int BASE, int STEPS, int NT>
+struct OutBlock {
+  static constexpr int P = F32 ? 3 : 2, V = F32 ? 4 : 8, RUNS = 16 / V;
   typedef typename std::conditional<F32, float, uint16_t>::type Y;
   typedef typename std::conditional<BASE == kBaseF32, float, uint16_t>::type X;
-  const int lane = threadIdx.x & 63, c = lane & 15, q = lane >> 4;
-  const int left = a.N - n0;
   Run<X, V> base[NT][RUNS];
-  if constexpr (BASE != kBaseNone) {
-#pragma unroll
-    for (int j = 0; j < NT; ++j) {
-      const X *p = static_cast<const X *>(a.base) + (size_t)(row[j] < 0 ? 0 : row[j]) * a.ldb + n0;
-#pragma unroll
-      for (int i = 0; i < RUNS; ++i) {
-        const int at = i * (kColBlock / RUNS) + q * V;
-        if (FULL || at + V <= left)
-          base[j][i] = load_run<X, V>(p + at);
-        else
-          base[j][i] = load_part<X, V>(p + at, left - at);
-      }
-    }
-  }
-  f32x4_t acc[NT][4] = {};
-  auto step_of = [&](int step) {
-    u32x4_t bv[4];
+  u32x4_t bv[STEPS ? STEPS : 1][4];
+
+  template <bool FULL>
+  CAI4_DEV void load_b(const Adapters &a, const uint16_t *B, int n0, int step, u32x4_t (&v)[4]) {
+    const int lane = threadIdx.x & 63, c = lane & 15, q = lane >> 4, left = a.N - n0;
     const int r = step * 32 + q * 8;
 #pragma unroll
     for (int m = 0; m < 4; ++m) {
       const int at = weight_col<F32>(m, c), n = FULL || at < left ? n0 + at : a.N - 1;
-      bv[m] = *reinterpret_cast<const u32x4_t *>(B + (size_t)n * a.R + (r < a.R ? r : 0));
+      v[m] = *reinterpret_cast<const u32x4_t *>(B + (size_t)n * a.R + (r < a.R ? r : 0));
     }
-    return std::array<u32x4_t, 4>{bv[0], bv[1], bv[2], bv[3]};
-  };
-  auto add = [&](int step, std::array<u32x4_t, 4> bv, u32x4_t keep) {
+  }
+  template <bool FULL>
+  CAI4_DEV void load(const Adapters &a, const uint16_t *B, const int (&row)[NT], int n0) {
+    const int q = (threadIdx.x & 63) >> 4, left = a.N - n0;
 #pragma unroll
-    for (int m = 0; m < 4; ++m) bv[m] &= keep;
-#pragma unroll
-    for (int p = 0; p < P; ++p)
+    for (int s = 0; s < STEPS; ++s) load_b<FULL>(a, B, n0, s, bv[s]);
+    if constexpr (BASE != kBaseNone) {
 #pragma unroll
       for (int j = 0; j < NT; ++j) {
-        const u32x4_t uv = us[((step * P + p) * kTiles + j) * 64 + lane];
+        const X *p =
+            static_cast<const X *>(a.base) + (size_t)(row[j] < 0 ? 0 : row[j]) * a.ldb + n0;
 #pragma unroll
-        for (int m = 0; m < 4; ++m) acc[j][m] = mfma_bf16(bv[m], uv, acc[j][m]);
+        for (int i = 0; i < RUNS; ++i) {
+          const int at = i * (kColBlock / RUNS) + q * V;
+          if constexpr (FULL)
+            base[j][i] = load_run<X, V>(p + at);
+          else
+            base[j][i] = load_part<X, V>(p + at, left - at);
+        }
       }
-  };
-  if constexpr (STEPS > 0) {
-    std::array<u32x4_t, 4> bv[STEPS];
-#pragma unroll
-    for (int s = 0; s < STEPS; ++s) bv[s] = step_of(s);
-#pragma unroll
-    for (int s = 0; s < STEPS; ++s) add(s, bv[s], mask[s]);
-  } else {
-    for (int s = 0; s < steps; ++s) add(s, step_of(s), keep_of(rank, s * 32 + q * 8));
-  }
-#pragma unroll
-  for (int j = 0; j < NT; ++j) {
-    if (row[j] < 0) continue;
-    Y *p = static_cast<Y *>(a.y) + (size_t)row[j] * a.ldy + n0;
-#pragma unroll
-    for (int i = 0; i < RUNS; ++i) {
-      const int at = i * (kColBlock / RUNS) + q * V;
-      Run<Y, V> y;
-#pragma unroll
-      for (int k = 0; k < V; ++k) {
-        const float d = acc[j][i * (V / 4) + k / 4][k % 4];
-        y.v[k] = row_value<Y>(BASE == kBaseNone ? d : value_of_row(base[j][i].v[k]) + d);
-      }
-      if (FULL || at + V <= left)
-        store_run<Y, V>(p + at, y);
-      else
-        store_part<Y, V>(p + at, y, left - at);
     }
   }
-}
+  template <bool FULL>
+  CAI4_DEV void finish(const Adapters &a, const uint16_t *B, int steps, int rank, const u32x4_t *us,
+                       const int (&row)[NT], int n0) {
+    const int lane = threadIdx.x & 63, q = lane >> 4, left = a.N - n0;
+    f32x4_t acc[NT][4] = {};
+    auto add = [&](int step, u32x4_t (&v)[4]) {
+      const u32x4_t keep = keep_of(rank, step * 32 + q * 8);
+#pragma unroll
+      for (int m = 0; m < 4; ++m) v[m] &= keep;
+#pragma unroll
+      for (int p = 0; p < P; ++p)
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+          const u32x4_t uv = us[((step * P + p) * NT + j) * 64 + lane];
+#pragma unroll
+          for (int m = 0; m < 4; ++m) acc[j][m] = mfma_bf16(v[m], uv, acc[j][m]);
+        }
+    };
+    if constexpr (STEPS > 0) {
+#pragma unroll
+      for (int s = 0; s < STEPS; ++s) add(s, bv[s]);
+    } else {
+      for (int s = 0; s < steps; ++s) {
+        load_b<FULL>(a, B, n0, s, bv[0]);
+        add(s, bv[0]);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      if (row[j] < 0) continue;
+      Y *p = static_cast<Y *>(a.y) + (size_t)row[j] * a.ldy + n0;
+#pragma unroll
+      for (int i = 0; i < RUNS; ++i) {
+        const int at = i * (kColBlock / RUNS) + q * V;
+        Run<Y, V> y;
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+          const float d = acc[j][i * (V / 4) + k / 4][k % 4];
+          y.v[k] = row_value<Y>(BASE == kBaseNone ? d : value_of_row(base[j][i].v[k]) + d);
+        }
+        if constexpr (FULL)
+          store_run(p + at, y);
+        else
+          store_part<Y, V>(p + at, y, left - at);
+      }
+    }
+  }
+};
 
-template <bool F32, int BASE, int STEPS>
-__global__ __launch_bounds__(64 * kOutWaves) void adapters_out_kernel(Adapters a, const float *u,
-                                                                      int slices, int cols,
-                                                                      int bare) {
-  constexpr int P = F32 ? 3 : 2;
-  extern __shared__ u32x4_t us[];  // [steps of 32 ranks][planes][tiles][lane]
+// A chunk's NT * 16 rows over columns [n_begin, n_end).  A block's loads are issued
+// before the one before it is multiplied, the first ones before u is read.
+template <bool F32, int BASE, int STEPS, int NT>
+CAI4_DEV void adapters_out_chunk(const Adapters &a, const Chunk &ch, const float *u, int slices,
+                                 int n_begin, int n_end, u32x4_t *us) {
+  constexpr int P = F32 ? 3 : 2, kStride = kOutWaves * kColBlock;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int c = lane & 15, q = lane >> 4;
-  const Chunk ch = find_chunk(a, blockIdx.x, bare);
-  if (ch.rows == 0) return;
   const bool own = ch.group < a.E;
-  const int rank = own ? rank_of(a, ch.group) : 0;
-  const int steps = STEPS ? STEPS : (rank + 31) / 32, tiles = ch.rows <= 16 ? 1 : kTiles;
+  const int rank = own ? rank_of(a, ch.group) : 0, steps = STEPS ? STEPS : (rank + 31) / 32;
   const float scale = own && a.scales ? a.scales[ch.group] : 1.0f;
-  int row[kTiles];
+  int row[NT];
 #pragma unroll
-  for (int j = 0; j < kTiles; ++j) row[j] = row_of(a, ch, j * 16 + c);
-  for (int k = wave; k < steps * tiles; k += kOutWaves) {
-    const int step = k / tiles, j = k % tiles;
+  for (int j = 0; j < NT; ++j) row[j] = row_of(a, ch, j * 16 + c);
+  const uint16_t *B = a.b + (size_t)(own ? ch.group : 0) * a.N * a.R;
+  int n0 = n_begin + wave * kColBlock;
+  const int n_full = n_end < a.N ? n_end : a.N / kColBlock * kColBlock;  // end of whole blocks
+  OutBlock<F32, BASE, STEPS, NT> now, next;
+  if (n0 < n_full) now.template load<true>(a, B, row, n0);
+  for (int k = wave; k < steps * NT; k += kOutWaves) {
+    const int step = k / NT, j = k % NT;
     const int r = step * 32 + q * 8, i0 = j * 16 + c;
     float v[8] = {};
     if (i0 < ch.rows && r < rank) {
@@ -321,27 +335,34 @@ __global__ __launch_bounds__(64 * kOutWaves) void adapters_out_kernel(Adapters a
     u32x4_t op[P];
     operands_of<P>(v, op);
 #pragma unroll
-    for (int p = 0; p < P; ++p) us[((step * P + p) * kTiles + j) * 64 + lane] = op[p];
+    for (int p = 0; p < P; ++p) us[((step * P + p) * NT + j) * 64 + lane] = op[p];
   }
-  u32x4_t mask[STEPS ? STEPS : 1];
-#pragma unroll
-  for (int s = 0; s < STEPS; ++s) mask[s] = keep_of(rank, s * 32 + q * 8);
   __syncthreads();
-  const uint16_t *B = a.b + (size_t)(own ? ch.group : 0) * a.N * a.R;
-  const int n_end = (blockIdx.y + 1) * cols < a.N ? (blockIdx.y + 1) * cols : a.N;
-  for (int n0 = blockIdx.y * cols + wave * kColBlock; n0 < n_end; n0 += kOutWaves * kColBlock) {
-    if (n0 + kColBlock <= a.N) {
-      if (tiles == 1)
-        adapters_out_block<F32, BASE, STEPS, 1, true>(a, B, steps, mask, rank, us, row, n0);
-      else
-        adapters_out_block<F32, BASE, STEPS, kTiles, true>(a, B, steps, mask, rank, us, row, n0);
-    } else {
-      if (tiles == 1)
-        adapters_out_block<F32, BASE, STEPS, 1, false>(a, B, steps, mask, rank, us, row, n0);
-      else
-        adapters_out_block<F32, BASE, STEPS, kTiles, false>(a, B, steps, mask, rank, us, row, n0);
-    }
+  while (n0 < n_full) {
+    const int n1 = n0 + kStride;
+    if (n1 < n_full) next.template load<true>(a, B, row, n1);
+    now.template finish<true>(a, B, steps, rank, us, row, n0);
+    now = next;
+    n0 = n1;
   }
+  if (n0 < n_end && n0 < a.N) {  // the last columns
+    now.template load<false>(a, B, row, n0);
+    now.template finish<false>(a, B, steps, rank, us, row, n0);
+  }
+}
+
+template <bool F32, int BASE, int STEPS>
+__global__ __launch_bounds__(64 * kOutWaves) void adapters_out_kernel(Adapters a, const float *u,
+                                                                      int slices, int cols,
+                                                                      int bare) {
+  extern __shared__ u32x4_t us[];  // [steps of 32 ranks][planes][tiles][lane]
+  const Chunk ch = find_chunk(a, blockIdx.x, bare);
+  if (ch.rows == 0) return;
+  const int n0 = blockIdx.y * cols, n1 = n0 + cols < a.N ? n0 + cols : a.N;
+  if (ch.rows <= 16)
+    adapters_out_chunk<F32, BASE, STEPS, 1>(a, ch, u, slices, n0, n1, us);
+  else
+    adapters_out_chunk<F32, BASE, STEPS, kTiles>(a, ch, u, slices, n0, n1, us);
 }
 
 // Chunks that T rows over E groups may make.

@@ -34,20 +34,26 @@ template <>
 struct Whole<8, 2> {
   typedef u32x2_by2_t type;
 };
-template <class T, int V>
+// STREAM: past the caches' replacement, for data that would fill them many times over.
+template <class T, int V, bool STREAM = false>
 CAI4_DEV Run<T, V> load_run(const T *p) {
   if constexpr (sizeof(T) * V == 32) {
     const Run<T, V / 2> h[2] = {load_run<T, V / 2>(p), load_run<T, V / 2>(p + V / 2)};
     return __builtin_bit_cast(Run<T, V>, h);
   } else {
     typedef typename Whole<sizeof(T) * V, sizeof(T)>::type W;
-    return __builtin_bit_cast(Run<T, V>, *reinterpret_cast<const W *>(p));
+    const W *w = reinterpret_cast<const W *>(p);
+    return __builtin_bit_cast(Run<T, V>, STREAM ? __builtin_nontemporal_load(w) : *w);
   }
 }
-template <class T, int V>
+template <bool STREAM = false, class T, int V>
 CAI4_DEV void store_run(T *p, const Run<T, V> &r) {
   typedef typename Whole<sizeof(T) * V, sizeof(T)>::type W;
-  *reinterpret_cast<W *>(p) = __builtin_bit_cast(W, r);
+  W *w = reinterpret_cast<W *>(p);
+  if constexpr (STREAM)
+    __builtin_nontemporal_store(__builtin_bit_cast(W, r), w);
+  else
+    *w = __builtin_bit_cast(W, r);
 }
 // The first n (< V) of them.
 template <class T, int V>
@@ -65,17 +71,17 @@ CAI4_DEV void store_part(T *p, const Run<T, V> &r, int n) {
 }
 // A whole run, or its first n values.  FULL is a constant of the code around: a run
 // that may be either is loaded value by value by the compiler.
-template <bool FULL, class T, int V>
+template <bool FULL, class T, int V, bool STREAM = false>
 CAI4_DEV Run<T, V> load_some(const T *p, int n) {
   if constexpr (FULL)
-    return load_run<T, V>(p);
+    return load_run<T, V, STREAM>(p);
   else
     return load_part<T, V>(p, n);
 }
-template <bool FULL, class T, int V>
+template <bool FULL, bool STREAM = false, class T, int V>
 CAI4_DEV void store_some(T *p, const Run<T, V> &r, int n) {
   if constexpr (FULL)
-    store_run<T, V>(p, r);
+    store_run<STREAM>(p, r);
   else
     store_part<T, V>(p, r, n);
 }

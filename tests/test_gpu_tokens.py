@@ -88,7 +88,8 @@ def test_sort_no_tokens_and_refusals(cl):
         with pytest.raises(ValueError):
             cl.sort_tokens(**a)
     ws = torch.empty(64, dtype=torch.uint8, device="cuda")
-    big = torch.zeros(4096, dtype=torch.int32, device="cuda")
+    big = torch.zeros(65536, dtype=torch.int32, device="cuda")
+    assert cl.sort_tokens_workspace_bytes(65536, 1, 8) > 64
     with pytest.raises(ValueError):
         cl.sort_tokens(big, 1, 8, off, big.clone(), big.clone(), workspace=ws)
 
