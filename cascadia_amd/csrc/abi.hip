@@ -2760,7 +2760,7 @@ int cascadia_int4_adapters_forward(const cascadia_int4_adapters *A, const int32_
   if (x_is_f32 > 1 || base_is_f32 > 1 || y_is_f32 > 1) return CASCADIA_INT4_ERR_ARG;
   if (n_tokens == 0) return CASCADIA_INT4_OK;
   if (!offsets || !slots || !xs || !ys) return CASCADIA_INT4_ERR_NULL;
-  constexpr size_t kMostStride = (size_t)1 << 40;
+  constexpr size_t kMostStride = (size_t)1 << 29;  // (bytes in 32 bits)
   if (x_stride < A->k_cols || y_stride < A->n_rows || (base && base_stride < A->n_rows) ||
       x_stride > kMostStride || y_stride > kMostStride || base_stride > kMostStride)
     return CASCADIA_INT4_ERR_ARG;
@@ -2786,9 +2786,9 @@ int cascadia_int4_adapters_forward(const cascadia_int4_adapters *A, const int32_
   a.x = xs;
   a.base = base;
   a.y = ys;
-  a.ldx = x_stride;
-  a.ldb = base_stride;
-  a.ldy = y_stride;
+  a.ldx = (uint32_t)(x_stride * (x_is_f32 ? 4 : 2));
+  a.ldb = (uint32_t)(base_stride * (base_is_f32 ? 4 : 2));
+  a.ldy = (uint32_t)(y_stride * (y_is_f32 ? 4 : 2));
   a.x_f32 = (int)x_is_f32;
   a.base_f32 = (int)base_is_f32;
   a.y_f32 = (int)y_is_f32;

@@ -69,7 +69,7 @@ constexpr int kInWaves = 8;  // of a workgroup: each has its own columns
 // one.  Rows and ranks past the last ones repeat a valid one: nobody reads their sums.
 template <bool F32, int RT, int NT>
 CAI4_DEV void adapters_in_chunk(const Adapters &a, const Chunk &ch, int rank, int r0, int b0, int b1,
-                                f32x4_t (*part)[RT * kTiles][64], float *u) {
+                                f32x4_t (*part)[RT * NT][64], float *u) {
   constexpr int P = F32 ? 3 : 1;
   constexpr int S = F32 && NT > 1 ? 2 : 4;  // steps of 32 columns loaded at a time
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, q = lane >> 4;
@@ -79,12 +79,12 @@ CAI4_DEV void adapters_in_chunk(const Adapters &a, const Chunk &ch, int rank, in
     const int r = r0 + i * 16 + c;
     A[i] = a.a + ((size_t)ch.group * a.R + (r < rank ? r : r0)) * a.K;
   }
-  size_t xo[NT];
+  const uint8_t *x[NT];
 #pragma unroll
   for (int i = 0; i < NT; ++i) {
     const int k = i * 16 + c;
     const int t = row_of(a, ch, k < ch.rows ? k : 0);
-    xo[i] = (size_t)(t < 0 ? 0 : t) * a.ldx;
+    x[i] = static_cast<const uint8_t *>(a.x) + (size_t)(t < 0 ? 0 : t) * a.ldx;
   }
   f32x4_t acc[RT][NT] = {};
   for (int at = b0 * 128; at < b1 * 128; at += S * 32) {
@@ -100,12 +100,12 @@ CAI4_DEV void adapters_in_chunk(const Adapters &a, const Chunk &ch, int rank, in
 #pragma unroll
       for (int i = 0; i < NT; ++i) {
         if constexpr (F32) {
-          const float *p = static_cast<const float *>(a.x) + xo[i] + col;
+          const float *p = reinterpret_cast<const float *>(x[i]) + col;
           xf[s][i][0] = __builtin_bit_cast(f32x4_t, load_run<float, 4>(p));
           xf[s][i][1] = __builtin_bit_cast(f32x4_t, load_run<float, 4>(p + 4));
         } else {
           xv[s][i] = __builtin_bit_cast(
-              u32x4_t, load_run<uint16_t, 8>(static_cast<const uint16_t *>(a.x) + xo[i] + col));
+              u32x4_t, load_run<uint16_t, 8>(reinterpret_cast<const uint16_t *>(x[i]) + col));
         }
       }
     }
@@ -167,23 +167,19 @@ CAI4_DEV void adapters_in_chunk(const Adapters &a, const Chunk &ch, int rank, in
   }
 }
 
-template <bool F32, int RT>
+template <bool F32, int RT, int NT>
 __global__ __launch_bounds__(64 * kInWaves) void adapters_in_kernel(Adapters a, float *u,
                                                                     int slices) {
-  __shared__ f32x4_t part[kInWaves / 2][RT * kTiles][64];
+  __shared__ f32x4_t part[kInWaves / 2][RT * NT][64];
   const int wave = threadIdx.x >> 6;
-  const Chunk ch = find_chunk(a, blockIdx.x, false);
+  const Chunk ch = find_chunk<16 * NT>(a, blockIdx.x, false);
   if (ch.rows == 0) return;
   const int rank = rank_of(a, ch.group), r0 = blockIdx.z * RT * 16;
   if (r0 >= rank) return;
   const int slice = blockIdx.y;
   const int blocks = (a.K + 127) / 128, parts = slices * kInWaves, me = slice * kInWaves + wave;
   const int b0 = (int)((int64_t)blocks * me / parts), b1 = (int)((int64_t)blocks * (me + 1) / parts);
-  u += (size_t)slice * a.T * a.R;
-  if (ch.rows <= 16)
-    adapters_in_chunk<F32, RT, 1>(a, ch, rank, r0, b0, b1, part, u);
-  else
-    adapters_in_chunk<F32, RT, kTiles>(a, ch, rank, r0, b0, b1, part, u);
+  adapters_in_chunk<F32, RT, NT>(a, ch, rank, r0, b0, b1, part, u + (size_t)slice * a.T * a.R);
 }
 
 // ---- y = base + B (s u) ----
@@ -192,16 +188,23 @@ constexpr int kOutWaves = 4, kColBlock = 64;  // columns of a wave at a time
 
 enum BaseType { kBaseNone, kBaseBf16, kBaseF32 };
 
-// Columns of a block that a lane (c, q) takes part with.  Its outputs are runs of 16
-// bytes, and four lanes' runs of a row are neighbours: f32 tile m is columns 16 m +
-// [0, 16); bf16 tiles 2 h and 2 h + 1 interleave four columns each.
+// Outputs leave the MFMAs as 16 columns of row c in lane (c, q), in RUNS runs of 16
+// bytes (of y's type).  Four lanes' runs of one row are 64 bytes, half a line; lanes c
+// and c ^ 1 exchange every second run, so that a store writes whole lines of the
+// eight even rows, the next those of the odd ones (4,096 x 14,336 in bf16 past the
+// caches, copied so: 37.5 us, in half lines 50).  f32: run m is columns 16 m + 4 q of
+// the block, tile m; bf16: run h is 32 h + 8 q, tiles 2 h and 2 h + 1 with four
+// columns each in turn.
 template <bool F32>
 CAI4_DEV int weight_col(int m, int c) {
   return F32 ? m * 16 + c : (m >> 1) * 32 + (c >> 2) * 8 + (m & 1) * 4 + (c & 3);
 }
+// Lane c ^ 1's value.
+CAI4_DEV float of_pair(float v) { return dpp_f32<0xB1>(v); }
 
 // What a block of 64 columns of NT * 16 rows reads: base, and B's rows (STEPS of 32
-// ranks; 0: as many as there are, read where they are multiplied).
+// ranks; 0: as many as there are, read where they are multiplied).  Run i of tile j of
+// a lane is of row pair_row[j][i & 1] (-1: none), columns run_col(i) on.
 template <bool F32, int BASE, int STEPS, int NT>
 struct OutBlock {
   static constexpr int P = F32 ? 3 : 2, V = F32 ? 4 : 8, RUNS = 16 / V;
@@ -209,6 +212,13 @@ struct OutBlock {
   typedef typename std::conditional<BASE == kBaseF32, float, uint16_t>::type X;
   Run<X, V> base[NT][RUNS];
   u32x4_t bv[STEPS ? STEPS : 1][4];
+
+  // Runs 2 i and 2 i + 1 of a lane after the exchange: both of the even lane's run 2 i
+  // (c even) or run 2 i + 1 (c odd), of the even row and of the odd one.
+  static CAI4_DEV int run_col(int i) {
+    const int lane = threadIdx.x & 63;
+    return ((i & ~1) + (lane & 1)) * (kColBlock / RUNS) + (lane >> 4) * V;
+  }
 
   template <bool FULL>
   CAI4_DEV void load_b(const Adapters &a, const uint16_t *B, int n0, int step, u32x4_t (&v)[4]) {
@@ -220,97 +230,123 @@ struct OutBlock {
       v[m] = *reinterpret_cast<const u32x4_t *>(B + (size_t)n * a.R + (r < a.R ? r : 0));
     }
   }
+  // Row r of p, made anew at each use: eight addresses kept would be 16 registers.
+  template <class T>
+  static CAI4_DEV T *row_at(T *p, uint32_t ld, int r) {
+    uint32_t t = r < 0 ? 0 : r;
+    asm volatile("" : "+v"(t));
+    typedef typename std::conditional<std::is_const<T>::value, const uint8_t, uint8_t>::type B;
+    return reinterpret_cast<T *>(reinterpret_cast<B *>(p) + (uint64_t)t * ld);
+  }
   template <bool FULL>
-  CAI4_DEV void load(const Adapters &a, const uint16_t *B, const int (&row)[NT], int n0) {
-    const int q = (threadIdx.x & 63) >> 4, left = a.N - n0;
+  CAI4_DEV void load(const Adapters &a, const uint16_t *B, const int (&row)[NT][2], int n0) {
+    const int left = a.N - n0;
 #pragma unroll
     for (int s = 0; s < STEPS; ++s) load_b<FULL>(a, B, n0, s, bv[s]);
     if constexpr (BASE != kBaseNone) {
 #pragma unroll
-      for (int j = 0; j < NT; ++j) {
-        const X *p =
-            static_cast<const X *>(a.base) + (size_t)(row[j] < 0 ? 0 : row[j]) * a.ldb + n0;
+      for (int j = 0; j < NT; ++j)
 #pragma unroll
-        for (int i = 0; i < RUNS; ++i) {
-          const int at = i * (kColBlock / RUNS) + q * V;
-          if constexpr (FULL)
-            base[j][i] = load_run<X, V>(p + at);
-          else
-            base[j][i] = load_part<X, V>(p + at, left - at);
+        for (int h = 0; h < 2; ++h) {
+          const X *p = row_at(static_cast<const X *>(a.base) + n0, a.ldb, row[j][h]);
+#pragma unroll
+          for (int i = h; i < RUNS; i += 2) {
+            const int at = run_col(i);
+            if constexpr (FULL)
+              base[j][i] = load_run<X, V>(p + at);
+            else
+              base[j][i] = load_part<X, V>(p + at, left - at);
+          }
         }
-      }
     }
   }
-  template <bool FULL>
+  // (A tile of 16 rows at a time: fewer sums at once, more waves.)
+  template <bool FULL, bool STREAM, int RW>
   CAI4_DEV void finish(const Adapters &a, const uint16_t *B, int steps, int rank, const u32x4_t *us,
-                       const int (&row)[NT], int n0) {
+                       const int (&row)[NT][2], int n0) {
     const int lane = threadIdx.x & 63, q = lane >> 4, left = a.N - n0;
-    f32x4_t acc[NT][4] = {};
-    auto add = [&](int step, u32x4_t (&v)[4]) {
-      const u32x4_t keep = keep_of(rank, step * 32 + q * 8);
+    const bool odd = lane & 1;
 #pragma unroll
-      for (int m = 0; m < 4; ++m) v[m] &= keep;
+    for (int s = 0; s < STEPS; ++s) {
+      const u32x4_t keep = keep_of(rank, s * 32 + q * 8);
 #pragma unroll
-      for (int p = 0; p < P; ++p)
-#pragma unroll
-        for (int j = 0; j < NT; ++j) {
-          const u32x4_t uv = us[((step * P + p) * NT + j) * 64 + lane];
-#pragma unroll
-          for (int m = 0; m < 4; ++m) acc[j][m] = mfma_bf16(v[m], uv, acc[j][m]);
-        }
-    };
-    if constexpr (STEPS > 0) {
-#pragma unroll
-      for (int s = 0; s < STEPS; ++s) add(s, bv[s]);
-    } else {
-      for (int s = 0; s < steps; ++s) {
-        load_b<FULL>(a, B, n0, s, bv[0]);
-        add(s, bv[0]);
-      }
+      for (int m = 0; m < 4; ++m) bv[s][m] &= keep;
     }
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
-      if (row[j] < 0) continue;
-      Y *p = static_cast<Y *>(a.y) + (size_t)row[j] * a.ldy + n0;
+      f32x4_t acc[4] = {};
+      auto add = [&](int step, const u32x4_t (&v)[4]) {
 #pragma unroll
-      for (int i = 0; i < RUNS; ++i) {
-        const int at = i * (kColBlock / RUNS) + q * V;
-        Run<Y, V> y;
+        for (int p = 0; p < P; ++p) {
+          const u32x4_t uv = us[((step * P + p) * RW * NT + j) * 64 + lane];
+#pragma unroll
+          for (int m = 0; m < 4; ++m) acc[m] = mfma_bf16(v[m], uv, acc[m]);
+        }
+      };
+      if constexpr (STEPS > 0) {
+#pragma unroll
+        for (int s = 0; s < STEPS; ++s) add(s, bv[s]);
+      } else {
+        for (int s = 0; s < steps; ++s) {
+          const u32x4_t keep = keep_of(rank, s * 32 + q * 8);
+          load_b<FULL>(a, B, n0, s, bv[0]);
+#pragma unroll
+          for (int m = 0; m < 4; ++m) bv[0][m] &= keep;
+          add(s, bv[0]);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < RUNS; i += 2) {
+        Run<Y, V> y[2];  // of the even row, of the odd one
 #pragma unroll
         for (int k = 0; k < V; ++k) {
-          const float d = acc[j][i * (V / 4) + k / 4][k % 4];
-          y.v[k] = row_value<Y>(BASE == kBaseNone ? d : value_of_row(base[j][i].v[k]) + d);
+          const float lo = acc[i * (V / 4) + k / 4][k % 4];
+          const float hi = acc[(i + 1) * (V / 4) + k / 4][k % 4];
+          const float got = of_pair(odd ? lo : hi);
+          const float d[2] = {odd ? got : lo, odd ? hi : got};
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+            y[h].v[k] = row_value<Y>(
+                BASE == kBaseNone ? d[h] : value_of_row(base[j][i + h].v[k]) + d[h]);
         }
-        if constexpr (FULL)
-          store_run(p + at, y);
-        else
-          store_part<Y, V>(p + at, y, left - at);
+        const int at = run_col(i);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          if (row[j][h] < 0) continue;
+          Y *p = row_at(static_cast<Y *>(a.y) + n0, a.ldy, row[j][h]);
+          if constexpr (FULL)
+            store_run<STREAM>(p + at, y[h]);
+          else
+            store_part<Y, V>(p + at, y[h], left - at);
+        }
       }
     }
   }
 };
 
-// A chunk's NT * 16 rows over columns [n_begin, n_end).  A block's loads are issued
-// before the one before it is multiplied, the first ones before u is read.
-template <bool F32, int BASE, int STEPS, int NT>
+// A chunk's rows over columns [n_begin, n_end): RW groups of NT * 16 rows, each with
+// kOutWaves / RW waves side by side.  The first loads are issued before u is read.
+template <bool F32, int BASE, int STEPS, int NT, int RW, bool STREAM>
 CAI4_DEV void adapters_out_chunk(const Adapters &a, const Chunk &ch, const float *u, int slices,
                                  int n_begin, int n_end, u32x4_t *us) {
-  constexpr int P = F32 ? 3 : 2, kStride = kOutWaves * kColBlock;
+  constexpr int P = F32 ? 3 : 2, kStride = kOutWaves / RW * kColBlock;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int c = lane & 15, q = lane >> 4;
+  const int c = lane & 15, q = lane >> 4, group = wave % RW;
   const bool own = ch.group < a.E;
   const int rank = own ? rank_of(a, ch.group) : 0, steps = STEPS ? STEPS : (rank + 31) / 32;
   const float scale = own && a.scales ? a.scales[ch.group] : 1.0f;
-  int row[NT];
+  int row[NT][2];
 #pragma unroll
-  for (int j = 0; j < NT; ++j) row[j] = row_of(a, ch, j * 16 + c);
+  for (int j = 0; j < NT; ++j)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) row[j][h] = row_of(a, ch, (group * NT + j) * 16 + (c & ~1) + h);
   const uint16_t *B = a.b + (size_t)(own ? ch.group : 0) * a.N * a.R;
-  int n0 = n_begin + wave * kColBlock;
+  int n0 = n_begin + wave / RW * kColBlock;
   const int n_full = n_end < a.N ? n_end : a.N / kColBlock * kColBlock;  // end of whole blocks
-  OutBlock<F32, BASE, STEPS, NT> now, next;
+  OutBlock<F32, BASE, STEPS, NT> now;
   if (n0 < n_full) now.template load<true>(a, B, row, n0);
-  for (int k = wave; k < steps * NT; k += kOutWaves) {
-    const int step = k / NT, j = k % NT;
+  for (int k = wave; k < steps * RW * NT; k += kOutWaves) {
+    const int step = k / (RW * NT), j = k % (RW * NT);
     const int r = step * 32 + q * 8, i0 = j * 16 + c;
     float v[8] = {};
     if (i0 < ch.rows && r < rank) {
@@ -335,52 +371,58 @@ CAI4_DEV void adapters_out_chunk(const Adapters &a, const Chunk &ch, const float
     u32x4_t op[P];
     operands_of<P>(v, op);
 #pragma unroll
-    for (int p = 0; p < P; ++p) us[((step * P + p) * NT + j) * 64 + lane] = op[p];
+    for (int p = 0; p < P; ++p) us[((step * P + p) * RW * NT + j) * 64 + lane] = op[p];
   }
   __syncthreads();
+  const u32x4_t *mine = us + group * NT * 64;
   while (n0 < n_full) {
-    const int n1 = n0 + kStride;
-    if (n1 < n_full) next.template load<true>(a, B, row, n1);
-    now.template finish<true>(a, B, steps, rank, us, row, n0);
-    now = next;
-    n0 = n1;
+    now.template finish<true, STREAM, RW>(a, B, steps, rank, mine, row, n0);
+    n0 += kStride;
+    if (n0 < n_full) now.template load<true>(a, B, row, n0);
   }
   if (n0 < n_end && n0 < a.N) {  // the last columns
     now.template load<false>(a, B, row, n0);
-    now.template finish<false>(a, B, steps, rank, us, row, n0);
+    now.template finish<false, false, RW>(a, B, steps, rank, mine, row, n0);
   }
 }
 
 template <bool F32, int BASE, int STEPS>
 __global__ __launch_bounds__(64 * kOutWaves) void adapters_out_kernel(Adapters a, const float *u,
                                                                       int slices, int cols,
-                                                                      int bare) {
+                                                                      int bare, int stream) {
   extern __shared__ u32x4_t us[];  // [steps of 32 ranks][planes][tiles][lane]
-  const Chunk ch = find_chunk(a, blockIdx.x, bare);
+  const Chunk ch = find_chunk<kChunkRows>(a, blockIdx.y, bare);
   if (ch.rows == 0) return;
-  const int n0 = blockIdx.y * cols, n1 = n0 + cols < a.N ? n0 + cols : a.N;
+  const int n0 = blockIdx.x * cols, n1 = n0 + cols < a.N ? n0 + cols : a.N;
   if (ch.rows <= 16)
-    adapters_out_chunk<F32, BASE, STEPS, 1>(a, ch, u, slices, n0, n1, us);
+    adapters_out_chunk<F32, BASE, STEPS, 1, 1, false>(a, ch, u, slices, n0, n1, us);
+  else if (stream)
+    adapters_out_chunk<F32, BASE, STEPS, 2, 2, true>(a, ch, u, slices, n0, n1, us);
   else
-    adapters_out_chunk<F32, BASE, STEPS, kTiles>(a, ch, u, slices, n0, n1, us);
+    adapters_out_chunk<F32, BASE, STEPS, 2, 2, false>(a, ch, u, slices, n0, n1, us);
 }
 
-// Chunks that T rows over E groups may make.
-int max_chunks(int T, int E) { return (T < E ? T : E) + T / kChunkRows; }
+// Chunks of `rows` rows that T rows over E groups may make.
+int max_chunks(int T, int E, int rows) { return (T < E ? T : E) + T / rows; }
 
-// Slices of K: enough that the first launch has some 512 workgroups, each wave at
-// least one block of 128 columns.
+// Rows of a chunk of the first launch, and slices of K: enough workgroups to fill the
+// chip, by fewer rows first (the second launch reads u once per slice).  Each wave has
+// at least one block of 128 columns.
 constexpr int kInWorkgroups = 512;
+int in_tiles(int T) { return T >= 16 * 1024 ? 4 : T >= 8 * 1024 ? 2 : 1; }
 int rank_tiles(int R) { return R <= 16 ? 1 : R <= 32 ? 2 : 4; }  // of a workgroup
 int rank_groups(int R) { return (R + 16 * rank_tiles(R) - 1) / (16 * rank_tiles(R)); }
 int slices_of(int K, int R, int E, int T) {
   const int most = ((K + 127) / 128 + kInWaves - 1) / kInWaves;
-  const int s = kInWorkgroups / (max_chunks(T, E) * rank_groups(R));
+  const int s = kInWorkgroups / (max_chunks(T, E, 16 * in_tiles(T)) * rank_groups(R));
   return s < 1 ? 1 : s < most ? s : most;
 }
 
+// Outputs that the caches would not hold, in whole lines, are written past them.
+constexpr size_t kStreamBytes = (size_t)64 << 20, kLine = 128;
+
 // Columns of a workgroup of the second launch: whole rounds of its waves.
-constexpr int kOutWorkgroups = 1536;
+constexpr int kOutWorkgroups = 3072;
 int cols_of(int N, int chunks) {
   const int each = kOutWaves * kColBlock, blocks = (N + each - 1) / each;
   const int per = (int)(((int64_t)blocks * chunks + kOutWorkgroups - 1) / kOutWorkgroups);
@@ -389,19 +431,22 @@ int cols_of(int N, int chunks) {
 
 template <bool F32, int BASE>
 void launch_out(const Adapters &a, const float *u, int slices, int bare, hipStream_t st) {
-  const int chunks = max_chunks(a.T, a.E + bare), cols = cols_of(a.N, chunks);
+  const int chunks = max_chunks(a.T, a.E + bare, kChunkRows), cols = cols_of(a.N, chunks);
   const int steps = (a.R + 31) / 32;
-  const dim3 grid(chunks, (a.N + cols - 1) / cols), block(64 * kOutWaves);
+  const size_t size = F32 ? 4 : 2;
+  const int stream = (size_t)a.T * a.N * size >= kStreamBytes && a.ldy % kLine == 0 &&
+                     (uintptr_t)a.y % kLine == 0;
+  const dim3 grid((a.N + cols - 1) / cols, chunks), block(64 * kOutWaves);
   const size_t lds = (size_t)steps * (F32 ? 3 : 2) * kTiles * 64 * 16;
   if (steps == 1)
     hipLaunchKernelGGL((adapters_out_kernel<F32, BASE, 1>), grid, block, lds, st, a, u, slices,
-                       cols, bare);
+                       cols, bare, stream);
   else if (steps == 2)
     hipLaunchKernelGGL((adapters_out_kernel<F32, BASE, 2>), grid, block, lds, st, a, u, slices,
-                       cols, bare);
+                       cols, bare, stream);
   else
     hipLaunchKernelGGL((adapters_out_kernel<F32, BASE, 0>), grid, block, lds, st, a, u, slices,
-                       cols, bare);
+                       cols, bare, stream);
 }
 template <bool F32>
 void launch_out(const Adapters &a, const float *u, int slices, int bare, hipStream_t st) {
@@ -413,23 +458,34 @@ void launch_out(const Adapters &a, const float *u, int slices, int bare, hipStre
     launch_out<F32, kBaseBf16>(a, u, slices, bare, st);
 }
 
+template <bool F32, int RT>
+void launch_in(const Adapters &a, float *u, int slices, hipStream_t st) {
+  const int tiles = in_tiles(a.T);
+  const dim3 grid(max_chunks(a.T, a.E, 16 * tiles), slices, rank_groups(a.R)),
+      block(64 * kInWaves);
+  if (tiles == 1)
+    hipLaunchKernelGGL((adapters_in_kernel<F32, RT, 1>), grid, block, 0, st, a, u, slices);
+  else if (tiles == 2)
+    hipLaunchKernelGGL((adapters_in_kernel<F32, RT, 2>), grid, block, 0, st, a, u, slices);
+  else
+    hipLaunchKernelGGL((adapters_in_kernel<F32, RT, 4>), grid, block, 0, st, a, u, slices);
+}
 template <bool F32>
 void launch_in(const Adapters &a, float *u, int slices, hipStream_t st) {
-  const dim3 grid(max_chunks(a.T, a.E), slices, rank_groups(a.R)), block(64 * kInWaves);
   const int rt = rank_tiles(a.R);
   if (rt == 1)
-    hipLaunchKernelGGL((adapters_in_kernel<F32, 1>), grid, block, 0, st, a, u, slices);
+    launch_in<F32, 1>(a, u, slices, st);
   else if (rt == 2)
-    hipLaunchKernelGGL((adapters_in_kernel<F32, 2>), grid, block, 0, st, a, u, slices);
+    launch_in<F32, 2>(a, u, slices, st);
   else
-    hipLaunchKernelGGL((adapters_in_kernel<F32, 4>), grid, block, 0, st, a, u, slices);
+    launch_in<F32, 4>(a, u, slices, st);
 }
 
 }  // namespace
 
 size_t adapters_workspace(int K, int R, int E, int T) {
   // (a call of fewer rows may take more slices: T * slices stays below
-  // kInWorkgroups * kChunkRows where there are any)
+  // kInWorkgroups * kChunkRows where there are several)
   const size_t most = ((size_t)((K + 127) / 128) + kInWaves - 1) / kInWaves;
   size_t rows = (size_t)T * most;
   if (rows > (size_t)kInWorkgroups * kChunkRows) rows = (size_t)kInWorkgroups * kChunkRows;

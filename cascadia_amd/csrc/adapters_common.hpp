@@ -6,7 +6,7 @@
 namespace cai4 {
 namespace {
 
-constexpr int kChunkRows = 64;
+constexpr int kChunkRows = 64;  // of the second launch; the first one's: 16, 32 or 64
 
 // Sorted rows row0 .. row0 + rows of one group (rows 0: there is no such chunk).
 struct Chunk {
@@ -19,8 +19,9 @@ CAI4_DEV int first_row(const Adapters &a, int e) {
   const int v = a.offsets[e < a.E ? e : a.E];  // (loaded in any case: no branch)
   return e > a.E || v > a.T ? a.T : v < 0 ? 0 : v;
 }
+template <int ROWS>
 CAI4_DEV int chunks_of(int first, int last) {
-  return last > first ? (last - first + kChunkRows - 1) / kChunkRows : 0;
+  return last > first ? (last - first + ROWS - 1) / ROWS : 0;
 }
 
 // Sum of v over the lanes up to this one.
@@ -34,8 +35,9 @@ CAI4_DEV int lanes_upto(int v) {
   return v;
 }
 
-// Chunk b of all groups' in order (bare: group E among them), by each wave for itself:
+// Chunk b (of ROWS rows) of all groups' in order (bare: group E among them), by each wave for itself:
 // lane i holds the offsets of `per` neighbouring groups and adds up their chunks.
+template <int ROWS>
 CAI4_DEV Chunk find_chunk(const Adapters &a, int b, bool bare) {
   constexpr int kMostPer = (kSortMaxGroups + 1 + 63) / 64;
   const int lane = threadIdx.x & 63;
@@ -48,7 +50,7 @@ CAI4_DEV Chunk find_chunk(const Adapters &a, int b, bool bare) {
   }
 #pragma unroll
   for (int i = 0; i < kMostPer; ++i)
-    if (i < per) n += chunks_of(row[i], row[i + 1]);
+    if (i < per) n += chunks_of<ROWS>(row[i], row[i + 1]);
   const int upto = lanes_upto(n);
   const uint64_t hit = __ballot(upto > b);
   if (!hit) return Chunk{0, 0, 0};
@@ -59,10 +61,10 @@ CAI4_DEV Chunk find_chunk(const Adapters &a, int b, bool bare) {
   for (int i = 0; i < kMostPer; ++i) {
     if (i < per) {
       const int first = __builtin_amdgcn_readlane(row[i], l);
-      const int last = __builtin_amdgcn_readlane(row[i + 1], l), m = chunks_of(first, last);
-      const int rows = last - first - left * kChunkRows;
+      const int last = __builtin_amdgcn_readlane(row[i + 1], l), m = chunks_of<ROWS>(first, last);
+      const int rows = last - first - left * ROWS;
       if (left >= 0 && left < m)
-        ch = Chunk{l * per + i, first + left * kChunkRows, rows < kChunkRows ? rows : kChunkRows};
+        ch = Chunk{l * per + i, first + left * ROWS, rows < ROWS ? rows : ROWS};
       left -= m;  // (negative once found)
     }
   }

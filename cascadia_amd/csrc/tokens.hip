@@ -18,12 +18,15 @@ namespace {
 
 // ---- sort ----
 
-// A thread per group; each wave places a run of neighbouring slots.
-constexpr int kSortThreads = kSortMaxGroups, kSortWaves = kSortThreads / 64;
+// Each wave of a workgroup places a run of neighbouring slots; its threads share the
+// groups among them.  Sixteen waves, or four for up to 1,024 slots (16 x 8 of them over
+// 256 experts: 3.2 us, by sixteen 4.6).
+constexpr int kSortWaves = 16, kFewWaves = 4;
 constexpr int kSteps = 4;  // steps of 64 slots whose ids are loaded together
 // Slots of a share, so that each wave takes one load of ids; at most 128 shares (a
 // placing workgroup adds up the counts of all shares).
 constexpr int kShareSlots = kSortWaves * kSteps * 64, kMaxShares = 128;
+constexpr int kFewSlots = kFewWaves * kSteps * 64;
 int shares_of(int n) {
   const int s = (n + kShareSlots - 1) / kShareSlots;
   return s < 1 ? 1 : s < kMaxShares ? s : kMaxShares;
@@ -32,10 +35,11 @@ int shares_of(int n) {
 __host__ __device__ inline int ld_counts(int E) { return E + 1; }
 
 // A wave's slots of share b: [first, last).
+template <int W>
 CAI4_DEV void wave_slots(const SortTokens &s, int shares, int b, int wave, int &first, int &last) {
-  const int waves = shares * kSortWaves;
+  const int waves = shares * W;
   const int per = ((s.n + waves - 1) / waves + 63) & ~63;
-  const int64_t at = ((int64_t)b * kSortWaves + wave) * per;
+  const int64_t at = ((int64_t)b * W + wave) * per;
   first = at < s.n ? (int)at : s.n;
   last = s.n - first < per ? s.n : first + per;
 }
@@ -58,14 +62,14 @@ CAI4_DEV void groups_of(const SortTokens &s, int at, int last, int (&e)[kSteps])
   }
 }
 
-__global__ __launch_bounds__(kSortThreads) void sort_count_kernel(SortTokens s, int shares,
-                                                                  int *counts) {
+__global__ __launch_bounds__(64 * kSortWaves) void sort_count_kernel(SortTokens s, int shares,
+                                                                     int *counts) {
   __shared__ int cnt[kSortMaxGroups + 1];
   const int b = blockIdx.x, ld = ld_counts(s.E);
-  for (int e = threadIdx.x; e <= s.E; e += kSortThreads) cnt[e] = 0;
+  for (int e = threadIdx.x; e <= s.E; e += 64 * kSortWaves) cnt[e] = 0;
   __syncthreads();
   int first, last, e[kSteps];
-  wave_slots(s, shares, b, threadIdx.x >> 6, first, last);
+  wave_slots<kSortWaves>(s, shares, b, threadIdx.x >> 6, first, last);
   for (int at = first; at < last; at += kSteps * 64) {
     groups_of(s, at, last, e);
 #pragma unroll
@@ -73,21 +77,23 @@ __global__ __launch_bounds__(kSortThreads) void sort_count_kernel(SortTokens s, 
       if (e[i] >= 0) atomicAdd(&cnt[e[i]], 1);
   }
   __syncthreads();
-  for (int i = threadIdx.x; i <= s.E; i += kSortThreads) counts[(size_t)b * ld + i] = cnt[i];
+  for (int i = threadIdx.x; i <= s.E; i += 64 * kSortWaves) counts[(size_t)b * ld + i] = cnt[i];
 }
 
-__global__ __launch_bounds__(kSortThreads) void sort_place_kernel(SortTokens s, int shares,
-                                                                  const int *counts) {
-  __shared__ int cnt[kSortWaves][kSortMaxGroups + 1];  // counts; then next rows
-  __shared__ int sums[kSortWaves + 1];
+template <int W>
+__global__ __launch_bounds__(64 * W) void sort_place_kernel(SortTokens s, int shares,
+                                                            const int *counts) {
+  constexpr int kThreads = 64 * W, kPer = kSortMaxGroups / kThreads;  // groups of a thread
+  __shared__ int cnt[W][kSortMaxGroups + 1];  // counts; then next rows
+  __shared__ int sums[W + 1];
   const int b = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int me = threadIdx.x, ld = ld_counts(s.E);  // me: this thread's group
+  const int e0 = threadIdx.x * kPer, ld = ld_counts(s.E);
   int first, last, e[kSteps];
-  wave_slots(s, shares, b, wave, first, last);
+  wave_slots<W>(s, shares, b, wave, first, last);
   if (first < last) groups_of(s, first, last, e);
-  for (int i = me; i <= s.E; i += kSortThreads)
+  for (int i = threadIdx.x; i <= s.E; i += kThreads)
 #pragma unroll
-    for (int w = 0; w < kSortWaves; ++w) cnt[w][i] = 0;
+    for (int w = 0; w < W; ++w) cnt[w][i] = 0;
   __syncthreads();
   for (int at = first; at < last; at += kSteps * 64) {
     if (at > first) groups_of(s, at, last, e);
@@ -95,19 +101,20 @@ __global__ __launch_bounds__(kSortThreads) void sort_place_kernel(SortTokens s, 
     for (int i = 0; i < kSteps; ++i)
       if (e[i] >= 0) atomicAdd(&cnt[wave][e[i]], 1);
   }
-  // the group's slots over all shares, and over those before this one
-  int total = 0, before = 0, left = 0;
-  if (shares > 1) {
+  // the groups' slots over all shares, and over those before this one
+  int total[kPer] = {}, before[kPer] = {}, left = 0;
+  if (W == kSortWaves && shares > 1) {
+    static_assert(kSortMaxGroups == 64 * kSortWaves, "a group per thread");
     constexpr int kLoads = 16;  // in flight
     for (int h0 = 0; h0 < shares; h0 += kLoads) {
       int v[kLoads];
 #pragma unroll
       for (int i = 0; i < kLoads; ++i)
-        v[i] = counts[(size_t)(h0 + i < shares ? h0 + i : h0) * ld + (me < s.E ? me : s.E)];
+        v[i] = counts[(size_t)(h0 + i < shares ? h0 + i : h0) * ld + (e0 < s.E ? e0 : s.E)];
 #pragma unroll
       for (int i = 0; i < kLoads; ++i) {
-        total += h0 + i < shares ? v[i] : 0;
-        before += h0 + i < b ? v[i] : 0;
+        total[0] += h0 + i < shares ? v[i] : 0;
+        before[0] += h0 + i < b ? v[i] : 0;
       }
     }
     if (wave == 0) {  // slots left out before this share: a share per lane
@@ -117,40 +124,49 @@ __global__ __launch_bounds__(kSortThreads) void sort_place_kernel(SortTokens s, 
     }
   }
   __syncthreads();
-  int c[kSortWaves];
+  int c[kPer][W], mine = 0;
 #pragma unroll
-  for (int w = 0; w < kSortWaves; ++w) c[w] = me < s.E ? cnt[w][me] : 0;
-  if (shares == 1)
+  for (int q = 0; q < kPer; ++q) {
+    const bool in = e0 + q < s.E;
 #pragma unroll
-    for (int w = 0; w < kSortWaves; ++w) total += c[w];
-  if (me >= s.E) total = 0;
+    for (int w = 0; w < W; ++w) {
+      c[q][w] = in ? cnt[w][e0 + q] : 0;
+      if (shares == 1) total[q] += c[q][w];
+    }
+    if (!in) total[q] = 0;
+    mine += total[q];
+  }
   // first rows: a sum over the threads before this one
-  int upto = total;
+  int row = mine;
 #pragma unroll
   for (int d = 1; d < 64; d *= 2) {
-    const int u = __shfl_up(upto, d);
-    if (lane >= d) upto += u;
+    const int u = __shfl_up(row, d);
+    if (lane >= d) row += u;
   }
-  if (lane == 63) sums[wave] = upto;
-  if (me == 0) sums[kSortWaves] = left;
+  if (lane == 63) sums[wave] = row;
+  if (threadIdx.x == 0) sums[W] = left;
   __syncthreads();
-  int row = upto - total;
+  row -= mine;
 #pragma unroll
-  for (int w = 0; w < kSortWaves; ++w) row += w < wave ? sums[w] : 0;
-  if (me < s.E) {
-    if (b == 0) s.offsets[me] = row;
-    int at = row + before;
+  for (int w = 0; w < W; ++w) row += w < wave ? sums[w] : 0;
 #pragma unroll
-    for (int w = 0; w < kSortWaves; ++w) {
-      cnt[w][me] = at;
-      at += c[w];
+  for (int q = 0; q < kPer; ++q) {
+    if (e0 + q < s.E) {
+      if (b == 0) s.offsets[e0 + q] = row;
+      int at = row + before[q];
+#pragma unroll
+      for (int w = 0; w < W; ++w) {
+        cnt[w][e0 + q] = at;
+        at += c[q][w];
+      }
     }
+    row += total[q];
   }
-  if (me == kSortThreads - 1) {  // (row + total: all that are kept)
-    if (b == 0) s.offsets[s.E] = row + total;
-    int at = row + total + sums[kSortWaves];
+  if (threadIdx.x == kThreads - 1) {  // (row: all that are kept)
+    if (b == 0) s.offsets[s.E] = row;
+    int at = row + sums[W];
 #pragma unroll
-    for (int w = 0; w < kSortWaves; ++w) {
+    for (int w = 0; w < W; ++w) {
       const int n = cnt[w][s.E];
       cnt[w][s.E] = at;
       at += n;
@@ -394,10 +410,14 @@ hipError_t sort_tokens(const SortTokens &s, void *workspace, hipStream_t st) {
   const int shares = shares_of(s.n);
   int *counts = static_cast<int *>(workspace);
   if (shares > 1)
-    hipLaunchKernelGGL(sort_count_kernel, dim3(shares), dim3(kSortThreads), 0, st, s, shares,
+    hipLaunchKernelGGL(sort_count_kernel, dim3(shares), dim3(64 * kSortWaves), 0, st, s, shares,
                        counts);
-  hipLaunchKernelGGL(sort_place_kernel, dim3(shares), dim3(kSortThreads), 0, st, s, shares,
-                     counts);
+  if (s.n <= kFewSlots)
+    hipLaunchKernelGGL(sort_place_kernel<kFewWaves>, dim3(1), dim3(64 * kFewWaves), 0, st, s, 1,
+                       counts);
+  else
+    hipLaunchKernelGGL(sort_place_kernel<kSortWaves>, dim3(shares), dim3(64 * kSortWaves), 0, st, s,
+                       shares, counts);
   return hipGetLastError();
 }
 

@@ -65,7 +65,7 @@ struct Adapters {
   int T;
   const void *x, *base;      // base null: zero
   void *y;
-  size_t ldx, ldb, ldy;      // row strides in values
+  uint32_t ldx, ldb, ldy;    // row strides in bytes
   int x_f32, base_f32, y_f32;
 };
 size_t adapters_workspace(int K, int R, int E, int T);

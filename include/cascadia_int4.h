@@ -645,8 +645,8 @@ typedef struct cascadia_int4_adapters {
  *     (-1: none) with top_k 1 and n_experts = n_adapters; one call of it serves all
  *     projections of a batch.
  *   xs [n_tokens, k_cols], base and ys [n_tokens, n_rows], f32 (*_is_f32) or bf16,
- *     rows *_stride values apart (parts of a wider buffer: the row of several
- *     projections); xs of a row without an adapter is not read.  ys may be base (then of
+ *     rows *_stride (<= 2^29) values apart (parts of a wider buffer: the row of
+ *     several projections); xs of a row without an adapter is not read.  ys may be base (then of
  *     its type and stride, and rows without an adapter are not touched), otherwise
  *     overlaps no input.
  * f32 sums; one rounding at the end.  f32 xs enter to 24 bits, the inner a_i xs[t]

@@ -100,8 +100,8 @@ def test_adapters_refusals(cl):
                dict(n_rows=(1 << 22) + 1), dict(max_rank=0), dict(max_rank=12), dict(max_rank=264),
                dict(n_adapters=0), dict(n_adapters=1025), dict(a=P + 8), dict(b=P + 8),
                dict(ranks=P + 2), dict(scales=P + 2), dict(T=(1 << 20) + 1), dict(xf=2), dict(bf=2),
-               dict(yf=2), dict(ldx=63), dict(ldy=47), dict(base=P, ldb=47), dict(ldx=1 << 41),
-               dict(ldy=1 << 41), dict(base=P, ldb=1 << 41), dict(off=P + 2), dict(slots=P + 2),
+               dict(yf=2), dict(ldx=63), dict(ldy=47), dict(base=P, ldb=47), dict(ldx=(1 << 29) + 1),
+               dict(ldy=(1 << 29) + 1), dict(base=P, ldb=(1 << 29) + 1), dict(off=P + 2), dict(slots=P + 2),
                dict(x=P + 1), dict(xf=1, x=P + 2), dict(y=P + 1), dict(yf=1, y=P + 2),
                dict(base=P + 1, ldb=48), dict(base=P + 2, bf=1, ldb=48), dict(ws=P + 8),
                dict(base=2 * P, ldb=49), dict(base=2 * P, bf=1, ldb=48)):
