@@ -1267,16 +1267,40 @@ def sort_tokens_workspace_bytes(n_tokens: int, top_k: int, n_experts: int) -> in
     return int(lib().cascadia_int4_sort_tokens_workspace_bytes(n_tokens, top_k, n_experts))
 
 
-def _int32(dev, t, n, name):
+def _flat(dev, t, dtype, n, name):
+    """The address of t: n contiguous values of dtype on the current device dev."""
+    if (t.__class__ is torch.Tensor and t.get_device() == dev and t.dtype is dtype
+            and t.numel() == n and t.is_contiguous()):  # (the common case in few steps)
+        return t.data_ptr()
     _here(dev, t, name)
-    if not (t.dtype is torch.int32 and t.numel() == n):
-        raise ValueError(f"{name}: int32 of {n} values")
+    if not (t.dtype is dtype and t.numel() == n):
+        raise ValueError(f"{name}: {dtype} of {n} values")
+    return t.data_ptr()
 
 
-def _row_weights(dev, weights, n):
-    _here(dev, weights, "weights")
-    if not (weights.dtype is torch.float32 and weights.numel() == n):
-        raise ValueError("weights: f32 [n_tokens, top_k]")
+def _values(dev, t, n, name):
+    """(address, is f32) of t: n contiguous values, f32 or bf16."""
+    if t.__class__ is not torch.Tensor or t.get_device() != dev or not t.is_contiguous():
+        _here(dev, t, name)
+    dtype = t.dtype
+    if not ((dtype is torch.bfloat16 or dtype is torch.float32) and t.numel() == n):
+        raise ValueError(f"{name}: f32 or bf16 of {n} values")
+    return t.data_ptr(), 1 if dtype is torch.float32 else 0
+
+
+def _slots(rows, top_k):
+    """Tokens of rows [n_tokens, top_k] (or ids)."""
+    n = rows.numel()
+    if not (1 <= top_k <= 16 and n % top_k == 0):
+        raise ValueError("top_k: 1 to 16, rows and ids [n_tokens, top_k]")
+    return n // top_k
+
+
+def _cols(t, n, name):
+    """Columns of t [n, cols]."""
+    if t.dim() != 2 or t.shape[0] != n:
+        raise ValueError(f"{name} must be [{n}, cols]")
+    return t.shape[1]
 
 
 def sort_tokens(ids, top_k: int, n_experts: int, offsets, slots, rows, *, weights=None,
@@ -1294,50 +1318,24 @@ def sort_tokens(ids, top_k: int, n_experts: int, offsets, slots, rows, *, weight
     (adapters_forward).  workspace: sort_tokens_workspace_bytes (for a graph capture)."""
     dev = _home(offsets, "offsets")
     top_k, n_experts = _index(top_k), _index(n_experts)
-    n = ids.numel()
-    _expect(1 <= top_k <= 16 and n % top_k == 0, "top_k: 1 to 16, ids [n_tokens, top_k]")
-    _expect(1 <= n_experts <= 1024, "n_experts: 1 to 1024")
-    _int32(dev, ids, n, "ids")
-    _int32(dev, offsets, n_experts + 1, "offsets")
-    _int32(dev, slots, n, "slots")
-    _int32(dev, rows, n, "rows")
-    wp = 0
-    if weights is not None:
-        _row_weights(dev, weights, n)
-        wp = weights.data_ptr()
+    T = _slots(ids, top_k)
+    n = T * top_k
+    if not 1 <= n_experts <= 1024:
+        raise ValueError("n_experts: 1 to 1024")
+    wp = 0 if weights is None else _flat(dev, weights, torch.float32, n, "weights")
     ws = 0
     if workspace is not None:
         _here(dev, workspace, "workspace")
-        need = _need("cascadia_int4_sort_tokens_workspace_bytes", 0, dev, n // top_k, top_k,
-                     n_experts)
+        need = _need("cascadia_int4_sort_tokens_workspace_bytes", 0, dev, T, top_k, n_experts)
         if workspace.nbytes < need:
             raise ValueError(f"workspace has {workspace.nbytes} bytes, the call needs {need}")
         ws = workspace.data_ptr()
+    i32 = torch.int32
     check("cascadia_int4_sort_tokens", lib().cascadia_int4_sort_tokens(
-        ids.data_ptr(), wp, threshold, n // top_k, top_k, n_experts, offsets.data_ptr(),
-        slots.data_ptr(), rows.data_ptr(), ws, _stream()))
+        _flat(dev, ids, i32, n, "ids"), wp, threshold, T, top_k, n_experts,
+        _flat(dev, offsets, i32, n_experts + 1, "offsets"), _flat(dev, slots, i32, n, "slots"),
+        _flat(dev, rows, i32, n, "rows"), ws, _stream()))
     return offsets, slots, rows
-
-
-def _token_rows(dev, t, rows, top_k, per, name):
-    """(n_tokens, cols) of a call over rows [n_tokens, top_k] and t [n_tokens * per, cols]."""
-    n = rows.numel()
-    if not (1 <= top_k <= 16 and n % top_k == 0):
-        raise ValueError("top_k: 1 to 16, rows [n_tokens, top_k]")
-    _int32(dev, rows, n, "rows")
-    T = n // top_k
-    if t.dim() != 2 or t.shape[0] != T * per:
-        raise ValueError(f"{name} must be [{T * per}, cols]")
-    return T, t.shape[1]
-
-
-def _values(dev, t, count, name):
-    """Whether t (count values, f32 or bf16) is f32."""
-    _here(dev, t, name)
-    f32 = t.dtype is torch.float32
-    if not ((f32 or t.dtype is torch.bfloat16) and t.numel() == count):
-        raise ValueError(f"{name}: f32 or bf16 of {count} values")
-    return f32
 
 
 def gather_tokens(x, rows, xs, *, top_k: int):
@@ -1346,7 +1344,8 @@ def gather_tokens(x, rows, xs, *, top_k: int):
     nearest even), or both e4m3 (or uint8).  The other rows of xs stay as they are."""
     dev = _home(x, "x")
     top_k = _index(top_k)
-    T, cols = _token_rows(dev, x, rows, top_k, 1, "x")
+    T = _slots(rows, top_k)
+    cols = _cols(x, T, "x")
     _here(dev, xs, "xs")
     xt, yt = _fp8_x_type(x.dtype), _fp8_x_type(xs.dtype)
     if (xt == FP8_X_E4M3) != (yt == FP8_X_E4M3):
@@ -1354,7 +1353,8 @@ def gather_tokens(x, rows, xs, *, top_k: int):
     if xs.numel() != T * top_k * cols:
         raise ValueError(f"xs must hold {T * top_k} rows of {cols}")
     check("cascadia_int4_gather_tokens", lib().cascadia_int4_gather_tokens(
-        x.data_ptr(), xt, rows.data_ptr(), T, top_k, cols, xs.data_ptr(), yt, _stream()))
+        x.data_ptr(), xt, _flat(dev, rows, torch.int32, T * top_k, "rows"), T, top_k, cols,
+        xs.data_ptr(), yt, _stream()))
     return xs
 
 
@@ -1366,21 +1366,16 @@ def combine_tokens(ys, rows, out, *, top_k: int, weights=None, residual=None):
     residual."""
     dev = _home(ys, "ys")
     top_k = _index(top_k)
-    T, cols = _token_rows(dev, ys, rows, top_k, top_k, "ys")
-    y_f32 = _values(dev, ys, T * top_k * cols, "ys")
-    out_f32 = _values(dev, out, T * cols, "out")
-    wp = rp = 0
-    if weights is not None:
-        _row_weights(dev, weights, T * top_k)
-        wp = weights.data_ptr()
-    if residual is not None:
-        _here(dev, residual, "residual")
-        _expect(residual.dtype is out.dtype and residual.numel() == T * cols,
-                "residual: [n_tokens, cols] of out's type")
-        rp = residual.data_ptr()
+    T = _slots(rows, top_k)
+    n = T * top_k
+    cols = _cols(ys, n, "ys")
+    yp, y_f32 = _values(dev, ys, n * cols, "ys")
+    op, out_f32 = _values(dev, out, T * cols, "out")
+    wp = 0 if weights is None else _flat(dev, weights, torch.float32, n, "weights")
+    rp = 0 if residual is None else _flat(dev, residual, out.dtype, T * cols, "residual")
     check("cascadia_int4_combine_tokens", lib().cascadia_int4_combine_tokens(
-        ys.data_ptr(), int(y_f32), rows.data_ptr(), wp, rp, T, top_k, cols, out.data_ptr(),
-        int(out_f32), _stream()))
+        yp, y_f32, _flat(dev, rows, torch.int32, n, "rows"), wp, rp, T, top_k, cols, op, out_f32,
+        _stream()))
     return out
 
 
@@ -1398,18 +1393,16 @@ def combine_tokens_grad(dout, ys, rows, weights, dys, dweights, *, top_k: int):
     bf16 or f32."""
     dev = _home(ys, "ys")
     top_k = _index(top_k)
-    T, cols = _token_rows(dev, ys, rows, top_k, top_k, "ys")
-    d_f32 = _values(dev, dout, T * cols, "dout")
-    y_f32 = _values(dev, ys, T * top_k * cols, "ys")
-    _here(dev, dys, "dys")
-    _expect(dys.dtype is ys.dtype and dys.numel() == ys.numel(), "dys: as ys")
-    _row_weights(dev, weights, T * top_k)
-    _here(dev, dweights, "dweights")
-    _expect(dweights.dtype is torch.float32 and dweights.numel() == T * top_k,
-            "dweights: f32 [n_tokens, top_k]")
+    T = _slots(rows, top_k)
+    n = T * top_k
+    cols = _cols(ys, n, "ys")
+    dp, d_f32 = _values(dev, dout, T * cols, "dout")
+    yp, y_f32 = _values(dev, ys, n * cols, "ys")
     check("cascadia_int4_combine_tokens_grad", lib().cascadia_int4_combine_tokens_grad(
-        dout.data_ptr(), int(d_f32), ys.data_ptr(), int(y_f32), rows.data_ptr(),
-        weights.data_ptr(), T, top_k, cols, dys.data_ptr(), dweights.data_ptr(), _stream()))
+        dp, d_f32, yp, y_f32, _flat(dev, rows, torch.int32, n, "rows"),
+        _flat(dev, weights, torch.float32, n, "weights"), T, top_k, cols,
+        _flat(dev, dys, ys.dtype, n * cols, "dys"),
+        _flat(dev, dweights, torch.float32, n, "dweights"), _stream()))
     return dys, dweights
 
 
@@ -1434,12 +1427,9 @@ class Adapters:
                 f"{E} adapters of rank {R}, {N} x {K}: ranks and columns are multiples of 8")
         rp = sp = 0
         if ranks is not None:
-            _int32(dev, ranks, E, "ranks")
-            rp = ranks.data_ptr()
+            rp = _flat(dev, ranks, torch.int32, E, "ranks")
         if scales is not None:
-            _here(dev, scales, "scales")
-            _expect(scales.dtype is torch.float32 and scales.numel() == E, "scales: f32 [n_adapters]")
-            sp = scales.data_ptr()
+            sp = _flat(dev, scales, torch.float32, E, "scales")
         self.a, self.b, self.ranks, self.scales = a, b, ranks, scales
         self.n_adapters, self.max_rank, self.k_cols, self.n_rows = E, R, K, N
         self._set = AdapterSet(K, N, R, E, a.data_ptr(), b.data_ptr(), rp, sp)
@@ -1458,19 +1448,19 @@ def _adapters_need(device, k_cols, n_rows, max_rank, n_adapters, n_tokens):
 
 
 def _strided(dev, t, T, cols, name):
-    """(is f32, row stride) of t [T, cols], whose rows may lie apart."""
-    if not (isinstance(t, torch.Tensor) and t.is_cuda):
-        raise ValueError(f"{name} must be a device (HBM) tensor")
-    if t.get_device() != dev:
+    """(address, is f32, row stride) of t [T, cols], whose rows may lie apart."""
+    if not (isinstance(t, torch.Tensor) and t.get_device() == dev):
+        _expect(isinstance(t, torch.Tensor) and t.is_cuda, f"{name} must be a device (HBM) tensor")
         raise ValueError(f"{name} is on {t.device}, the current device is {dev}")
     f32 = t.dtype is torch.float32
-    if not ((f32 or t.dtype is torch.bfloat16) and t.dim() == 2 and t.shape[0] == T
-            and t.shape[1] == cols):
+    if not (f32 or t.dtype is torch.bfloat16) or t.shape != (T, cols):
         raise ValueError(f"{name}: f32 or bf16 [{T}, {cols}]")
-    ld = t.stride(0) if T > 1 else cols
-    if (cols > 1 and t.stride(1) != 1) or ld < cols:
-        raise ValueError(f"{name}: rows of neighbouring values that do not overlap")
-    return f32, ld
+    ld = cols
+    if not t.is_contiguous():
+        ld = t.stride(0) if T > 1 else cols
+        if (cols > 1 and t.stride(1) != 1) or ld < cols:
+            raise ValueError(f"{name}: rows of neighbouring values that do not overlap")
+    return t.data_ptr(), 1 if f32 else 0, ld
 
 
 def adapters_forward(adapters: Adapters, xs, offsets, slots, ys, *, base=None, workspace=None):
@@ -1484,28 +1474,27 @@ def adapters_forward(adapters: Adapters, xs, offsets, slots, ys, *, base=None, w
     workspace: adapters_workspace_bytes (for a graph capture)."""
     dev = _home(offsets, "offsets")
     A = adapters
-    _here(dev, A.a, "adapters")
-    T = slots.numel()
-    _int32(dev, offsets, A.n_adapters + 1, "offsets")
-    _int32(dev, slots, T, "slots")
-    x_f32, ldx = _strided(dev, xs, T, A.k_cols, "xs")
-    y_f32, ldy = _strided(dev, ys, T, A.n_rows, "ys")
-    b_f32, ldb, bp = False, 0, 0
+    if A.a.get_device() != dev:
+        _here(dev, A.a, "adapters")
+    T, K, N = slots.numel(), A.k_cols, A.n_rows
+    xp, x_f32, ldx = _strided(dev, xs, T, K, "xs")
+    yp, y_f32, ldy = _strided(dev, ys, T, N, "ys")
+    bp = b_f32 = ldb = 0
     if base is not None:
-        b_f32, ldb = _strided(dev, base, T, A.n_rows, "base")
-        bp = base.data_ptr()
-        if bp == ys.data_ptr() and (b_f32 != y_f32 or ldb != ldy):
+        bp, b_f32, ldb = _strided(dev, base, T, N, "base")
+        if bp == yp and (b_f32 != y_f32 or ldb != ldy):
             raise ValueError("ys over base: of its type and stride")
     ws = 0
     if workspace is not None:
         _here(dev, workspace, "workspace")
-        need = _adapters_need(dev, A.k_cols, A.n_rows, A.max_rank, A.n_adapters, T)
+        need = _adapters_need(dev, K, N, A.max_rank, A.n_adapters, T)
         if workspace.nbytes < need:
             raise ValueError(f"workspace has {workspace.nbytes} bytes, the call needs {need}")
         ws = workspace.data_ptr()
     check("cascadia_int4_adapters_forward", lib().cascadia_int4_adapters_forward(
-        A._ref, offsets.data_ptr(), slots.data_ptr(), xs.data_ptr(), int(x_f32), ldx, bp,
-        int(b_f32), ldb, T, ys.data_ptr(), int(y_f32), ldy, ws, _stream()))
+        A._ref, _flat(dev, offsets, torch.int32, A.n_adapters + 1, "offsets"),
+        _flat(dev, slots, torch.int32, T, "slots"), xp, x_f32, ldx, bp, b_f32, ldb, T, yp, y_f32,
+        ldy, ws, _stream()))
     return ys
 
 

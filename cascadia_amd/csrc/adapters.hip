@@ -1,7 +1,7 @@
 // adapters.hip -- low-rank adapters of many requests at once:
 //   y_t = base_t + s_a B_a (A_a x_t),  a: row t's adapter (rows without one: base_t)
 //
-// Rows come sorted by adapter, in chunks of up to kChunkRows rows of one adapter.
+// Rows come sorted by adapter, in chunks of up to 64 rows of one adapter.
 // Two launches: u = A x for every chunk (K in slices where chunks are few; their
 // partial sums stay f32), then y = base + B (s u), which adds the slices in order.
 //
@@ -17,8 +17,6 @@
 
 namespace cai4 {
 namespace {
-
-constexpr int kTiles = kChunkRows / 16;
 
 // v as N bf16 planes whose sum holds 8 N bits of it.  An infinity or NaN is in the
 // first alone: what it leaves over would be NaN.
@@ -185,6 +183,7 @@ __global__ __launch_bounds__(64 * kInWaves) void adapters_in_kernel(Adapters a, 
 // ---- y = base + B (s u) ----
 
 constexpr int kOutWaves = 4, kColBlock = 64;  // columns of a wave at a time
+constexpr int kOutRows = 32;                  // rows of a chunk
 
 enum BaseType { kBaseNone, kBaseBf16, kBaseF32 };
 
@@ -261,7 +260,7 @@ struct OutBlock {
     }
   }
   // (A tile of 16 rows at a time: fewer sums at once, more waves.)
-  template <bool FULL, bool STREAM, int RW>
+  template <bool FULL, bool STREAM>
   CAI4_DEV void finish(const Adapters &a, const uint16_t *B, int steps, int rank, const u32x4_t *us,
                        const int (&row)[NT][2], int n0) {
     const int lane = threadIdx.x & 63, q = lane >> 4, left = a.N - n0;
@@ -278,7 +277,7 @@ struct OutBlock {
       auto add = [&](int step, const u32x4_t (&v)[4]) {
 #pragma unroll
         for (int p = 0; p < P; ++p) {
-          const u32x4_t uv = us[((step * P + p) * RW * NT + j) * 64 + lane];
+          const u32x4_t uv = us[((step * P + p) * NT + j) * 64 + lane];
 #pragma unroll
           for (int m = 0; m < 4; ++m) acc[m] = mfma_bf16(v[m], uv, acc[m]);
         }
@@ -324,14 +323,14 @@ struct OutBlock {
   }
 };
 
-// A chunk's rows over columns [n_begin, n_end): RW groups of NT * 16 rows, each with
-// kOutWaves / RW waves side by side.  The first loads are issued before u is read.
-template <bool F32, int BASE, int STEPS, int NT, int RW, bool STREAM>
+// A chunk's NT * 16 rows over columns [n_begin, n_end), a block of 64 per wave at a
+// time.  The first loads are issued before u is read.
+template <bool F32, int BASE, int STEPS, int NT, bool STREAM>
 CAI4_DEV void adapters_out_chunk(const Adapters &a, const Chunk &ch, const float *u, int slices,
                                  int n_begin, int n_end, u32x4_t *us) {
-  constexpr int P = F32 ? 3 : 2, kStride = kOutWaves / RW * kColBlock;
+  constexpr int P = F32 ? 3 : 2, kStride = kOutWaves * kColBlock;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int c = lane & 15, q = lane >> 4, group = wave % RW;
+  const int c = lane & 15, q = lane >> 4;
   const bool own = ch.group < a.E;
   const int rank = own ? rank_of(a, ch.group) : 0, steps = STEPS ? STEPS : (rank + 31) / 32;
   const float scale = own && a.scales ? a.scales[ch.group] : 1.0f;
@@ -339,14 +338,14 @@ CAI4_DEV void adapters_out_chunk(const Adapters &a, const Chunk &ch, const float
 #pragma unroll
   for (int j = 0; j < NT; ++j)
 #pragma unroll
-    for (int h = 0; h < 2; ++h) row[j][h] = row_of(a, ch, (group * NT + j) * 16 + (c & ~1) + h);
+    for (int h = 0; h < 2; ++h) row[j][h] = row_of(a, ch, j * 16 + (c & ~1) + h);
   const uint16_t *B = a.b + (size_t)(own ? ch.group : 0) * a.N * a.R;
-  int n0 = n_begin + wave / RW * kColBlock;
+  int n0 = n_begin + wave * kColBlock;
   const int n_full = n_end < a.N ? n_end : a.N / kColBlock * kColBlock;  // end of whole blocks
   OutBlock<F32, BASE, STEPS, NT> now;
   if (n0 < n_full) now.template load<true>(a, B, row, n0);
-  for (int k = wave; k < steps * RW * NT; k += kOutWaves) {
-    const int step = k / (RW * NT), j = k % (RW * NT);
+  for (int k = wave; k < steps * NT; k += kOutWaves) {
+    const int step = k / NT, j = k % NT;
     const int r = step * 32 + q * 8, i0 = j * 16 + c;
     float v[8] = {};
     if (i0 < ch.rows && r < rank) {
@@ -371,18 +370,17 @@ CAI4_DEV void adapters_out_chunk(const Adapters &a, const Chunk &ch, const float
     u32x4_t op[P];
     operands_of<P>(v, op);
 #pragma unroll
-    for (int p = 0; p < P; ++p) us[((step * P + p) * RW * NT + j) * 64 + lane] = op[p];
+    for (int p = 0; p < P; ++p) us[((step * P + p) * NT + j) * 64 + lane] = op[p];
   }
   __syncthreads();
-  const u32x4_t *mine = us + group * NT * 64;
   while (n0 < n_full) {
-    now.template finish<true, STREAM, RW>(a, B, steps, rank, mine, row, n0);
+    now.template finish<true, STREAM>(a, B, steps, rank, us, row, n0);
     n0 += kStride;
     if (n0 < n_full) now.template load<true>(a, B, row, n0);
   }
   if (n0 < n_end && n0 < a.N) {  // the last columns
     now.template load<false>(a, B, row, n0);
-    now.template finish<false, false, RW>(a, B, steps, rank, mine, row, n0);
+    now.template finish<false, false>(a, B, steps, rank, us, row, n0);
   }
 }
 
@@ -391,15 +389,15 @@ __global__ __launch_bounds__(64 * kOutWaves) void adapters_out_kernel(Adapters a
                                                                       int slices, int cols,
                                                                       int bare, int stream) {
   extern __shared__ u32x4_t us[];  // [steps of 32 ranks][planes][tiles][lane]
-  const Chunk ch = find_chunk<kChunkRows>(a, blockIdx.y, bare);
+  const Chunk ch = find_chunk<kOutRows>(a, blockIdx.y, bare);
   if (ch.rows == 0) return;
   const int n0 = blockIdx.x * cols, n1 = n0 + cols < a.N ? n0 + cols : a.N;
   if (ch.rows <= 16)
-    adapters_out_chunk<F32, BASE, STEPS, 1, 1, false>(a, ch, u, slices, n0, n1, us);
+    adapters_out_chunk<F32, BASE, STEPS, 1, false>(a, ch, u, slices, n0, n1, us);
   else if (stream)
-    adapters_out_chunk<F32, BASE, STEPS, 2, 2, true>(a, ch, u, slices, n0, n1, us);
+    adapters_out_chunk<F32, BASE, STEPS, kOutRows / 16, true>(a, ch, u, slices, n0, n1, us);
   else
-    adapters_out_chunk<F32, BASE, STEPS, 2, 2, false>(a, ch, u, slices, n0, n1, us);
+    adapters_out_chunk<F32, BASE, STEPS, kOutRows / 16, false>(a, ch, u, slices, n0, n1, us);
 }
 
 // Chunks of `rows` rows that T rows over E groups may make.
@@ -408,13 +406,13 @@ int max_chunks(int T, int E, int rows) { return (T < E ? T : E) + T / rows; }
 // Rows of a chunk of the first launch, and slices of K: enough workgroups to fill the
 // chip, by fewer rows first (the second launch reads u once per slice).  Each wave has
 // at least one block of 128 columns.
-constexpr int kInWorkgroups = 512;
-int in_tiles(int T) { return T >= 16 * 1024 ? 4 : T >= 8 * 1024 ? 2 : 1; }
+constexpr int kInWorkgroups = 1024;
+int in_tiles(int R, int T) { return T < 1024 ? 1 : R > 32 && T >= 2048 ? 4 : 2; }
 int rank_tiles(int R) { return R <= 16 ? 1 : R <= 32 ? 2 : 4; }  // of a workgroup
 int rank_groups(int R) { return (R + 16 * rank_tiles(R) - 1) / (16 * rank_tiles(R)); }
 int slices_of(int K, int R, int E, int T) {
   const int most = ((K + 127) / 128 + kInWaves - 1) / kInWaves;
-  const int s = kInWorkgroups / (max_chunks(T, E, 16 * in_tiles(T)) * rank_groups(R));
+  const int s = kInWorkgroups / (max_chunks(T, E, 16 * in_tiles(R, T)) * rank_groups(R));
   return s < 1 ? 1 : s < most ? s : most;
 }
 
@@ -429,24 +427,24 @@ int cols_of(int N, int chunks) {
   return each * (per < 1 ? 1 : per < blocks ? per : blocks);
 }
 
+template <bool F32, int BASE, int STEPS>
+void launch_out(const Adapters &a, const float *u, int slices, int bare, hipStream_t st) {
+  const int chunks = max_chunks(a.T, a.E + bare, kOutRows), cols = cols_of(a.N, chunks);
+  const int stream = (size_t)a.T * a.N * (F32 ? 4 : 2) >= kStreamBytes && a.ldy % kLine == 0 &&
+                     (uintptr_t)a.y % kLine == 0;
+  const size_t lds = (size_t)((a.R + 31) / 32) * (F32 ? 3 : 2) * (kOutRows / 16) * 64 * 16;
+  hipLaunchKernelGGL((adapters_out_kernel<F32, BASE, STEPS>),
+                     dim3((a.N + cols - 1) / cols, chunks), dim3(64 * kOutWaves), lds, st, a, u,
+                     slices, cols, bare, stream);
+}
 template <bool F32, int BASE>
 void launch_out(const Adapters &a, const float *u, int slices, int bare, hipStream_t st) {
-  const int chunks = max_chunks(a.T, a.E + bare, kChunkRows), cols = cols_of(a.N, chunks);
-  const int steps = (a.R + 31) / 32;
-  const size_t size = F32 ? 4 : 2;
-  const int stream = (size_t)a.T * a.N * size >= kStreamBytes && a.ldy % kLine == 0 &&
-                     (uintptr_t)a.y % kLine == 0;
-  const dim3 grid((a.N + cols - 1) / cols, chunks), block(64 * kOutWaves);
-  const size_t lds = (size_t)steps * (F32 ? 3 : 2) * kTiles * 64 * 16;
-  if (steps == 1)
-    hipLaunchKernelGGL((adapters_out_kernel<F32, BASE, 1>), grid, block, lds, st, a, u, slices,
-                       cols, bare, stream);
-  else if (steps == 2)
-    hipLaunchKernelGGL((adapters_out_kernel<F32, BASE, 2>), grid, block, lds, st, a, u, slices,
-                       cols, bare, stream);
+  if (a.R <= 32)
+    launch_out<F32, BASE, 1>(a, u, slices, bare, st);
+  else if (a.R <= 64)
+    launch_out<F32, BASE, 2>(a, u, slices, bare, st);
   else
-    hipLaunchKernelGGL((adapters_out_kernel<F32, BASE, 0>), grid, block, lds, st, a, u, slices,
-                       cols, bare, stream);
+    launch_out<F32, BASE, 0>(a, u, slices, bare, st);
 }
 template <bool F32>
 void launch_out(const Adapters &a, const float *u, int slices, int bare, hipStream_t st) {
@@ -460,7 +458,7 @@ void launch_out(const Adapters &a, const float *u, int slices, int bare, hipStre
 
 template <bool F32, int RT>
 void launch_in(const Adapters &a, float *u, int slices, hipStream_t st) {
-  const int tiles = in_tiles(a.T);
+  const int tiles = in_tiles(a.R, a.T);
   const dim3 grid(max_chunks(a.T, a.E, 16 * tiles), slices, rank_groups(a.R)),
       block(64 * kInWaves);
   if (tiles == 1)
@@ -485,10 +483,10 @@ void launch_in(const Adapters &a, float *u, int slices, hipStream_t st) {
 
 size_t adapters_workspace(int K, int R, int E, int T) {
   // (a call of fewer rows may take more slices: T * slices stays below
-  // kInWorkgroups * kChunkRows where there are several)
+  // kInWorkgroups * 64 where there are several)
   const size_t most = ((size_t)((K + 127) / 128) + kInWaves - 1) / kInWaves;
   size_t rows = (size_t)T * most;
-  if (rows > (size_t)kInWorkgroups * kChunkRows) rows = (size_t)kInWorkgroups * kChunkRows;
+  if (rows > (size_t)kInWorkgroups * 64) rows = (size_t)kInWorkgroups * 64;
   if (rows < (size_t)T) rows = T;
   return rows * R * 4;
 }

@@ -6,8 +6,6 @@
 namespace cai4 {
 namespace {
 
-constexpr int kChunkRows = 64;  // of the second launch; the first one's: 16, 32 or 64
-
 // Sorted rows row0 .. row0 + rows of one group (rows 0: there is no such chunk).
 struct Chunk {
   int group, row0, rows;
