@@ -48,6 +48,25 @@ CAI4_DEV void operands_of(const float (&v)[8], u32x4_t (&op)[N]) {
   }
 }
 
+// The same for x, of which there is much more, in a third of the instructions: three
+// planes, the first one truncated (so that no finite value becomes infinite), which
+// hold 23 bits.  An infinity is in the first alone, a NaN in any.
+CAI4_DEV void operands_of_x(const float (&v)[8], u32x4_t (&op)[3]) {
+  auto pair = [](float a, float b) {
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2_t{a, b}, bf16x2_t));
+  };
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float a = v[2 * i], b = v[2 * i + 1];
+    op[0][i] = __builtin_amdgcn_perm(fbits(b), fbits(a), 0x07060302u);
+    float ra = a - bitsf(fbits(a) & 0xFFFF0000u), rb = b - bitsf(fbits(b) & 0xFFFF0000u);
+    ra = fabsf(a) == INFINITY ? 0.f : ra;
+    rb = fabsf(b) == INFINITY ? 0.f : rb;
+    op[1][i] = pair(ra, rb);
+    op[2][i] = pair(ra - bitsf(op[1][i] << 16), rb - bitsf(op[1][i] & 0xFFFF0000u));
+  }
+}
+
 // Bits to keep of columns r .. r + 7 of a row of B: those below the rank (the others
 // may hold anything).
 CAI4_DEV u32x4_t keep_of(int rank, int r) {
@@ -130,7 +149,7 @@ CAI4_DEV void adapters_in_chunk(const Adapters &a, const Chunk &ch, int rank, in
           float v[8];
 #pragma unroll
           for (int i = 0; i < 8; ++i) v[i] = xf[s][j][i / 4][i % 4];
-          operands_of<P>(v, op);
+          operands_of_x(v, op);
         } else {
           op[0] = xv[s][j];
         }

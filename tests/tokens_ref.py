@@ -64,8 +64,9 @@ def combine_grad(dout, ys, rows, weights, dys, y_bf16):
 def adapters(a, b, ranks, scales, ids, x, base, y_bf16):
     """(ys, bound).  Products of bf16 values are exact in f32; a sum of n of them, in
     some order, is off by 2^-23 of the terms' magnitudes each (a matrix core may
-    truncate).  f32 x enters as three bf16 values that hold it to 2^-24, the inner
-    values as three (f32 y) or two (2^-16)."""
+    truncate).  f32 x enters as three bf16 values that hold it to 2^-23 (the first one
+    truncated: 2^-7, then halves of steps: 2^-8 each), the inner values as three that hold
+    them to 2^-24 (f32 y) or two (2^-16)."""
     T, N, K = len(ids), b.shape[1], a.shape[2]
     out = np.zeros((T, N)) if base is None else np.array(base, np.float64)
     bound = np.zeros((T, N))
@@ -77,7 +78,7 @@ def adapters(a, b, ranks, scales, ids, x, base, y_bf16):
         A, B = a[i, :r].astype(np.float64), b[i, :, :r].astype(np.float64)
         xt = x[t].astype(np.float64)
         u = A @ xt
-        du = ((3 * K + 64) * 2 * U32 + U32) * (np.abs(A) @ np.abs(xt))
+        du = ((3 * K + 64) * 2 * U32 + 2 * U32) * (np.abs(A) @ np.abs(xt))
         su = s * u
         dsu = abs(s) * du + (2 * U32 + plane) * (np.abs(su) + abs(s) * du)
         out[t] += B @ su
