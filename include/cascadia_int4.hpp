@@ -1144,6 +1144,180 @@ inline void fp8_moe_forward(const Fp8Experts &experts, const Fp8Rows &x,
                   residual_bf16.data, residual_bf16.len, call);
 }
 
+// ---- tokens sorted by expert and back, and low-rank adapters ----
+//
+// No counterpart in the crate: cascadia_int4.h states what each computes.
+
+// Rows that a call writes: f32, bf16 bits, or (gather_tokens) e4m3 codes.
+struct RowsOut {
+  void *data;
+  size_t len;
+  uint32_t type;
+  RowsOut(DeviceSlice<float> y) : data(y.data), len(y.len), type(CASCADIA_INT4_FP8_X_F32) {}
+  RowsOut(DeviceSlice<uint16_t> y_bf16)
+      : data(y_bf16.data), len(y_bf16.len), type(CASCADIA_INT4_FP8_X_BF16) {}
+  RowsOut(DeviceSlice<uint8_t> codes)
+      : data(codes.data), len(codes.len), type(CASCADIA_INT4_FP8_X_E4M3) {}
+  // whether f32; codes are refused
+  bool f32() const {
+    detail::require(type != CASCADIA_INT4_FP8_X_E4M3, "rows of f32 or bf16");
+    return type == CASCADIA_INT4_FP8_X_F32;
+  }
+};
+
+inline size_t sort_tokens_workspace_bytes(size_t n_tokens, size_t top_k, size_t n_experts) {
+  detail::require(n_tokens <= UINT32_MAX && top_k <= UINT32_MAX && n_experts <= UINT32_MAX,
+                  "unsupported sizes");
+  return cascadia_int4_sort_tokens_workspace_bytes((uint32_t)n_tokens, (uint32_t)top_k,
+                                                   (uint32_t)n_experts);
+}
+
+// offsets [n_experts + 1], slots [n_tokens * top_k] (sorted row -> slot), rows
+// [n_tokens, top_k] (slot -> sorted row, -1: left out) of ids [n_tokens, top_k]; weights
+// (empty: none) below threshold are left out.
+inline void sort_tokens(DeviceSlice<const int32_t> ids, size_t top_k, size_t n_experts,
+                        DeviceSlice<int32_t> offsets, DeviceSlice<int32_t> slots,
+                        DeviceSlice<int32_t> rows, DeviceSlice<const float> weights = {},
+                        float threshold = 0.0f, const Options &call = {}) {
+  detail::require(top_k >= 1 && top_k <= 16 && ids.len % top_k == 0, "ids: n_tokens x top_k");
+  const size_t t = ids.len / top_k;
+  detail::require(n_experts <= 1024 && offsets.len == n_experts + 1, "offsets: n_experts + 1");
+  detail::require(t <= UINT32_MAX && slots.len == ids.len && rows.len == ids.len &&
+                      (!weights.data || weights.len == ids.len),
+                  "slots, rows and weights: n_tokens x top_k");
+  detail::check(cascadia_int4_sort_tokens(ids.data, weights.data, threshold, (uint32_t)t,
+                                          (uint32_t)top_k, (uint32_t)n_experts, offsets.data,
+                                          slots.data, rows.data, call.workspace, call.stream),
+                "cascadia_int4_sort_tokens");
+  detail::finish(call);
+}
+
+namespace detail {
+// Tokens and columns of rows [n_tokens, top_k] and of `len` values in n_tokens * per rows.
+inline std::pair<uint32_t, uint32_t> token_rows(DeviceSlice<const int32_t> rows, size_t top_k,
+                                                size_t len, size_t per, size_t cols) {
+  require(top_k >= 1 && top_k <= 16 && rows.len % top_k == 0, "rows: n_tokens x top_k");
+  const size_t t = rows.len / top_k;
+  require(t <= UINT32_MAX && cols <= UINT32_MAX && len == t * per * cols,
+          "rows of cols values");
+  return {(uint32_t)t, (uint32_t)cols};
+}
+}  // namespace detail
+
+// xs[rows[t, j]] = x[t]: f32 and bf16 in any pair, codes (Fp8Rows(codes, {})) to codes.
+inline void gather_tokens(const Fp8Rows &x, DeviceSlice<const int32_t> rows, size_t top_k,
+                          size_t cols, const RowsOut &xs, const Options &call = {}) {
+  const auto d = detail::token_rows(rows, top_k, x.len, 1, cols);
+  detail::require(xs.len == x.len * top_k, "xs: n_tokens * top_k rows of cols");
+  detail::check(cascadia_int4_gather_tokens(x.data, x.type, rows.data, d.first, (uint32_t)top_k,
+                                            d.second, xs.data, xs.type, call.stream),
+                "cascadia_int4_gather_tokens");
+  detail::finish(call);
+}
+
+// out[t] = residual[t] + sum_j weights[t, j] * ys[rows[t, j]]; empty weights: 1, empty
+// residual (of out's type): 0.
+inline void combine_tokens(const Fp8Rows &ys, DeviceSlice<const int32_t> rows, size_t top_k,
+                           size_t cols, const RowsOut &out,
+                           DeviceSlice<const float> weights = {}, const Fp8Rows *residual = nullptr,
+                           const Options &call = {}) {
+  detail::require(ys.type != CASCADIA_INT4_FP8_X_E4M3, "ys is f32 or bf16");
+  const auto d = detail::token_rows(rows, top_k, ys.len, top_k, cols);
+  const size_t n = (size_t)d.first * cols;
+  const bool f32 = out.f32();
+  detail::require(out.len == n && (!residual || (residual->len == n && residual->type == out.type)),
+                  "out and residual: n_tokens x cols of one type");
+  detail::require(!weights.data || weights.len == rows.len, "weights: n_tokens x top_k");
+  detail::check(cascadia_int4_combine_tokens(ys.data, ys.type == CASCADIA_INT4_FP8_X_F32, rows.data,
+                                             weights.data, residual ? residual->data : nullptr,
+                                             d.first, (uint32_t)top_k, d.second, out.data, f32,
+                                             call.stream),
+                "cascadia_int4_combine_tokens");
+  detail::finish(call);
+}
+
+// The gradient of gather_tokens: dx[t] = sum_j dxs[rows[t, j]].
+inline void gather_tokens_grad(const Fp8Rows &dxs, DeviceSlice<const int32_t> rows, size_t top_k,
+                               size_t cols, const RowsOut &dx, const Options &call = {}) {
+  combine_tokens(dxs, rows, top_k, cols, dx, {}, nullptr, call);
+}
+
+// The gradient of combine_tokens: dys[rows[t, j]] = weights[t, j] * dout[t] (of ys's
+// type), dweights[t, j] = ys[rows[t, j]] . dout[t].
+inline void combine_tokens_grad(const Fp8Rows &dout, const Fp8Rows &ys,
+                                DeviceSlice<const int32_t> rows, DeviceSlice<const float> weights,
+                                size_t top_k, size_t cols, const RowsOut &dys,
+                                DeviceSlice<float> dweights, const Options &call = {}) {
+  detail::require(ys.type != CASCADIA_INT4_FP8_X_E4M3 && dout.type != CASCADIA_INT4_FP8_X_E4M3,
+                  "ys and dout are f32 or bf16");
+  const auto d = detail::token_rows(rows, top_k, ys.len, top_k, cols);
+  const bool f32 = ys.type == CASCADIA_INT4_FP8_X_F32;
+  detail::require(dout.len == (size_t)d.first * cols && dys.len == ys.len && dys.type == ys.type,
+                  "dout: n_tokens x cols, dys as ys");
+  detail::require(weights.len == rows.len && dweights.len == rows.len,
+                  "weights and dweights: n_tokens x top_k");
+  detail::check(cascadia_int4_combine_tokens_grad(dout.data, dout.type == CASCADIA_INT4_FP8_X_F32,
+                                                  ys.data, f32, rows.data, weights.data, d.first,
+                                                  (uint32_t)top_k, d.second, dys.data,
+                                                  dweights.data, call.stream),
+                "cascadia_int4_combine_tokens_grad");
+  detail::finish(call);
+}
+
+// Low-rank adapters of one projection, bf16 bits read where they are: a [n_adapters,
+// max_rank, k_cols], b [n_adapters, n_rows, max_rank]; ranks and scales (empty: max_rank,
+// 1) [n_adapters].
+class Adapters {
+ public:
+  Adapters(DeviceSlice<const uint16_t> a, DeviceSlice<const uint16_t> b, size_t n_adapters,
+           size_t max_rank, size_t n_rows, size_t k_cols, DeviceSlice<const int32_t> ranks = {},
+           DeviceSlice<const float> scales = {}) {
+    detail::require(n_adapters >= 1 && n_adapters <= 1024 && max_rank >= 8 && max_rank <= 256 &&
+                        max_rank % 8 == 0 && k_cols >= 8 && k_cols % 8 == 0 &&
+                        k_cols <= UINT32_MAX && n_rows >= 1 && n_rows <= UINT32_MAX,
+                    "1 to 1024 adapters, ranks and columns in multiples of 8");
+    detail::require(a.len == n_adapters * max_rank * k_cols &&
+                        b.len == n_adapters * n_rows * max_rank &&
+                        (!ranks.data || ranks.len == n_adapters) &&
+                        (!scales.data || scales.len == n_adapters),
+                    "a: n_adapters x max_rank x k_cols, b: n_adapters x n_rows x max_rank, ranks and "
+                    "scales: n_adapters");
+    s_ = {(uint32_t)k_cols, (uint32_t)n_rows, (uint32_t)max_rank, (uint32_t)n_adapters,
+          a.data,           b.data,           ranks.data,         scales.data};
+  }
+  const cascadia_int4_adapters &c_adapters() const { return s_; }
+  size_t workspace_bytes(size_t n_tokens) const {
+    return cascadia_int4_adapters_workspace_bytes(&s_, (uint32_t)n_tokens);
+  }
+
+ private:
+  cascadia_int4_adapters s_{};
+};
+
+// ys[t] = base[t] + scale b (a xs[t]) of row t's adapter; offsets and slots:
+// sort_tokens of the rows' adapters with top_k 1; base null: 0.  Contiguous rows (the
+// C call takes others).
+inline void adapters_forward(const Adapters &adapters, const Fp8Rows &xs,
+                             DeviceSlice<const int32_t> offsets, DeviceSlice<const int32_t> slots,
+                             const RowsOut &ys, const Fp8Rows *base = nullptr,
+                             const Options &call = {}) {
+  const cascadia_int4_adapters &s = adapters.c_adapters();
+  const size_t t = slots.len, n = t * s.n_rows;
+  detail::require(xs.type != CASCADIA_INT4_FP8_X_E4M3 &&
+                      (!base || base->type != CASCADIA_INT4_FP8_X_E4M3),
+                  "xs and base are f32 or bf16");
+  detail::require(t <= UINT32_MAX && offsets.len == (size_t)s.n_adapters + 1 &&
+                      xs.len == t * s.k_cols && ys.len == n && (!base || base->len == n),
+                  "offsets: n_adapters + 1, xs: n_tokens x k_cols, ys and base: n_tokens x n_rows");
+  detail::check(cascadia_int4_adapters_forward(
+                    &s, offsets.data, slots.data, xs.data, xs.type == CASCADIA_INT4_FP8_X_F32,
+                    s.k_cols, base ? base->data : nullptr,
+                    base && base->type == CASCADIA_INT4_FP8_X_F32, s.n_rows, (uint32_t)t, ys.data,
+                    ys.f32(), s.n_rows, call.workspace, call.stream),
+                "cascadia_int4_adapters_forward");
+  detail::finish(call);
+}
+
 // ---- the crate's C handle API (c_ffi.rs:35-341) as an owning object ----
 
 // A model directory (safetensors, or an int4_bin manifest with flat expert
