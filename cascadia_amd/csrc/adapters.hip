@@ -4,10 +4,21 @@
 // Rows come sorted by adapter, in chunks of up to 64 rows of one adapter.
 // Two launches: u = A x for every chunk (K in slices where chunks are few; their
 // partial sums stay f32), then y = base + B (s u), which adds the slices in order.
+// (Both in one launch, u made again by every workgroup: one row of rank 16 took 10 us of
+// kernel time for 4.9 + 5.4, but rank 32, or 16 rows and more, 15 to 65 % more than two.)
 //
 // Both products run on bf16 MFMAs with f32 sums.  A and B are bf16; f32 x, and u,
 // enter as a sum of bf16 planes, each the rounding of what the ones before left
-// over: three hold 24 bits, two (for bf16 y) 16.
+// over: u to 24 bits (f32 y, three planes) or 16 (bf16 y, two: its own rounding is
+// 2^-8), x to 23 (three).
+//
+// Bound: HBM, by base and y (x, A and B besides); rows that are few, by two launches of
+// some three dependent round trips each.  4,096 rows, rank 32, 4,096 -> 14,336, all
+// bf16: u 17 us (27 MB of x, and A from the L2), y 57 (235 MB, 4.1 TB/s; a copy of the
+// same rows takes 44), 70 to 75 in all.  Rank 64: 23 + 78: the second launch's u and B
+// from the L2 cost it what the matrix cores do not.  One row, rank 16, 4,096 -> 4,096: 4.9 +
+// 5.4.  64 rows of 33 adapters of rank 4 to 64 in f32, 4,096 -> 14,336: 9.2 + 14.3; the
+// second reads rows of B of 128 bytes of which the rank fills half.
 #include <array>
 #include <type_traits>
 
@@ -202,17 +213,19 @@ __global__ __launch_bounds__(64 * kInWaves) void adapters_in_kernel(Adapters a, 
 // ---- y = base + B (s u) ----
 
 constexpr int kOutWaves = 4, kColBlock = 64;  // columns of a wave at a time
-constexpr int kOutRows = 32;                  // rows of a chunk
+// Rows of a chunk.  32 / 64 / 128: 256 rows of as many adapters 24.2 / 25.6 / 30.1 us, 8,192 of
+// rank 32 60.7 / 65.4 / 70.5, 4,096 of rank 64 100 / 102 / 114.
+constexpr int kOutRows = 32;
 
 enum BaseType { kBaseNone, kBaseBf16, kBaseF32 };
 
 // Outputs leave the MFMAs as 16 columns of row c in lane (c, q), in RUNS runs of 16
 // bytes (of y's type).  Four lanes' runs of one row are 64 bytes, half a line; lanes c
 // and c ^ 1 exchange every second run, so that a store writes whole lines of the
-// eight even rows, the next those of the odd ones (4,096 x 14,336 in bf16 past the
-// caches, copied so: 37.5 us, in half lines 50).  f32: run m is columns 16 m + 4 q of
-// the block, tile m; bf16: run h is 32 h + 8 q, tiles 2 h and 2 h + 1 with four
-// columns each in turn.
+// eight even rows, the next those of the odd ones (4,096 x 14,336 in bf16, copied so past
+// the caches: 47 us, in half lines 56).  f32: run m is columns 16 m + 4 q of the block,
+// tile m; bf16: run h is 32 h + 8 q, tiles 2 h and 2 h + 1 with four columns each in
+// turn.
 template <bool F32>
 CAI4_DEV int weight_col(int m, int c) {
   return F32 ? m * 16 + c : (m >> 1) * 32 + (c >> 2) * 8 + (m & 1) * 4 + (c & 3);
@@ -422,9 +435,13 @@ __global__ __launch_bounds__(64 * kOutWaves) void adapters_out_kernel(Adapters a
 // Chunks of `rows` rows that T rows over E groups may make.
 int max_chunks(int T, int E, int rows) { return (T < E ? T : E) + T / rows; }
 
-// Rows of a chunk of the first launch, and slices of K: enough workgroups to fill the
-// chip, by fewer rows first (the second launch reads u once per slice).  Each wave has
-// at least one block of 128 columns.
+// Rows of a chunk of the first launch: more of them read A less often, fewer make more
+// workgroups.  16 / 32 / 64 rows, us of the whole call: 512 rows of rank 32 20.9 / 22.6 /
+// 24.6; 1,024 of rank 16 19.2 / 18.2 / 20.5; 4,096 of rank 32 80 / 75 / 77; 2,048 of rank 64
+// 40.4 / 40.4 / 35.0, 4,096 of it 111 / 107 / 102.
+// Slices of K, each read again by the second launch: up to some 1,024 workgroups, each
+// wave at least one block of 128 columns.  1,024 / 512 / 256: 256 adapters' rows 23.9 / 27.3 /
+// 27.4, 8,192 rows of rank 32 60.8 / 66.1 / 66.2, 4,096 of rank 64 99.9 / 99.6 / 96.2.
 constexpr int kInWorkgroups = 1024;
 int in_tiles(int R, int T) { return T < 1024 ? 1 : R > 32 && T >= 2048 ? 4 : 2; }
 int rank_tiles(int R) { return R <= 16 ? 1 : R <= 32 ? 2 : 4; }  // of a workgroup
@@ -435,10 +452,14 @@ int slices_of(int K, int R, int E, int T) {
   return s < 1 ? 1 : s < most ? s : most;
 }
 
-// Outputs that the caches would not hold, in whole lines, are written past them.
+// Outputs of 64 MiB and more, in whole lines, are written past the caches, so or not:
+// 117 MB 74.9 / 78.7 us, 67 MB 55.2 / 61.7.  (15 MB: 19.4 / 21.3, but what reads those next
+// finds them there.)
 constexpr size_t kStreamBytes = (size_t)64 << 20, kLine = 128;
 
-// Columns of a workgroup of the second launch: whole rounds of its waves.
+// Columns of a workgroup of the second launch: whole rounds of its waves, for some 3,072
+// workgroups.  1,536 / 3,072 / 6,144: 4,096 rows of rank 32 81 / 75 / 74 us, 64 rows of mixed
+// ranks 27.3 / 27.0 / 32.9.
 constexpr int kOutWorkgroups = 3072;
 int cols_of(int N, int chunks) {
   const int each = kOutWaves * kColBlock, blocks = (N + each - 1) / each;

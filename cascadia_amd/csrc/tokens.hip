@@ -1,14 +1,21 @@
 // tokens.hip -- a layer's slots (token, choice) sorted by expert, rows moved to that
 // order and back with the slots' weights, and the gradient of the way back.
 //
-// Sorting is a counting sort that keeps the slots' order within a group: shares of
-// the slots are counted (one launch), then every share adds up the counts before its
-// own and places its slots (another); one share does both by itself.  The rank of a
-// slot among the slots of its group comes from ballots, not from the order in which
-// atomics return, so that the result is the same every time.
+// Sorting is a counting sort that keeps the slots' order within a group: row of slot i =
+// slots of smaller groups + slots before i of its own.  Shares of the slots are counted
+// (one launch), then every share adds up the counts before its own and places its slots
+// (another); up to 4,096 slots are one share, which does both by itself.  A slot's rank
+// among the 64 of a wave comes from ballots, not from the order in which atomics
+// return, so that the result is the same every time.  Bound: launches and a handful of
+// dependent loads (12 bytes a slot).  8,192 x 8 slots over 384 experts: 4.2 + 9 us.
 //
-// The other three move rows and are bound by HBM: a token's row is read once for all
-// of its slots.
+// The other three move rows and are bound by HBM:
+//   gather   xs[row(t, j)] = x[t]            a token's row read once for its slots
+//   combine  out[t] = res[t] + sum w y       each slot's row read once
+//   gradient dy[row] = w dout, dw = y . dout  both in one pass over y
+// 4,096 tokens, 8 slots each, rows of 7,168 in bf16: gather 88 us (514 MB, 5.8 TB/s),
+// combine 97 to 111 (574 MB, 5.2 to 5.9); the gradient of rows of 4,096: 104 us (555 MB,
+// 5.3).  A copy of 2 GiB reaches 4.9: these write and read past the caches (below).
 #include "fp8.hpp"
 #include "rows.hpp"
 #include "tokens.hpp"
@@ -19,8 +26,8 @@ namespace {
 // ---- sort ----
 
 // Each wave of a workgroup places a run of neighbouring slots; its threads share the
-// groups among them.  Sixteen waves, or four for up to 1,024 slots (16 x 8 of them over
-// 256 experts: 3.2 us, by sixteen 4.6).
+// groups among them.  Sixteen waves, or four for up to 1,024 slots (128 slots of 256
+// experts: the kernel takes 4.6 us, with sixteen 5.3).
 constexpr int kSortWaves = 16, kFewWaves = 4;
 constexpr int kSteps = 4;  // steps of 64 slots whose ids are loaded together
 // Slots of a share, so that each wave takes one load of ids; at most 128 shares (a
@@ -62,11 +69,6 @@ CAI4_DEV void groups_of(const SortTokens &s, int at, int last, int (&e)[kSteps])
   }
 }
 
-// Groups from which a lane's own atomic counts its slot; of fewer, many lanes of a wave
-// would add to one word of LDS and take their turns, so one of them adds for all.
-// (Counting 65,536 slots of 384 groups: 4.2 us by atomics, 5.0 by ballots.)
-constexpr int kManyGroups = 64;
-
 // The lanes of this lane's group e (-1: none), in `bits` ballots.
 CAI4_DEV uint64_t lanes_of(int e, int bits) {
   uint64_t same = __ballot(e >= 0);
@@ -91,8 +93,7 @@ CAI4_DEV int take_places(int e, int bits, int *next) {
 __global__ __launch_bounds__(64 * kSortWaves) void sort_count_kernel(SortTokens s, int shares,
                                                                      int *counts) {
   __shared__ int cnt[kSortMaxGroups + 1];
-  const int b = blockIdx.x, ld = ld_counts(s.E), lane = threadIdx.x & 63;
-  const int bits = 32 - __builtin_clz(s.E);
+  const int b = blockIdx.x, ld = ld_counts(s.E);
   for (int e = threadIdx.x; e <= s.E; e += 64 * kSortWaves) cnt[e] = 0;
   __syncthreads();
   int first, last, e[kSteps];
@@ -100,14 +101,8 @@ __global__ __launch_bounds__(64 * kSortWaves) void sort_count_kernel(SortTokens 
   for (int at = first; at < last; at += kSteps * 64) {
     groups_of(s, at, last, e);
 #pragma unroll
-    for (int i = 0; i < kSteps; ++i) {
-      if (s.E >= kManyGroups) {
-        if (e[i] >= 0) atomicAdd(&cnt[e[i]], 1);
-        continue;
-      }
-      const uint64_t same = lanes_of(e[i], bits);
-      if (e[i] >= 0 && !(same & ((1ull << lane) - 1))) atomicAdd(&cnt[e[i]], __popcll(same));
-    }
+    for (int i = 0; i < kSteps; ++i)
+      if (e[i] >= 0) atomicAdd(&cnt[e[i]], 1);  // (sums: in any order)
   }
   __syncthreads();
   for (int i = threadIdx.x; i <= s.E; i += 64 * kSortWaves) counts[(size_t)b * ld + i] = cnt[i];
@@ -384,8 +379,11 @@ dim3 move_grid(int T, int cols, int V) {
   return dim3(T, (cols + kMoveThreads * V - 1) / (kMoveThreads * V));
 }
 
-// Whether rows are written past the caches: more of them than the Infinity Cache holds,
-// in whole lines.
+// Whether the slots' rows are written or read past the caches' replacement: more of them
+// than the Infinity Cache (256 MiB) holds, in whole lines.  Gather, written so or not:
+// 470 MB 89 / 106 us, 134 MB 26.2 / 26.9, 67 MB 12.7 / 12.6; combine, read so or not: 470 MB
+// 97 / 119, 101 MB 29.3 / 22.2 (then still in that cache); the gradient, both: 268 MB 104 /
+// 114; rows of an odd number of bytes, written so: 37 / 31.
 constexpr size_t kStreamBytes = (size_t)256 << 20, kLine = 128;
 bool streams(const void *p, int rows, int cols, size_t size) {
   return (size_t)rows * cols * size >= kStreamBytes && cols * size % kLine == 0 &&
