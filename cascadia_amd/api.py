@@ -1298,8 +1298,8 @@ def _slots(rows, top_k):
 
 def _cols(t, n, name):
     """Columns of t [n, cols]."""
-    if t.dim() != 2 or t.shape[0] != n:
-        raise ValueError(f"{name} must be [{n}, cols]")
+    if t.dim() != 2 or t.shape[0] != n or not 1 <= t.shape[1] <= 1 << 20:
+        raise ValueError(f"{name} must be [{n}, cols], 1 to 2^20 columns")
     return t.shape[1]
 
 

@@ -9,8 +9,8 @@
 //
 // Both products run on bf16 MFMAs with f32 sums.  A and B are bf16; f32 x, and u,
 // enter as a sum of bf16 planes, each the rounding of what the ones before left
-// over: u to 24 bits (f32 y, three planes) or 16 (bf16 y, two: its own rounding is
-// 2^-8), x to 23 (three).
+// over: x and, for f32 y, u in three (24 bits), for bf16 y u in two (16 bits: y's own
+// rounding is 2^-8).
 //
 // Bound: HBM, by base and y (x, A and B besides); rows that are few, by two launches of
 // some three dependent round trips each.  4,096 rows, rank 32, 4,096 -> 14,336, all
@@ -30,7 +30,7 @@ namespace cai4 {
 namespace {
 
 // v as N bf16 planes whose sum holds 8 N bits of it.  An infinity or NaN is in the
-// first alone: what it leaves over would be NaN.
+// first alone: what an infinity leaves over would be NaN.
 template <int N>
 CAI4_DEV void planes_of(float v, uint32_t (&p)[N]) {
   p[0] = split_hi(v);
@@ -60,8 +60,9 @@ CAI4_DEV void operands_of(const float (&v)[8], u32x4_t (&op)[N]) {
 }
 
 // The same for x, of which there is much more, in a third of the instructions: three
-// planes, the first one truncated (so that no finite value becomes infinite), which
-// hold 23 bits.  An infinity is in the first alone, a NaN in any.
+// planes, the first one truncated (so that no finite value becomes infinite).  It
+// leaves 16 bits, the second half a step of its 8, the third the rest: all 24 bits.  An
+// infinity is in the first alone, a NaN in any.
 CAI4_DEV void operands_of_x(const float (&v)[8], u32x4_t (&op)[3]) {
   auto pair = [](float a, float b) {
     return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2_t{a, b}, bf16x2_t));

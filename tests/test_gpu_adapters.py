@@ -277,3 +277,39 @@ def test_repeats_streams_and_recorded_calls(cl):
     graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(y, base)
+
+
+@pytest.mark.parametrize("rows", [1, 40])
+def test_unit_weights_return_x(cl, rows):
+    """Adapters that pick columns: f32 values come back whole, from the largest to small
+    ones.  (A value's three planes are added twice, in the inner product and in the
+    outer one: two additions each, of 2^-23 at most.)"""
+    K, N, R = 264, 96, 24
+    g = gen(13)
+    cols = torch.randperm(K, generator=g)[:R]
+    a, b = torch.zeros((1, R, K), dtype=BF16), torch.zeros((1, N, R), dtype=BF16)
+    a[0, torch.arange(R), cols] = 1.0
+    b[0, torch.arange(N), torch.arange(N) % R] = 1.0
+    for scale in (1.0, 3.4e38, 1e-30):
+        x = (torch.rand((rows, K), generator=g) * 2 - 1) * scale
+        x[0, cols[0]] = scale
+        off, slots = plan(cl, torch.zeros(rows, dtype=torch.int32), 1)
+        y = cl.adapters_forward(cl.Adapters(a.cuda(), b.cuda()), x.cuda(), off, slots,
+                                torch.empty((rows, N), device="cuda"))
+        want = host(x[:, cols])[:, np.arange(N) % R]
+        assert np.all(np.abs(host(y) - want) <= 2.0 ** -21 * np.abs(want))
+
+
+def test_signs_of_zero_rows_and_small_values(cl):
+    """Rows without an adapter: base as it is, subnormal values among it."""
+    T, E, N, K = 40, 2, 100, 16
+    base = torch.tensor([1e-40, -3e-39, 1.4e-45, 0.0, 1.1754944e-38]).repeat(T, N // 5)
+    off, slots = plan(cl, torch.full((T,), -1, dtype=torch.int32), E)
+    A = cl.Adapters(torch.ones((E, 8, K), dtype=BF16, device="cuda"),
+                    torch.ones((E, N, 8), dtype=BF16, device="cuda"))
+    x = torch.ones((T, K), device="cuda")
+    for b in (base, base.to(BF16)):
+        for t in (F32, BF16):
+            y = cl.adapters_forward(A, x, off, slots, torch.empty((T, N), dtype=t, device="cuda"),
+                                    base=b.cuda())
+            assert torch.equal(y.cpu(), b.to(t))

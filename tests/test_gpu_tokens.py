@@ -219,6 +219,15 @@ def test_combine_grad(cl, y_type, d_type, cols):
 
 def test_rows_with_infinities_and_large_values(cl):
     """Infinities and NaN of a slot reach its own token only; bf16 rounding at the top."""
+    small = torch.tensor([[1e-40, -3e-39, 1.4e-45, 9.2e-41, 4.6e-41, 1.1754944e-38, -1e-45, 0.0]])
+    r = torch.tensor([[0, 1]], dtype=torch.int32).cuda()
+    for t in (F32, BF16):  # subnormal values stay
+        xs = torch.empty((2, 8), dtype=t, device="cuda")
+        cl.gather_tokens(small.cuda(), r, xs, top_k=2)
+        assert same(host(xs), small.to(t).double().expand(2, 8).numpy())
+        out = torch.empty((1, 8), dtype=t, device="cuda")
+        cl.combine_tokens(xs, r, out, top_k=2, weights=torch.tensor([[1.0, 0.0]]).cuda())
+        assert same(host(out), small.to(t).double().numpy())
     x = torch.tensor([[float("inf"), -float("inf"), NAN, 3.4e38, 3.3895e38, -3.4e38, 1e-45, -0.0]])
     rows = torch.tensor([[1, 0]], dtype=torch.int32).cuda()
     for t in (F32, BF16):
@@ -265,6 +274,7 @@ def test_moves_of_nothing_and_refusals(cl):
               lambda: cl.gather_tokens(x.to(FP8), r, y, top_k=2),
               lambda: cl.gather_tokens(x.t(), r, y, top_k=2),
               lambda: cl.gather_tokens(x, r.long(), y, top_k=2),
+              lambda: cl.gather_tokens(x[:, :0], r, y[:, :0], top_k=2),
               lambda: cl.gather_tokens(x, r, y, top_k=4), lambda: cl.gather_tokens(x, r, y, top_k=0),
               lambda: cl.combine_tokens(y, r, x.half(), top_k=2),
               lambda: cl.combine_tokens(y, r, x, top_k=2, weights=w[:2]),

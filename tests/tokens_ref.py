@@ -64,9 +64,8 @@ def combine_grad(dout, ys, rows, weights, dys, y_bf16):
 def adapters(a, b, ranks, scales, ids, x, base, y_bf16):
     """(ys, bound).  Products of bf16 values are exact in f32; a sum of n of them, in
     some order, is off by 2^-23 of the terms' magnitudes each (a matrix core may
-    truncate).  f32 x enters as three bf16 values that hold it to 2^-23 (the first one
-    truncated: 2^-7, then halves of steps: 2^-8 each), the inner values as three that hold
-    them to 2^-24 (f32 y) or two (2^-16)."""
+    truncate).  f32 x enters as three bf16 values that hold it, the inner values as three
+    that hold them to 2^-24 (f32 y) or two (2^-16)."""
     T, N, K = len(ids), b.shape[1], a.shape[2]
     out = np.zeros((T, N)) if base is None else np.array(base, np.float64)
     bound = np.zeros((T, N))
