@@ -33,8 +33,8 @@ CAI4_DEV int lanes_upto(int v) {
   return v;
 }
 
-// Chunk b (of ROWS rows) of all groups' in order (bare: group E among them), by each wave for itself:
-// lane i holds the offsets of `per` neighbouring groups and adds up their chunks.
+// Chunk b (of ROWS rows) of all groups' in order (bare: group E among them), by each wave
+// for itself: lane i holds the offsets of `per` neighbouring groups and adds up their chunks.
 template <int ROWS>
 CAI4_DEV Chunk find_chunk(const Adapters &a, int b, bool bare) {
   constexpr int kMostPer = (kSortMaxGroups + 1 + 63) / 64;
