@@ -8,9 +8,8 @@
 // kernel time for 4.9 + 5.4, but rank 32, or 16 rows and more, 15 to 65 % more than two.)
 //
 // Both products run on bf16 MFMAs with f32 sums.  A and B are bf16; f32 x, and u,
-// enter as a sum of bf16 planes, each the rounding of what the ones before left
-// over: x and, for f32 y, u in three (24 bits), for bf16 y u in two (16 bits: y's own
-// rounding is 2^-8).
+// enter as a sum of three bf16 planes, each what the ones before left over: all 24 bits,
+// also where y is bf16, since an f32 base may take away the sum's upper ones.
 //
 // Bound: HBM, by base and y (x, A and B besides); rows that are few, by two launches of
 // some three dependent round trips each.  4,096 rows, rank 32, 4,096 -> 14,336, all
@@ -29,41 +28,12 @@
 namespace cai4 {
 namespace {
 
-// v as N bf16 planes whose sum holds 8 N bits of it.  An infinity or NaN is in the
-// first alone: what an infinity leaves over would be NaN.
-template <int N>
-CAI4_DEV void planes_of(float v, uint32_t (&p)[N]) {
-  p[0] = split_hi(v);
-  float rest = v - bitsf(p[0] << 16);
-  if (!(fabsf(v) < INFINITY)) {
-    p[0] = f32_to_bf16_rne(v);
-    rest = 0.f;
-  }
-#pragma unroll
-  for (int i = 1; i < N; ++i) {
-    p[i] = f32_to_bf16_rne(rest);
-    rest -= bitsf(p[i] << 16);
-  }
-}
+constexpr int kPlanes = 3;  // of an f32 value
 
-// Eight values as the operands of N MFMAs.
-template <int N>
-CAI4_DEV void operands_of(const float (&v)[8], u32x4_t (&op)[N]) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    uint32_t lo[N], hi[N];
-    planes_of<N>(v[2 * i], lo);
-    planes_of<N>(v[2 * i + 1], hi);
-#pragma unroll
-    for (int p = 0; p < N; ++p) op[p][i] = lo[p] | hi[p] << 16;
-  }
-}
-
-// The same for x, of which there is much more, in a third of the instructions: three
-// planes, the first one truncated (so that no finite value becomes infinite).  It
-// leaves 16 bits, the second half a step of its 8, the third the rest: all 24 bits.  An
-// infinity is in the first alone, a NaN in any.
-CAI4_DEV void operands_of_x(const float (&v)[8], u32x4_t (&op)[3]) {
+// Eight values as the operands of three MFMAs: bf16 planes, the first one truncated (so
+// that no finite value becomes infinite).  It leaves 16 bits, the second half a step of
+// its 8, the third the rest: all 24 bits.  An infinity is in the first alone, a NaN in any.
+CAI4_DEV void operands_of(const float (&v)[8], u32x4_t (&op)[kPlanes]) {
   auto pair = [](float a, float b) {
     return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2_t{a, b}, bf16x2_t));
   };
@@ -99,7 +69,7 @@ constexpr int kInWaves = 8;  // of a workgroup: each has its own columns
 template <bool F32, int RT, int NT>
 CAI4_DEV void adapters_in_chunk(const Adapters &a, const Chunk &ch, int rank, int r0, int b0, int b1,
                                 f32x4_t (*part)[RT * NT][64], float *u) {
-  constexpr int P = F32 ? 3 : 1;
+  constexpr int P = F32 ? kPlanes : 1;
   constexpr int S = F32 && NT > 1 ? 2 : 4;  // steps of 32 columns loaded at a time
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, q = lane >> 4;
   const uint16_t *A[RT];
@@ -161,7 +131,7 @@ CAI4_DEV void adapters_in_chunk(const Adapters &a, const Chunk &ch, int rank, in
           float v[8];
 #pragma unroll
           for (int i = 0; i < 8; ++i) v[i] = xf[s][j][i / 4][i % 4];
-          operands_of_x(v, op);
+          operands_of(v, op);
         } else {
           op[0] = xv[s][j];
         }
@@ -239,7 +209,7 @@ CAI4_DEV float of_pair(float v) { return dpp_f32<0xB1>(v); }
 // a lane is of row pair_row[j][i & 1] (-1: none), columns run_col(i) on.
 template <bool F32, int BASE, int STEPS, int NT>
 struct OutBlock {
-  static constexpr int P = F32 ? 3 : 2, V = F32 ? 4 : 8, RUNS = 16 / V;
+  static constexpr int P = kPlanes, V = F32 ? 4 : 8, RUNS = 16 / V;
   typedef typename std::conditional<F32, float, uint16_t>::type Y;
   typedef typename std::conditional<BASE == kBaseF32, float, uint16_t>::type X;
   Run<X, V> base[NT][RUNS];
@@ -361,7 +331,7 @@ struct OutBlock {
 template <bool F32, int BASE, int STEPS, int NT, bool STREAM>
 CAI4_DEV void adapters_out_chunk(const Adapters &a, const Chunk &ch, const float *u, int slices,
                                  int n_begin, int n_end, u32x4_t *us) {
-  constexpr int P = F32 ? 3 : 2, kStride = kOutWaves * kColBlock;
+  constexpr int P = kPlanes, kStride = kOutWaves * kColBlock;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int c = lane & 15, q = lane >> 4;
   const bool own = ch.group < a.E;
@@ -401,7 +371,7 @@ CAI4_DEV void adapters_out_chunk(const Adapters &a, const Chunk &ch, const float
       for (int i = 0; i < 8; ++i) v[i] = r + i < rank ? v[i] * scale : 0.f;
     }
     u32x4_t op[P];
-    operands_of<P>(v, op);
+    operands_of(v, op);
 #pragma unroll
     for (int p = 0; p < P; ++p) us[((step * P + p) * NT + j) * 64 + lane] = op[p];
   }
@@ -473,7 +443,7 @@ void launch_out(const Adapters &a, const float *u, int slices, int bare, hipStre
   const int chunks = max_chunks(a.T, a.E + bare, kOutRows), cols = cols_of(a.N, chunks);
   const int stream = (size_t)a.T * a.N * (F32 ? 4 : 2) >= kStreamBytes && a.ldy % kLine == 0 &&
                      (uintptr_t)a.y % kLine == 0;
-  const size_t lds = (size_t)((a.R + 31) / 32) * (F32 ? 3 : 2) * (kOutRows / 16) * 64 * 16;
+  const size_t lds = (size_t)((a.R + 31) / 32) * kPlanes * (kOutRows / 16) * 64 * 16;
   hipLaunchKernelGGL((adapters_out_kernel<F32, BASE, STEPS>),
                      dim3((a.N + cols - 1) / cols, chunks), dim3(64 * kOutWaves), lds, st, a, u,
                      slices, cols, bare, stream);

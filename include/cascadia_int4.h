@@ -649,8 +649,8 @@ typedef struct cascadia_int4_adapters {
  *     several projections); xs of a row without an adapter is not read.  ys may be base (then of
  *     its type and stride, and rows without an adapter are not touched), otherwise
  *     overlaps no input.
- * f32 sums; one rounding at the end.  f32 xs enter whole, the inner a_i xs[t] to
- * 24 bits (f32 ys) or 16 (bf16).  An infinity of b may give NaN in place of an
+ * f32 sums; one rounding at the end (bf16 ys are f32 ys rounded).  f32 xs and the
+ * inner a_i xs[t] enter whole.  An infinity of b may give NaN in place of an
  * infinity.  n_tokens <= 2^20.  workspace: 16-byte aligned, of at least
  * _workspace_bytes for n_tokens rows or more, or NULL for the library's. */
 size_t cascadia_int4_adapters_workspace_bytes(const cascadia_int4_adapters *adapters,
