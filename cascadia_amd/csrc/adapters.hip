@@ -242,9 +242,13 @@ struct OutBlock {
   }
   template <bool FULL>
   CAI4_DEV void load(const Adapters &a, const uint16_t *B, const int (&row)[NT][2], int n0) {
-    const int left = a.N - n0;
 #pragma unroll
     for (int s = 0; s < STEPS; ++s) load_b<FULL>(a, B, n0, s, bv[s]);
+    load_base<FULL>(a, row, n0);
+  }
+  template <bool FULL>
+  CAI4_DEV void load_base(const Adapters &a, const int (&row)[NT][2], int n0) {
+    const int left = a.N - n0;
     if constexpr (BASE != kBaseNone) {
 #pragma unroll
       for (int j = 0; j < NT; ++j)
@@ -262,11 +266,40 @@ struct OutBlock {
         }
     }
   }
+  template <bool FULL, bool STREAM>
+  static CAI4_DEV void store(const Adapters &a, int row, int n0, int at, const Run<Y, V> &y) {
+    if (row < 0) return;
+    Y *p = row_at(static_cast<Y *>(a.y) + n0, a.ldy, row) + at;
+    if constexpr (FULL)
+      store_run<STREAM>(p, y);
+    else
+      store_part<Y, V>(p, y, a.N - n0 - at);
+  }
+  // y = base, every bit of it where both are of one type.
+  template <bool FULL, bool STREAM>
+  CAI4_DEV void copy(const Adapters &a, const int (&row)[NT][2], int n0) {
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int i = 0; i < RUNS; ++i) {
+        Run<Y, V> y = {};
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+          if constexpr (BASE == kBaseNone)
+            continue;
+          else if constexpr (std::is_same<X, Y>::value)
+            y.v[k] = base[j][i].v[k];
+          else
+            y.v[k] = row_value<Y>(value_of_row(base[j][i].v[k]));
+        }
+        store<FULL, STREAM>(a, row[j][i & 1], n0, run_col(i), y);
+      }
+  }
   // (A tile of 16 rows at a time: fewer sums at once, more waves.)
   template <bool FULL, bool STREAM>
   CAI4_DEV void finish(const Adapters &a, const uint16_t *B, int steps, int rank, const u32x4_t *us,
                        const int (&row)[NT][2], int n0) {
-    const int lane = threadIdx.x & 63, q = lane >> 4, left = a.N - n0;
+    const int lane = threadIdx.x & 63, q = lane >> 4;
     const bool odd = lane & 1;
 #pragma unroll
     for (int s = 0; s < STEPS; ++s) {
@@ -313,14 +346,7 @@ struct OutBlock {
         }
         const int at = run_col(i);
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          if (row[j][h] < 0) continue;
-          Y *p = row_at(static_cast<Y *>(a.y) + n0, a.ldy, row[j][h]);
-          if constexpr (FULL)
-            store_run<STREAM>(p + at, y[h]);
-          else
-            store_part<Y, V>(p + at, y[h], left - at);
-        }
+        for (int h = 0; h < 2; ++h) store<FULL, STREAM>(a, row[j][h], n0, at, y[h]);
       }
     }
   }
@@ -346,6 +372,18 @@ CAI4_DEV void adapters_out_chunk(const Adapters &a, const Chunk &ch, const float
   int n0 = n_begin + wave * kColBlock;
   const int n_full = n_end < a.N ? n_end : a.N / kColBlock * kColBlock;  // end of whole blocks
   OutBlock<F32, BASE, STEPS, NT> now;
+  if (rank == 0) {  // no product: base + 0 would lose the sign of a zero
+    if (a.base == a.y) return;
+    for (; n0 < n_full; n0 += kStride) {
+      now.template load_base<true>(a, row, n0);
+      now.template copy<true, STREAM>(a, row, n0);
+    }
+    if (n0 < n_end && n0 < a.N) {
+      now.template load_base<false>(a, row, n0);
+      now.template copy<false, false>(a, row, n0);
+    }
+    return;
+  }
   if (n0 < n_full) now.template load<true>(a, B, row, n0);
   for (int k = wave; k < steps * NT; k += kOutWaves) {
     const int step = k / NT, j = k % NT;

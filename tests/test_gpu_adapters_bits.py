@@ -1,4 +1,5 @@
-"""What adapters_forward keeps of its values: the bits of the inner values."""
+"""What adapters_forward keeps of its values: the bits of the inner values, rows without
+an adapter as they are."""
 import numpy as np
 import pytest
 import torch
@@ -48,3 +49,51 @@ def test_a_base_that_cancels_the_adapter(cl, T):
     want = host(base) + host(picked)
     bound = 2.0 ** -8 * np.abs(want) + 2.0 ** -21 * np.abs(host(picked))
     assert np.all(np.abs(host(forward(cl, c, BF16)) - want) <= bound)
+
+
+def bits(t):
+    return t.view(torch.int16 if t.dtype is BF16 else torch.int32).cpu()
+
+
+@pytest.mark.parametrize("base_type", [F32, BF16])
+@pytest.mark.parametrize("y_type", [F32, BF16])
+@pytest.mark.parametrize("rank_zero", [False, True])
+def test_rows_without_an_adapter_keep_every_bit(cl, base_type, y_type, rank_zero):
+    """Zeros of either sign, subnormal values, infinities and the largest values, beside rows
+    that have an adapter; out of place and in place."""
+    T, E, N, K, R = 75, 3, 104, 64, 16
+    g = gen(22)
+    a, b = torch.randn((E, R, K), generator=g).to(BF16), torch.randn((E, N, R), generator=g).to(BF16)
+    ranks = torch.tensor([R, 0, 8], dtype=torch.int32)
+    ids = torch.arange(T, dtype=torch.int32) % E
+    if not rank_zero:
+        ids[ids == 1] = -1
+    bare = (ids == 1) | (ids < 0)
+    v = torch.tensor([-0.0, 0.0, -1e-40, 1.0, float("-inf"), 3.3e38, -1.1754944e-38, 0.1])
+    base = v[torch.randint(0, 8, (T, N), generator=g)].to(base_type)
+    base[~bare] = 0.5
+    x = torch.randn((T, K), generator=g).to(BF16)
+    c = (a, b, ranks, torch.ones(E), ids, x, base)
+    out = forward(cl, c, y_type)
+    assert torch.equal(bits(out)[bare], bits(base.to(y_type))[bare])
+    assert bool((out.cpu()[~bare] != 0.5).any(1).all())
+    if base_type is y_type:
+        off, slots = plan(cl, ids, E)
+        A = cl.Adapters(a.cuda(), b.cuda(), ranks=ranks.cuda())
+        y = base.cuda()
+        cl.adapters_forward(A, x.cuda(), off, slots, y, base=y)
+        assert torch.equal(bits(y), bits(out))
+
+
+def test_rows_without_an_adapter_over_many_rows(cl):
+    """The same where whole lines are written past the caches."""
+    T, E, N, K, R = 9000, 3, 4096, 16, 8
+    ids = torch.arange(T, dtype=torch.int32) % 4 - 1
+    bare = ids < 0
+    x, a, b = torch.ones((T, K)), torch.ones((E, R, K), dtype=BF16), torch.ones((E, N, R), dtype=BF16)
+    base = torch.full((T, N), -0.0)
+    c = (a, b, torch.full((E,), R, dtype=torch.int32), torch.ones(E), ids, x, base)
+    for t in (F32, BF16):
+        out = forward(cl, c, t).cpu()
+        assert bool((bits(out)[bare] == bits(base[:1].to(t))).all())
+        assert bool((out[~bare] == K * R).all())
