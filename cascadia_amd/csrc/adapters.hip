@@ -49,6 +49,66 @@ CAI4_DEV void operands_of(const float (&v)[8], u32x4_t (&op)[kPlanes]) {
   }
 }
 
+// What an infinity w meets in planes: 0 times it in those that a value leaves empty, or
+// two infinities of unlike sign, both NaN.  So where a sum comes out as NaN it is taken
+// again, with the infinities (and NaN) of each side apart, times the other side's signs;
+// the other sums of the wave keep their bits, to which it adds zeros.  Each function
+// takes words of two bf16 values.
+CAI4_DEV uint32_t halves_of(uint32_t tops) { return ((tops & 0x80008000u) >> 15) * 0xFFFFu; }
+CAI4_DEV uint32_t nonfinite(uint32_t w) { return halves_of((w & 0x7F807F80u) + 0x00800080u); }
+CAI4_DEV uint32_t nonzero(uint32_t w) { return halves_of((w & 0x7FFF7FFFu) + 0x7FFF7FFFu); }
+CAI4_DEV uint32_t sign_of(uint32_t w) { return nonzero(w) & ((w & 0x80008000u) | 0x3F803F80u); }
+struct Sides {
+  u32x4_t finite, infinite, sign;
+};
+CAI4_DEV Sides sides_of(u32x4_t w) {
+  Sides s;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    s.infinite[i] = w[i] & nonfinite(w[i]);
+    s.finite[i] = w[i] & ~nonfinite(w[i]);
+    s.sign[i] = sign_of(w[i]);
+  }
+  return s;
+}
+// The same of a value's planes, the first of which alone says whether it is finite; an
+// infinite one leaves them.
+CAI4_DEV Sides sides_of(u32x4_t (&op)[kPlanes]) {
+  Sides s;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t infinite = nonfinite(op[0][i]);
+    uint32_t first = op[kPlanes - 1][i];  // of the planes, the first that is not zero
+#pragma unroll
+    for (int p = kPlanes - 2; p >= 0; --p)
+      first = (op[p][i] & nonzero(op[p][i])) | (first & ~nonzero(op[p][i]));
+    s.infinite[i] = op[0][i] & infinite;
+    s.sign[i] = sign_of(first);
+#pragma unroll
+    for (int p = 0; p < kPlanes; ++p) op[p][i] &= ~infinite;
+  }
+  return s;
+}
+// acc + w times a value in planes, of sides s.  (One at a time: few registers, since the
+// kernels that may come here need theirs for loads in flight.)
+CAI4_DEV void add_sides(u32x4_t w, const u32x4_t (&op)[kPlanes], const Sides &s, f32x4_t &acc) {
+  const Sides ws = sides_of(w);
+#pragma unroll
+  for (int p = 0; p < kPlanes; ++p) acc = mfma_bf16(ws.finite, op[p], acc);
+  acc = mfma_bf16(ws.infinite, s.sign, acc);
+  acc = mfma_bf16(ws.sign, s.infinite, acc);
+  __builtin_amdgcn_sched_barrier(0);
+}
+// Whether any lane has a NaN.
+template <int N>
+CAI4_DEV bool any_nan(const f32x4_t (&acc)[N]) {
+  bool nan = false;
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+    nan |= __builtin_isunordered(acc[i][0], acc[i][1]) || __builtin_isunordered(acc[i][2], acc[i][3]);
+  return __builtin_expect(__ballot(nan) != 0, 0);
+}
+
 // Bits to keep of columns r .. r + 7 of a row of B: those below the rank (the others
 // may hold anything).
 CAI4_DEV u32x4_t keep_of(int rank, int r) {
@@ -62,6 +122,38 @@ CAI4_DEV u32x4_t keep_of(int rank, int r) {
 // ---- u = A x ----
 
 constexpr int kInWaves = 8;  // of a workgroup: each has its own columns
+
+// A wave's sums over blocks [b0, b1) of 128 columns with infinities apart (f32 x).
+template <int RT, int NT>
+CAI4_DEV void sums_of_sides(const Adapters &a, const uint16_t *const (&A)[RT],
+                            const uint8_t *const (&x)[NT], int b0, int b1,
+                            f32x4_t (&acc)[RT][NT]) {
+#pragma unroll
+  for (int i = 0; i < RT; ++i)
+#pragma unroll
+    for (int j = 0; j < NT; ++j) acc[i][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  const int q = (threadIdx.x & 63) >> 4;
+  for (int at = b0 * 128; at < b1 * 128; at += 32) {
+    const bool in = at + q * 8 < a.K;
+    const int col = in ? at + q * 8 : 0;
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      const Run<float, 8> r = load_run<float, 8>(reinterpret_cast<const float *>(x[j]) + col);
+      float v[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = in ? r.v[i] : 0.f;
+      u32x4_t op[kPlanes];
+      operands_of(v, op);
+      const Sides s = sides_of(op);
+#pragma unroll
+      for (int i = 0; i < RT; ++i) {
+        u32x4_t w = *reinterpret_cast<const u32x4_t *>(A[i] + col);
+        w = in ? w : u32x4_t{0, 0, 0, 0};
+        add_sides(w, op, s, acc[i][j]);
+      }
+    }
+  }
+}
 
 // A workgroup's slice of K for RT * 16 ranks and NT * 16 rows of a chunk.  A wave has
 // blocks [b0, b1) of 128 columns; the waves' sums are added in LDS, eight to four to
@@ -141,6 +233,12 @@ CAI4_DEV void adapters_in_chunk(const Adapters &a, const Chunk &ch, int rank, in
           for (int p = 0; p < P; ++p) acc[i][j] = mfma_bf16(av[s][i], op[p], acc[i][j]);
       }
     }
+  }
+  if constexpr (F32) {
+    bool nan = false;
+#pragma unroll
+    for (int i = 0; i < RT; ++i) nan |= any_nan(acc[i]);
+    if (nan) sums_of_sides(a, A, x, b0, b1, acc);
   }
   constexpr int kHalf = kInWaves / 2;
   if (wave >= kHalf)
@@ -222,15 +320,19 @@ struct OutBlock {
     return ((i & ~1) + (lane & 1)) * (kColBlock / RUNS) + (lane >> 4) * V;
   }
 
+  // Ranks step * 32 + 8 q on of row m's column of B.
+  template <bool FULL>
+  static CAI4_DEV const u32x4_t *weights_at(const Adapters &a, const uint16_t *B, int n0, int step,
+                                            int m) {
+    const int lane = threadIdx.x & 63, c = lane & 15, q = lane >> 4, left = a.N - n0;
+    const int r = step * 32 + q * 8, at = weight_col<F32>(m, c);
+    const int n = FULL || at < left ? n0 + at : a.N - 1;
+    return reinterpret_cast<const u32x4_t *>(B + (size_t)n * a.R + (r < a.R ? r : 0));
+  }
   template <bool FULL>
   CAI4_DEV void load_b(const Adapters &a, const uint16_t *B, int n0, int step, u32x4_t (&v)[4]) {
-    const int lane = threadIdx.x & 63, c = lane & 15, q = lane >> 4, left = a.N - n0;
-    const int r = step * 32 + q * 8;
 #pragma unroll
-    for (int m = 0; m < 4; ++m) {
-      const int at = weight_col<F32>(m, c), n = FULL || at < left ? n0 + at : a.N - 1;
-      v[m] = *reinterpret_cast<const u32x4_t *>(B + (size_t)n * a.R + (r < a.R ? r : 0));
-    }
+    for (int m = 0; m < 4; ++m) v[m] = *weights_at<FULL>(a, B, n0, step, m);
   }
   // Row r of p, made anew at each use: eight addresses kept would be 16 registers.
   template <class T>
@@ -295,18 +397,42 @@ struct OutBlock {
         store<FULL, STREAM>(a, row[j][i & 1], n0, run_col(i), y);
       }
   }
+  CAI4_DEV void keep_ranks(int rank) {
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s) {
+      const u32x4_t keep = keep_of(rank, s * 32 + (threadIdx.x & 63) / 16 * 8);
+#pragma unroll
+      for (int m = 0; m < 4; ++m) bv[s][m] &= keep;
+    }
+  }
+  // The sums of tile j's rows with infinities apart.
+  template <bool FULL>
+  static CAI4_DEV void sums_of_sides(const Adapters &a, const uint16_t *B, int steps, int rank,
+                                     const u32x4_t *us, int j, int n0, f32x4_t (&acc)[4]) {
+    const int lane = threadIdx.x & 63, q = lane >> 4;
+#pragma unroll
+    for (int m = 0; m < 4; ++m) acc[m] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+    for (int s = 0; s < steps; ++s) {
+      u32x4_t op[P];
+#pragma unroll
+      for (int p = 0; p < P; ++p) op[p] = us[((s * P + p) * NT + j) * 64 + lane];
+      const Sides sides = sides_of(op);
+      const u32x4_t keep = keep_of(rank, s * 32 + q * 8);
+#pragma unroll
+      for (int m = 0; m < 4; ++m) {
+        const u32x4_t w = *weights_at<FULL>(a, B, n0, s, m);
+        add_sides(w & keep, op, sides, acc[m]);
+      }
+    }
+  }
   // (A tile of 16 rows at a time: fewer sums at once, more waves.)
   template <bool FULL, bool STREAM>
   CAI4_DEV void finish(const Adapters &a, const uint16_t *B, int steps, int rank, const u32x4_t *us,
                        const int (&row)[NT][2], int n0) {
     const int lane = threadIdx.x & 63, q = lane >> 4;
     const bool odd = lane & 1;
-#pragma unroll
-    for (int s = 0; s < STEPS; ++s) {
-      const u32x4_t keep = keep_of(rank, s * 32 + q * 8);
-#pragma unroll
-      for (int m = 0; m < 4; ++m) bv[s][m] &= keep;
-    }
+    keep_ranks(rank);
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
       f32x4_t acc[4] = {};
@@ -330,8 +456,18 @@ struct OutBlock {
           add(s, bv[0]);
         }
       }
+      if (any_nan(acc)) {
+        // (what was loaded is loaded again: it and its addresses, kept meanwhile, would
+        // take registers)
+        int again = n0;
+        asm volatile("" : "+v"(again));
+        sums_of_sides<FULL>(a, B, steps, rank, us, j, again, acc);
+        load<FULL>(a, B, row, again);
+        keep_ranks(rank);
+      }
 #pragma unroll
       for (int i = 0; i < RUNS; i += 2) {
+        __builtin_amdgcn_sched_barrier(0);  // (one pair of runs at a time: registers)
         Run<Y, V> y[2];  // of the even row, of the odd one
 #pragma unroll
         for (int k = 0; k < V; ++k) {

@@ -650,8 +650,8 @@ typedef struct cascadia_int4_adapters {
  *     its type and stride, and rows without an adapter are not touched), otherwise
  *     overlaps no input.
  * f32 sums; one rounding at the end (bf16 ys are f32 ys rounded).  f32 xs and the
- * inner a_i xs[t] enter whole.  An infinity of b may give NaN in place of an
- * infinity.  n_tokens <= 2^20.  workspace: 16-byte aligned, of at least
+ * inner a_i xs[t] enter whole (bits below 2^-133 apart), infinities and NaN of xs, a and
+ * b as in the formula.  n_tokens <= 2^20.  workspace: 16-byte aligned, of at least
  * _workspace_bytes for n_tokens rows or more, or NULL for the library's. */
 size_t cascadia_int4_adapters_workspace_bytes(const cascadia_int4_adapters *adapters,
                                               uint32_t n_tokens);
