@@ -2612,6 +2612,14 @@ bool slots_ok(uint32_t n_tokens, uint32_t top_k) {
   return n_tokens <= (uint32_t)cai4::kSortMaxTokens && top_k >= 1 &&
          top_k <= (uint32_t)cai4::kSortMaxTopK;
 }
+struct Bytes {
+  const void *at;
+  size_t n;
+};
+bool overlap(const Bytes &x, const Bytes &y) {
+  const uintptr_t p = (uintptr_t)x.at, q = (uintptr_t)y.at;
+  return x.at && y.at && x.n && y.n && p < q + y.n && q < p + x.n;
+}
 bool row_cols_ok(uint32_t cols) { return cols >= 1 && cols <= (uint32_t)cai4::kRowMaxCols; }
 
 int adapters_check(const cascadia_int4_adapters *A, uint32_t n_tokens) {
@@ -2658,9 +2666,19 @@ int cascadia_int4_sort_tokens(const int32_t *ids, const float *weights, float th
   s.offsets = offsets;
   s.slots = slots;
   s.rows = rows;
+  const size_t need = cai4::sort_tokens_workspace(s.n, s.E);
+  // (slots whose ids change between the launches would be written where no slot belongs)
+  const size_t each = (size_t)s.n * 4;
+  const Bytes out[4] = {{offsets, (size_t)(s.E + 1) * 4}, {slots, each}, {rows, each},
+                        {workspace, need}};
+  for (int i = 0; i < 4; ++i) {
+    if (overlap(out[i], {ids, each}) || overlap(out[i], {weights, each}))
+      return CASCADIA_INT4_ERR_ARG;
+    for (int j = 0; j < i; ++j)
+      if (overlap(out[i], out[j])) return CASCADIA_INT4_ERR_ARG;
+  }
   const hipStream_t st = (hipStream_t)stream;
   Workspace own;
-  const size_t need = cai4::sort_tokens_workspace(s.n, s.E);
   if (need && !workspace) {
     int dev;
     if (int rc = current_device(&dev)) return rc;

@@ -217,7 +217,9 @@ __global__ __launch_bounds__(64 * W) void sort_place_kernel(SortTokens s, int sh
 #pragma unroll
     for (int i = 0; i < kSteps; ++i) {
       const int p = once ? (e[i] >= 0 ? next[e[i]] : 0) + place[i] : take_places(e[i], bits, next);
-      if (e[i] < 0) continue;
+      // (p is out of range only where ids or the counts changed meanwhile: another call over
+      // the same workspace)
+      if (e[i] < 0 || (uint32_t)p >= (uint32_t)s.n) continue;
       const int k = at + i * 64 + lane;
       s.slots[p] = k;
       s.rows[k] = e[i] < s.E ? p : -1;
