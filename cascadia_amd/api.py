@@ -86,6 +86,15 @@ def _expect(cond: bool, msg: str) -> None:
         raise ValueError(msg)
 
 
+def _sizes(*values):
+    """Sizes as the library takes them: ctypes would cut others off to 32 bits."""
+    out = tuple(map(_index, values))
+    for v in out:
+        if not 0 <= v < 1 << 32:
+            raise ValueError(f"a size of {v} is not one of 32 bits")
+    return out
+
+
 def _is_bf16_bits(t: torch.Tensor) -> bool:
     return t.dtype in (torch.bfloat16, torch.int16, torch.uint16)
 
@@ -317,6 +326,7 @@ def gemm_workspace_bytes(n_rows, k_cols, seq, x_f32, group_size=GROUP_SIZE,
                          tiling=TILING_CRATE) -> int:
     """Workspace bytes of dequant_gemm_int4_multi_auto / gemm_int4_bf16 for up to
     seq rows on the current device."""
+    n_rows, k_cols, seq, group_size = _sizes(n_rows, k_cols, seq, group_size)
     return int(lib().cascadia_int4_gemm_workspace_bytes(
         _layout(n_rows, k_cols, group_size, SCALE_BF16, tiling), int(x_f32), seq))
 
@@ -569,7 +579,7 @@ def gate_up_silu(x, gate_packed, gate_scale, up_packed, up_scale, inter_out,
 def ffn_workspace_bytes(hidden, inter, n_tokens, group_size=GROUP_SIZE) -> int:
     """Workspace bytes of expert_forward / ffn_forward_sparse_f32 for up to
     n_tokens rows on the current device."""
-    return int(lib().cascadia_int4_ffn_workspace_bytes(hidden, inter, group_size, n_tokens))
+    return int(lib().cascadia_int4_ffn_workspace_bytes(*_sizes(hidden, inter, group_size, n_tokens)))
 
 
 def expert_forward(x_bf16, gate_packed, gate_scale, up_packed, up_scale, down_packed,
@@ -637,8 +647,8 @@ def _sparse_call(x, weights, out, threshold, thresholds, group_size, scale_dtype
 
 
 def ffn_sparse_axpy_workspace_bytes(hidden, inter, n_tokens, group_size=GROUP_SIZE) -> int:
-    return int(lib().cascadia_int4_ffn_sparse_axpy_workspace_bytes(hidden, inter, group_size,
-                                                                    n_tokens))
+    return int(lib().cascadia_int4_ffn_sparse_axpy_workspace_bytes(
+        *_sizes(hidden, inter, group_size, n_tokens)))
 
 
 def ffn_forward_sparse_axpy_f32_mode(x_f32, hidden, intermediate, gate_packed, gate_scale,
@@ -760,8 +770,8 @@ dequant_axpy_int4_active_auto = dequant_axpy_int4_active  # ffn_axpy.rs:274
 
 def ffn_sparse_workspace_bytes(hidden, inter, n_tokens, group_size=GROUP_SIZE) -> int:
     """Workspace bytes of the sparse entry points for up to n_tokens rows."""
-    return int(lib().cascadia_int4_ffn_sparse_workspace_bytes(hidden, inter, group_size,
-                                                              n_tokens))
+    return int(lib().cascadia_int4_ffn_sparse_workspace_bytes(
+        *_sizes(hidden, inter, group_size, n_tokens)))
 
 
 def expert_forward_sparse(x_bf16, gate_packed, gate_scale, up_packed, up_scale, down_packed,
@@ -898,7 +908,8 @@ class MoEExperts:
 
 
 def moe_workspace_bytes(experts: MoEExperts, top_k: int, n_tokens: int) -> int:
-    return int(lib().cascadia_int4_moe_workspace_bytes(C.byref(experts._struct()), top_k, n_tokens))
+    return int(lib().cascadia_int4_moe_workspace_bytes(C.byref(experts._struct()),
+                                                       *_sizes(top_k, n_tokens)))
 
 
 @functools.lru_cache(maxsize=1024)
@@ -1112,6 +1123,7 @@ def _fp8_x_type(dtype) -> int:
 
 def fp8_gemm_workspace_bytes(n_rows: int, k_cols: int, seq: int, x_dtype=torch.bfloat16) -> int:
     """Workspace bytes of fp8_gemm for up to seq rows of x_dtype."""
+    n_rows, k_cols, seq = _sizes(n_rows, k_cols, seq)
     return int(lib().cascadia_int4_fp8_gemm_workspace_bytes(n_rows, k_cols, _fp8_x_type(x_dtype),
                                                             seq))
 
@@ -1204,7 +1216,7 @@ class Fp8Experts:
 
 def fp8_moe_workspace_bytes(experts: Fp8Experts, top_k: int, n_tokens: int) -> int:
     """Workspace bytes of fp8_moe_forward for up to n_tokens rows."""
-    return int(lib().cascadia_int4_fp8_moe_workspace_bytes(experts._ref, top_k, n_tokens))
+    return int(lib().cascadia_int4_fp8_moe_workspace_bytes(experts._ref, *_sizes(top_k, n_tokens)))
 
 
 @functools.lru_cache(maxsize=1024)
@@ -1264,7 +1276,7 @@ def fp8_moe_forward(experts: Fp8Experts, x, out, *, top_k: int, ids, weights,
 
 def sort_tokens_workspace_bytes(n_tokens: int, top_k: int, n_experts: int) -> int:
     """Workspace bytes of sort_tokens for up to n_tokens tokens."""
-    return int(lib().cascadia_int4_sort_tokens_workspace_bytes(n_tokens, top_k, n_experts))
+    return int(lib().cascadia_int4_sort_tokens_workspace_bytes(*_sizes(n_tokens, top_k, n_experts)))
 
 
 def _flat(dev, t, dtype, n, name):
@@ -1439,7 +1451,7 @@ class Adapters:
 
 def adapters_workspace_bytes(adapters: Adapters, n_tokens: int) -> int:
     """Workspace bytes of adapters_forward for up to n_tokens rows."""
-    return int(lib().cascadia_int4_adapters_workspace_bytes(adapters._ref, n_tokens))
+    return int(lib().cascadia_int4_adapters_workspace_bytes(adapters._ref, *_sizes(n_tokens)))
 
 
 @functools.lru_cache(maxsize=1024)

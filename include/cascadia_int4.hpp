@@ -148,6 +148,12 @@ inline void check(int rc, const char *fn) {
   throw DeviceError(fn, rc);
 }
 
+// A size as the C ABI takes it.
+inline uint32_t size32(size_t n) {
+  require(n <= UINT32_MAX, "sizes exceed 32 bits");
+  return (uint32_t)n;
+}
+
 inline void finish(const Options &o) {
   if (o.synchronize) check(cascadia_int4_synchronize(o.stream), "cascadia_int4_synchronize");
 }
@@ -852,7 +858,7 @@ class MoeLayer {
   const cascadia_int4_moe_layer &c_layer() const { return l_; }
   // device workspace bytes of moe_forward (Options::workspace)
   size_t workspace_bytes(size_t top_k, size_t n_tokens) const {
-    return cascadia_int4_moe_workspace_bytes(&l_, (uint32_t)top_k, (uint32_t)n_tokens);
+    return cascadia_int4_moe_workspace_bytes(&l_, detail::size32(top_k), detail::size32(n_tokens));
   }
 
  private:
@@ -1096,7 +1102,8 @@ class Fp8Experts {
   size_t hidden() const { return l_.hidden; }
   const cascadia_int4_fp8_moe_layer &c_layer() const { return l_; }
   size_t workspace_bytes(size_t top_k, size_t n_tokens) const {
-    return cascadia_int4_fp8_moe_workspace_bytes(&l_, (uint32_t)top_k, (uint32_t)n_tokens);
+    return cascadia_int4_fp8_moe_workspace_bytes(&l_, detail::size32(top_k),
+                                                 detail::size32(n_tokens));
   }
 
  private:
@@ -1166,10 +1173,8 @@ struct RowsOut {
 };
 
 inline size_t sort_tokens_workspace_bytes(size_t n_tokens, size_t top_k, size_t n_experts) {
-  detail::require(n_tokens <= UINT32_MAX && top_k <= UINT32_MAX && n_experts <= UINT32_MAX,
-                  "unsupported sizes");
-  return cascadia_int4_sort_tokens_workspace_bytes((uint32_t)n_tokens, (uint32_t)top_k,
-                                                   (uint32_t)n_experts);
+  return cascadia_int4_sort_tokens_workspace_bytes(
+      detail::size32(n_tokens), detail::size32(top_k), detail::size32(n_experts));
 }
 
 // offsets [n_experts + 1], slots [n_tokens * top_k] (sorted row -> slot), rows
@@ -1287,7 +1292,7 @@ class Adapters {
   }
   const cascadia_int4_adapters &c_adapters() const { return s_; }
   size_t workspace_bytes(size_t n_tokens) const {
-    return cascadia_int4_adapters_workspace_bytes(&s_, (uint32_t)n_tokens);
+    return cascadia_int4_adapters_workspace_bytes(&s_, detail::size32(n_tokens));
   }
 
  private:
