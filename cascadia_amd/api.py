@@ -1400,8 +1400,8 @@ def gather_tokens_grad(dxs, rows, dx, *, top_k: int):
 
 def combine_tokens_grad(dout, ys, rows, weights, dys, dweights, *, top_k: int):
     """The gradient of combine_tokens from that of its output, dout [n_tokens, cols]
-    (which is the residual's): dys[rows[t, j]] = weights[t, j] * dout[t], of ys's type
-    (rows that no slot has stay as they are; dys may be ys), and dweights[t, j] =
+    (which is the residual's): dys[rows[t, j]] = weights[t, j] * dout[t], rounded to f32,
+    then to ys's type (rows that no slot has stay as they are; dys may be ys), and dweights[t, j] =
     sum_c ys[rows[t, j], c] * dout[t, c] in f32 (0 for a slot left out).  dout and ys
     bf16 or f32."""
     dev = _home(ys, "ys")

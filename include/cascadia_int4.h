@@ -616,8 +616,9 @@ int cascadia_int4_combine_tokens(const void *ys, uint32_t y_is_f32, const int32_
 
 /* The gradient of cascadia_int4_combine_tokens from that of out, dout [n_tokens, cols]
  * f32 (dout_is_f32) or bf16 (the residual's is dout itself):
- *   dys[rows[t, j]] = weights[t, j] * dout[t], of ys's type, one rounding; rows that
- *     no slot has are left as they are.  dys may be ys, otherwise overlaps no input.
+ *   dys[rows[t, j]] = weights[t, j] * dout[t], rounded to f32 and then to ys's type;
+ *     rows that no slot has are left as they are.  dys may be ys, otherwise overlaps no
+ *     input.
  *   dweights[t, j] = sum_c ys[rows[t, j], c] * dout[t, c] in f32; 0 for a slot left
  *     out.  Sums in an order that depends on cols alone. */
 int cascadia_int4_combine_tokens_grad(const void *dout, uint32_t dout_is_f32, const void *ys,
