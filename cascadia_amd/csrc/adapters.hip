@@ -141,7 +141,8 @@ CAI4_DEV void sums_of_sides(const Adapters &a, const uint16_t *const (&A)[RT],
       const Run<float, 8> r = load_run<float, 8>(reinterpret_cast<const float *>(x[j]) + col);
       float v[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = in ? r.v[i] : 0.f;
+      for (int i = 0; i < 8; ++i)  // (quiet: the first plane of a NaN is one)
+        v[i] = in ? __builtin_canonicalizef(r.v[i]) : 0.f;
       u32x4_t op[kPlanes];
       operands_of(v, op);
       const Sides s = sides_of(op);

@@ -86,3 +86,20 @@ def test_one_infinite_weight_alone(cl, x_type, y_type, T):
             want[:, 5], want[:, 6] = sign * INF, sign
         assert torch.equal(got[at], want)
         assert not got[~at].any()
+
+
+@pytest.mark.parametrize("T", [1, 20, 1100, 2100])
+@pytest.mark.parametrize("nan", [0x7F800001, 0x7FC00000, -0x7FFF01, 0x7FFFFFFF])
+def test_every_nan_of_x_stays_one(cl, T, nan):
+    """Signalling ones too, whose upper half alone would be an infinity."""
+    K, N, R = 136, 70, 40
+    g = gen(24)
+    a, b = (torch.rand(s, generator=g).to(BF16) + 1.0 for s in ((1, R, K), (1, N, R)))
+    x = torch.randn((T, K), generator=g)
+    x.view(torch.int32)[T // 2, 9] = nan
+    c = (a, b, torch.tensor([R], dtype=torch.int32), torch.ones(1), torch.zeros(T, dtype=torch.int32), x,
+         None)
+    got = forward(cl, c, F32).cpu()
+    assert bool(got[T // 2].isnan().all())
+    got[T // 2] = 0
+    assert bool(got.isfinite().all())
