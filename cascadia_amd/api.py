@@ -1326,7 +1326,8 @@ def sort_tokens(ids, top_k: int, n_experts: int, offsets, slots, rows, *, weight
       rows [n_tokens, top_k]: the sorted row of each slot, -1 where left out.
     All int32.  Left out: ids outside [0, n_experts) (padding: -1) and, where weights
     (f32 [n_tokens, top_k]) are given, slots of weight < threshold.  n_experts <= 1024,
-    top_k <= 16, n_tokens <= 2^20; the outputs overlap neither each other nor the inputs.
+    top_k <= 16, n_tokens <= 2^20; rows may be ids, otherwise the outputs overlap neither
+    each other nor the inputs.
     With top_k 1 it groups rows by adapter (adapters_forward).  workspace:
     sort_tokens_workspace_bytes (for a graph capture)."""
     dev = _home(offsets, "offsets")

@@ -2672,7 +2672,9 @@ int cascadia_int4_sort_tokens(const int32_t *ids, const float *weights, float th
   const Bytes out[4] = {{offsets, (size_t)(s.E + 1) * 4}, {slots, each}, {rows, each},
                         {workspace, need}};
   for (int i = 0; i < 4; ++i) {
-    if (overlap(out[i], {ids, each}) || overlap(out[i], {weights, each}))
+    // (rows in place of ids: a wave reads a run of ids before it writes their rows)
+    const bool in_place = out[i].at == rows && rows == ids;
+    if ((overlap(out[i], {ids, each}) && !in_place) || overlap(out[i], {weights, each}))
       return CASCADIA_INT4_ERR_ARG;
     for (int j = 0; j < i; ++j)
       if (overlap(out[i], out[j])) return CASCADIA_INT4_ERR_ARG;

@@ -579,8 +579,8 @@ int cascadia_int4_debug_fp8_moe_form(const cascadia_int4_fp8_moe_layer *layer, u
  *     expert; behind the last row the slots left out, ascending.
  *   rows [n_tokens, top_k]: the sorted row of each slot, -1 where left out.
  * n_experts <= 1024, top_k <= 16, n_tokens <= 2^20; zero tokens set offsets to 0.
- * offsets, slots, rows and workspace overlap neither each other nor the inputs (refused:
- * CASCADIA_INT4_ERR_ARG).
+ * rows may be ids; otherwise offsets, slots, rows and workspace overlap neither each
+ * other nor the inputs (refused: CASCADIA_INT4_ERR_ARG).
  * workspace: 16-byte aligned, of at least _workspace_bytes for these sizes or larger
  * ones, or NULL for the library's.  With top_k 1 the same call groups a batch's
  * rows by adapter (below). */

@@ -1,9 +1,11 @@
-"""sort_tokens refuses buffers that overlap: its launches count the slots twice and write
-where the counts say.  On the CPU: no call here reaches the device."""
+"""sort_tokens refuses buffers that overlap (on the CPU: no call that is refused reaches the
+device), except rows in place of ids."""
 import itertools
 
 import pytest
 import torch
+
+import tokens_ref as ref
 
 P = 1 << 24  # addresses that no call may read
 NAMES = ("ids", "w", "off", "slots", "rows", "ws")
@@ -34,6 +36,8 @@ def test_overlapping_buffers_are_refused(cl, T, k, E):
         at = far[x]
         last = at + (size[x] - 4) // 16 * 16  # (workspaces lie on 16 bytes)
         for where in (at, last, at - (size[y] - 4) // 16 * 16):
+            if {x, y} == {"ids", "rows"} and where == at:
+                continue  # (rows may be ids)
             assert call(**{y: where}) == arg, (x, y, where - at)
 
 
@@ -47,3 +51,18 @@ def test_neighbours_are_not_refused(cl):
         ids, o, slots, rows, w = at
         assert L.cascadia_int4_sort_tokens(ids, w, 0.0, T, k, E, o, slots, rows, None, None) != arg
         assert L.cascadia_int4_sort_tokens(ids, ids, 0.0, T, k, E, o, slots, rows, None, None) != arg
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,k,E", [(1, 1, 1), (100, 8, 60), (3000, 2, 5), (9000, 8, 384),
+                                   (70001, 8, 1024), (200000, 3, 17)])
+def test_rows_in_place_of_ids(cl, T, k, E):
+    g = torch.Generator()
+    g.manual_seed(T)
+    ids = torch.randint(-1, E + 1, (T, k), generator=g, dtype=torch.int32)
+    want = ref.sort(ids.numpy(), E)
+    rows = ids.cuda()
+    off, slots = (torch.empty(n, dtype=torch.int32, device="cuda") for n in (E + 1, T * k))
+    cl.sort_tokens(rows, k, E, off, slots, rows)
+    for a, b in zip((off, slots, rows), want):
+        assert torch.equal(a.cpu(), torch.from_numpy(b))
