@@ -562,10 +562,12 @@ CAI4_DEV void adapters_out_chunk(const Adapters &a, const Chunk &ch, const float
   }
 }
 
+// (Ranks past 64, whose B is read where it is multiplied, want four waves per SIMD rather
+// than three: 2,048 rows of rank 96, 4,096 -> 4,096, 33 / 36 us.  Fewer ranks do not fit
+// four, for lack of registers.)
 template <bool F32, int BASE, int STEPS>
-__global__ __launch_bounds__(64 * kOutWaves) void adapters_out_kernel(Adapters a, const float *u,
-                                                                      int slices, int cols,
-                                                                      int bare, int stream) {
+__global__ __launch_bounds__(64 * kOutWaves, STEPS ? 1 : 4) void adapters_out_kernel(
+    Adapters a, const float *u, int slices, int cols, int bare, int stream) {
   extern __shared__ u32x4_t us[];  // [steps of 32 ranks][planes][tiles][lane]
   const Chunk ch = find_chunk<kOutRows>(a, blockIdx.y, bare);
   if (ch.rows == 0) return;
