@@ -1,9 +1,10 @@
 // adapters.hip -- low-rank adapters of many requests at once:
 //   y_t = base_t + s_a B_a (A_a x_t),  a: row t's adapter (rows without one: base_t)
 //
-// Rows come sorted by adapter, in chunks of up to 64 rows of one adapter.
-// Two launches: u = A x for every chunk (K in slices where chunks are few; their
-// partial sums stay f32), then y = base + B (s u), which adds the slices in order.
+// Rows come sorted by adapter, in chunks of one adapter: 16 to 64 rows in the first
+// launch, 32 in the second.  The first is u = A x for every chunk (K in slices where
+// chunks are few; their partial sums stay f32), the other y = base + B (s u), which adds
+// the slices in order; a chunk without an adapter, or of rank 0, is copied from base.
 // (Both in one launch, u made again by every workgroup: one row of rank 16 took 10 us of
 // kernel time for 4.9 + 5.4, but rank 32, or 16 rows and more, 15 to 65 % more than two.)
 //
@@ -13,10 +14,12 @@
 //
 // Bound: HBM, by base and y (x, A and B besides); rows that are few, by two launches of
 // some three dependent round trips each.  4,096 rows, rank 32, 4,096 -> 14,336, all
-// bf16: u 17 us (27 MB of x, and A from the L2), y 57 (235 MB, 4.1 TB/s; a copy of the
-// same rows takes 44), 70 to 75 in all.  Rank 64: 23 + 78: the second launch's u and B
-// from the L2 cost it what the matrix cores do not.  One row, rank 16, 4,096 -> 4,096: 4.9 +
-// 5.4.  64 rows of 33 adapters of rank 4 to 64 in f32, 4,096 -> 14,336: 9.2 + 14.3; the
+// bf16: u 17.5 us (27 MB of x, and A from the L2), y 57 (235 MB, 4.1 TB/s; the runtime's
+// copy of as many bytes takes 44, the rows copied by this kernel for want of adapters
+// 48), 67 to 75 in all.  Rank 64: 23 + 81: the second launch's u and B from the L2 cost it
+// what the matrix cores do not.  Rank 128: 36 + 172, rank 256: 59 + 300: past 64, B is read
+// once per tile of 16 rows, where it is multiplied.  One row, rank 16, 4,096 -> 4,096: 4.9 +
+// 5.4.  64 rows of 33 adapters of rank 4 to 64 in f32, 4,096 -> 14,336: 9.7 + 15.1; the
 // second reads rows of B of 128 bytes of which the rank fills half.
 #include <array>
 #include <type_traits>
@@ -293,7 +296,7 @@ enum BaseType { kBaseNone, kBaseBf16, kBaseF32 };
 // bytes (of y's type).  Four lanes' runs of one row are 64 bytes, half a line; lanes c
 // and c ^ 1 exchange every second run, so that a store writes whole lines of the
 // eight even rows, the next those of the odd ones (4,096 x 14,336 in bf16, copied so past
-// the caches: 47 us, in half lines 56).  f32: run m is columns 16 m + 4 q of the block,
+// the caches: 48 us, in half lines 56).  f32: run m is columns 16 m + 4 q of the block,
 // tile m; bf16: run h is 32 h + 8 q, tiles 2 h and 2 h + 1 with four columns each in
 // turn.
 template <bool F32>
@@ -584,9 +587,11 @@ __global__ __launch_bounds__(64 * kOutWaves, STEPS ? 1 : 4) void adapters_out_ke
 int max_chunks(int T, int E, int rows) { return (T < E ? T : E) + T / rows; }
 
 // Rows of a chunk of the first launch: more of them read A less often, fewer make more
-// workgroups.  16 / 32 / 64 rows, us of the whole call: 512 rows of rank 32 20.9 / 22.6 /
-// 24.6; 1,024 of rank 16 19.2 / 18.2 / 20.5; 4,096 of rank 32 80 / 75 / 77; 2,048 of rank 64
-// 40.4 / 40.4 / 35.0, 4,096 of it 111 / 107 / 102.
+// workgroups.  16 / 32 / 64 rows, nine adapters, us of the whole call: 512 rows of rank 32
+// 20.9 / 22.6 / 24.6; 1,024 of rank 16 19.2 / 18.2 / 20.5; 4,096 of rank 32 80 / 75 / 77;
+// 2,048 of rank 64 40.4 / 40.4 / 35.0, 4,096 of it 111 / 107 / 102.  (By T and R alone: with
+// 256 adapters a chunk of 32 holds some eight of 2,048 rows; rank 32, 4,096 -> 4,096, 17 us
+// of the call's 36.)
 // Slices of K, each read again by the second launch: up to some 1,024 workgroups, each
 // wave at least one block of 128 columns.  1,024 / 512 / 256: 256 adapters' rows 23.9 / 27.3 /
 // 27.4, 8,192 rows of rank 32 60.8 / 66.1 / 66.2, 4,096 of rank 64 99.9 / 99.6 / 96.2.

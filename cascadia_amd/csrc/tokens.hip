@@ -14,8 +14,8 @@
 //   combine  out[t] = res[t] + sum w y       each slot's row read once
 //   gradient dy[row] = w dout, dw = y . dout  both in one pass over y
 // 4,096 tokens, 8 slots each, rows of 7,168 in bf16: gather 88 us (514 MB, 5.8 TB/s),
-// combine 97 to 111 (574 MB, 5.2 to 5.9); the gradient of rows of 4,096: 104 us (555 MB,
-// 5.3).  A copy of 2 GiB reaches 4.9: these write and read past the caches (below).
+// combine 111 (574 MB, 5.2); the gradient of rows of 4,096: 104 us (555 MB, 5.3).  A copy
+// of 2 GiB reaches 4.9: these write and read past the caches (below).
 #include "fp8.hpp"
 #include "rows.hpp"
 #include "tokens.hpp"
@@ -383,8 +383,9 @@ dim3 move_grid(int T, int cols, int V) {
 
 // Whether the slots' rows are written or read past the caches' replacement: more of them
 // than the Infinity Cache (256 MiB) holds, in whole lines.  Gather, written so or not:
-// 470 MB 89 / 106 us, 134 MB 26.2 / 26.9, 67 MB 12.7 / 12.6; combine, read so or not: 470 MB
-// 97 / 119, 101 MB 29.3 / 22.2 (then still in that cache); the gradient, both: 268 MB 104 /
+// 470 MB 89 / 106 us, 134 MB 26.2 / 26.9, 67 MB 12.7 / 12.6; combine, read so or not
+// (residual and output in that cache): 470 MB 97 / 119, 101 MB 29.3 / 22.2 (then the rows
+// are in it as well); the gradient, both: 268 MB 104 /
 // 114; rows of an odd number of bytes, written so: 37 / 31.
 constexpr size_t kStreamBytes = (size_t)256 << 20, kLine = 128;
 bool streams(const void *p, int rows, int cols, size_t size) {
