@@ -4,8 +4,8 @@ import numpy as np
 import pytest
 import torch
 
-from test_gpu_adapters import cl, gen, host  # noqa: F401
-from test_gpu_adapters_bits import forward
+from test_gpu_adapters import case, cl, gen, host, plan  # noqa: F401
+from test_gpu_adapters_bits import bits, forward
 
 pytestmark = pytest.mark.gpu
 F32, BF16 = torch.float32, torch.bfloat16
@@ -103,3 +103,26 @@ def test_every_nan_of_x_stays_one(cl, T, nan):
     assert bool(got[T // 2].isnan().all())
     got[T // 2] = 0
     assert bool(got.isfinite().all())
+
+
+@pytest.mark.parametrize("t", [BF16, F32])
+@pytest.mark.parametrize("R", [16, 40, 72])
+def test_in_place_where_sums_are_taken_again(cl, t, R):
+    """Rows with infinite sums in either tile of a chunk, over base: as out of place, and
+    the rows between them as without any infinity."""
+    T, E, K, N = 150, 2, 136, 330
+    a, b, ranks, scales, ids, x, base = case(25, T, E, R, K, N, t, t, mixed=False, bare=0.1)
+    clean = forward(cl, (a, b, ranks, scales, ids, x, base), t)
+    hit = torch.zeros(T, dtype=torch.bool)
+    hit[::9] = True
+    hit &= (ids >= 0) & (ids < E)
+    x = x.clone()
+    x[hit, 3], x[hit, 4] = INF, -INF
+    out = forward(cl, (a, b, ranks, scales, ids, x, base), t)
+    off, slots = plan(cl, ids, E)
+    A = cl.Adapters(a.cuda(), b.cuda(), ranks=ranks.cuda(), scales=scales.cuda())
+    y = base.cuda()
+    cl.adapters_forward(A, x.cuda(), off, slots, y, base=y)
+    assert torch.equal(bits(y), bits(out))
+    assert torch.equal(bits(out)[~hit], bits(clean)[~hit])
+    assert not out.cpu()[hit].isfinite().any()
